@@ -280,6 +280,150 @@ TS_API int ts_decode_attention(const void* qkv, int64_t qkv_row_stride, int batc
                                int64_t cache_head_stride, int attn_len, int max_seq, void* out,
                                int64_t out_row_stride, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged key-value cache for sequences of unequal length (no counterpart in
+ * the reference, whose models keep their own caches).
+ *
+ * k_pages / v_pages: fp16 or bf16 [num_pages, n_kv, page_size, head_dim] with
+ * the given element strides, the same for both (multiples of 8; rows of
+ * head_dim contiguous; a token-major pool is a choice of strides). Slot s of
+ * sequence b lies in page page_table[b * table_stride + s / page_size] at
+ * offset s % page_size; entries outside [0, num_pages) have no memory and
+ * are never touched. seq_lens[b] counts the cached tokens of sequence b; a
+ * negative count marks a sequence that takes no part in a call. scores
+ * (fp32) and slot_pos (int32), both contiguous [num_pages, n_kv, page_size]
+ * or NULL, hold each slot's accumulated attention weight and its token's
+ * position; ts_paged_evict needs both. head_dim: a multiple of 16 up to 256.
+ */
+typedef struct ts_paged_cache {
+  void* k_pages;
+  void* v_pages;
+  int64_t page_stride, head_stride, token_stride;
+  const int32_t* page_table;  /* device [batch, max_pages] */
+  int64_t table_stride;
+  int32_t* seq_lens;          /* device [batch] */
+  float* scores;
+  int32_t* slot_pos;
+  int32_t dtype;              /* TS_F16 or TS_BF16 */
+  int32_t batch, n_kv, head_dim, page_size, num_pages, max_pages;
+  int32_t reserved0;
+} ts_paged_cache;
+
+/*
+ * Stores `tokens` new tokens per sequence in slots seq_lens[b] + t (n_new,
+ * device [batch] or NULL, gives a smaller count per sequence). k / v:
+ * [batch, tokens, n_kv, head_dim] in the cache's type with element strides
+ * (sequence, token, head). With rotary tables (fp32 [rope_rows, head_dim / 2])
+ * keys are rotated to position first[b] + t (first: device int64, or NULL for
+ * the slot's number). scores (fp32 [batch, n_kv, tokens], strides (sequence,
+ * head, token)) initialise the slots' scores, 0 without. Tokens without a
+ * slot, a page or a rotary row are dropped. seq_lens is not changed.
+ */
+TS_API int ts_paged_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                           int tokens, const int32_t* n_new, const ts_paged_cache* cache, const int64_t* first,
+                           const float* rope_cos, const float* rope_sin, int64_t rope_rows, const float* scores,
+                           const int64_t* score_strides, void* stream);
+
+/*
+ * One decode step of grouped-query attention: for each sequence, q and k of
+ * the new token are rotated to positions[b] (no rotation without tables), k
+ * and v stored in slot seq_lens[b], and every query head attends over slots
+ * [0, seq_lens[b]] with scores scale * q.k. With accumulate != 0 each slot's
+ * score grows by the weights that the kv head's query heads gave it (the new
+ * slot's starts from 0; it is set to 0 too when nothing is accumulated). A
+ * sequence whose count is negative, that has no page left for the token, or
+ * whose position has no rotary row answers with zeros and stores nothing.
+ * seq_lens is not changed. qkv, out as in ts_decode_attention, in the
+ * cache's type. workspace: zero-filled once; its first 256 KB are zero again
+ * after every call and the rest is scratch (one workspace may serve all
+ * ts_paged_* and ts_fp4_* calls of a stream).
+ */
+TS_API size_t ts_paged_attention_workspace_size(const ts_paged_cache* cache, int n_q, int accumulate);
+TS_API int ts_paged_decode_attention(const void* qkv, int64_t qkv_row_stride, int n_q, const ts_paged_cache* cache,
+                                     const int64_t* positions, const float* rope_cos, const float* rope_sin,
+                                     int64_t rope_rows, float scale, int accumulate, void* out,
+                                     int64_t out_row_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Cuts every sequence longer than `budget` back to `budget` slots per kv
+ * head: the slots of the `recent` newest positions stay, then those of the
+ * largest scores (equal scores: the lowest slot; NaN counts as -inf). Kept
+ * slots at or behind `budget` move into the holes before it, both in
+ * ascending order, and seq_lens becomes `budget`. A sequence's pages must
+ * not be shared with another one. Workspace as ts_paged_decode_attention.
+ */
+TS_API size_t ts_paged_evict_workspace_size(const ts_paged_cache* cache, int budget);
+TS_API int ts_paged_evict(const ts_paged_cache* cache, int budget, int recent, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Microscaled 4-bit floating point. Elements are E2M1, the even column in a
+ * byte's low nibble, columns padded with zeros to a multiple of 64:
+ *   TS_NVFP4  blocks of 16 columns with an E4M3 scale s and one fp32 scale g
+ *             of the tensor: value = e2m1 * (s * g)
+ *   TS_MXFP4  blocks of 32 columns with an E8M0 scale: value = e2m1 * 2^(s - 127)
+ * codes: [rows, padded_cols / 2]. scales: tiles of 128 rows x 4 blocks, 512
+ * bytes each, the tiles of a row of tiles one after another; the byte of
+ * (row r, block j) within its tile is (r % 32) * 16 + (r % 128) / 32 * 4 + j % 4.
+ * Bytes of rows behind the last one are never read.
+ */
+typedef enum ts_fp4_format {
+  TS_NVFP4 = 0,
+  TS_MXFP4 = 1
+} ts_fp4_format;
+
+typedef struct ts_fp4_tensor {
+  uint8_t* codes;        /* device, 16-byte aligned */
+  uint8_t* scales;       /* device, 16-byte aligned */
+  float* global_scale;   /* device [1] (TS_NVFP4), or NULL (counts as 1) */
+  int64_t rows, cols;
+  int32_t format;
+  int32_t reserved0;
+} ts_fp4_tensor;
+
+/*
+ * Quantises x [rows, cols] (fp16, bf16 or fp32) into t. TS_NVFP4:
+ *   s = e4m3(min(max|block| * (1 / (6 g)), 448)),  e2m1(x * (1 / (s g)))
+ * with every operation rounded to fp32 and both conversions to nearest even
+ * (saturating); g is t->global_scale[0], which find_scale != 0 first sets to
+ * max(max|x| * fp32(1 / 2688), 2^-100) over the finite elements. TS_MXFP4:
+ *   s = 2^(floor(log2 max|block|) - 2), at least 2^-127;  e2m1(x / s)
+ * A block that holds an infinity or a NaN gets a NaN scale and zero codes.
+ * A given g outside [2^-100, 2^118] counts as the nearer bound, a NaN as the
+ * lower. workspace: ts_fp4_quantize_workspace_size() bytes when find_scale is set.
+ */
+TS_API size_t ts_fp4_scales_bytes(int64_t rows, int64_t cols, int format);
+TS_API size_t ts_fp4_quantize_workspace_size(void);
+TS_API int ts_fp4_quantize(const void* x, int x_dtype, int64_t x_row_stride, const ts_fp4_tensor* t, int find_scale,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* The values of t in out_dtype, rounded once from e2m1 * fp32(s * g). */
+TS_API int ts_fp4_dequantize(const ts_fp4_tensor* t, void* out, int out_dtype, int64_t out_row_stride, void* stream);
+
+/*
+ * out[M, N] = a . b^T (+ bias) for a [M, K] and b [N, K] of one format on the
+ * block-scaled tensor cores, fp32 sums: ga * gb * sum + bias, rounded once
+ * to out_dtype. Workspace as ts_paged_decode_attention.
+ */
+TS_API size_t ts_fp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int format);
+TS_API int ts_fp4_matmul(const ts_fp4_tensor* a, const ts_fp4_tensor* b, const void* bias, int bias_dtype, void* out,
+                         int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/*
+ * out[M, N] = x . w^T (+ bias): ts_fp4_quantize of x [M, cols] (with the given
+ * device scale x_scale for TS_NVFP4, NULL: 1) into the workspace, then
+ * ts_fp4_matmul.
+ */
+TS_API size_t ts_fp4_linear_workspace_size(int64_t M, int64_t N, int64_t K, int format);
+TS_API int ts_fp4_linear(const void* x, int x_dtype, int64_t M, int64_t x_row_stride, float* x_scale,
+                         const ts_fp4_tensor* w, const void* bias, int bias_dtype, void* out, int out_dtype,
+                         int64_t out_row_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ts_qlinear_status for the fp4 product (a per-device flag); with clear the
+ * counters at the workspace's start are zeroed too (workspace may be NULL). */
+TS_API int ts_fp4_status(void* workspace, size_t workspace_bytes, int clear, void* stream);
+
 /* Dense reconstruction W[rows, cols] in `out_dtype`.
  * Replaces triton_kernels.py:1114-1186 `dequantize_weight` (which covers only
  * 4/8-bit; this covers 2/4/8 and the double-quantized metadata). With

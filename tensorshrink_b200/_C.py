@@ -76,6 +76,24 @@ class TsQlinearOp(C.Structure):
     ]
 
 
+class TsPagedCache(C.Structure):
+    """struct ts_paged_cache."""
+    _fields_ = [
+        ("k_pages", _vp), ("v_pages", _vp), ("page_stride", _i64), ("head_stride", _i64), ("token_stride", _i64),
+        ("page_table", _vp), ("table_stride", _i64), ("seq_lens", _vp), ("scores", _vp), ("slot_pos", _vp),
+        ("dtype", _i32), ("batch", _i32), ("n_kv", _i32), ("head_dim", _i32), ("page_size", _i32),
+        ("num_pages", _i32), ("max_pages", _i32), ("reserved0", _i32),
+    ]
+
+
+class TsFp4Tensor(C.Structure):
+    """struct ts_fp4_tensor."""
+    _fields_ = [("codes", _vp), ("scales", _vp), ("global_scale", _vp), ("rows", _i64), ("cols", _i64),
+                ("format", _i32), ("reserved0", _i32)]
+
+
+TS_NVFP4, TS_MXFP4 = 0, 1
+
 OP_GATED = 1
 OP_RMSNORM = 2
 
@@ -107,6 +125,24 @@ _SIGNATURES = [
     ("ts_allreduce_oneshot", C.c_int, [C.POINTER(C.c_void_p), C.c_int, C.c_int, _i64, _vp, _vp, _vp, _i64, _vp, _vp]),
     ("ts_decode_attention", C.c_int, [_vp, _i64, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp,
                                       _i64, _i64, C.c_int, C.c_int, _vp, _i64, _vp]),
+    ("ts_paged_append", C.c_int, [_vp, C.POINTER(_i64), _vp, C.POINTER(_i64), C.c_int, _vp, C.POINTER(TsPagedCache),
+                                  _vp, _vp, _vp, _i64, _vp, C.POINTER(_i64), _vp]),
+    ("ts_paged_attention_workspace_size", C.c_size_t, [C.POINTER(TsPagedCache), C.c_int, C.c_int]),
+    ("ts_paged_decode_attention", C.c_int, [_vp, _i64, C.c_int, C.POINTER(TsPagedCache), _vp, _vp, _vp, _i64,
+                                            C.c_float, C.c_int, _vp, _i64, _vp, C.c_size_t, _vp]),
+    ("ts_paged_evict_workspace_size", C.c_size_t, [C.POINTER(TsPagedCache), C.c_int]),
+    ("ts_paged_evict", C.c_int, [C.POINTER(TsPagedCache), C.c_int, C.c_int, _vp, C.c_size_t, _vp]),
+    ("ts_fp4_scales_bytes", C.c_size_t, [_i64, _i64, C.c_int]),
+    ("ts_fp4_quantize_workspace_size", C.c_size_t, []),
+    ("ts_fp4_quantize", C.c_int, [_vp, C.c_int, _i64, C.POINTER(TsFp4Tensor), C.c_int, _vp, C.c_size_t, _vp]),
+    ("ts_fp4_dequantize", C.c_int, [C.POINTER(TsFp4Tensor), _vp, C.c_int, _i64, _vp]),
+    ("ts_fp4_matmul_workspace_size", C.c_size_t, [_i64, _i64, _i64, C.c_int]),
+    ("ts_fp4_matmul", C.c_int, [C.POINTER(TsFp4Tensor), C.POINTER(TsFp4Tensor), _vp, C.c_int, _vp, C.c_int, _i64,
+                                _vp, C.c_size_t, _vp]),
+    ("ts_fp4_linear_workspace_size", C.c_size_t, [_i64, _i64, _i64, C.c_int]),
+    ("ts_fp4_linear", C.c_int, [_vp, C.c_int, _i64, _i64, _vp, C.POINTER(TsFp4Tensor), _vp, C.c_int, _vp, C.c_int,
+                                _i64, _vp, C.c_size_t, _vp]),
+    ("ts_fp4_status", C.c_int, [_vp, C.c_size_t, C.c_int, _vp]),
     ("ts_dequantize_weight", C.c_int, [C.POINTER(TsQWeight), _vp, C.c_int, _i64, C.c_int, _vp]),
     ("ts_quantize_workspace_size", C.c_size_t, [C.POINTER(TsQuantParams)]),
     ("ts_quantize_pack", C.c_int, [_vp, C.c_int, C.POINTER(TsQuantParams), C.POINTER(TsQuantOutputs),

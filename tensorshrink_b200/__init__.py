@@ -35,6 +35,20 @@ from .kernels import (
     apply_outlier_correction,
     dequantize_weight,
 )
+from .fp4 import (
+    Fp4Tensor,
+    Fp4Linear,
+    fp4_quantize,
+    fp4_dequantize,
+    fp4_matmul,
+    fp4_linear,
+)
+from .paged import (
+    PagedKVCache,
+    paged_append,
+    paged_decode_attention,
+    paged_evict,
+)
 
 __version__ = "0.1.0"
 
@@ -44,4 +58,6 @@ __all__ = [
     "T5_EXTRA_SKIP_PATTERNS", "suggest_max_dequant_rows", "quantize_tensor_gpu",
     "quantize_tensor_gpu_adaptive", "quantize_module_gpu", "fused_quantized_linear",
     "apply_outlier_correction", "dequantize_weight", "ChainStep", "qlinear_chain",
+    "Fp4Tensor", "Fp4Linear", "fp4_quantize", "fp4_dequantize", "fp4_matmul", "fp4_linear",
+    "PagedKVCache", "paged_append", "paged_decode_attention", "paged_evict",
 ]

@@ -1,0 +1,749 @@
+// Attention of one new token per sequence over a paged key-value cache.
+//
+//   q, k, v of the new token from its projection; q and k rotated to the
+//   token's position; k and v stored in slot len of the sequence; then, for
+//   each query head of the kv head's group,
+//     s_t = scale q . k_t,  t = 0 .. len,      p = softmax(s),   o = sum_t p_t v_t
+//   and, when weights are accumulated, score_t += sum over the group of p_t
+//   (the new slot's score is set, not added to).
+//
+// What bounds it: the cache is read once, 2 len D elements per kv head, and
+// every element meets only the group's few query heads, so DRAM bandwidth
+// does. The work is cut into units of 64 slots of one kv head, the units of
+// all sequences laid end to end, and CTA i takes an equal range of them: a
+// batch of unequal lengths, or a single long sequence, loads every SM alike.
+// A head whose units lie in several CTAs is joined by the last of them to
+// arrive, from fp32 partial sums in the workspace, in CTA order (so results
+// do not depend on timing).
+//
+// Inside a CTA each warp owns 16 slots of every unit and streams them through
+// its own ring of shared-memory stages with cp.async (no CTA barrier in the
+// loop). Scores and outputs use mma.m16n8k16 with the group's heads as the 16
+// rows: padding a small group to 16 rows costs tensor-core time that the
+// kernel has to spare, and P passes from the score accumulators to the second
+// product without leaving registers. Softmax statistics and sums are fp32; P
+// is rounded to the cache's type for its product, as wide as v itself: the
+// rounding errors of a row's weights average out in the sum over slots.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace ts {
+namespace paged {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 16;                  // slots of a warp's share of a unit
+constexpr int kUnit = kWarps * kRows;      // slots of a unit
+constexpr int kHeads = 16;                 // query heads of an MMA tile
+
+struct AttnArgs {
+  Cache c;
+  const uint16_t* qkv;
+  int64_t qkv_stride;
+  int n_q, group, head_tiles;
+  const int64_t* positions;
+  const float* cos_t;
+  const float* sin_t;
+  int64_t rope_rows;
+  float scale2;          // scale * log2(e)
+  uint16_t* out;
+  int64_t out_stride;
+  int* counters;
+  float* partials;       // [grid][2][16][D + 2]: the group's rows, each with its max and sum
+  float* lse2;           // [batch * n_q] log2 of the softmax denominators, or NULL
+  float* logits;         // [batch * n_q][cap] scores in log2 units, or NULL
+  int64_t logit_stride;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+template <bool BF>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};" : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};" : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Units of sequence b for one kv head, 0 when the call cannot take it: no
+// slot for the new token, or a position outside the rotary tables.
+__device__ __forceinline__ int units_of(const AttnArgs& a, int b) {
+  const int len = a.c.seq_lens[b];
+  if (len < 0 || len >= capacity(a.c)) return 0;
+  if (a.cos_t != nullptr) {
+    const int64_t pos = a.positions[b];
+    if (pos < 0 || pos >= a.rope_rows) return 0;
+  }
+  if (page_of(a.c, b, len) < 0) return 0;
+  return len / kUnit + 1;
+}
+
+// Shared memory: the warps' rings [kWarps][S][K, V][16 rows][pitch], the
+// query tile [16][DP + 8] and the prefix sums of the sequences' units. Row r
+// keeps its 16-byte chunk c at c ^ (r & 7), so that ldmatrix reads of eight
+// rows touch every bank once.
+template <int DP>
+constexpr int stages_for() { return DP == 64 ? 6 : 3; }
+template <int DP>
+constexpr size_t ring_bytes() { return (size_t)kWarps * stages_for<DP>() * 2 * kRows * DP * 2; }
+template <int DP>
+constexpr size_t attn_smem(int batch) {
+  return ring_bytes<DP>() + kHeads * (DP + 8) * 2 + (size_t)(batch + 1) * 4 + 64;
+}
+
+template <bool BF, int DP>
+__global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArgs a) {
+  constexpr int S = stages_for<DP>();
+  constexpr int kPitch = DP * 2;                 // bytes of a staged row
+  constexpr int kStage = 2 * kRows * kPitch;     // bytes of a stage: K rows, then V rows
+  constexpr int kSteps = DP / 16;
+  constexpr bool kKeepQ = DP <= 128;             // query fragments stay in registers
+  extern __shared__ __align__(128) char smem[];
+  uint16_t* qs = reinterpret_cast<uint16_t*>(smem + ring_bytes<DP>());
+  int* prefix = reinterpret_cast<int*>(smem + ring_bytes<DP>() + kHeads * (DP + 8) * 2);
+  __shared__ int warp_sums[kWarps];
+  __shared__ int is_last;
+  const Cache& c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int D = c.head_dim, chunks = D / 8, steps = D / 16, rows_per_b = c.n_kv * a.head_tiles;
+
+  // prefix sums of the sequences' units; every thread takes a run of sequences
+  {
+    const int per = (c.batch + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) sum += units_of(a, b);
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    int at = inc - sum;
+    for (int w = 0; w < warp; ++w) at += warp_sums[w];
+    for (int b = b0; b < b1; ++b) {
+      prefix[b] = at;
+      at += units_of(a, b);
+    }
+    if (b1 == c.batch && b0 < b1) prefix[c.batch] = at;
+  }
+  // rows of the query tile that no head fills: zeros, so that their scores are finite
+  for (int i = tid; i < kHeads * (DP + 8) / 2; i += kThreads) reinterpret_cast<uint32_t*>(qs)[i] = 0;
+  __syncthreads();
+  // a sequence that the call cannot take answers with zeros
+  for (int b = blockIdx.x; b < c.batch; b += gridDim.x)
+    if (prefix[b] == prefix[b + 1])
+      for (int i = tid; i < a.n_q * D; i += kThreads) a.out[b * a.out_stride + i] = 0;
+
+  const int64_t total = (int64_t)prefix[c.batch] * rows_per_b;
+  const int64_t n_cta = min((int64_t)gridDim.x, total);
+  if ((int64_t)blockIdx.x >= n_cta) return;
+  const int64_t u0 = total * blockIdx.x / n_cta, u1 = total * (blockIdx.x + 1) / n_cta;
+
+  char* ring = smem + (size_t)warp * S * kStage;
+  const uint32_t ring_u = smem_u32(ring);
+  const uint32_t qs_u = smem_u32(qs);
+
+  for (int64_t u = u0; u < u1;) {
+    // the segment: units [t0, t1) of (sequence b, kv head h, head tile ht)
+    int b;
+    {
+      int lo = 0, hi = c.batch - 1;   // last b with prefix[b] * rows_per_b <= u and units
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((int64_t)prefix[mid] * rows_per_b <= u) lo = mid; else hi = mid - 1;
+      }
+      b = lo;
+    }
+    const int nt = prefix[b + 1] - prefix[b];
+    const int64_t in_b = u - (int64_t)prefix[b] * rows_per_b;
+    const int row = (int)(in_b / nt);
+    const int t0 = (int)(in_b - (int64_t)row * nt);
+    const int t1 = (int)min((int64_t)nt, t0 + (u1 - u));
+    const int h = row / a.head_tiles, ht = row - h * a.head_tiles;
+    const int heads = min(kHeads, a.group - ht * kHeads);
+    const int head0 = h * a.group + ht * kHeads;       // first query head of the tile
+    const int len = c.seq_lens[b];
+    const int64_t pos = a.positions != nullptr ? a.positions[b] : 0;
+    const uint16_t* new_row = a.qkv + b * a.qkv_stride;
+    const float* cs = a.cos_t != nullptr ? a.cos_t + pos * (D / 2) : nullptr;
+    const float* sn = a.cos_t != nullptr ? a.sin_t + pos * (D / 2) : nullptr;
+
+    // rows of warp-unit t: slots t * 64 + warp * 16 + r. Lane r (< 16) finds
+    // the element offset of row r, -1 where nothing is to be copied.
+    auto row_offset = [&](int t) -> int64_t {
+      const int slot = t * kUnit + warp * kRows + (lane & 15);
+      if (t >= t1 || slot >= len) return -1;
+      const int page = page_of(c, b, slot);
+      return page < 0 ? -1 : row_at(c, page, h, slot % c.page_size);
+    };
+    auto issue = [&](int t, int stage, int64_t off) {
+      if (t < t1) {
+        const uint32_t base = ring_u + stage * kStage;
+        for (int i = lane; i < kRows * chunks; i += 32) {   // a multiple of 32 pieces: D % 16 == 0
+          const int r = i / chunks, ch = i - r * chunks;
+          const int64_t o = __shfl_sync(0xffffffffu, off, r);
+          const uint32_t dst = base + r * kPitch + ((ch ^ (r & 7)) << 4);
+          const int64_t e = o < 0 ? 0 : (o + ch * 8) * 2;
+          cp16(dst, c.k + e, o < 0 ? 0 : 16);
+          cp16(dst + kRows * kPitch, c.v + e, o < 0 ? 0 : 16);
+        }
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) issue(t0 + s, s, row_offset(t0 + s));
+    int64_t next_off = row_offset(t0 + S - 1);
+
+    // the rotated query heads of the tile
+    for (int i = tid; i < heads * (D / 2); i += kThreads) {
+      const int g = i / (D / 2), j = i - g * (D / 2);
+      const uint16_t* qr = new_row + (int64_t)(head0 + g) * D;
+      uint16_t x1 = qr[j], x2 = qr[j + D / 2];
+      if (cs != nullptr) {
+        const float2 f = unpack2<BF>((uint32_t)x1 | ((uint32_t)x2 << 16));
+        const float2 y = rotate(f.x, f.y, cs[j], sn[j]);
+        const uint32_t p = pack2<BF>(y.x, y.y);
+        x1 = (uint16_t)p;
+        x2 = (uint16_t)(p >> 16);
+      }
+      qs[g * (DP + 8) + j] = x1;
+      qs[g * (DP + 8) + j + D / 2] = x2;
+    }
+    __syncthreads();
+    uint32_t qf[kKeepQ ? kSteps : 1][4];
+    const uint32_t q_addr = qs_u + ((lane & 15) * (DP + 8) + (lane >> 4) * 8) * 2;
+    if (kKeepQ) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        if (s < steps) ldsm4(q_addr + s * 32, qf[kKeepQ ? s : 0]);
+    }
+
+    float o[DP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const int r7 = lane & 7;
+
+    int stage = 0;
+    for (int t = t0; t < t1; ++t) {
+      issue(t + S - 1, stage == 0 ? S - 1 : stage - 1, next_off);
+      next_off = row_offset(t + S);
+      cp_wait<S - 1>();
+      __syncwarp();
+      const int slot0 = t * kUnit + warp * kRows;
+      const uint32_t kb = ring_u + stage * kStage, vb = kb + kRows * kPitch;
+      stage = stage + 1 == S ? 0 : stage + 1;
+      if (slot0 > len) continue;                       // warp-uniform: nothing left for this warp
+      if (len < slot0 + kRows) {
+        // the new token's row: into the stage and, once per kv head, the cache
+        const int r = len - slot0;
+        char* st = ring + (kb - ring_u);
+        const int page = page_of(c, b, len);
+        const int64_t at = row_at(c, page, h, len % c.page_size);
+        uint16_t* kc = reinterpret_cast<uint16_t*>(c.k) + at;
+        uint16_t* vc = reinterpret_cast<uint16_t*>(c.v) + at;
+        const uint16_t* kr = new_row + (int64_t)(a.n_q + h) * D;
+        const uint16_t* vr = new_row + (int64_t)(a.n_q + c.n_kv + h) * D;
+        for (int j = lane; j < D / 2; j += 32) {
+          uint16_t x1 = kr[j], x2 = kr[j + D / 2];
+          if (cs != nullptr) {
+            const float2 f = unpack2<BF>((uint32_t)x1 | ((uint32_t)x2 << 16));
+            const float2 y = rotate(f.x, f.y, cs[j], sn[j]);
+            const uint32_t p = pack2<BF>(y.x, y.y);
+            x1 = (uint16_t)p;
+            x2 = (uint16_t)(p >> 16);
+          }
+          const uint16_t v1 = vr[j], v2 = vr[j + D / 2];
+          const int j2 = j + D / 2;
+          auto at16 = [&](int e) { return r * kPitch + (((e >> 3) ^ (r & 7)) << 4) + (e & 7) * 2; };
+          *reinterpret_cast<uint16_t*>(st + at16(j)) = x1;
+          *reinterpret_cast<uint16_t*>(st + at16(j2)) = x2;
+          *reinterpret_cast<uint16_t*>(st + kRows * kPitch + at16(j)) = v1;
+          *reinterpret_cast<uint16_t*>(st + kRows * kPitch + at16(j2)) = v2;
+          if (ht == 0) {
+            kc[j] = x1;
+            kc[j2] = x2;
+            vc[j] = v1;
+            vc[j2] = v2;
+          }
+        }
+        if (lane == 0 && ht == 0) {
+          const int64_t sa = stat_at(c, page, h, len % c.page_size);
+          if (c.scores != nullptr) c.scores[sa] = 0.f;
+          if (c.slot_pos != nullptr) c.slot_pos[sa] = (int32_t)pos;
+        }
+        __syncwarp();
+      }
+
+      // scores of 16 heads x 16 slots
+      float sc[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+      const int krow = (lane & 7) + ((lane >> 4) << 3);
+      const uint32_t k_addr = kb + krow * kPitch;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if (s >= steps) break;
+        uint32_t kf[4];
+        ldsm4(k_addr + (((2 * s + ((lane >> 3) & 1)) ^ r7) << 4), kf);
+        if (!kKeepQ) ldsm4(q_addr + s * 32, qf[0]);
+        mma<BF>(sc[0], qf[kKeepQ ? s : 0], kf[0], kf[1]);
+        mma<BF>(sc[1], qf[kKeepQ ? s : 0], kf[2], kf[3]);
+      }
+      // slots that exist: below the new one, or it, and with memory
+      const int64_t mine = row_offset(t);              // of row (lane & 15)
+      const int my_slot = slot0 + (lane & 15);
+      const unsigned live = __ballot_sync(0xffffffffu, my_slot == len || mine >= 0);
+      const int c0 = (lane & 3) * 2;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = n * 8 + c0 + (e & 1);
+          sc[n][e] = (live >> r) & 1 ? sc[n][e] * a.scale2 : -INFINITY;
+        }
+      if (a.logits != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int g = (lane >> 2) + 8 * e;
+          if (g < heads) {
+            float* lg = a.logits + (int64_t)(b * a.n_q + head0 + g) * a.logit_stride + slot0 + c0;
+            *reinterpret_cast<float2*>(lg) = make_float2(sc[0][2 * e], sc[0][2 * e + 1]);
+            *reinterpret_cast<float2*>(lg + 8) = make_float2(sc[1][2 * e], sc[1][2 * e + 1]);
+          }
+        }
+      }
+      // online softmax of the two rows this thread holds parts of
+      float mn[2], base[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = fmaxf(fmaxf(sc[0][2 * e], sc[0][2 * e + 1]), fmaxf(sc[1][2 * e], sc[1][2 * e + 1]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        mn[e] = fmaxf(m[e], x);
+        base[e] = mn[e] == -INFINITY ? 0.f : mn[e];
+      }
+      if (__any_sync(0xffffffffu, mn[0] > m[0] || mn[1] > m[1])) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float corr = exp2f(m[e] - base[e]);
+          l[e] *= corr;
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) {
+            o[i][2 * e] *= corr;
+            o[i][2 * e + 1] *= corr;
+          }
+          m[e] = mn[e];
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sc[n][e] = exp2f(sc[n][e] - base[e >> 1]);
+          l[e >> 1] += sc[n][e];
+        }
+      const uint32_t pf[4] = {pack2<BF>(sc[0][0], sc[0][1]), pack2<BF>(sc[0][2], sc[0][3]),
+                              pack2<BF>(sc[1][0], sc[1][1]), pack2<BF>(sc[1][2], sc[1][3])};
+      const int vrow = lane & 15;
+      const uint32_t v_addr = vb + vrow * kPitch;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if (s >= steps) break;
+        uint32_t vf[4];
+        ldsm4t(v_addr + (((2 * s + (lane >> 4)) ^ r7) << 4), vf);
+        mma<BF>(o[2 * s], pf, vf[0], vf[1]);
+        mma<BF>(o[2 * s + 1], pf, vf[2], vf[3]);
+      }
+      __syncwarp();   // the stage is refilled at the top of the next round
+    }
+    cp_wait<0>();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+    }
+    __syncthreads();
+
+    // join the warps through shared memory (over the drained rings)
+    constexpr int kJoin = DP + 4;                    // floats of a row: its sums, max, sum
+    float* jo = reinterpret_cast<float*>(smem);      // [kWarps][16][kJoin]
+    static_assert((size_t)kWarps * kHeads * kJoin * 4 <= ring_bytes<DP>() + kHeads * (DP + 8) * 2, "join area");
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float* r = jo + (warp * kHeads + (lane >> 2) + 8 * e) * kJoin;
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+        *reinterpret_cast<float2*>(r + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+      if ((lane & 3) == 0) {
+        r[DP] = m[e];
+        r[DP + 1] = l[e];
+      }
+    }
+    __syncthreads();
+    const int64_t row_u0 = (int64_t)prefix[b] * rows_per_b + (int64_t)row * nt;   // the row's units
+    const bool whole = t0 == 0 && t1 == nt;
+    const int64_t prow = (int64_t)kHeads * (D + 2);
+    float* part = whole ? nullptr : a.partials + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * prow;
+    for (int i = tid; i < heads * D; i += kThreads) {
+      const int g = i / D, d = i - g * D;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, jo[(w * kHeads + g) * kJoin + DP]);
+      const float bs = mm == -INFINITY ? 0.f : mm;
+      float acc = 0.f, ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float* r = jo + (w * kHeads + g) * kJoin;
+        const float f = exp2f(r[DP] - bs);
+        acc = fmaf(f, r[d], acc);
+        ll = fmaf(f, r[DP + 1], ll);
+      }
+      if (whole) {
+        const float y = acc / ll;
+        a.out[b * a.out_stride + (int64_t)(head0 + g) * D + d] = (uint16_t)pack2<BF>(y, 0.f);
+        if (d == 0 && a.lse2 != nullptr) a.lse2[b * a.n_q + head0 + g] = bs + log2f(ll);
+      } else {
+        part[g * (D + 2) + d] = acc;
+        if (d == 0) {
+          part[g * (D + 2) + D] = mm;
+          part[g * (D + 2) + D + 1] = ll;
+        }
+      }
+    }
+    if (!whole) {
+      const int64_t last_u = row_u0 + nt - 1;
+      const int cta0 = (int)(((row_u0 + 1) * n_cta - 1) / total), cta1 = (int)(((last_u + 1) * n_cta - 1) / total);
+      int* cnt = a.counters + b * rows_per_b + row;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        is_last = atomicAdd(cnt, 1) == cta1 - cta0;
+        if (is_last) *cnt = 0;                       // zero for the next call
+      }
+      __syncthreads();
+      if (is_last) {
+        __threadfence();
+        for (int i = tid; i < heads * D; i += kThreads) {
+          const int g = i / D, d = i - g * D;
+          float mm = -INFINITY, acc = 0.f, ll = 0.f;
+          for (int ct = cta0; ct <= cta1; ++ct) {
+            const int slot = total * ct / n_cta >= row_u0 ? 0 : 1;
+            const float* r = a.partials + ((int64_t)ct * 2 + slot) * prow + g * (D + 2);
+            const float pm = __ldcg(r + D), pl = __ldcg(r + D + 1), pa = __ldcg(r + d);
+            const float nm = fmaxf(mm, pm), bs = nm == -INFINITY ? 0.f : nm;
+            const float f0 = exp2f(mm - bs), f1 = exp2f(pm - bs);
+            acc = acc * f0 + pa * f1;
+            ll = ll * f0 + pl * f1;
+            mm = nm;
+          }
+          const float y = acc / ll;
+          a.out[b * a.out_stride + (int64_t)(head0 + g) * D + d] = (uint16_t)pack2<BF>(y, 0.f);
+          if (d == 0 && a.lse2 != nullptr) a.lse2[b * a.n_q + head0 + g] = mm + log2f(ll);
+        }
+      }
+    }
+    __syncthreads();   // the join area becomes the rings again
+    u += t1 - t0;
+  }
+}
+
+// score[slot] (+)= sum over the group of exp2(logit - lse2): one thread per
+// slot of a kv head. Reads 4 bytes per slot and query head, next to the
+// 4 D bytes per slot that the attention read.
+__global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a) {
+  const Cache& c = a.c;
+  const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv;
+  if (units_of(a, b) == 0) return;
+  const int len = c.seq_lens[b];
+  for (int slot = blockIdx.x * blockDim.x + threadIdx.x; slot <= len; slot += gridDim.x * blockDim.x) {
+    const int page = page_of(c, b, slot);
+    if (page < 0) continue;
+    float w = 0.f;
+    for (int g = 0; g < a.group; ++g) {
+      const int64_t q = (int64_t)b * a.n_q + h * a.group + g;
+      w += exp2f(__ldcs(a.logits + q * a.logit_stride + slot) - a.lse2[q]);
+    }
+    c.scores[stat_at(c, page, h, slot % c.page_size)] += w;   // the attention has set the new slot's to 0
+  }
+}
+
+// Stores tokens behind a sequence's cached ones: slot len + t of every kv
+// head gets k (rotated when tables are given) and v; scores and positions
+// are set. One warp per (sequence, token, kv head), 16 bytes per lane.
+struct AppendArgs {
+  Cache c;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t kb, kt, kh, vb, vt, vh;   // element strides of sequence, token, head
+  const int64_t* first;
+  const int32_t* n_new;
+  int tokens;
+  const float* cos_t;
+  const float* sin_t;
+  int64_t rope_rows;
+  const float* scores;
+  int64_t sb, sh, st;
+};
+
+template <bool BF>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 31;
+  const int64_t items = (int64_t)c.batch * a.tokens * c.n_kv;
+  const int D = c.head_dim, chunks = D / 8, half = chunks / 2;
+  const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < items; i += step) {
+    const int h = (int)(i % c.n_kv);
+    const int64_t bt = i / c.n_kv;
+    const int t = (int)(bt % a.tokens), b = (int)(bt / a.tokens);
+    const int len = c.seq_lens[b];
+    if (len < 0 || (a.n_new != nullptr && t >= a.n_new[b])) continue;
+    const int64_t slot = (int64_t)len + t;
+    if (slot >= capacity(c)) continue;
+    const int page = page_of(c, b, (int)slot);
+    if (page < 0) continue;
+    const int off = (int)(slot % c.page_size);
+    const int64_t pos = a.first != nullptr ? a.first[b] + t : slot;
+    if (a.cos_t != nullptr && (pos < 0 || pos >= a.rope_rows)) continue;
+    const int64_t at = row_at(c, page, h, off);
+    const uint16_t* ks = a.k + b * a.kb + t * a.kt + h * a.kh;
+    const uint16_t* vs = a.v + b * a.vb + t * a.vt + h * a.vh;
+    uint16_t* kd = reinterpret_cast<uint16_t*>(c.k) + at;
+    uint16_t* vd = reinterpret_cast<uint16_t*>(c.v) + at;
+    for (int ch = lane; ch < 2 * chunks; ch += 32) {
+      const bool is_v = ch >= chunks;
+      const int cc = is_v ? ch - chunks : ch;
+      uint4 w = *reinterpret_cast<const uint4*>((is_v ? vs : ks) + cc * 8);
+      if (!is_v && a.cos_t != nullptr) {
+        const bool hi = cc >= half;
+        const uint4 p = *reinterpret_cast<const uint4*>(ks + (hi ? cc - half : cc + half) * 8);
+        const int j = (hi ? cc - half : cc) * 8;
+        const float* cs = a.cos_t + pos * (D / 2) + j;
+        const float* sn = a.sin_t + pos * (D / 2) + j;
+        uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+        const uint32_t* pw = reinterpret_cast<const uint32_t*>(&p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = unpack2<BF>(ww[e]), y = unpack2<BF>(pw[e]);
+          float2 r0, r1;
+          if (hi) {
+            r0 = rotate(y.x, x.x, cs[2 * e], sn[2 * e]);
+            r1 = rotate(y.y, x.y, cs[2 * e + 1], sn[2 * e + 1]);
+            ww[e] = pack2<BF>(r0.y, r1.y);
+          } else {
+            r0 = rotate(x.x, y.x, cs[2 * e], sn[2 * e]);
+            r1 = rotate(x.y, y.y, cs[2 * e + 1], sn[2 * e + 1]);
+            ww[e] = pack2<BF>(r0.x, r1.x);
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>((is_v ? vd : kd) + cc * 8) = w;
+    }
+    if (lane == 0) {
+      const int64_t sa = stat_at(c, page, h, off);
+      if (c.scores != nullptr) c.scores[sa] = a.scores != nullptr ? a.scores[b * a.sb + h * a.sh + t * a.st] : 0.f;
+      if (c.slot_pos != nullptr) c.slot_pos[sa] = (int32_t)pos;
+    }
+  }
+}
+
+int make_cache(const ts_paged_cache* p, Cache* o) {
+  TS_REQUIRE(p != nullptr, "NULL cache");
+  TS_REQUIRE(p->k_pages && p->v_pages && p->page_table && p->seq_lens, "NULL pointer in the cache");
+  TS_UNSUPPORTED(p->dtype == TS_F16 || p->dtype == TS_BF16, "the cache holds fp16 or bf16");
+  TS_REQUIRE(p->batch >= 0 && p->n_kv > 0 && p->page_size > 0 && p->num_pages > 0 && p->max_pages > 0,
+             "bad cache sizes");
+  TS_UNSUPPORTED(p->head_dim % 16 == 0 && p->head_dim >= 16 && p->head_dim <= 256,
+                 "head_dim must be a multiple of 16, <= 256");
+  TS_REQUIRE((int64_t)p->max_pages * p->page_size <= (int64_t)1 << 30, "more than 2^30 slots per sequence");
+  TS_REQUIRE(is_aligned(p->k_pages, 16) && is_aligned(p->v_pages, 16) && p->page_stride % 8 == 0 &&
+                 p->head_stride % 8 == 0 && p->token_stride % 8 == 0,
+             "cache rows must be 16-byte aligned");
+  o->k = reinterpret_cast<char*>(p->k_pages);
+  o->v = reinterpret_cast<char*>(p->v_pages);
+  o->page_stride = p->page_stride;
+  o->head_stride = p->head_stride;
+  o->token_stride = p->token_stride;
+  o->table = p->page_table;
+  o->table_stride = p->table_stride;
+  o->seq_lens = p->seq_lens;
+  o->scores = p->scores;
+  o->slot_pos = p->slot_pos;
+  o->batch = p->batch;
+  o->n_kv = p->n_kv;
+  o->head_dim = p->head_dim;
+  o->page_size = p->page_size;
+  o->num_pages = p->num_pages;
+  o->max_pages = p->max_pages;
+  return TS_OK;
+}
+
+static size_t grid_of(int head_dim) { return (size_t)sm_count() * (head_dim > 128 ? 1 : 2); }
+
+struct Layout {
+  size_t partials, lse, logits, bytes;
+  int64_t logit_stride;
+};
+
+static Layout attn_layout(const ts_paged_cache& p, int n_q, bool weights) {
+  Layout L;
+  L.partials = kCounterBytes;
+  L.lse = align_up(L.partials + grid_of(p.head_dim) * 2 * kHeads * (p.head_dim + 2) * 4, 256);
+  L.logits = align_up(L.lse + (weights ? (size_t)p.batch * n_q * 4 : 0), 256);
+  L.logit_stride = (int64_t)align_up((size_t)p.max_pages * p.page_size, kUnit);
+  L.bytes = L.logits + (weights ? (size_t)p.batch * n_q * L.logit_stride * 4 : 0);
+  return L;
+}
+
+template <bool BF, int DP>
+static int launch_attention(const AttnArgs& a, int grid, cudaStream_t st) {
+  auto k = paged_attention_kernel<BF, DP>;
+  const size_t smem = attn_smem<DP>(a.c.batch);
+  TS_UNSUPPORTED(smem <= (size_t)max_smem_optin(), "batch too large for the kernel's tables");
+  static thread_local int configured_dev = -1;
+  static thread_local size_t configured_smem = 0;
+  int dev = 0;
+  TS_CUDA_TRY(cudaGetDevice(&dev));
+  if (configured_dev != dev || configured_smem < smem) {
+    TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    configured_dev = dev;
+    configured_smem = smem;
+  }
+  k<<<grid, kThreads, smem, st>>>(a);
+  TS_LAUNCH_CHECK();
+  return TS_OK;
+}
+
+template <bool BF>
+static int launch_attention(const AttnArgs& a, int grid, cudaStream_t st) {
+  if (a.c.head_dim <= 64) return launch_attention<BF, 64>(a, grid, st);
+  if (a.c.head_dim <= 128) return launch_attention<BF, 128>(a, grid, st);
+  return launch_attention<BF, 256>(a, grid, st);
+}
+
+}  // namespace paged
+}  // namespace ts
+
+using namespace ts;
+using namespace ts::paged;
+
+extern "C" size_t ts_paged_attention_workspace_size(const ts_paged_cache* cache, int n_q, int accumulate) {
+  if (cache == nullptr) return 0;
+  return attn_layout(*cache, n_q, accumulate != 0).bytes;
+}
+
+extern "C" int ts_paged_decode_attention(const void* qkv, int64_t qkv_row_stride, int n_q, const ts_paged_cache* cache,
+                                         const int64_t* positions, const float* rope_cos, const float* rope_sin,
+                                         int64_t rope_rows, float scale, int accumulate, void* out,
+                                         int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                                         void* stream) {
+  AttnArgs a;
+  const int rc = make_cache(cache, &a.c);
+  if (rc != TS_OK) return rc;
+  TS_REQUIRE(qkv && out, "NULL pointer");
+  TS_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), "rope_cos and rope_sin come both or neither");
+  TS_REQUIRE(positions != nullptr || (rope_cos == nullptr && a.c.slot_pos == nullptr),
+             "positions are needed for the rotation and for slot_pos");
+  TS_REQUIRE(n_q > 0 && n_q % a.c.n_kv == 0, "bad head counts");
+  TS_REQUIRE(!accumulate || a.c.scores != nullptr, "the cache has no scores to accumulate into");
+  if (a.c.batch == 0) return TS_OK;
+  a.group = n_q / a.c.n_kv;
+  a.head_tiles = (a.group + kHeads - 1) / kHeads;
+  TS_UNSUPPORTED((int64_t)a.c.batch * a.c.n_kv * a.head_tiles <= (int64_t)kCounters, "too many heads in one call");
+  const Layout L = attn_layout(*cache, n_q, accumulate != 0);
+  if (workspace == nullptr || workspace_bytes < L.bytes) {
+    set_error("workspace of %zu bytes, %zu needed", workspace_bytes, L.bytes);
+    return TS_ERR_WORKSPACE;
+  }
+  TS_REQUIRE(is_aligned(workspace, 16), "workspace must be 16-byte aligned");
+  char* ws = reinterpret_cast<char*>(workspace);
+  a.qkv = reinterpret_cast<const uint16_t*>(qkv);
+  a.qkv_stride = qkv_row_stride;
+  a.n_q = n_q;
+  a.positions = positions;
+  a.cos_t = rope_cos;
+  a.sin_t = rope_sin;
+  a.rope_rows = rope_rows;
+  a.scale2 = scale * 1.4426950408889634f;
+  a.out = reinterpret_cast<uint16_t*>(out);
+  a.out_stride = out_row_stride;
+  a.counters = reinterpret_cast<int*>(ws);
+  a.partials = reinterpret_cast<float*>(ws + L.partials);
+  a.lse2 = accumulate ? reinterpret_cast<float*>(ws + L.lse) : nullptr;
+  a.logits = accumulate ? reinterpret_cast<float*>(ws + L.logits) : nullptr;
+  a.logit_stride = L.logit_stride;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int grid = (int)grid_of(a.c.head_dim);
+  const int r = cache->dtype == TS_BF16 ? launch_attention<true>(a, grid, st) : launch_attention<false>(a, grid, st);
+  if (r != TS_OK || !accumulate) return r;
+  const int rows = a.c.batch * a.c.n_kv;
+  const int64_t cap = (int64_t)a.c.max_pages * a.c.page_size;
+  const int per_row = (int)std::max<int64_t>(1, std::min<int64_t>((cap + 255) / 256, (4 * sm_count() + rows - 1) / rows));
+  paged_weights_kernel<<<dim3(per_row, rows), 256, 0, st>>>(a);
+  TS_LAUNCH_CHECK();
+  return TS_OK;
+}
+
+extern "C" int ts_paged_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                               int tokens, const int32_t* n_new, const ts_paged_cache* cache, const int64_t* first,
+                               const float* rope_cos, const float* rope_sin, int64_t rope_rows, const float* scores,
+                               const int64_t* score_strides, void* stream) {
+  AppendArgs a;
+  const int rc = make_cache(cache, &a.c);
+  if (rc != TS_OK) return rc;
+  TS_REQUIRE(k && v && k_strides && v_strides && tokens >= 0, "bad tokens");
+  TS_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), "rope_cos and rope_sin come both or neither");
+  TS_REQUIRE(scores == nullptr || (a.c.scores != nullptr && score_strides != nullptr),
+             "scores were given for a cache that keeps none");
+  for (int i = 0; i < 3; ++i)
+    TS_REQUIRE(k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0, "k and v rows must be 16-byte aligned");
+  TS_REQUIRE(is_aligned(k, 16) && is_aligned(v, 16), "k and v must be 16-byte aligned");
+  if (a.c.batch == 0 || tokens == 0) return TS_OK;
+  a.k = reinterpret_cast<const uint16_t*>(k);
+  a.v = reinterpret_cast<const uint16_t*>(v);
+  a.kb = k_strides[0]; a.kt = k_strides[1]; a.kh = k_strides[2];
+  a.vb = v_strides[0]; a.vt = v_strides[1]; a.vh = v_strides[2];
+  a.first = first;
+  a.n_new = n_new;
+  a.tokens = tokens;
+  a.cos_t = rope_cos;
+  a.sin_t = rope_sin;
+  a.rope_rows = rope_rows;
+  a.scores = scores;
+  a.sb = scores ? score_strides[0] : 0;
+  a.sh = scores ? score_strides[1] : 0;
+  a.st = scores ? score_strides[2] : 0;
+  const int64_t items = (int64_t)a.c.batch * tokens * a.c.n_kv;
+  const int grid = (int)std::min<int64_t>((items + 7) / 8, (int64_t)sm_count() * 8);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (cache->dtype == TS_BF16) paged_append_kernel<true><<<grid, 256, 0, st>>>(a);
+  else paged_append_kernel<false><<<grid, 256, 0, st>>>(a);
+  TS_LAUNCH_CHECK();
+  return TS_OK;
+}

@@ -1,0 +1,282 @@
+// Eviction from a paged key-value cache by accumulated attention weight.
+//
+// For each sequence longer than `budget` and each kv head, `budget` slots
+// stay: those whose position is among the `recent` newest, then those of the
+// largest score (ties to the lowest slot; a NaN score counts as -inf, and
+// a slot without memory goes first). Kept slots at or behind `budget` move
+// into the holes before it, both taken in ascending order, with k, v, score
+// and position; the sequence's length becomes `budget`. Attention does not
+// depend on the order of slots, so nothing else has to move: after one new
+// token a single slot does, where a shift that keeps the order would rewrite
+// most of the cache. Sources lie behind `budget` and targets before it, so
+// all moves of a call are independent of one another.
+//
+// select: one CTA per (sequence, kv head) finds the budget-th largest key by
+// radix selection over monotone 32-bit keys (three digits of 11, 11 and 10
+// bits, histograms in shared memory) and lists holes and movers by block
+// scans. move: a warp per moved slot copies both rows, 16 bytes per lane.
+// What bounds them: select reads 8 bytes per slot and is latency-bound at one
+// CTA per head; move is DRAM traffic of the moved slots only.
+#include <algorithm>
+#include <climits>
+
+#include "paged.cuh"
+
+namespace ts {
+namespace paged {
+
+constexpr int kSelThreads = 1024;
+constexpr int kBins = 2048;
+constexpr int kMoveWarps = 8;
+
+struct EvictArgs {
+  Cache c;
+  int budget, recent;
+  int* n_move;            // [batch * n_kv]
+  int32_t* holes;         // [batch * n_kv][list]
+  int32_t* movers;
+  int list;
+  uint32_t* keys;         // [batch * n_kv][cap] when they do not fit shared memory, else NULL
+  int64_t cap;
+  int smem_keys;          // keys that fit shared memory
+};
+
+// Monotone key: larger scores have larger keys, -0 equals +0, NaN counts as -inf.
+__device__ __forceinline__ uint32_t key_of(float s) {
+  const uint32_t u = isnan(s) ? 0xFF800000u : __float_as_uint(s == 0.f ? 0.f : s);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Exclusive block scan of one int per thread; *sum receives the total.
+__device__ __forceinline__ int block_scan(int v, int* sum, int* warp_tot) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  __syncthreads();
+  if (lane == 31) warp_tot[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    int w = lane < kSelThreads / 32 ? warp_tot[lane] : 0;
+    int wi = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, wi, o);
+      if (lane >= o) wi += t;
+    }
+    warp_tot[lane] = wi - w;
+    if (lane == 31) warp_tot[32] = wi;
+  }
+  __syncthreads();
+  *sum = warp_tot[32];
+  return warp_tot[warp] + inc - v;
+}
+
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
+  extern __shared__ uint32_t skeys[];
+  __shared__ int hist[kBins];
+  __shared__ int warp_tot[33];
+  __shared__ int s_newest, s_digit, s_left;
+  const Cache& c = a.c;
+  const int row = blockIdx.x, b = row / c.n_kv, h = row - b * c.n_kv, tid = threadIdx.x;
+  const int n = (int)min((int64_t)max(c.seq_lens[b], 0), capacity(c));
+  if (n <= a.budget) {
+    if (tid == 0) a.n_move[row] = 0;
+    return;
+  }
+  uint32_t* keys = n <= a.smem_keys ? skeys : a.keys + (int64_t)row * a.cap;
+
+  if (tid == 0) s_newest = INT_MIN;
+  __syncthreads();
+  int newest = INT_MIN;
+  for (int i = tid; i < n; i += kSelThreads) {
+    const int page = page_of(c, b, i);
+    if (page >= 0) newest = max(newest, c.slot_pos[stat_at(c, page, h, i % c.page_size)]);
+  }
+  newest = __reduce_max_sync(0xffffffffu, newest);
+  if ((tid & 31) == 0) atomicMax(&s_newest, newest);
+  __syncthreads();
+  const int64_t limit = (int64_t)s_newest - a.recent;
+  for (int i = tid; i < n; i += kSelThreads) {
+    const int page = page_of(c, b, i);
+    uint32_t k = 0;
+    if (page >= 0) {
+      const int64_t at = stat_at(c, page, h, i % c.page_size);
+      k = (int64_t)c.slot_pos[at] > limit ? 0xFF800000u : key_of(c.scores[at]);   // the key of +inf
+    }
+    keys[i] = k;
+  }
+
+  // radix selection of the budget-th largest key
+  uint32_t prefix = 0, mask = 0;
+  int left = a.budget;   // how many of the keys with this prefix stay
+  const int shifts[3] = {21, 10, 0};
+  const int widths[3] = {11, 11, 10};
+#pragma unroll
+  for (int d = 0; d < 3; ++d) {
+    const int bins = 1 << widths[d];
+    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSelThreads) {
+      const uint32_t k = keys[i];
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shifts[d]) & (bins - 1)], 1);
+    }
+    __syncthreads();
+    // thread t holds the two bins 2047 - 2t and 2046 - 2t: a scan from the top
+    const int hi = kBins - 1 - 2 * tid;
+    const int n1 = hist[hi], n0 = hist[hi - 1];
+    int total;
+    const int before = block_scan(n1 + n0, &total, warp_tot);
+    if (before < left && left <= before + n1) {
+      s_digit = hi;
+      s_left = left - before;
+    } else if (before + n1 < left && left <= before + n1 + n0) {
+      s_digit = hi - 1;
+      s_left = left - before - n1;
+    }
+    __syncthreads();
+    prefix |= (uint32_t)s_digit << shifts[d];
+    mask |= (uint32_t)(bins - 1) << shifts[d];
+    left = s_left;
+    __syncthreads();
+  }
+
+  // of the keys equal to the threshold the first `left` stay. Every thread
+  // takes a run of slots (an odd number, so that their keys fall in
+  // different banks).
+  const int per = ((n + kSelThreads - 1) / kSelThreads) | 1;
+  const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+  int eq = 0;
+  for (int i = i0; i < i1; ++i) eq += keys[i] == prefix;
+  int dummy;
+  const int eq0 = block_scan(eq, &dummy, warp_tot);
+  int holes = 0, movers = 0, e = eq0;
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t k = keys[i];
+    const bool keep = k > prefix || (k == prefix && e++ < left);
+    if (i < a.budget) holes += !keep;
+    else movers += keep;
+  }
+  int n_holes, n_movers;
+  int at_h = block_scan(holes, &n_holes, warp_tot);
+  int at_m = block_scan(movers, &n_movers, warp_tot);
+  e = eq0;
+  int32_t* lh = a.holes + (int64_t)row * a.list;
+  int32_t* lm = a.movers + (int64_t)row * a.list;
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t k = keys[i];
+    const bool keep = k > prefix || (k == prefix && e++ < left);
+    if (i < a.budget) {
+      if (!keep) lh[at_h++] = i;
+    } else if (keep) {
+      lm[at_m++] = i;
+    }
+  }
+  if (tid == 0) a.n_move[row] = n_movers;   // == n_holes
+}
+
+__global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictArgs a) {
+  const Cache& c = a.c;
+  const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv, lane = threadIdx.x & 31;
+  const int n = a.n_move[row], chunks = c.head_dim / 8;
+  const int32_t* lh = a.holes + (int64_t)row * a.list;
+  const int32_t* lm = a.movers + (int64_t)row * a.list;
+  for (int i = blockIdx.x * kMoveWarps + (threadIdx.x >> 5); i < n; i += gridDim.x * kMoveWarps) {
+    const int to = lh[i], from = lm[i];
+    const int pt = page_of(c, b, to), pf = page_of(c, b, from);
+    if (pt < 0 || pf < 0) continue;
+    const int ot = to % c.page_size, of = from % c.page_size;
+    const int64_t rt = row_at(c, pt, h, ot) * 2, rf = row_at(c, pf, h, of) * 2;
+    for (int ch = lane; ch < 2 * chunks; ch += 32) {
+      char* base = ch < chunks ? c.k : c.v;
+      const int64_t e = (ch < chunks ? ch : ch - chunks) * 16;
+      *reinterpret_cast<uint4*>(base + rt + e) = *reinterpret_cast<const uint4*>(base + rf + e);
+    }
+    if (lane == 0) {
+      const int64_t st = stat_at(c, pt, h, ot), sf = stat_at(c, pf, h, of);
+      c.scores[st] = c.scores[sf];
+      c.slot_pos[st] = c.slot_pos[sf];
+    }
+  }
+  // nothing in this kernel reads the lengths, so they can be set here
+  if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0 && c.seq_lens[b] > a.budget) c.seq_lens[b] = a.budget;
+}
+
+struct EvictLayout {
+  size_t n_move, holes, movers, keys, bytes;
+  int64_t list;
+  int smem_keys;
+};
+
+static EvictLayout evict_layout(const ts_paged_cache& p, int budget) {
+  EvictLayout L;
+  const int64_t cap = (int64_t)p.max_pages * p.page_size, rows = (int64_t)p.batch * p.n_kv;
+  L.list = std::max<int64_t>(1, std::min<int64_t>(budget, cap - budget));
+  L.smem_keys = (int)std::min<int64_t>(cap, 48 * 1024);
+  L.n_move = kCounterBytes;
+  L.holes = align_up(L.n_move + rows * 4, 256);
+  L.movers = align_up(L.holes + rows * L.list * 4, 256);
+  L.keys = align_up(L.movers + rows * L.list * 4, 256);
+  L.bytes = L.keys + (cap > L.smem_keys ? (size_t)rows * cap * 4 : 0);
+  return L;
+}
+
+}  // namespace paged
+}  // namespace ts
+
+using namespace ts;
+using namespace ts::paged;
+
+extern "C" size_t ts_paged_evict_workspace_size(const ts_paged_cache* cache, int budget) {
+  if (cache == nullptr) return 0;
+  return evict_layout(*cache, budget).bytes;
+}
+
+extern "C" int ts_paged_evict(const ts_paged_cache* cache, int budget, int recent, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  EvictArgs a;
+  const int rc = make_cache(cache, &a.c);
+  if (rc != TS_OK) return rc;
+  TS_REQUIRE(a.c.scores != nullptr && a.c.slot_pos != nullptr, "eviction needs the cache's scores and slot_pos");
+  TS_REQUIRE(budget > 0, "budget must be positive");
+  TS_REQUIRE(recent >= 0 && recent <= budget, "recent must be in [0, budget]");
+  const int64_t cap = (int64_t)a.c.max_pages * a.c.page_size;
+  if (a.c.batch == 0 || cap <= budget) return TS_OK;
+  const EvictLayout L = evict_layout(*cache, budget);
+  if (workspace == nullptr || workspace_bytes < L.bytes) {
+    set_error("workspace of %zu bytes, %zu needed", workspace_bytes, L.bytes);
+    return TS_ERR_WORKSPACE;
+  }
+  TS_REQUIRE(is_aligned(workspace, 16), "workspace must be 16-byte aligned");
+  char* ws = reinterpret_cast<char*>(workspace);
+  a.budget = budget;
+  a.recent = recent;
+  a.n_move = reinterpret_cast<int*>(ws + L.n_move);
+  a.holes = reinterpret_cast<int32_t*>(ws + L.holes);
+  a.movers = reinterpret_cast<int32_t*>(ws + L.movers);
+  a.list = (int)L.list;
+  a.keys = reinterpret_cast<uint32_t*>(ws + L.keys);
+  a.cap = cap;
+  a.smem_keys = L.smem_keys;
+  const int rows = a.c.batch * a.c.n_kv;
+  TS_UNSUPPORTED(rows <= 65535, "too many heads in one call");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const size_t smem = (size_t)L.smem_keys * 4;
+  static thread_local int configured_dev = -1;
+  int dev = 0;
+  TS_CUDA_TRY(cudaGetDevice(&dev));
+  if (configured_dev != dev) {
+    TS_CUDA_TRY(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 48 * 1024 * 4));
+    configured_dev = dev;
+  }
+  evict_select_kernel<<<rows, kSelThreads, smem, st>>>(a);
+  TS_LAUNCH_CHECK();
+  const int per_row = (int)std::max<int64_t>(
+      1, std::min<int64_t>((L.list + kMoveWarps * 4 - 1) / (kMoveWarps * 4), (8 * sm_count() + rows - 1) / rows));
+  evict_move_kernel<<<dim3(per_row, rows), kMoveWarps * 32, 0, st>>>(a);
+  TS_LAUNCH_CHECK();
+  return TS_OK;
+}
