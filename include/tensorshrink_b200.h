@@ -334,8 +334,8 @@ TS_API int ts_paged_append(const void* k, const int64_t* k_strides, const void* 
  * sequence whose count is negative, that has no page left for the token, or
  * whose position has no rotary row answers with zeros and stores nothing.
  * seq_lens is not changed. qkv, out as in ts_decode_attention, in the
- * cache's type. workspace: zero-filled once; its first 256 KB are zero again
- * after every call and the rest is scratch (one workspace may serve all
+ * cache's type. workspace: zero-filled once; its first
+ * ts_serving_counter_bytes() are zero again after every call and the rest is scratch (one workspace may serve all
  * ts_paged_* and ts_fp4_* calls of a stream).
  */
 TS_API size_t ts_paged_attention_workspace_size(const ts_paged_cache* cache, int n_q, int accumulate);
@@ -419,6 +419,10 @@ TS_API size_t ts_fp4_linear_workspace_size(int64_t M, int64_t N, int64_t K, int 
 TS_API int ts_fp4_linear(const void* x, int x_dtype, int64_t M, int64_t x_row_stride, float* x_scale,
                          const ts_fp4_tensor* w, const void* bias, int bias_dtype, void* out, int out_dtype,
                          int64_t out_row_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes at a serving workspace's start that hold counters: zero before the
+ * first call and between calls. */
+TS_API size_t ts_serving_counter_bytes(void);
 
 /* ts_qlinear_status for the fp4 product (a per-device flag); with clear the
  * counters at the workspace's start are zeroed too (workspace may be NULL). */

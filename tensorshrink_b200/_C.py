@@ -142,6 +142,7 @@ _SIGNATURES = [
     ("ts_fp4_linear_workspace_size", C.c_size_t, [_i64, _i64, _i64, C.c_int]),
     ("ts_fp4_linear", C.c_int, [_vp, C.c_int, _i64, _i64, _vp, C.POINTER(TsFp4Tensor), _vp, C.c_int, _vp, C.c_int,
                                 _i64, _vp, C.c_size_t, _vp]),
+    ("ts_serving_counter_bytes", C.c_size_t, []),
     ("ts_fp4_status", C.c_int, [_vp, C.c_size_t, C.c_int, _vp]),
     ("ts_dequantize_weight", C.c_int, [C.POINTER(TsQWeight), _vp, C.c_int, _i64, C.c_int, _vp]),
     ("ts_quantize_workspace_size", C.c_size_t, [C.POINTER(TsQuantParams)]),
@@ -208,6 +209,15 @@ def torch_ops():
             torch.ops.load_library(str(_TORCH_LIB_PATH))
             _ops = torch.ops.tensorshrink
     return _ops or None
+
+
+def serving_ops():
+    """`torch.ops.tensorshrink` for the operators that have no other form (the
+    fp4 and paged ones); raises if the library was not built."""
+    ops = torch_ops()
+    if ops is None:
+        raise ImportError(f"{_TORCH_LIB_PATH} is missing: build it with `python -m tensorshrink_b200.build`")
+    return ops
 
 
 def launch_count(reset: bool = False) -> int:

@@ -29,7 +29,7 @@ LIBDIR = PKG / "_lib"
 OBJDIR = PKG / "_lib" / "obj"
 LIBNAME = "libtensorshrink_b200.so"
 TORCH_LIBNAME = "libtensorshrink_torch.so"
-TORCH_SRC = PKG / "csrc_torch" / "ops.cpp"
+TORCH_SRCS = [PKG / "csrc_torch" / "ops.cpp", PKG / "csrc_torch" / "serving.cpp"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
@@ -105,12 +105,12 @@ def build_torch_ops(lib: Path, verbose: bool = False) -> Path:
     thin C++ layer (host code only) over the C ABI library."""
     import torch.utils.cpp_extension as ce
     out = LIBDIR / TORCH_LIBNAME
-    deps = [TORCH_SRC, lib] + list(INCLUDE.glob("*.h"))
+    deps = [*TORCH_SRCS, lib] + list(INCLUDE.glob("*.h"))
     if out.exists() and out.stat().st_mtime >= max(f.stat().st_mtime for f in deps):
         return out
     import torch
     cuda_inc = Path(nvcc()).resolve().parent.parent / "include"
-    cmd = ["g++", "-O2", "-shared", "-fPIC", "-std=c++17", str(TORCH_SRC), "-o", str(out),
+    cmd = ["g++", "-O2", "-shared", "-fPIC", "-std=c++17", *map(str, TORCH_SRCS), "-o", str(out),
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{p}" for p in ce.include_paths()], f"-I{cuda_inc}", f"-I{INCLUDE}",
            *[f"-L{p}" for p in ce.library_paths()], "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",

@@ -511,6 +511,8 @@ extern "C" int ts_fp4_matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, con
   return w->format == TS_NVFP4 ? launch<true>(p.BT, wm, xm, a, p.grid, st) : launch<false>(p.BT, wm, xm, a, p.grid, st);
 }
 
+extern "C" size_t ts_serving_counter_bytes(void) { return paged::kCounterBytes; }
+
 extern "C" int ts_fp4_status(void* workspace, size_t workspace_bytes, int clear, void* stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   TS_REQUIRE(workspace == nullptr || workspace_bytes >= paged::kCounterBytes, "workspace of %zu bytes, %zu needed",

@@ -54,7 +54,22 @@ struct AttnArgs {
   float* lse2;           // [batch * n_q] log2 of the softmax denominators, or NULL
   float* logits;         // [batch * n_q][cap] scores in log2 units, or NULL
   int64_t logit_stride;
+  int page_shift;        // log2(page_size), or -1
+  int one_page;          // page_size % 16 == 0: a warp's 16 slots share a page
 };
+
+constexpr int kMaxPieces = 64;   // CTAs that share a kv head's units at most
+
+// s / page_size and s % page_size.
+__device__ __forceinline__ void split_slot(const AttnArgs& a, int s, int* page, int* off) {
+  if (a.page_shift >= 0) {
+    *page = s >> a.page_shift;
+    *off = s & (a.c.page_size - 1);
+  } else {
+    *page = s / a.c.page_size;
+    *off = s - *page * a.c.page_size;
+  }
+}
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -101,7 +116,7 @@ __device__ __forceinline__ int units_of(const AttnArgs& a, int b) {
 // keeps its 16-byte chunk c at c ^ (r & 7), so that ldmatrix reads of eight
 // rows touch every bank once.
 template <int DP>
-constexpr int stages_for() { return DP == 64 ? 6 : 3; }
+constexpr int stages_for() { return DP == 64 ? 4 : 3; }
 template <int DP>
 constexpr size_t ring_bytes() { return (size_t)kWarps * stages_for<DP>() * 2 * kRows * DP * 2; }
 template <int DP>
@@ -116,29 +131,42 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
   constexpr int kStage = 2 * kRows * kPitch;     // bytes of a stage: K rows, then V rows
   constexpr int kSteps = DP / 16;
   constexpr bool kKeepQ = DP <= 128;             // query fragments stay in registers
+  constexpr int kRowChunks = DP / 8;             // 16-byte columns of a staged row
+  constexpr int kRowsPer = 32 / kRowChunks;      // rows that a warp copies at once
   extern __shared__ __align__(128) char smem[];
   uint16_t* qs = reinterpret_cast<uint16_t*>(smem + ring_bytes<DP>());
   int* prefix = reinterpret_cast<int*>(smem + ring_bytes<DP>() + kHeads * (DP + 8) * 2);
-  __shared__ int warp_sums[kWarps];
+  __shared__ int warp_sums[kWarps], warp_most[kWarps];
   __shared__ int is_last;
   const Cache& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int D = c.head_dim, chunks = D / 8, steps = D / 16, rows_per_b = c.n_kv * a.head_tiles;
 
   // prefix sums of the sequences' units; every thread takes a run of sequences
+  int longest = 0;
   {
     const int per = (c.batch + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += units_of(a, b);
+    int sum = 0, most = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int n = units_of(a, b);
+      sum += n;
+      most = max(most, n);
+    }
     int inc = sum;
+    most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += t;
     }
-    if (lane == 31) warp_sums[warp] = inc;
+    if (lane == 31) {
+      warp_sums[warp] = inc;
+      warp_most[warp] = most;
+    }
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) longest = max(longest, warp_most[w]);
     int at = inc - sum;
     for (int w = 0; w < warp; ++w) at += warp_sums[w];
     for (int b = b0; b < b1; ++b) {
@@ -156,8 +184,11 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
       for (int i = tid; i < a.n_q * D; i += kThreads) a.out[b * a.out_stride + i] = 0;
 
   const int64_t total = (int64_t)prefix[c.batch] * rows_per_b;
-  const int64_t n_cta = min((int64_t)gridDim.x, total);
-  if ((int64_t)blockIdx.x >= n_cta) return;
+  // every CTA gets units, unless that cut the longest row into more pieces
+  // than its join takes in its stride
+  const int64_t n_cta =
+      max((int64_t)1, min(min((int64_t)gridDim.x, total), kMaxPieces * total / max(longest, 1)));
+  if (total == 0 || (int64_t)blockIdx.x >= n_cta) return;
   const int64_t u0 = total * blockIdx.x / n_cta, u1 = total * (blockIdx.x + 1) / n_cta;
 
   char* ring = smem + (size_t)warp * S * kStage;
@@ -189,31 +220,67 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
     const float* cs = a.cos_t != nullptr ? a.cos_t + pos * (D / 2) : nullptr;
     const float* sn = a.cos_t != nullptr ? a.sin_t + pos * (D / 2) : nullptr;
 
-    // rows of warp-unit t: slots t * 64 + warp * 16 + r. Lane r (< 16) finds
-    // the element offset of row r, -1 where nothing is to be copied.
-    auto row_offset = [&](int t) -> int64_t {
-      const int slot = t * kUnit + warp * kRows + (lane & 15);
-      if (t >= t1 || slot >= len) return -1;
-      const int page = page_of(c, b, slot);
-      return page < 0 ? -1 : row_at(c, page, h, slot % c.page_size);
-    };
-    auto issue = [&](int t, int stage, int64_t off) {
+    // A warp's share of unit t: slots t * 64 + warp * 16 + r. It copies the
+    // rows of cached slots and zeros for the others; `live` is a bit per row
+    // that has a cached token, queued until the stage is consumed.
+    const int cl = lane % kRowChunks, rl = lane / kRowChunks;   // this lane's 16-byte column and first row
+    const bool col = cl < chunks;
+    auto issue = [&](int t, int stage) -> uint32_t {
+      uint32_t live = 0;
       if (t < t1) {
-        const uint32_t base = ring_u + stage * kStage;
-        for (int i = lane; i < kRows * chunks; i += 32) {   // a multiple of 32 pieces: D % 16 == 0
-          const int r = i / chunks, ch = i - r * chunks;
-          const int64_t o = __shfl_sync(0xffffffffu, off, r);
-          const uint32_t dst = base + r * kPitch + ((ch ^ (r & 7)) << 4);
-          const int64_t e = o < 0 ? 0 : (o + ch * 8) * 2;
-          cp16(dst, c.k + e, o < 0 ? 0 : 16);
-          cp16(dst + kRows * kPitch, c.v + e, o < 0 ? 0 : 16);
+        const int slot0 = t * kUnit + warp * kRows;
+        const uint32_t dst = ring_u + stage * kStage + rl * kPitch;
+        const int n = min(kRows, len - slot0);          // rows with cached tokens
+        if (a.one_page) {
+          int pg, off;
+          split_slot(a, slot0, &pg, &off);
+          const int page = n > 0 && pg < c.max_pages ? c.table[b * c.table_stride + pg] : -1;
+          const int rows = (unsigned)page < (unsigned)c.num_pages ? n : 0;
+          live = rows > 0 ? (1u << rows) - 1 : 0;
+          int64_t e = rows > 0 ? (row_at(c, page, h, off + rl) + cl * 8) * 2 : 0;
+          const int64_t step = rows > 0 ? c.token_stride * (kRowsPer * 2) : 0;
+          if (col) {
+#pragma unroll
+            for (int i = 0; i < kRows / kRowsPer; ++i) {
+              const int r = i * kRowsPer + rl;
+              const int ok = r < rows;
+              const uint32_t d = dst + i * kRowsPer * kPitch + ((cl ^ (r & 7)) << 4);
+              cp16(d, c.k + (ok ? e : 0), ok * 16);
+              cp16(d + kRows * kPitch, c.v + (ok ? e : 0), ok * 16);
+              e += step;
+            }
+          }
+        } else {
+          // pages may end inside the rows: lane r (< 16) looks row r up
+          const int r0 = lane & 15;
+          int64_t o = -1;
+          if (r0 < n) {
+            int pg, off;
+            split_slot(a, slot0 + r0, &pg, &off);
+            const int page = pg < c.max_pages ? c.table[b * c.table_stride + pg] : -1;
+            if ((unsigned)page < (unsigned)c.num_pages) o = row_at(c, page, h, off);
+          }
+          live = __ballot_sync(0xffffffffu, o >= 0) & 0xFFFFu;
+#pragma unroll
+          for (int i = 0; i < kRows / kRowsPer; ++i) {
+            const int r = i * kRowsPer + rl;
+            const int64_t ro = __shfl_sync(0xffffffffu, o, r);
+            const int ok = ro >= 0;
+            const int64_t e = ok ? (ro + cl * 8) * 2 : 0;
+            const uint32_t d = dst + i * kRowsPer * kPitch + ((cl ^ (r & 7)) << 4);
+            if (col) {
+              cp16(d, c.k + e, ok * 16);
+              cp16(d + kRows * kPitch, c.v + e, ok * 16);
+            }
+          }
         }
       }
       cp_commit();
+      return live;
     };
+    uint64_t live_q = 0;
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) issue(t0 + s, s, row_offset(t0 + s));
-    int64_t next_off = row_offset(t0 + S - 1);
+    for (int s = 0; s < S - 1; ++s) live_q |= (uint64_t)issue(t0 + s, s) << (16 * s);
 
     // the rotated query heads of the tile
     for (int i = tid; i < heads * (D / 2); i += kThreads) {
@@ -249,8 +316,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
 
     int stage = 0;
     for (int t = t0; t < t1; ++t) {
-      issue(t + S - 1, stage == 0 ? S - 1 : stage - 1, next_off);
-      next_off = row_offset(t + S);
+      live_q |= (uint64_t)issue(t + S - 1, stage == 0 ? S - 1 : stage - 1) << (16 * (S - 1));
+      uint32_t live = (uint32_t)live_q & 0xFFFFu;
+      live_q >>= 16;
       cp_wait<S - 1>();
       __syncwarp();
       const int slot0 = t * kUnit + warp * kRows;
@@ -260,6 +328,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
       if (len < slot0 + kRows) {
         // the new token's row: into the stage and, once per kv head, the cache
         const int r = len - slot0;
+        live |= 1u << r;
         char* st = ring + (kb - ring_u);
         const int page = page_of(c, b, len);
         const int64_t at = row_at(c, page, h, len % c.page_size);
@@ -315,10 +384,6 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
         mma<BF>(sc[0], qf[kKeepQ ? s : 0], kf[0], kf[1]);
         mma<BF>(sc[1], qf[kKeepQ ? s : 0], kf[2], kf[3]);
       }
-      // slots that exist: below the new one, or it, and with memory
-      const int64_t mine = row_offset(t);              // of row (lane & 15)
-      const int my_slot = slot0 + (lane & 15);
-      const unsigned live = __ballot_sync(0xffffffffu, my_slot == len || mine >= 0);
       const int c0 = (lane & 3) * 2;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -449,22 +514,48 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
       __syncthreads();
       if (is_last) {
         __threadfence();
-        for (int i = tid; i < heads * D; i += kThreads) {
-          const int g = i / D, d = i - g * D;
-          float mm = -INFINITY, acc = 0.f, ll = 0.f;
-          for (int ct = cta0; ct <= cta1; ++ct) {
-            const int slot = total * ct / n_cta >= row_u0 ? 0 : 1;
-            const float* r = a.partials + ((int64_t)ct * 2 + slot) * prow + g * (D + 2);
-            const float pm = __ldcg(r + D), pl = __ldcg(r + D + 1), pa = __ldcg(r + d);
-            const float nm = fmaxf(mm, pm), bs = nm == -INFINITY ? 0.f : nm;
-            const float f0 = exp2f(mm - bs), f1 = exp2f(pm - bs);
-            acc = acc * f0 + pa * f1;
-            ll = ll * f0 + pl * f1;
-            mm = nm;
+        // factors exp2(m_piece - m) / l of every piece and head, then the sums
+        const int pieces = cta1 - cta0 + 1;            // at most kMaxPieces + 2
+        float* fac = jo;                               // [pieces][kHeads]
+        // a row's pieces lie at the start of their CTAs' ranges, except that
+        // the first may lie at its CTA's end
+        const float* piece0 = a.partials + ((int64_t)cta0 * 2 + (total * cta0 / n_cta >= row_u0 ? 0 : 1)) * prow;
+        const float* piece1 = a.partials + (int64_t)cta0 * 2 * prow;
+        auto piece = [&](int i) { return i == 0 ? piece0 : piece1 + (int64_t)i * 2 * prow; };
+        __syncthreads();                               // the join of the warps has been read
+        for (int g = warp; g < heads; g += kWarps) {
+          float mm = -INFINITY;
+          for (int i = lane; i < pieces; i += 32) mm = fmaxf(mm, __ldcg(piece(i) + g * (D + 2) + D));
+#pragma unroll
+          for (int o2 = 16; o2 > 0; o2 >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o2));
+          const float bs = mm == -INFINITY ? 0.f : mm;
+          float ll = 0.f;
+          for (int i = lane; i < pieces; i += 32) {
+            const float* r = piece(i) + g * (D + 2) + D;
+            const float f = exp2f(__ldcg(r) - bs);
+            ll = fmaf(f, __ldcg(r + 1), ll);
+            fac[i * kHeads + g] = f;
           }
-          const float y = acc / ll;
-          a.out[b * a.out_stride + (int64_t)(head0 + g) * D + d] = (uint16_t)pack2<BF>(y, 0.f);
-          if (d == 0 && a.lse2 != nullptr) a.lse2[b * a.n_q + head0 + g] = mm + log2f(ll);
+          ll = warp_sum(ll);
+          if (lane == 0) {
+            fac[pieces * kHeads + g] = 1.f / ll;
+            if (a.lse2 != nullptr) a.lse2[b * a.n_q + head0 + g] = bs + log2f(ll);
+          }
+        }
+        __syncthreads();
+        for (int i = tid; i < heads * (D / 2); i += kThreads) {
+          const int g = i / (D / 2), d = 2 * (i - g * (D / 2));
+          float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 8
+          for (int p = 0; p < pieces; ++p) {
+            const float2 v = __ldcg(reinterpret_cast<const float2*>(piece(p) + g * (D + 2) + d));
+            const float f = fac[p * kHeads + g];
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+          }
+          const float inv = fac[pieces * kHeads + g];
+          *reinterpret_cast<uint32_t*>(a.out + b * a.out_stride + (int64_t)(head0 + g) * D + d) =
+              pack2<BF>(acc.x * inv, acc.y * inv);
         }
       }
     }
@@ -495,7 +586,10 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a) {
 
 // Stores tokens behind a sequence's cached ones: slot len + t of every kv
 // head gets k (rotated when tables are given) and v; scores and positions
-// are set. One warp per (sequence, token, kv head), 16 bytes per lane.
+// are set. A warp takes four tokens of a head at a time, 16 bytes per lane
+// and token. Bound by DRAM traffic: every row is read and written once.
+constexpr int kTok = 4;
+
 struct AppendArgs {
   Cache c;
   const uint16_t* k;
@@ -515,60 +609,71 @@ template <bool BF>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
   const Cache& c = a.c;
   const int lane = threadIdx.x & 31;
-  const int64_t items = (int64_t)c.batch * a.tokens * c.n_kv;
   const int D = c.head_dim, chunks = D / 8, half = chunks / 2;
-  const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < items; i += step) {
-    const int h = (int)(i % c.n_kv);
-    const int64_t bt = i / c.n_kv;
-    const int t = (int)(bt % a.tokens), b = (int)(bt / a.tokens);
-    const int len = c.seq_lens[b];
-    if (len < 0 || (a.n_new != nullptr && t >= a.n_new[b])) continue;
-    const int64_t slot = (int64_t)len + t;
-    if (slot >= capacity(c)) continue;
-    const int page = page_of(c, b, (int)slot);
-    if (page < 0) continue;
-    const int off = (int)(slot % c.page_size);
-    const int64_t pos = a.first != nullptr ? a.first[b] + t : slot;
-    if (a.cos_t != nullptr && (pos < 0 || pos >= a.rope_rows)) continue;
-    const int64_t at = row_at(c, page, h, off);
-    const uint16_t* ks = a.k + b * a.kb + t * a.kt + h * a.kh;
-    const uint16_t* vs = a.v + b * a.vb + t * a.vt + h * a.vh;
-    uint16_t* kd = reinterpret_cast<uint16_t*>(c.k) + at;
-    uint16_t* vd = reinterpret_cast<uint16_t*>(c.v) + at;
+  const int b = blockIdx.z, len = c.seq_lens[b];
+  const int tokens = a.n_new != nullptr ? min(a.tokens, a.n_new[b]) : a.tokens;
+  if (len < 0) return;
+  // a warp takes kTok tokens of one head, so that their loads overlap
+  const int h = blockIdx.y;
+  const int64_t first = a.first != nullptr ? a.first[b] : len;
+  for (int t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kTok; t0 < tokens; t0 += gridDim.x * 8 * kTok) {
+    int64_t at[kTok];
+    bool ok[kTok];
     for (int ch = lane; ch < 2 * chunks; ch += 32) {
       const bool is_v = ch >= chunks;
       const int cc = is_v ? ch - chunks : ch;
-      uint4 w = *reinterpret_cast<const uint4*>((is_v ? vs : ks) + cc * 8);
-      if (!is_v && a.cos_t != nullptr) {
-        const bool hi = cc >= half;
-        const uint4 p = *reinterpret_cast<const uint4*>(ks + (hi ? cc - half : cc + half) * 8);
-        const int j = (hi ? cc - half : cc) * 8;
-        const float* cs = a.cos_t + pos * (D / 2) + j;
-        const float* sn = a.sin_t + pos * (D / 2) + j;
-        uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
-        const uint32_t* pw = reinterpret_cast<const uint32_t*>(&p);
+      const bool hi = cc >= half;
+      const bool turn = !is_v && a.cos_t != nullptr;
+      const uint16_t* src = is_v ? a.v + b * a.vb + h * a.vh : a.k + b * a.kb + h * a.kh;
+      const int64_t step = is_v ? a.vt : a.kt;
+      // the rows are on their way while the pages are looked up
+      uint4 w[kTok], p[kTok];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 x = unpack2<BF>(ww[e]), y = unpack2<BF>(pw[e]);
-          float2 r0, r1;
-          if (hi) {
-            r0 = rotate(y.x, x.x, cs[2 * e], sn[2 * e]);
-            r1 = rotate(y.y, x.y, cs[2 * e + 1], sn[2 * e + 1]);
-            ww[e] = pack2<BF>(r0.y, r1.y);
-          } else {
-            r0 = rotate(x.x, y.x, cs[2 * e], sn[2 * e]);
-            r1 = rotate(x.y, y.y, cs[2 * e + 1], sn[2 * e + 1]);
-            ww[e] = pack2<BF>(r0.x, r1.x);
+      for (int i = 0; i < kTok; ++i)
+        if (t0 + i < tokens) {
+          const uint16_t* r = src + (t0 + i) * step;
+          w[i] = *reinterpret_cast<const uint4*>(r + cc * 8);
+          if (turn) p[i] = *reinterpret_cast<const uint4*>(r + (hi ? cc - half : cc + half) * 8);
+        }
+      if (ch == lane) {
+#pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+          const int64_t slot = (int64_t)len + t0 + i, pos = first + t0 + i;
+          ok[i] = t0 + i < tokens && slot < capacity(c) && (a.cos_t == nullptr || (pos >= 0 && pos < a.rope_rows));
+          at[i] = 0;
+          const int page = ok[i] ? page_of(c, b, (int)slot) : -1;
+          ok[i] = page >= 0;
+          if (ok[i]) {
+            const int off = (int)slot % c.page_size;
+            at[i] = row_at(c, page, h, off);
+            if (lane == 0) {
+              const int64_t sa = stat_at(c, page, h, off);
+              if (c.scores != nullptr)
+                c.scores[sa] = a.scores != nullptr ? a.scores[b * a.sb + h * a.sh + (t0 + i) * a.st] : 0.f;
+              if (c.slot_pos != nullptr) c.slot_pos[sa] = (int32_t)pos;
+            }
           }
         }
       }
-      *reinterpret_cast<uint4*>((is_v ? vd : kd) + cc * 8) = w;
-    }
-    if (lane == 0) {
-      const int64_t sa = stat_at(c, page, h, off);
-      if (c.scores != nullptr) c.scores[sa] = a.scores != nullptr ? a.scores[b * a.sb + h * a.sh + t * a.st] : 0.f;
-      if (c.slot_pos != nullptr) c.slot_pos[sa] = (int32_t)pos;
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) {
+        if (!ok[i]) continue;
+        if (turn) {
+          const int64_t j = (first + t0 + i) * (D / 2) + (hi ? cc - half : cc) * 8;
+          const float* cs = a.cos_t + j;
+          const float* sn = a.sin_t + j;
+          uint32_t* ww = reinterpret_cast<uint32_t*>(&w[i]);
+          const uint32_t* pw = reinterpret_cast<const uint32_t*>(&p[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 x = unpack2<BF>(hi ? pw[e] : ww[e]), y = unpack2<BF>(hi ? ww[e] : pw[e]);
+            const float2 r0 = rotate(x.x, y.x, cs[2 * e], sn[2 * e]);
+            const float2 r1 = rotate(x.y, y.y, cs[2 * e + 1], sn[2 * e + 1]);
+            ww[e] = hi ? pack2<BF>(r0.y, r1.y) : pack2<BF>(r0.x, r1.x);
+          }
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(is_v ? c.v : c.k) + at[i] + cc * 8) = w[i];
+      }
     }
   }
 }
@@ -604,7 +709,7 @@ int make_cache(const ts_paged_cache* p, Cache* o) {
   return TS_OK;
 }
 
-static size_t grid_of(int head_dim) { return (size_t)sm_count() * (head_dim > 128 ? 1 : 2); }
+static size_t grid_of(int head_dim) { return (size_t)sm_count() * (head_dim > 128 ? 1 : head_dim > 64 ? 2 : 3); }
 
 struct Layout {
   size_t partials, lse, logits, bytes;
@@ -671,6 +776,7 @@ extern "C" int ts_paged_decode_attention(const void* qkv, int64_t qkv_row_stride
   TS_REQUIRE(positions != nullptr || (rope_cos == nullptr && a.c.slot_pos == nullptr),
              "positions are needed for the rotation and for slot_pos");
   TS_REQUIRE(n_q > 0 && n_q % a.c.n_kv == 0, "bad head counts");
+  TS_REQUIRE(is_aligned(out, 4) && out_row_stride % 2 == 0, "rows of out must be 4-byte aligned");
   TS_REQUIRE(!accumulate || a.c.scores != nullptr, "the cache has no scores to accumulate into");
   if (a.c.batch == 0) return TS_OK;
   a.group = n_q / a.c.n_kv;
@@ -698,6 +804,10 @@ extern "C" int ts_paged_decode_attention(const void* qkv, int64_t qkv_row_stride
   a.lse2 = accumulate ? reinterpret_cast<float*>(ws + L.lse) : nullptr;
   a.logits = accumulate ? reinterpret_cast<float*>(ws + L.logits) : nullptr;
   a.logit_stride = L.logit_stride;
+  a.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (a.c.page_size == 1 << i) a.page_shift = i;
+  a.one_page = a.c.page_size % kRows == 0 ? 1 : 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int grid = (int)grid_of(a.c.head_dim);
   const int r = cache->dtype == TS_BF16 ? launch_attention<true>(a, grid, st) : launch_attention<false>(a, grid, st);
@@ -739,8 +849,10 @@ extern "C" int ts_paged_append(const void* k, const int64_t* k_strides, const vo
   a.sb = scores ? score_strides[0] : 0;
   a.sh = scores ? score_strides[1] : 0;
   a.st = scores ? score_strides[2] : 0;
-  const int64_t items = (int64_t)a.c.batch * tokens * a.c.n_kv;
-  const int grid = (int)std::min<int64_t>((items + 7) / 8, (int64_t)sm_count() * 8);
+  TS_UNSUPPORTED(a.c.batch <= 65535 && a.c.n_kv <= 65535, "too many sequences or heads in one call");
+  const int rows = a.c.batch * a.c.n_kv;
+  const dim3 grid((unsigned)std::max(1, std::min((tokens + 8 * kTok - 1) / (8 * kTok), (16 * sm_count() + rows - 1) / rows)),
+                  (unsigned)a.c.n_kv, (unsigned)a.c.batch);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (cache->dtype == TS_BF16) paged_append_kernel<true><<<grid, 256, 0, st>>>(a);
   else paged_append_kernel<false><<<grid, 256, 0, st>>>(a);

@@ -188,28 +188,12 @@ def device_status(device: Optional[torch.device] = None, clear: bool = True) -> 
             else:
                 rc = lib.ts_qlinear_status(b.data_ptr(), int(b.numel()), 1 if clear else 0, stream)
             _C.check(rc, "ts_qlinear_status")
-        timeout = 0
-        for b in _SERVING.on_device(dev.index):
-            # the flag is one per device and the first call clears it: zero
-            # the counters of the other workspaces here
-            if timeout and clear:
-                b[:1 << 18].zero_()
-            else:
-                timeout = lib.ts_fp4_status(b.data_ptr(), int(b.numel()), 1 if clear else 0, stream)
-        _C.check(timeout, "ts_fp4_status")
+        if ops is not None:       # the fp4 and paged operators
+            ops.serving_status(dev.index, clear)
 
 
 def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
     return _WORKSPACES.get(device, nbytes)
-
-
-# scratch of the ts_paged_* and ts_fp4_* calls, whose counters lie elsewhere
-# than those of ts_qlinear
-_SERVING = _Workspaces()
-
-
-def _serving_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    return _SERVING.get(device, nbytes)
 
 
 # ---------------------------------------------------------------------------
