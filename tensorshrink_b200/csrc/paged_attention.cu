@@ -36,6 +36,8 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;                  // slots of a warp's share of a unit
 constexpr int kUnit = kWarps * kRows;      // slots of a unit
 constexpr int kHeads = 16;                 // query heads of an MMA tile
+constexpr int kRowCost = 6;                // units that starting and joining a row costs
+constexpr int kFullUnits = 8;              // units per CTA from which that cost is counted
 
 struct AttnArgs {
   Cache c;
@@ -74,6 +76,9 @@ __device__ __forceinline__ void split_slot(const AttnArgs& a, int s, int* page, 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -98,17 +103,35 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Units of sequence b for one kv head, 0 when the call cannot take it: no
-// slot for the new token, or a position outside the rotary tables.
-__device__ __forceinline__ int units_of(const AttnArgs& a, int b) {
-  const int len = a.c.seq_lens[b];
-  if (len < 0 || len >= capacity(a.c)) return 0;
-  if (a.cos_t != nullptr) {
-    const int64_t pos = a.positions[b];
-    if (pos < 0 || pos >= a.rope_rows) return 0;
+// Units of a sequence of `len` cached tokens for one kv head; 0 without a
+// slot for the new one.
+__device__ __forceinline__ int units_of(const AttnArgs& a, int len) {
+  return len < 0 || len >= capacity(a.c) ? 0 : len / kUnit + 1;
+}
+
+// Whether sequence b, with a slot for its new token, can take it: the slot
+// has memory and the position a row in the rotary tables.
+__device__ __forceinline__ bool takes(const AttnArgs& a, int b, int len, int64_t pos) {
+  int pg, off;
+  split_slot(a, len, &pg, &off);
+  const int page = a.c.table[b * a.c.table_stride + pg];
+  return (unsigned)page < (unsigned)a.c.num_pages && (a.cos_t == nullptr || (pos >= 0 && pos < a.rope_rows));
+}
+
+// Equal shares of `total` units for n CTAs: the first total % n get one more.
+struct Shares {
+  unsigned q, r;
+  __device__ __forceinline__ Shares(unsigned total, unsigned n) : q(total / n), r(total - total / n * n) {}
+  __device__ __forceinline__ unsigned begin(unsigned i) const { return i * q + min(i, r); }
+  __device__ __forceinline__ unsigned owner(unsigned u) const {
+    return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q;
   }
-  if (page_of(a.c, b, len) < 0) return 0;
-  return len / kUnit + 1;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Shared memory: the warps' rings [kWarps][S][K, V][16 rows][pitch], the
@@ -121,11 +144,11 @@ template <int DP>
 constexpr size_t ring_bytes() { return (size_t)kWarps * stages_for<DP>() * 2 * kRows * DP * 2; }
 template <int DP>
 constexpr size_t attn_smem(int batch) {
-  return ring_bytes<DP>() + kHeads * (DP + 8) * 2 + (size_t)(batch + 1) * 4 + 64;
+  return ring_bytes<DP>() + kHeads * (DP + 8) * 2 + (size_t)(2 * batch + 1) * 4;
 }
 
 template <bool BF, int DP>
-__global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) paged_attention_kernel(const AttnArgs a) {
   constexpr int S = stages_for<DP>();
   constexpr int kPitch = DP * 2;                 // bytes of a staged row
   constexpr int kStage = 2 * kRows * kPitch;     // bytes of a stage: K rows, then V rows
@@ -133,31 +156,35 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
   constexpr bool kKeepQ = DP <= 128;             // query fragments stay in registers
   constexpr int kRowChunks = DP / 8;             // 16-byte columns of a staged row
   constexpr int kRowsPer = 32 / kRowChunks;      // rows that a warp copies at once
-  extern __shared__ __align__(128) char smem[];
+  extern __shared__ __align__(1024) char smem[];
   uint16_t* qs = reinterpret_cast<uint16_t*>(smem + ring_bytes<DP>());
-  int* prefix = reinterpret_cast<int*>(smem + ring_bytes<DP>() + kHeads * (DP + 8) * 2);
-  __shared__ int warp_sums[kWarps], warp_most[kWarps];
+  int* prefix = reinterpret_cast<int*>(smem + ring_bytes<DP>() + kHeads * (DP + 8) * 2);   // [batch + 1]
+  __shared__ uint64_t warp_sums[kWarps];
+  __shared__ int warp_most[kWarps];
   __shared__ int is_last;
   const Cache& c = a.c;
+  int* lens = prefix + c.batch + 1;                                                        // [batch]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int D = c.head_dim, chunks = D / 8, steps = D / 16, rows_per_b = c.n_kv * a.head_tiles;
 
   // prefix sums of the sequences' units; every thread takes a run of sequences
-  int longest = 0;
+  int longest = 0, front = 0;
   {
     const int per = (c.batch + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
-    int sum = 0, most = 0;
+    uint64_t sum = 0;                             // units, and sequences with units in the upper half
+    int most = 0;
     for (int b = b0; b < b1; ++b) {
-      const int n = units_of(a, b);
-      sum += n;
+      lens[b] = c.seq_lens[b];
+      const int n = units_of(a, lens[b]);
+      sum += n > 0 ? ((uint64_t)1 << 32) + n : 0;
       most = max(most, n);
     }
-    int inc = sum;
+    uint64_t inc = sum;
     most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, inc, o);
+      const uint64_t t = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += t;
     }
     if (lane == 31) {
@@ -165,15 +192,25 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
       warp_most[warp] = most;
     }
     __syncthreads();
+    uint64_t all = 0, at = inc - sum;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) longest = max(longest, warp_most[w]);
-    int at = inc - sum;
-    for (int w = 0; w < warp; ++w) at += warp_sums[w];
-    for (int b = b0; b < b1; ++b) {
-      prefix[b] = at;
-      at += units_of(a, b);
+    for (int w = 0; w < kWarps; ++w) {
+      longest = max(longest, warp_most[w]);
+      if (w < warp) at += warp_sums[w];
+      all += warp_sums[w];
     }
-    if (b1 == c.batch && b0 < b1) prefix[c.batch] = at;
+    // With units enough for every CTA, a row counts kRowCost units in front of
+    // its own, so that a CTA of many short rows gets fewer units than one of
+    // few long ones.
+    front = (uint64_t)(uint32_t)all * rows_per_b >= (uint64_t)kFullUnits * gridDim.x ? kRowCost : 0;
+    longest += front;
+    int v = (int)(uint32_t)at + front * (int)(at >> 32);
+    for (int b = b0; b < b1; ++b) {
+      prefix[b] = v;
+      const int n = units_of(a, lens[b]);
+      v += n > 0 ? n + front : 0;
+    }
+    if (b1 == c.batch && b0 < b1) prefix[c.batch] = v;
   }
   // rows of the query tile that no head fills: zeros, so that their scores are finite
   for (int i = tid; i < kHeads * (DP + 8) / 2; i += kThreads) reinterpret_cast<uint32_t*>(qs)[i] = 0;
@@ -183,49 +220,63 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
     if (prefix[b] == prefix[b + 1])
       for (int i = tid; i < a.n_q * D; i += kThreads) a.out[b * a.out_stride + i] = 0;
 
-  const int64_t total = (int64_t)prefix[c.batch] * rows_per_b;
-  // every CTA gets units, unless that cut the longest row into more pieces
-  // than its join takes in its stride
-  const int64_t n_cta =
-      max((int64_t)1, min(min((int64_t)gridDim.x, total), kMaxPieces * total / max(longest, 1)));
-  if (total == 0 || (int64_t)blockIdx.x >= n_cta) return;
-  const int64_t u0 = total * blockIdx.x / n_cta, u1 = total * (blockIdx.x + 1) / n_cta;
+  const unsigned total = (unsigned)prefix[c.batch] * rows_per_b;   // (the host keeps it below 2^31)
+  if (total == 0) return;
+  // as many CTAs as get a whole unit each, unless that cut the longest row
+  // into more pieces than its join takes in its stride
+  const unsigned n_cta = max(1u, min(min(gridDim.x, total / (front + 1)),
+                                     (unsigned)min((float)kMaxPieces * total / longest, 1e6f)));
+  if (blockIdx.x >= n_cta) return;
+  const Shares shares(total, n_cta);
+  const unsigned u1 = shares.begin(blockIdx.x + 1);
 
   char* ring = smem + (size_t)warp * S * kStage;
   const uint32_t ring_u = smem_u32(ring);
   const uint32_t qs_u = smem_u32(qs);
 
-  for (int64_t u = u0; u < u1;) {
+  // the first row: sequence b is the last with prefix[b] * rows_per_b <= u
+  unsigned u = shares.begin(blockIdx.x);
+  int b = 0;
+  for (int hi = c.batch - 1; b < hi;) {
+    const int mid = (b + hi + 1) >> 1;
+    if ((unsigned)prefix[mid] * rows_per_b <= u) b = mid; else hi = mid - 1;
+  }
+  int row = (int)((u - (unsigned)prefix[b] * rows_per_b) / (unsigned)(prefix[b + 1] - prefix[b]));
+  for (; u < u1; ++row) {
     // the segment: units [t0, t1) of (sequence b, kv head h, head tile ht)
-    int b;
-    {
-      int lo = 0, hi = c.batch - 1;   // last b with prefix[b] * rows_per_b <= u and units
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if ((int64_t)prefix[mid] * rows_per_b <= u) lo = mid; else hi = mid - 1;
-      }
-      b = lo;
+    if (row == rows_per_b) {
+      row = 0;
+      do ++b; while (prefix[b + 1] == prefix[b]);
     }
-    const int nt = prefix[b + 1] - prefix[b];
-    const int64_t in_b = u - (int64_t)prefix[b] * rows_per_b;
-    const int row = (int)(in_b / nt);
-    const int t0 = (int)(in_b - (int64_t)row * nt);
-    const int t1 = (int)min((int64_t)nt, t0 + (u1 - u));
+    const int cost = prefix[b + 1] - prefix[b], nt = cost - front;
+    const unsigned row_u = (unsigned)prefix[b] * rows_per_b + (unsigned)(row * cost);
+    const int v0 = (int)(u - row_u), v1 = (int)min((unsigned)cost, v0 + (u1 - u));
+    u += v1 - v0;
+    if (v1 <= front) continue;                         // only the row's front
+    const int t0 = max(v0 - front, 0), t1 = v1 - front;
     const int h = row / a.head_tiles, ht = row - h * a.head_tiles;
     const int heads = min(kHeads, a.group - ht * kHeads);
     const int head0 = h * a.group + ht * kHeads;       // first query head of the tile
-    const int len = c.seq_lens[b];
-    const int64_t pos = a.positions != nullptr ? a.positions[b] : 0;
+    const int len = lens[b];
+    const int32_t* table = c.table + b * c.table_stride;
+    int64_t pos = a.positions != nullptr ? a.positions[b] : 0;
+    const bool ok = takes(a, b, len, pos);             // (a sequence that cannot take its token answers with zeros)
+    if (!ok) pos = 0;
     const uint16_t* new_row = a.qkv + b * a.qkv_stride;
-    const float* cs = a.cos_t != nullptr ? a.cos_t + pos * (D / 2) : nullptr;
-    const float* sn = a.cos_t != nullptr ? a.sin_t + pos * (D / 2) : nullptr;
+    const bool turn = a.cos_t != nullptr;
 
     // A warp's share of unit t: slots t * 64 + warp * 16 + r. It copies the
     // rows of cached slots and zeros for the others; `live` is a bit per row
     // that has a cached token, queued until the stage is consumed.
     const int cl = lane % kRowChunks, rl = lane / kRowChunks;   // this lane's 16-byte column and first row
     const bool col = cl < chunks;
-    auto issue = [&](int t, int stage) -> uint32_t {
+    auto page_at = [&](int t) {                        // (one_page) the page of unit t's rows
+      const int slot0 = t * kUnit + warp * kRows;
+      int pg, off;
+      split_slot(a, slot0, &pg, &off);
+      return t < t1 && slot0 < len ? table[pg] : -1;
+    };
+    auto issue = [&](int t, int stage, int page) -> uint32_t {
       uint32_t live = 0;
       if (t < t1) {
         const int slot0 = t * kUnit + warp * kRows;
@@ -234,20 +285,32 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
         if (a.one_page) {
           int pg, off;
           split_slot(a, slot0, &pg, &off);
-          const int page = n > 0 && pg < c.max_pages ? c.table[b * c.table_stride + pg] : -1;
           const int rows = (unsigned)page < (unsigned)c.num_pages ? n : 0;
           live = rows > 0 ? (1u << rows) - 1 : 0;
-          int64_t e = rows > 0 ? (row_at(c, page, h, off + rl) + cl * 8) * 2 : 0;
-          const int64_t step = rows > 0 ? c.token_stride * (kRowsPer * 2) : 0;
-          if (col) {
+          // row 2 i + rl of a 256-byte row (and alike for the other widths):
+          // its swizzled column is this lane's with bits of i flipped
+          const uint32_t x0 = (uint32_t)(cl ^ rl) << 4;
+          const int64_t e = rows > 0 ? (row_at(c, page, h, off + rl) + cl * 8) * 2 : 0;
+          const char* kp = c.k + e;
+          const int64_t step = c.token_stride * (kRowsPer * 2), kv = c.v - c.k;
+          if (rows == kRows) {
+            if (col) {
+#pragma unroll
+              for (int i = 0; i < kRows / kRowsPer; ++i) {
+                const uint32_t d = dst + i * kRowsPer * kPitch + (x0 ^ (((i * kRowsPer) & 7) << 4));
+                cp16(d, kp);
+                cp16(d + kRows * kPitch, kp + kv);
+                kp += step;
+              }
+            }
+          } else if (col) {
 #pragma unroll
             for (int i = 0; i < kRows / kRowsPer; ++i) {
-              const int r = i * kRowsPer + rl;
-              const int ok = r < rows;
-              const uint32_t d = dst + i * kRowsPer * kPitch + ((cl ^ (r & 7)) << 4);
-              cp16(d, c.k + (ok ? e : 0), ok * 16);
-              cp16(d + kRows * kPitch, c.v + (ok ? e : 0), ok * 16);
-              e += step;
+              const int ok = i * kRowsPer + rl < rows;
+              const uint32_t d = dst + i * kRowsPer * kPitch + (x0 ^ (((i * kRowsPer) & 7) << 4));
+              cp16(d, ok ? kp : c.k, ok * 16);
+              cp16(d + kRows * kPitch, ok ? kp + kv : c.v, ok * 16);
+              if (ok) kp += step;
             }
           }
         } else {
@@ -257,8 +320,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
           if (r0 < n) {
             int pg, off;
             split_slot(a, slot0 + r0, &pg, &off);
-            const int page = pg < c.max_pages ? c.table[b * c.table_stride + pg] : -1;
-            if ((unsigned)page < (unsigned)c.num_pages) o = row_at(c, page, h, off);
+            const int p = table[pg];
+            if ((unsigned)p < (unsigned)c.num_pages) o = row_at(c, p, h, off);
           }
           live = __ballot_sync(0xffffffffu, o >= 0) & 0xFFFFu;
 #pragma unroll
@@ -278,24 +341,49 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
       cp_commit();
       return live;
     };
-    uint64_t live_q = 0;
+    // The rotated query heads of the tile, kQ pairs of a thread at a time; the
+    // first are loaded before the copies, which would hold them up.
+    constexpr int kQ = 4;
+    const float* cs = a.cos_t + pos * (D / 2);
+    const float* sn = a.sin_t + pos * (D / 2);
+    uint32_t qx[kQ];
+    float2 rot[kQ];
+    auto load_q = [&](int i0) {
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) live_q |= (uint64_t)issue(t0 + s, s) << (16 * s);
-
-    // the rotated query heads of the tile
-    for (int i = tid; i < heads * (D / 2); i += kThreads) {
-      const int g = i / (D / 2), j = i - g * (D / 2);
-      const uint16_t* qr = new_row + (int64_t)(head0 + g) * D;
-      uint16_t x1 = qr[j], x2 = qr[j + D / 2];
-      if (cs != nullptr) {
-        const float2 f = unpack2<BF>((uint32_t)x1 | ((uint32_t)x2 << 16));
-        const float2 y = rotate(f.x, f.y, cs[j], sn[j]);
-        const uint32_t p = pack2<BF>(y.x, y.y);
-        x1 = (uint16_t)p;
-        x2 = (uint16_t)(p >> 16);
+      for (int k = 0; k < kQ; ++k) {
+        const int i = i0 + k * kThreads, g = i / (D / 2), j = i - g * (D / 2);
+        if (i < heads * (D / 2)) {
+          const uint16_t* qr = new_row + (int64_t)(head0 + g) * D + j;
+          qx[k] = (uint32_t)qr[0] | ((uint32_t)qr[D / 2] << 16);
+          if (turn) rot[k] = make_float2(cs[j], sn[j]);
+        }
       }
-      qs[g * (DP + 8) + j] = x1;
-      qs[g * (DP + 8) + j + D / 2] = x2;
+    };
+    load_q(tid);
+    uint64_t live_q = 0;
+    int page_next;
+    {
+      int pages[S];
+#pragma unroll
+      for (int s = 0; s < S; ++s) pages[s] = a.one_page ? page_at(t0 + s) : -1;
+#pragma unroll
+      for (int s = 0; s < S - 1; ++s) live_q |= (uint64_t)issue(t0 + s, s, pages[s]) << (16 * s);
+      page_next = pages[S - 1];
+    }
+    for (int i0 = tid; i0 < heads * (D / 2); i0 += kQ * kThreads) {
+      if (i0 != tid) load_q(i0);
+#pragma unroll
+      for (int k = 0; k < kQ; ++k) {
+        const int i = i0 + k * kThreads, g = i / (D / 2), j = i - g * (D / 2);
+        if (i >= heads * (D / 2)) continue;
+        if (turn) {
+          const float2 f = unpack2<BF>(qx[k]);
+          const float2 y = rotate(f.x, f.y, rot[k].x, rot[k].y);
+          qx[k] = pack2<BF>(y.x, y.y);
+        }
+        qs[g * (DP + 8) + j] = (uint16_t)qx[k];
+        qs[g * (DP + 8) + j + D / 2] = (uint16_t)(qx[k] >> 16);
+      }
     }
     __syncthreads();
     uint32_t qf[kKeepQ ? kSteps : 1][4];
@@ -316,7 +404,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
 
     int stage = 0;
     for (int t = t0; t < t1; ++t) {
-      live_q |= (uint64_t)issue(t + S - 1, stage == 0 ? S - 1 : stage - 1) << (16 * (S - 1));
+      live_q |= (uint64_t)issue(t + S - 1, stage == 0 ? S - 1 : stage - 1, page_next) << (16 * (S - 1));
+      if (a.one_page) page_next = page_at(t + S);
       uint32_t live = (uint32_t)live_q & 0xFFFFu;
       live_q >>= 16;
       cp_wait<S - 1>();
@@ -325,7 +414,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
       const uint32_t kb = ring_u + stage * kStage, vb = kb + kRows * kPitch;
       stage = stage + 1 == S ? 0 : stage + 1;
       if (slot0 > len) continue;                       // warp-uniform: nothing left for this warp
-      if (len < slot0 + kRows) {
+      if (ok && len < slot0 + kRows) {
         // the new token's row: into the stage and, once per kv head, the cache
         const int r = len - slot0;
         live |= 1u << r;
@@ -338,7 +427,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
         const uint16_t* vr = new_row + (int64_t)(a.n_q + c.n_kv + h) * D;
         for (int j = lane; j < D / 2; j += 32) {
           uint16_t x1 = kr[j], x2 = kr[j + D / 2];
-          if (cs != nullptr) {
+          if (turn) {
             const float2 f = unpack2<BF>((uint32_t)x1 | ((uint32_t)x2 << 16));
             const float2 y = rotate(f.x, f.y, cs[j], sn[j]);
             const uint32_t p = pack2<BF>(y.x, y.y);
@@ -374,36 +463,37 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
       const int krow = (lane & 7) + ((lane >> 4) << 3);
-      const uint32_t k_addr = kb + krow * kPitch;
+      const uint32_t k_addr = (kb + krow * kPitch) | ((((lane >> 3) & 1) ^ r7) << 4);   // rows start at multiples of their pitch
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         if (s >= steps) break;
         uint32_t kf[4];
-        ldsm4(k_addr + (((2 * s + ((lane >> 3) & 1)) ^ r7) << 4), kf);
+        ldsm4(k_addr ^ (s << 5), kf);
         if (!kKeepQ) ldsm4(q_addr + s * 32, qf[0]);
         mma<BF>(sc[0], qf[kKeepQ ? s : 0], kf[0], kf[1]);
         mma<BF>(sc[1], qf[kKeepQ ? s : 0], kf[2], kf[3]);
       }
       const int c0 = (lane & 3) * 2;
+      if (live != 0xFFFFu) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = n * 8 + c0 + (e & 1);
-          sc[n][e] = (live >> r) & 1 ? sc[n][e] * a.scale2 : -INFINITY;
-        }
+          for (int e = 0; e < 4; ++e)
+            if (!((live >> (n * 8 + c0 + (e & 1))) & 1)) sc[n][e] = -INFINITY;
+      }
       if (a.logits != nullptr) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int g = (lane >> 2) + 8 * e;
           if (g < heads) {
             float* lg = a.logits + (int64_t)(b * a.n_q + head0 + g) * a.logit_stride + slot0 + c0;
-            *reinterpret_cast<float2*>(lg) = make_float2(sc[0][2 * e], sc[0][2 * e + 1]);
-            *reinterpret_cast<float2*>(lg + 8) = make_float2(sc[1][2 * e], sc[1][2 * e + 1]);
+            *reinterpret_cast<float2*>(lg) = make_float2(sc[0][2 * e] * a.scale2, sc[0][2 * e + 1] * a.scale2);
+            *reinterpret_cast<float2*>(lg + 8) = make_float2(sc[1][2 * e] * a.scale2, sc[1][2 * e + 1] * a.scale2);
           }
         }
       }
-      // online softmax of the two rows this thread holds parts of
+      // online softmax of the two rows this thread holds parts of; m and the
+      // maxima are unscaled, weights are 2^(s scale2 - m scale2)
       float mn[2], base[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -411,12 +501,12 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
         mn[e] = fmaxf(m[e], x);
-        base[e] = mn[e] == -INFINITY ? 0.f : mn[e];
+        base[e] = mn[e] == -INFINITY ? 0.f : mn[e] * a.scale2;
       }
       if (__any_sync(0xffffffffu, mn[0] > m[0] || mn[1] > m[1])) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float corr = exp2f(m[e] - base[e]);
+          const float corr = ex2(fmaf(m[e], a.scale2, -base[e]));
           l[e] *= corr;
 #pragma unroll
           for (int i = 0; i < DP / 8; ++i) {
@@ -429,19 +519,18 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[n][e] = exp2f(sc[n][e] - base[e >> 1]);
-          l[e >> 1] += sc[n][e];
-        }
+        for (int e = 0; e < 4; ++e) sc[n][e] = ex2(fmaf(sc[n][e], a.scale2, -base[e >> 1]));
+      l[0] += (sc[0][0] + sc[0][1]) + (sc[1][0] + sc[1][1]);
+      l[1] += (sc[0][2] + sc[0][3]) + (sc[1][2] + sc[1][3]);
       const uint32_t pf[4] = {pack2<BF>(sc[0][0], sc[0][1]), pack2<BF>(sc[0][2], sc[0][3]),
                               pack2<BF>(sc[1][0], sc[1][1]), pack2<BF>(sc[1][2], sc[1][3])};
       const int vrow = lane & 15;
-      const uint32_t v_addr = vb + vrow * kPitch;
+      const uint32_t v_addr = (vb + vrow * kPitch) | (((lane >> 4) ^ r7) << 4);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         if (s >= steps) break;
         uint32_t vf[4];
-        ldsm4t(v_addr + (((2 * s + (lane >> 4)) ^ r7) << 4), vf);
+        ldsm4t(v_addr ^ (s << 5), vf);
         mma<BF>(o[2 * s], pf, vf[0], vf[1]);
         mma<BF>(o[2 * s + 1], pf, vf[2], vf[3]);
       }
@@ -458,7 +547,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
     // join the warps through shared memory (over the drained rings)
     constexpr int kJoin = DP + 4;                    // floats of a row: its sums, max, sum
     float* jo = reinterpret_cast<float*>(smem);      // [kWarps][16][kJoin]
-    static_assert((size_t)kWarps * kHeads * kJoin * 4 <= ring_bytes<DP>() + kHeads * (DP + 8) * 2, "join area");
+    static_assert((size_t)kWarps * kHeads * (kJoin + 2) * 4 <= ring_bytes<DP>() &&
+                      (size_t)kHeads * (2 * (kMaxPieces + 4) + 1) * 4 <= ring_bytes<DP>(), "join areas");
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float* r = jo + (warp * kHeads + (lane >> 2) + 8 * e) * kJoin;
@@ -466,101 +556,122 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
       for (int i = 0; i < DP / 8; ++i)
         *reinterpret_cast<float2*>(r + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
       if ((lane & 3) == 0) {
-        r[DP] = m[e];
+        r[DP] = m[e] * a.scale2;                       // in log2 units from here on
         r[DP + 1] = l[e];
       }
     }
     __syncthreads();
-    const int64_t row_u0 = (int64_t)prefix[b] * rows_per_b + (int64_t)row * nt;   // the row's units
-    const bool whole = t0 == 0 && t1 == nt;
-    const int64_t prow = (int64_t)kHeads * (D + 2);
-    float* part = whole ? nullptr : a.partials + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * prow;
-    for (int i = tid; i < heads * D; i += kThreads) {
-      const int g = i / D, d = i - g * D;
-      float mm = -INFINITY;
+    // factors 2^(m_warp - m) of every warp and head, then the sums
+    float* fac = jo + kWarps * kHeads * kJoin;       // [kWarps][16], then [16] maxima, [16] sums
+    if (tid < kHeads) {
+      float wm[kWarps], mm = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, jo[(w * kHeads + g) * kJoin + DP]);
+      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, wm[w] = jo[(w * kHeads + tid) * kJoin + DP]);
       const float bs = mm == -INFINITY ? 0.f : mm;
-      float acc = 0.f, ll = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float* r = jo + (w * kHeads + g) * kJoin;
-        const float f = exp2f(r[DP] - bs);
-        acc = fmaf(f, r[d], acc);
-        ll = fmaf(f, r[DP + 1], ll);
+        const float f = ex2(wm[w] - bs);
+        fac[w * kHeads + tid] = f;
+        ll = fmaf(f, jo[(w * kHeads + tid) * kJoin + DP + 1], ll);
+      }
+      fac[kWarps * kHeads + tid] = mm;
+      fac[(kWarps + 1) * kHeads + tid] = ll;
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == nt;
+    const int64_t prow = (int64_t)kHeads * (D + 2);  // a piece: [16][D] sums, [16] (max, sum)
+    // a CTA has at most two partial rows: one that it ends, one that it begins
+    float* part = a.partials + ((int64_t)blockIdx.x * 2 + (t0 > 0 ? 0 : 1)) * prow;
+    uint16_t* out = a.out + b * a.out_stride + (int64_t)head0 * D;
+    for (int i = tid; i < heads * (D / 4); i += kThreads) {
+      const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float4 v = *reinterpret_cast<const float4*>(jo + (w * kHeads + g) * kJoin + d);
+        const float f = fac[w * kHeads + g];
+        acc.x = fmaf(f, v.x, acc.x);
+        acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z);
+        acc.w = fmaf(f, v.w, acc.w);
       }
       if (whole) {
-        const float y = acc / ll;
-        a.out[b * a.out_stride + (int64_t)(head0 + g) * D + d] = (uint16_t)pack2<BF>(y, 0.f);
-        if (d == 0 && a.lse2 != nullptr) a.lse2[b * a.n_q + head0 + g] = bs + log2f(ll);
+        const float inv = 1.f / fac[(kWarps + 1) * kHeads + g];
+        uint32_t* dst = reinterpret_cast<uint32_t*>(out + g * D + d);
+        dst[0] = ok ? pack2<BF>(acc.x * inv, acc.y * inv) : 0;
+        dst[1] = ok ? pack2<BF>(acc.z * inv, acc.w * inv) : 0;
       } else {
-        part[g * (D + 2) + d] = acc;
-        if (d == 0) {
-          part[g * (D + 2) + D] = mm;
-          part[g * (D + 2) + D + 1] = ll;
-        }
+        *reinterpret_cast<float4*>(part + g * D + d) = acc;
       }
     }
+    if (tid < heads) {
+      const float mm = fac[kWarps * kHeads + tid], ll = fac[(kWarps + 1) * kHeads + tid];
+      if (!whole) reinterpret_cast<float2*>(part + kHeads * D)[tid] = make_float2(mm, ll);
+      else if (a.lse2 != nullptr) a.lse2[b * a.n_q + head0 + tid] = mm + log2f(ll);
+    }
     if (!whole) {
-      const int64_t last_u = row_u0 + nt - 1;
-      const int cta0 = (int)(((row_u0 + 1) * n_cta - 1) / total), cta1 = (int)(((last_u + 1) * n_cta - 1) / total);
+      const unsigned first_u = row_u + front;        // the row's first unit
+      const int cta0 = (int)shares.owner(first_u), cta1 = (int)shares.owner(first_u + nt - 1);
       int* cnt = a.counters + b * rows_per_b + row;
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
+        __threadfence();                             // the CTA's piece, before its arrival
         is_last = atomicAdd(cnt, 1) == cta1 - cta0;
         if (is_last) *cnt = 0;                       // zero for the next call
+        __threadfence();
       }
       __syncthreads();
       if (is_last) {
-        __threadfence();
-        // factors exp2(m_piece - m) / l of every piece and head, then the sums
-        const int pieces = cta1 - cta0 + 1;            // at most kMaxPieces + 2
-        float* fac = jo;                               // [pieces][kHeads]
-        // a row's pieces lie at the start of their CTAs' ranges, except that
-        // the first may lie at its CTA's end
-        const float* piece0 = a.partials + ((int64_t)cta0 * 2 + (total * cta0 / n_cta >= row_u0 ? 0 : 1)) * prow;
-        const float* piece1 = a.partials + (int64_t)cta0 * 2 * prow;
-        auto piece = [&](int i) { return i == 0 ? piece0 : piece1 + (int64_t)i * 2 * prow; };
-        __syncthreads();                               // the join of the warps has been read
+        const int pieces = cta1 - cta0 + 1;          // at most kMaxPieces + 2
+        // a row's pieces lie first in their CTAs' slots, but for its beginning
+        const float* begun = a.partials + ((int64_t)cta0 * 2 + 1) * prow;
+        const float* others = a.partials + (int64_t)cta0 * 2 * prow;
+        auto piece = [&](int i) { return i == 0 ? begun : others + (int64_t)i * 2 * prow; };
+        float2* ml = reinterpret_cast<float2*>(jo);  // [pieces][16]: (max, sum), then (factor, -)
+        float* inv_l = jo + 2 * kHeads * (kMaxPieces + 4);
+        for (int i = tid; i < pieces * kHeads; i += kThreads) {
+          const int pc = i / kHeads, g = i % kHeads;
+          if (g < heads) ml[i] = __ldcg(reinterpret_cast<const float2*>(piece(pc) + kHeads * D) + g);
+        }
+        __syncthreads();
         for (int g = warp; g < heads; g += kWarps) {
           float mm = -INFINITY;
-          for (int i = lane; i < pieces; i += 32) mm = fmaxf(mm, __ldcg(piece(i) + g * (D + 2) + D));
+          for (int i = lane; i < pieces; i += 32) mm = fmaxf(mm, ml[i * kHeads + g].x);
 #pragma unroll
           for (int o2 = 16; o2 > 0; o2 >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o2));
           const float bs = mm == -INFINITY ? 0.f : mm;
           float ll = 0.f;
           for (int i = lane; i < pieces; i += 32) {
-            const float* r = piece(i) + g * (D + 2) + D;
-            const float f = exp2f(__ldcg(r) - bs);
-            ll = fmaf(f, __ldcg(r + 1), ll);
-            fac[i * kHeads + g] = f;
+            const float f = ex2(ml[i * kHeads + g].x - bs);
+            ll = fmaf(f, ml[i * kHeads + g].y, ll);
+            ml[i * kHeads + g].x = f;
           }
           ll = warp_sum(ll);
           if (lane == 0) {
-            fac[pieces * kHeads + g] = 1.f / ll;
+            inv_l[g] = 1.f / ll;
             if (a.lse2 != nullptr) a.lse2[b * a.n_q + head0 + g] = bs + log2f(ll);
           }
         }
         __syncthreads();
-        for (int i = tid; i < heads * (D / 2); i += kThreads) {
-          const int g = i / (D / 2), d = 2 * (i - g * (D / 2));
-          float2 acc = make_float2(0.f, 0.f);
+        for (int i = tid; i < heads * (D / 4); i += kThreads) {
+          const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
           for (int p = 0; p < pieces; ++p) {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(piece(p) + g * (D + 2) + d));
-            const float f = fac[p * kHeads + g];
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(p) + g * D + d));
+            const float f = ml[p * kHeads + g].x;
             acc.x = fmaf(f, v.x, acc.x);
             acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
           }
-          const float inv = fac[pieces * kHeads + g];
-          *reinterpret_cast<uint32_t*>(a.out + b * a.out_stride + (int64_t)(head0 + g) * D + d) =
-              pack2<BF>(acc.x * inv, acc.y * inv);
+          uint32_t* dst = reinterpret_cast<uint32_t*>(out + g * D + d);
+          dst[0] = ok ? pack2<BF>(acc.x * inv_l[g], acc.y * inv_l[g]) : 0;
+          dst[1] = ok ? pack2<BF>(acc.z * inv_l[g], acc.w * inv_l[g]) : 0;
         }
       }
     }
     __syncthreads();   // the join area becomes the rings again
-    u += t1 - t0;
   }
 }
 
@@ -570,15 +681,15 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const AttnArg
 __global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a) {
   const Cache& c = a.c;
   const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv;
-  if (units_of(a, b) == 0) return;
   const int len = c.seq_lens[b];
+  if (units_of(a, len) == 0 || !takes(a, b, len, a.positions != nullptr ? a.positions[b] : 0)) return;
   for (int slot = blockIdx.x * blockDim.x + threadIdx.x; slot <= len; slot += gridDim.x * blockDim.x) {
     const int page = page_of(c, b, slot);
     if (page < 0) continue;
     float w = 0.f;
     for (int g = 0; g < a.group; ++g) {
       const int64_t q = (int64_t)b * a.n_q + h * a.group + g;
-      w += exp2f(__ldcs(a.logits + q * a.logit_stride + slot) - a.lse2[q]);
+      w += ex2(__ldcs(a.logits + q * a.logit_stride + slot) - a.lse2[q]);
     }
     c.scores[stat_at(c, page, h, slot % c.page_size)] += w;   // the attention has set the new slot's to 0
   }
@@ -776,12 +887,16 @@ extern "C" int ts_paged_decode_attention(const void* qkv, int64_t qkv_row_stride
   TS_REQUIRE(positions != nullptr || (rope_cos == nullptr && a.c.slot_pos == nullptr),
              "positions are needed for the rotation and for slot_pos");
   TS_REQUIRE(n_q > 0 && n_q % a.c.n_kv == 0, "bad head counts");
+  TS_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
   TS_REQUIRE(is_aligned(out, 4) && out_row_stride % 2 == 0, "rows of out must be 4-byte aligned");
   TS_REQUIRE(!accumulate || a.c.scores != nullptr, "the cache has no scores to accumulate into");
   if (a.c.batch == 0) return TS_OK;
   a.group = n_q / a.c.n_kv;
   a.head_tiles = (a.group + kHeads - 1) / kHeads;
   TS_UNSUPPORTED((int64_t)a.c.batch * a.c.n_kv * a.head_tiles <= (int64_t)kCounters, "too many heads in one call");
+  TS_UNSUPPORTED(((int64_t)a.c.max_pages * a.c.page_size / kUnit + 1 + kRowCost) * a.c.batch * a.c.n_kv * a.head_tiles <
+                     (int64_t)1 << 31,
+                 "too many slots in one call");
   const Layout L = attn_layout(*cache, n_q, accumulate != 0);
   if (workspace == nullptr || workspace_bytes < L.bytes) {
     set_error("workspace of %zu bytes, %zu needed", workspace_bytes, L.bytes);
