@@ -8,9 +8,12 @@
 // one 32-bit TMEM column holding the four scales of a row (nvfp4; two of the
 // four per instruction for mxfp4).
 //
-// A tile is 128 rows of b (the weight's output features; the MMA's M) x BT
-// rows of a (tokens; its N), K in stages of 256. Roles in one persistent CTA
-// per SM:
+// Two kernels: fp4_gemm_kernel for decode-sized calls and small layers,
+// fp4_pair_kernel (below) for prefill.
+//
+// fp4_gemm_kernel: a tile is 128 rows of b (the weight's output features; the
+// MMA's M) x BT <= 128 rows of a (tokens; its N), K in stages of 256. Roles in
+// one persistent CTA per SM:
 //   warp 0      TMA producer: codes of both operands (128-byte rows, 128-byte
 //               swizzle) and, as bulk copies, the scale tiles of the stage
 //   warp 1      one thread copies the stage's scale tiles to TMEM
@@ -19,11 +22,9 @@
 //               stage's columns are rewritten only after the MMAs that read
 //               them have released the stage.
 //   warps 2-5   epilogue: tcgen05.ld, tensor scales, bias, stores
-//
-// Decode-sized calls are bound by the weight's bytes, prefill by the tensor
-// cores. Few tokens make few tiles: their stages are laid end to end and each
-// CTA takes an equal share (split along K), partial sums being added by the
-// last CTA of a tile to arrive, in CTA order.
+// Bound by the weight's bytes. The tiles are few, so their stages are laid end
+// to end and each CTA takes an equal share (split along K); partial sums are
+// added by the last CTA of a tile to arrive, in CTA order.
 //
 // Every wait is bounded in wall-clock time: a role whose wait runs out records
 // a code and unwinds; the TMEM is freed at the end in any case.
@@ -52,15 +53,13 @@ struct GemmArgs {
   int64_t M, N;
   int wblocks, tblocks, kblocks;   // tiles of weight rows, of tokens, stages
   int kt, steps;                   // scale tiles along K, MMA steps of 64 columns
-  int x_tiles;                     // scale tiles along the tokens
   const void* bias;
   int bias_dtype;
   void* out;
   int out_dtype;
   int64_t out_stride;
-  int split;
-  int* counters;
-  float* partials;                 // split: [grid][2][128][BT]
+  int* counters;                   // one per tile, zero between calls
+  float* partials;                 // [grid][2][BT / 4][128][4]
   uint64_t wait_ns;
   int stall;                       // test hook: the producer issues nothing
 };
@@ -68,13 +67,11 @@ struct GemmArgs {
 template <bool NV, int BT>
 struct Shape {
   static constexpr int kTiles = NV ? 4 : 2;                    // scale tiles of a stage, per 128 rows
-  static constexpr int kXRowTiles = BT > 128 ? 2 : 1;
-  static constexpr int kSfA = kTiles * kTileBytes;
-  static constexpr int kSfB = kXRowTiles * kTiles * kTileBytes;
+  static constexpr int kSf = kTiles * kTileBytes;              // an operand's scales in a stage
   static constexpr int kXBytes = BT * 128;
-  static constexpr int kStage = kABytes + kXBytes + kSfA + kSfB;
-  static constexpr int kSfCols = 4 * kTiles * (1 + kXRowTiles);  // TMEM columns of a stage's scales
-  static constexpr int kAcc = BT <= 128 ? 2 : 1;               // accumulators
+  static constexpr int kStage = kABytes + kXBytes + 2 * kSf;
+  static constexpr int kSfCols = 8 * kTiles;                   // TMEM columns of a stage's scales
+  static constexpr int kAcc = 2;                               // accumulators
   static constexpr int kAccCols = BT < 32 ? 32 : BT;
   static constexpr int kFitTmem = (kTmemCols - kAcc * kAccCols) / kSfCols;
   static constexpr int kFitSmem = (227 * 1024 - 2048) / kStage;
@@ -93,12 +90,22 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 
-// Instruction descriptor: E2M1 operands, K-major, fp32 sums, M = 128 x N;
+// Instruction descriptor: E2M1 operands, K-major, fp32 sums, M x N;
 // sf: which of a column's scales the instruction starts from (mxfp4: 0 or 2).
 template <bool NV>
-__host__ __device__ constexpr uint32_t idesc_fp4(int N, uint32_t sf) {
+__host__ __device__ constexpr uint32_t idesc_fp4(int M, int N, uint32_t sf) {
   return (sf << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (NV ? 0u : 1u << 23) |
-         ((uint32_t)(kBW >> 7) << 27) | (sf << 29);
+         ((uint32_t)(M >> 7) << 27) | (sf << 29);
+}
+
+// One lane of a converged warp. Unlike `lane == 0` it tells the compiler that
+// the code behind it runs once per warp, and the descriptors of tensor-core
+// instructions then go to uniform registers without a loop over lanes (the
+// same kernel, 8192 x 28672 x 8192: 2035 us with lane == 0, 1284 us with this).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
 }
 
 template <bool NV>
@@ -120,40 +127,21 @@ __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint
 
 // Work items of a CTA: a tile and the stages [k0, k1) of it that are its own.
 struct Item {
-  int tile, k0, k1, slot;
+  int tile, k0, k1;
 };
 struct ItemIter {
   int64_t u, u1;
-  int64_t begin;
 };
 __device__ __forceinline__ ItemIter items_begin(const GemmArgs& a, int ntiles) {
-  ItemIter it;
-  if (a.split) {
-    const int64_t U = (int64_t)ntiles * a.kblocks;
-    it.u = U * blockIdx.x / gridDim.x;
-    it.u1 = U * (blockIdx.x + 1) / gridDim.x;
-  } else {
-    it.u = blockIdx.x;
-    it.u1 = ntiles;
-  }
-  it.begin = it.u;
-  return it;
+  const int64_t U = (int64_t)ntiles * a.kblocks;
+  return {U * blockIdx.x / gridDim.x, U * (blockIdx.x + 1) / gridDim.x};
 }
 __device__ __forceinline__ bool items_next(const GemmArgs& a, ItemIter& it, Item& x) {
   if (it.u >= it.u1) return false;
-  if (a.split) {
-    x.tile = (int)(it.u / a.kblocks);
-    x.k0 = (int)(it.u - (int64_t)x.tile * a.kblocks);
-    x.k1 = (int)min((int64_t)a.kblocks, x.k0 + (it.u1 - it.u));
-    x.slot = it.u == it.begin ? 0 : 1;
-    it.u += x.k1 - x.k0;
-  } else {
-    x.tile = (int)it.u;
-    x.k0 = 0;
-    x.k1 = a.kblocks;
-    x.slot = 0;
-    it.u += gridDim.x;
-  }
+  x.tile = (int)(it.u / a.kblocks);
+  x.k0 = (int)(it.u - (int64_t)x.tile * a.kblocks);
+  x.k1 = (int)min((int64_t)a.kblocks, x.k0 + (it.u1 - it.u));
+  it.u += x.k1 - x.k0;
   return true;
 }
 
@@ -168,8 +156,8 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
   char* s_w = smem;                                  // [S][128][128]
   char* s_x = s_w + S * kABytes;                     // [S][BT][128]
   char* s_sw = s_x + S * P::kXBytes;                 // [S][tiles][512]
-  char* s_sx = s_sw + S * P::kSfA;                   // [S][row tiles][tiles][512]
-  uint64_t* full = reinterpret_cast<uint64_t*>(s_sx + S * P::kSfB);
+  char* s_sx = s_sw + S * P::kSf;                    // the same of the tokens
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_sx + S * P::kSf);
   uint64_t* empty = full + S;
   uint64_t* tfull = empty + S;
   uint64_t* tempty = tfull + P::kAcc;
@@ -203,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0 && !a.stall) {
+    if (elect_one() && !a.stall) {
       int s = 0;
       uint32_t ph = 0;
       ItemIter it = items_begin(a, ntiles);
@@ -218,15 +206,13 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
             break;
           }
           const int t0 = kb * P::kTiles, nt = min(P::kTiles, a.kt - t0);
-          const int xt = min(P::kXRowTiles, a.x_tiles - tb * P::kXRowTiles);   // (BT < 128 has one token tile)
           const uint32_t sf_bytes = nt * kTileBytes;
-          mbar_arrive_expect_tx(full + s, kABytes + P::kXBytes + sf_bytes * (1 + xt));
+          mbar_arrive_expect_tx(full + s, kABytes + P::kXBytes + 2 * sf_bytes);
           tma_load_2d(s_w + s * kABytes, &wmap, kb * 128, wb * kBW, full + s);
           tma_load_2d(s_x + s * P::kXBytes, &xmap, kb * 128, tb * BT, full + s);
-          bulk_load(s_sw + s * P::kSfA, a.wscales + ((int64_t)wb * a.kt + t0) * kTileBytes, sf_bytes, full + s);
-          for (int r = 0; r < xt; ++r)
-            bulk_load(s_sx + s * P::kSfB + r * P::kSfA,
-                      a.xscales + ((int64_t)(tb * P::kXRowTiles + r) * a.kt + t0) * kTileBytes, sf_bytes, full + s);
+          bulk_load(s_sw + s * P::kSf, a.wscales + ((int64_t)wb * a.kt + t0) * kTileBytes, sf_bytes, full + s);
+          // (tb > 0 only with BT = 128: token tiles are scale tiles)
+          bulk_load(s_sx + s * P::kSf, a.xscales + ((int64_t)tb * a.kt + t0) * kTileBytes, sf_bytes, full + s);
           ++issued;
           if (++s == S) {
             s = 0;
@@ -243,7 +229,7 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint64_t wd0 = umma_desc_sw128(smem_u32(s_w)), xd0 = umma_desc_sw128(smem_u32(s_x));
       const uint64_t swd0 = desc_scales(smem_u32(s_sw)), sxd0 = desc_scales(smem_u32(s_sx));
       const uint32_t sf0 = tmem + P::kAcc * P::kAccCols;
@@ -265,19 +251,17 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
           const uint32_t sfa = sf0 + s * P::kSfCols, sfb = sfa + 4 * P::kTiles;
           const int nt = min(P::kTiles, a.kt - kb * P::kTiles);
           for (int t = 0; t < nt; ++t) {
-            copy_scales(sfa + 4 * t, swd0 + (uint64_t)((s * P::kSfA + t * kTileBytes) >> 4));
-#pragma unroll
-            for (int r = 0; r < P::kXRowTiles; ++r)
-              copy_scales(sfb + 4 * (t * P::kXRowTiles + r),
-                          sxd0 + (uint64_t)((s * P::kSfB + r * P::kSfA + t * kTileBytes) >> 4));
+            const uint64_t at = (uint64_t)((s * P::kSf + t * kTileBytes) >> 4);
+            copy_scales(sfa + 4 * t, swd0 + at);
+            copy_scales(sfb + 4 * t, sxd0 + at);
           }
           const int nk = min(kBK / kColPad, a.steps - kb * (kBK / kColPad));
           const uint64_t wd = wd0 + (uint64_t)((s * kABytes) >> 4), xd = xd0 + (uint64_t)((s * P::kXBytes) >> 4);
           for (int k = 0; k < nk; ++k) {
             const int t = NV ? k : k >> 1;
             const uint32_t sf = NV ? 0u : (uint32_t)(k & 1) * 2;
-            mma_fp4<NV>(d, wd + 2 * k, xd + 2 * k, idesc_fp4<NV>(BT, sf), sfa + 4 * t,
-                        sfb + 4 * t * P::kXRowTiles, (kb != x.k0 || k != 0) ? 1u : 0u);
+            mma_fp4<NV>(d, wd + 2 * k, xd + 2 * k, idesc_fp4<NV>(kBW, BT, sf), sfa + 4 * t,
+                        sfb + 4 * t, (kb != x.k0 || k != 0) ? 1u : 0u);
           }
           umma_commit(empty + s);
           if (++s == S) {
@@ -312,7 +296,7 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
       const bool valid = n < a.N;
       const bool whole = x.k0 == 0 && x.k1 == a.kblocks;
       const int jn_all = (int)min((int64_t)BT, a.M - m0);
-      float* pp = whole ? nullptr : a.partials + ((size_t)blockIdx.x * 2 + x.slot) * (BT * kBW);
+      float* pp = whole ? nullptr : a.partials + ((size_t)blockIdx.x * 2 + (x.k0 > 0 ? 0 : 1)) * (BT * kBW);
       const float bias = a.bias && valid ? load_f(a.bias, a.bias_dtype, n) : 0.f;
       const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * P::kAccCols;
 #pragma unroll 1
@@ -325,9 +309,11 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
           mbar_arrive(tempty + buf);
         }
         if (!whole) {
-          float4* dst = reinterpret_cast<float4*>(pp + (size_t)r * BT + c * CW);
+          // a piece: [BT / 4 tokens][128 rows][4 tokens], coalesced both ways
+          float4* dst = reinterpret_cast<float4*>(pp) + (size_t)(c * CW / 4) * kBW + r;
 #pragma unroll
-          for (int j = 0; j < CW / 4; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          for (int j = 0; j < CW / 4; ++j)
+            if (c * CW + 4 * j < jn_all) dst[j * kBW] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           continue;
         }
         if (!valid) continue;
@@ -343,9 +329,12 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
       }
       if (whole) continue;
       // a tile split over several CTAs: the last to arrive adds the pieces
-      __threadfence();
       named_bar_sync(3, kEpiWarps * 32);
-      if (r == 0) *epi_flag = atomicAdd(a.counters + x.tile, 1);
+      if (r == 0) {
+        __threadfence();                               // the CTA's piece, before its arrival
+        *epi_flag = atomicAdd(a.counters + x.tile, 1);
+        __threadfence();
+      }
       named_bar_sync(3, kEpiWarps * 32);
       const int64_t U = (int64_t)ntiles * a.kblocks;
       const int G = gridDim.x;
@@ -354,33 +343,36 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
       const int old = *epi_flag;
       named_bar_sync(3, kEpiWarps * 32);
       if (old != c_last - c_first) continue;
-      __threadfence();
       if (r == 0) a.counters[x.tile] = 0;
       if (!valid) continue;
-      constexpr int RT = 16;
-      for (int j0 = 0; j0 < jn_all; j0 += RT) {
-        float sum[RT];
+      // the tile's beginning lies in its CTA's second slot, the other pieces
+      // in their CTAs' first; 16 tokens of 4 pieces in flight
+      constexpr int kPiece4 = BT * kBW / 4;
+      const float4* base = reinterpret_cast<const float4*>(a.partials) + (size_t)c_first * 2 * kPiece4 + r;
+      const int pieces = c_last - c_first + 1;
+      for (int j0 = 0; j0 < jn_all; j0 += 16) {
+        float4 sum[4];
 #pragma unroll
-        for (int u = 0; u < RT; ++u) sum[u] = 0.f;
-        for (int c = c_first; c <= c_last; ++c) {
-          const int slot = U * c / G >= u_lo ? 0 : 1;
-          const float4* src =
-              reinterpret_cast<const float4*>(a.partials + ((size_t)c * 2 + slot) * (BT * kBW) + (size_t)r * BT + j0);
-          float4 t[RT / 4];
+        for (int u = 0; u < 4; ++u) sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int c = 0; c < pieces; ++c) {
+          const float4* src = base + (c == 0 ? (size_t)kPiece4 : (size_t)c * 2 * kPiece4) + (size_t)(j0 / 4) * kBW;
 #pragma unroll
-          for (int u = 0; u < RT / 4; ++u) t[u] = __ldcg(src + u);
-#pragma unroll
-          for (int u = 0; u < RT / 4; ++u) {
-            sum[4 * u] += t[u].x;
-            sum[4 * u + 1] += t[u].y;
-            sum[4 * u + 2] += t[u].z;
-            sum[4 * u + 3] += t[u].w;
+          for (int u = 0; u < 4; ++u) {
+            if (j0 + 4 * u < jn_all) {
+              const float4 t = __ldcg(src + u * kBW);
+              sum[u].x += t.x;
+              sum[u].y += t.y;
+              sum[u].z += t.z;
+              sum[u].w += t.w;
+            }
           }
         }
+        const float* f = reinterpret_cast<const float*>(sum);
 #pragma unroll
-        for (int u = 0; u < RT; ++u)
+        for (int u = 0; u < 16; ++u)
           if (j0 + u < jn_all)
-            store_f(a.out, a.out_dtype, (m0 + j0 + u) * a.out_stride + n, fmaf(sum[u], alpha, bias));
+            store_f(a.out, a.out_dtype, (m0 + j0 + u) * a.out_stride + n, fmaf(f[u], alpha, bias));
       }
     }
   }
@@ -393,23 +385,391 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
   }
 }
 
+// ---- prefill: tiles of 256 tokens x 256 weight rows on CTA pairs ------------------
+//
+// Two CTAs of a cluster share one MMA (cta_group::2, M = 256): each holds its
+// 128 token rows of A, half of B's rows and the accumulator of its own
+// tokens, so every operand byte is fetched by one of the two and feeds both
+// tensor cores; a stage of 256 columns brings 38 KB per CTA for 128 x BN x 256
+// products where a lone CTA's 128 x 256 tile needs 54 KB. Loads of both CTAs
+// complete on the leader's barrier; the leader's thread issues scale copies
+// and MMAs for both; commits release the stage in both. Tokens are the
+// accumulator's lanes, so that a thread stores runs of its token's outputs.
+
+constexpr int BN = 256;
+
+template <bool NV>
+struct Pair {
+  static constexpr int kTiles = NV ? 4 : 2;                    // scale tiles of a stage, per 128 rows
+  static constexpr int kRowTiles = BN / 128;
+  static constexpr int kBBytes = BN / 2 * 128;
+  static constexpr int kSfA = kTiles * kTileBytes;
+  static constexpr int kSfB = kRowTiles * kSfA;
+  static constexpr int kStage = kABytes + kBBytes + kSfA + kSfB;
+  static constexpr int kSfCols = 4 * kTiles * (1 + kRowTiles);
+  static constexpr int kFitTmem = (kTmemCols - BN) / kSfCols;
+  static constexpr int kFitSmem = (227 * 1024 - 2048) / kStage;
+  static constexpr int S = kFitTmem < kFitSmem ? kFitTmem : kFitSmem;
+  static constexpr size_t kSmem = 1024 + (size_t)S * kStage + (2 * S + 3) * 8 + 16;
+};
+
+struct PairArgs {
+  const float* wg;
+  const float* xg;
+  int64_t M, N;
+  int mblocks, nblocks, kblocks;
+  int kt, steps;
+  const void* bias;
+  int bias_dtype;
+  void* out;
+  int out_dtype;
+  int64_t out_stride;
+  int vec;                         // rows of out take 16-byte stores
+  uint64_t wait_ns;
+  int stall;
+};
+
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address of the same shared-memory location in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+// TMA tile load into this CTA's shared memory, completing on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void copy_scales_pair(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+template <bool NV>
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+  if (NV)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+template <bool NV>
+__global__ void __launch_bounds__(kThreads) __cluster_dims__(2, 1, 1)
+    fp4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                    const __grid_constant__ CUtensorMap asmap, const __grid_constant__ CUtensorMap bsmap,
+                    const PairArgs a) {
+  using P = Pair<NV>;
+  constexpr int S = P::S;
+  extern __shared__ char smem_raw[];
+  // both CTAs have one layout: the dynamic area starts at the same address in each
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  char* s_a = smem;
+  char* s_b = s_a + S * kABytes;
+  char* s_sa = s_b + S * P::kBBytes;
+  char* s_sb = s_sa + S * P::kSfA;
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_sb + S * P::kSfB);
+  uint64_t* empty = full + S;
+  uint64_t* tfull = empty + S;
+  uint64_t* tempty = tfull + 1;
+  uint64_t* drain = tempty + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int ntiles = a.mblocks * a.nblocks;
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&amap);
+    prefetch_tensormap(&bmap);
+    prefetch_tensormap(&asmap);
+    prefetch_tensormap(&bsmap);
+    for (int i = 0; i < S; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(tfull, 1);
+    mbar_init(tempty, 2 * kEpiWarps);
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (elect_one() && !a.stall) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < ntiles; tile += pairs) {
+        const int mb = tile % a.mblocks, nb = tile / a.mblocks;
+        const int arow = mb * 256 + (int)rank * 128, brow = nb * BN + (int)rank * (BN / 2);
+        const int at = (mb * 2 + (int)rank) * a.kt, bt = nb * P::kRowTiles * a.kt;
+        for (int kb = 0; kb < a.kblocks; ++kb) {
+          if (!mbar_wait_hint(empty + s, ph ^ 1, &g_err, 31, a.wait_ns)) {
+            ok = false;
+            break;
+          }
+          // both CTAs' copies count on the leader's barrier
+          const uint32_t bar = map_cta(smem_u32(full + s), 0);
+          if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * P::kStage);
+          tma_load_pair(smem_u32(s_a + s * kABytes), &amap, kb * 128, arow, bar);
+          tma_load_pair(smem_u32(s_b + s * P::kBBytes), &bmap, kb * 128, brow, bar);
+          // scale tiles are rows of 512 bytes; tiles behind a row's end are
+          // loaded too (of the next row, or zeros) and not used
+          tma_load_pair(smem_u32(s_sa + s * P::kSfA), &asmap, 0, at + kb * P::kTiles, bar);
+#pragma unroll
+          for (int r = 0; r < P::kRowTiles; ++r)
+            tma_load_pair(smem_u32(s_sb + s * P::kSfB + r * P::kSfA), &bsmap, 0, bt + r * a.kt + kb * P::kTiles, bar);
+          if (++s == S) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      // every stage has been released to this CTA before it ends; after a
+      // timeout, the copies in flight have landed
+      for (int i = 0; i < S; ++i) {
+        if (ok) {
+          if (!mbar_wait_hint(empty + s, ph ^ 1, &g_err, 35, a.wait_ns)) break;
+        } else if (rank == 0) {
+          mbar_wait_hint(full + s, ph ^ 1, nullptr, 0, a.wait_ns);
+        }
+        if (++s == S) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank != 0) {
+      // the last commit reaches this CTA's barrier too: it stays until then
+      if (elect_one()) mbar_wait_hint(drain, 0, nullptr, 0, a.wait_ns);
+    } else if (elect_one()) {
+      const uint64_t ad0 = umma_desc_sw128(smem_u32(s_a)), bd0 = umma_desc_sw128(smem_u32(s_b));
+      const uint64_t sad0 = desc_scales(smem_u32(s_sa)), sbd0 = desc_scales(smem_u32(s_sb));
+      const uint32_t sf0 = tmem + BN;
+      int s = 0, n = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < ntiles; tile += pairs, ++n) {
+        if (!mbar_wait_hint(tempty, (n & 1) ^ 1, &g_err, 32, a.wait_ns)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < a.kblocks; ++kb) {
+          if (!mbar_wait_hint(full + s, ph, &g_err, 33, a.wait_ns)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sfa = sf0 + s * P::kSfCols, sfb = sfa + 4 * P::kTiles;
+#pragma unroll
+          for (int t = 0; t < P::kTiles; ++t) {
+            copy_scales_pair(sfa + 4 * t, sad0 + (uint64_t)((s * P::kSfA + t * kTileBytes) >> 4));
+#pragma unroll
+            for (int r = 0; r < P::kRowTiles; ++r)
+              copy_scales_pair(sfb + 4 * (t * P::kRowTiles + r),
+                               sbd0 + (uint64_t)((s * P::kSfB + r * P::kSfA + t * kTileBytes) >> 4));
+          }
+          const int nk = min(kBK / kColPad, a.steps - kb * (kBK / kColPad));
+          const uint64_t ad = ad0 + (uint64_t)((s * kABytes) >> 4), bd = bd0 + (uint64_t)((s * P::kBBytes) >> 4);
+#pragma unroll
+          for (int k = 0; k < kBK / kColPad; ++k) {
+            if (k < nk) {
+              const int t = NV ? k : k >> 1;
+              const uint32_t sf = NV ? 0u : (uint32_t)(k & 1) * 2;
+              mma_pair<NV>(tmem, ad + 2 * k, bd + 2 * k, idesc_fp4<NV>(256, BN, sf), sfa + 4 * t,
+                           sfb + 4 * t * P::kRowTiles, (kb != 0 || k != 0) ? 1u : 0u);
+            }
+          }
+          commit_pair(empty + s);
+          if (++s == S) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (ok) commit_pair(tfull);
+      }
+      // every MMA issued has finished before the TMEM is freed
+      commit_pair(drain);
+      mbar_wait_hint(drain, 0, nullptr, 0, a.wait_ns);
+    }
+  } else {
+    const int quad = warp & 3;
+    const float alpha = usable_scale(a.wg) * usable_scale(a.xg);
+    const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t free_bar = map_cta(smem_u32(tempty), 0);
+    int n = 0;
+    for (int tile = pair; tile < ntiles; tile += pairs, ++n) {
+      const int64_t m = (int64_t)(tile % a.mblocks) * 256 + rank * 128 + quad * 32 + lane;
+      const int64_t n0 = (int64_t)(tile / a.mblocks) * BN;
+      const int cols = (int)min((int64_t)BN, a.N - n0);
+      const bool got = mbar_wait_hint(tfull, n & 1, &g_err, 34, a.wait_ns);
+      if (!__all_sync(0xffffffffu, got)) break;
+      tc_fence_after();
+      if (a.out_dtype == TS_F32) {
+        float* row = reinterpret_cast<float*>(a.out) + m * a.out_stride + n0;
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          float v[32];
+          tmem_ld32(acc + c * 32, v);
+          if (c == BN / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(free_bar);
+          }
+          if (m >= a.M) continue;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int col = c * 32 + j;
+            if (col < cols) row[col] = fmaf(v[j], alpha, a.bias ? load_f(a.bias, a.bias_dtype, n0 + col) : 0.f);
+          }
+        }
+        continue;
+      }
+      // 16-bit outputs wait in registers, so that the accumulator is free
+      // again before the first of them is stored
+      uint32_t w[BN / 2];
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) {
+        float v[32];
+        tmem_ld32(acc + c * 32, v);
+        if (a.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int col = c * 32 + j;
+            v[j] = fmaf(v[j], alpha, col < cols ? load_f(a.bias, a.bias_dtype, n0 + col) : 0.f);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= alpha;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (a.out_dtype == TS_BF16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            w[c * 16 + j] = *reinterpret_cast<const uint32_t*>(&h);
+          } else {
+            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            w[c * 16 + j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(free_bar);
+      if (m >= a.M) continue;
+      uint16_t* row = reinterpret_cast<uint16_t*>(a.out) + m * a.out_stride + n0;
+      if (a.vec) {
+#pragma unroll
+        for (int i = 0; i < BN / 8; ++i)
+          if (i * 8 < cols)   // N is a multiple of 8 here
+            *reinterpret_cast<uint4*>(row + i * 8) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < BN / 2; ++i) {
+          if (2 * i < cols) row[2 * i] = (uint16_t)w[i];
+          if (2 * i + 1 < cols) row[2 * i + 1] = (uint16_t)(w[i] >> 16);
+        }
+      }
+    }
+  }
+
+  // neither CTA leaves, nor frees TMEM, while the other's copies, MMAs or
+  // arrivals may still reach it
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
 // ---- host -------------------------------------------------------------------
 
 struct Plan {
+  bool pair;        // CTA pairs on tiles of 256 tokens x 256 weight rows
   int BT, tblocks, wblocks, kblocks, ntiles, grid;
-  bool split;
 };
 
 static Plan plan(int64_t M, int64_t N, int64_t K) {
-  Plan p;
-  p.BT = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  Plan p{};
+  const int sms = sm_count(), pairs = sms / 2;
+  p.kblocks = (int)((padded_cols(K) + kBK - 1) / kBK);
+  const int64_t mb = (M + 255) / 256, nb = (N + BN - 1) / BN;
+  if (M > 128 && mb * nb * 2 >= pairs) {
+    p.pair = true;
+    p.tblocks = (int)mb;
+    p.wblocks = (int)nb;
+    p.ntiles = (int)(mb * nb);
+    p.grid = 2 * (int)std::min<int64_t>(mb * nb, pairs);
+    return p;
+  }
+  p.BT = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   p.wblocks = (int)((N + kBW - 1) / kBW);
   p.tblocks = (int)((M + p.BT - 1) / p.BT);
-  p.kblocks = (int)((padded_cols(K) + kBK - 1) / kBK);
   p.ntiles = p.wblocks * p.tblocks;
-  p.split = p.BT <= 128;
-  p.grid = (int)std::min<int64_t>(p.split ? (int64_t)p.ntiles * p.kblocks : p.ntiles, sm_count());
+  p.grid = (int)std::min<int64_t>((int64_t)p.ntiles * p.kblocks, sms);
   return p;
+}
+
+template <bool NV>
+static int launch_pair(const CUtensorMap (&m)[4], const PairArgs& a, int grid, cudaStream_t st) {
+  auto k = fp4_pair_kernel<NV>;
+  constexpr size_t smem = Pair<NV>::kSmem;
+  static_assert(smem <= 227 * 1024, "shared memory");
+  static thread_local int configured_dev = -1;
+  int dev = 0;
+  TS_CUDA_TRY(cudaGetDevice(&dev));
+  if (configured_dev != dev) {
+    TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    configured_dev = dev;
+  }
+  k<<<grid, kThreads, smem, st>>>(m[0], m[1], m[2], m[3], a);
+  TS_LAUNCH_CHECK();
+  return TS_OK;
+}
+
+// Tensor map of a tensor's scale tiles: rows of 512 bytes, boxes of the tiles of a stage.
+static int scale_map(CUtensorMap* map, const ts_fp4_tensor& t) {
+  const uint64_t rows = (uint64_t)((t.rows + kTileRows - 1) / kTileRows) * scale_tiles(t.cols, t.format);
+  return encode_tmap_2d(map, t.scales, CU_TENSOR_MAP_DATA_TYPE_UINT16, kTileBytes / 2, rows, kTileBytes, kTileBytes / 2,
+                        kBK / block_of(t.format) / 4, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 template <bool NV, int BT>
@@ -435,8 +795,7 @@ static int launch(int BT, const CUtensorMap& wm, const CUtensorMap& xm, const Ge
     case 16: return launch<NV, 16>(wm, xm, a, grid, st);
     case 32: return launch<NV, 32>(wm, xm, a, grid, st);
     case 64: return launch<NV, 64>(wm, xm, a, grid, st);
-    case 128: return launch<NV, 128>(wm, xm, a, grid, st);
-    default: return launch<NV, 256>(wm, xm, a, grid, st);
+    default: return launch<NV, 128>(wm, xm, a, grid, st);
   }
 }
 
@@ -451,7 +810,7 @@ extern "C" size_t ts_fp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K, 
   (void)format;
   if (M <= 0 || N <= 0 || K <= 0) return paged::kCounterBytes;
   const Plan p = plan(M, N, K);
-  return paged::kCounterBytes + (p.split ? (size_t)p.grid * 2 * kBW * p.BT * 4 : 0);
+  return paged::kCounterBytes + (!p.pair ? (size_t)p.grid * 2 * kBW * p.BT * 4 : 0);
 }
 
 extern "C" int ts_fp4_matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, const void* bias, int bias_dtype, void* out,
@@ -470,36 +829,69 @@ extern "C" int ts_fp4_matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, con
   TS_REQUIRE(out, "NULL pointer");
   const Plan p = plan(x->rows, w->rows, w->cols);
   const size_t need = ts_fp4_matmul_workspace_size(x->rows, w->rows, w->cols, w->format);
-  if (p.split && (workspace == nullptr || workspace_bytes < need)) {
+  if (!p.pair && (workspace == nullptr || workspace_bytes < need)) {
     set_error("workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return TS_ERR_WORKSPACE;
   }
   TS_REQUIRE(is_aligned(workspace, 16), "workspace must be 16-byte aligned");
-  TS_UNSUPPORTED(!p.split || p.ntiles <= (int)paged::kCounters, "too many output features in one call");
+  TS_UNSUPPORTED(p.pair || p.ntiles <= (int)paged::kCounters, "too many output features in one call");
+  const float* wg = w->format == TS_NVFP4 ? w->global_scale : nullptr;
+  const float* xg = x->format == TS_NVFP4 ? x->global_scale : nullptr;
+  const int kt = (int)scale_tiles(w->cols, w->format), steps = (int)(padded_cols(w->cols) / kColPad);
+  const uint64_t row = (uint64_t)padded_cols(w->cols) / 2;
+  const int stall = take_test_stall() ? 1 : 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p.pair) {
+    PairArgs a;
+    a.wg = wg;
+    a.xg = xg;
+    a.M = x->rows;
+    a.N = w->rows;
+    a.mblocks = p.tblocks;
+    a.nblocks = p.wblocks;
+    a.kblocks = p.kblocks;
+    a.kt = kt;
+    a.steps = steps;
+    a.bias = bias;
+    a.bias_dtype = bias_dtype;
+    a.out = out;
+    a.out_dtype = out_dtype;
+    a.out_stride = out_row_stride;
+    a.vec = w->rows % 8 == 0 && out_row_stride % 8 == 0 && is_aligned(out, 16);
+    a.wait_ns = wait_limit_ns();
+    a.stall = stall;
+    CUtensorMap m[4];
+    rc = encode_tmap_2d(&m[0], x->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)x->rows, row, 128, 128,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TS_OK)
+      rc = encode_tmap_2d(&m[1], w->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)w->rows, row, 128, BN / 2,
+                          CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TS_OK) rc = scale_map(&m[2], *x);
+    if (rc == TS_OK) rc = scale_map(&m[3], *w);
+    if (rc != TS_OK) return rc;
+    return w->format == TS_NVFP4 ? launch_pair<true>(m, a, p.grid, st) : launch_pair<false>(m, a, p.grid, st);
+  }
   GemmArgs a;
   a.wscales = w->scales;
   a.xscales = x->scales;
-  a.wg = w->format == TS_NVFP4 ? w->global_scale : nullptr;
-  a.xg = x->format == TS_NVFP4 ? x->global_scale : nullptr;
+  a.wg = wg;
+  a.xg = xg;
   a.M = x->rows;
   a.N = w->rows;
   a.wblocks = p.wblocks;
   a.tblocks = p.tblocks;
   a.kblocks = p.kblocks;
-  a.kt = (int)scale_tiles(w->cols, w->format);
-  a.steps = (int)(padded_cols(w->cols) / kColPad);
-  a.x_tiles = (int)((x->rows + kTileRows - 1) / kTileRows);
+  a.kt = kt;
+  a.steps = steps;
   a.bias = bias;
   a.bias_dtype = bias_dtype;
   a.out = out;
   a.out_dtype = out_dtype;
   a.out_stride = out_row_stride;
-  a.split = p.split ? 1 : 0;
   a.counters = reinterpret_cast<int*>(workspace);
-  a.partials = p.split ? reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + paged::kCounterBytes) : nullptr;
+  a.partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + paged::kCounterBytes);
   a.wait_ns = wait_limit_ns();
-  a.stall = take_test_stall() ? 1 : 0;
-  const uint64_t row = (uint64_t)padded_cols(w->cols) / 2;
+  a.stall = stall;
   CUtensorMap wm, xm;
   rc = encode_tmap_2d(&wm, w->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)w->rows, row, 128, kBW,
                       CU_TENSOR_MAP_SWIZZLE_128B);
@@ -507,7 +899,6 @@ extern "C" int ts_fp4_matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, con
   rc = encode_tmap_2d(&xm, x->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)x->rows, row, 128, p.BT,
                       CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != TS_OK) return rc;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return w->format == TS_NVFP4 ? launch<true>(p.BT, wm, xm, a, p.grid, st) : launch<false>(p.BT, wm, xm, a, p.grid, st);
 }
 

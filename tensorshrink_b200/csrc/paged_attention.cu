@@ -222,10 +222,10 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
 
   const unsigned total = (unsigned)prefix[c.batch] * rows_per_b;   // (the host keeps it below 2^31)
   if (total == 0) return;
-  // as many CTAs as get a whole unit each, unless that cut the longest row
-  // into more pieces than its join takes in its stride
-  const unsigned n_cta = max(1u, min(min(gridDim.x, total / (front + 1)),
-                                     (unsigned)min((float)kMaxPieces * total / longest, 1e6f)));
+  // as many CTAs as get a whole unit each, but none with less than 1 / kMaxPieces
+  // of the longest row: a row is then cut into at most kMaxPieces + 1 pieces
+  const unsigned least = max(front + 1, (longest + kMaxPieces - 1) / kMaxPieces);
+  const unsigned n_cta = max(1u, min(gridDim.x, total / least));
   if (blockIdx.x >= n_cta) return;
   const Shares shares(total, n_cta);
   const unsigned u1 = shares.begin(blockIdx.x + 1);
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
       }
       __syncthreads();
       if (is_last) {
-        const int pieces = cta1 - cta0 + 1;          // at most kMaxPieces + 2
+        const int pieces = cta1 - cta0 + 1;          // at most kMaxPieces + 1
         // a row's pieces lie first in their CTAs' slots, but for its beginning
         const float* begun = a.partials + ((int64_t)cta0 * 2 + 1) * prow;
         const float* others = a.partials + (int64_t)cta0 * 2 * prow;

@@ -202,7 +202,24 @@ def test_product(ts, fmt, m, n, k):
                   bias.to(torch.bfloat16), k)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 4096, 14336), (2048, 1024, 4096)])
+# enough tiles for CTA pairs, with edges in every direction
+PAIRS = [(200, 9500, 320), (257, 5000, 1088), (1000, 2561, 576), (129, 19000, 64), (600, 3200, 2000),
+         (130, 16576, 256), (512, 8288, 640), (400, 8100, 1344), (256, 16500, 832)]
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m,n,k", PAIRS)
+def test_product_on_pairs(ts, fmt, m, n, k):
+    a = ts.fp4_quantize(data(m, k, torch.bfloat16, m + k), fmt)
+    b = ts.fp4_quantize(data(n, k, torch.float32, n), fmt)
+    bias = torch.randn(n, device="cuda").to(torch.float16)
+    va, vb = values64(a), values64(b)
+    for dt in (torch.float32, torch.bfloat16):
+        check_product(ts.fp4_matmul(a, b, out_dtype=dt), va, vb, None, k)
+    check_product(ts.fp4_matmul(a, b, bias=bias, out_dtype=torch.float16), va, vb, bias, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 14336), (2048, 1024, 4096), (2047, 14336, 4096), (2048, 4096, 14336)])
 def test_product_of_large_shapes(ts, m, n, k):
     a, b = ts.fp4_quantize(data(m, k, torch.bfloat16, 1)), ts.fp4_quantize(data(n, k, torch.bfloat16, 2))
     check_product(ts.fp4_matmul(a, b, out_dtype=torch.float32), values64(a), values64(b), None, k)
@@ -309,11 +326,12 @@ def test_refusals(ts):
             bad()
 
 
-def test_stalled_product_reports_and_recovers(ts):
+@pytest.mark.parametrize("m", [1, 200])
+def test_stalled_product_reports_and_recovers(ts, m):
     """A launch whose producer issues nothing: its waits run out, the status
     says so, and the same workspace serves the next call."""
     from tensorshrink_b200 import _C, kernels
-    a, b = ts.fp4_quantize(data(1, 4096, torch.bfloat16, 1)), ts.fp4_quantize(data(2000, 4096, torch.bfloat16, 2))
+    a, b = ts.fp4_quantize(data(m, 1024, torch.bfloat16, 1)), ts.fp4_quantize(data(9500, 1024, torch.bfloat16, 2))
     want = ts.fp4_matmul(a, b)
     kernels.device_status()
     assert _C.load().ts_test_inject_stall(1_000_000) == 0
