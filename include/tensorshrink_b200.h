@@ -390,7 +390,8 @@ typedef struct ts_fp4_tensor {
  *   s = 2^(floor(log2 max|block|) - 2), at least 2^-127;  e2m1(x / s)
  * A block that holds an infinity or a NaN gets a NaN scale and zero codes.
  * A given g outside [2^-100, 2^118] counts as the nearer bound, a NaN as the
- * lower. workspace: ts_fp4_quantize_workspace_size() bytes when find_scale is set.
+ * lower. workspace (as of ts_paged_decode_attention): needed when find_scale is
+ * set, ts_fp4_quantize_workspace_size() bytes.
  */
 TS_API size_t ts_fp4_scales_bytes(int64_t rows, int64_t cols, int format);
 TS_API size_t ts_fp4_quantize_workspace_size(void);

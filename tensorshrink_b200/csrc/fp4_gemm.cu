@@ -62,6 +62,7 @@ struct GemmArgs {
   float* partials;                 // [grid][2][BT / 4][128][4]
   uint64_t wait_ns;
   int stall;                       // test hook: the producer issues nothing
+  int overlap;                     // launched while the quantisation of x may still run
 };
 
 template <bool NV, int BT>
@@ -146,7 +147,7 @@ __device__ __forceinline__ bool items_next(const GemmArgs& a, ItemIter& it, Item
 }
 
 template <bool NV, int BT>
-__global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constant__ CUtensorMap wmap,
+__global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_constant__ CUtensorMap wmap,
                                                             const __grid_constant__ CUtensorMap xmap,
                                                             const GemmArgs a) {
   using P = Shape<NV, BT>;
@@ -191,28 +192,44 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (elect_one() && !a.stall) {
-      int s = 0;
+    if (elect_one()) {
+      auto load_w = [&](const Item& x, int kb, int s) {
+        const int wb = x.tile / a.tblocks, t0 = kb * P::kTiles;
+        const uint32_t sf_bytes = min(P::kTiles, a.kt - t0) * kTileBytes;
+        mbar_arrive_expect_tx(full + s, kABytes + P::kXBytes + 2 * sf_bytes);
+        tma_load_2d(s_w + s * kABytes, &wmap, kb * 128, wb * kBW, full + s);
+        bulk_load(s_sw + s * P::kSf, a.wscales + ((int64_t)wb * a.kt + t0) * kTileBytes, sf_bytes, full + s);
+      };
+      auto load_x = [&](const Item& x, int kb, int s) {
+        const int tb = x.tile % a.tblocks, t0 = kb * P::kTiles;
+        const uint32_t sf_bytes = min(P::kTiles, a.kt - t0) * kTileBytes;
+        tma_load_2d(s_x + s * P::kXBytes, &xmap, kb * 128, tb * BT, full + s);
+        // (tb > 0 only with BT = 128: token tiles are scale tiles)
+        bulk_load(s_sx + s * P::kSf, a.xscales + ((int64_t)tb * a.kt + t0) * kTileBytes, sf_bytes, full + s);
+      };
+      // The weight's first S stages are loaded while the kernel that writes
+      // the tokens' codes may still run; everything else follows its end.
+      const int ahead = a.stall ? 0 : (int)min((int64_t)S, items_begin(a, ntiles).u1 - items_begin(a, ntiles).u);
+      int s = 0, issued = 0;
       uint32_t ph = 0;
-      ItemIter it = items_begin(a, ntiles);
+      bool ok = !a.stall;
       Item x;
-      bool ok = true;
-      int issued = 0;
+      ItemIter it = items_begin(a, ntiles);
+      while (issued < ahead && items_next(a, it, x))
+        for (int kb = x.k0; kb < x.k1 && issued < ahead; ++kb) load_w(x, kb, issued++);
+      pdl_wait_primary();
+      issued = 0;
+      it = items_begin(a, ntiles);
       while (ok && items_next(a, it, x)) {
-        const int tb = x.tile % a.tblocks, wb = x.tile / a.tblocks;
         for (int kb = x.k0; kb < x.k1; ++kb) {
-          if (!mbar_wait_hint(empty + s, ph ^ 1, &g_err, 21, a.wait_ns)) {
-            ok = false;
-            break;
+          if (issued >= ahead) {
+            if (!mbar_wait_hint(empty + s, ph ^ 1, &g_err, 21, a.wait_ns)) {
+              ok = false;
+              break;
+            }
+            load_w(x, kb, s);
           }
-          const int t0 = kb * P::kTiles, nt = min(P::kTiles, a.kt - t0);
-          const uint32_t sf_bytes = nt * kTileBytes;
-          mbar_arrive_expect_tx(full + s, kABytes + P::kXBytes + 2 * sf_bytes);
-          tma_load_2d(s_w + s * kABytes, &wmap, kb * 128, wb * kBW, full + s);
-          tma_load_2d(s_x + s * P::kXBytes, &xmap, kb * 128, tb * BT, full + s);
-          bulk_load(s_sw + s * P::kSf, a.wscales + ((int64_t)wb * a.kt + t0) * kTileBytes, sf_bytes, full + s);
-          // (tb > 0 only with BT = 128: token tiles are scale tiles)
-          bulk_load(s_sx + s * P::kSf, a.xscales + ((int64_t)tb * a.kt + t0) * kTileBytes, sf_bytes, full + s);
+          load_x(x, kb, s);
           ++issued;
           if (++s == S) {
             s = 0;
@@ -354,17 +371,25 @@ __global__ void __launch_bounds__(kThreads) fp4_gemm_kernel(const __grid_constan
         float4 sum[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int c = 0; c < pieces; ++c) {
-          const float4* src = base + (c == 0 ? (size_t)kPiece4 : (size_t)c * 2 * kPiece4) + (size_t)(j0 / 4) * kBW;
+        for (int c = 0; c < pieces; c += 4) {
+          // (tokens behind the last one were not written: read, never stored)
+          float4 t[4][4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (j0 + 4 * u < jn_all) {
-              const float4 t = __ldcg(src + u * kBW);
-              sum[u].x += t.x;
-              sum[u].y += t.y;
-              sum[u].z += t.z;
-              sum[u].w += t.w;
+          for (int i = 0; i < 4; ++i) {
+            const int cc = min(c + i, pieces - 1);
+            const float4* src = base + (cc == 0 ? (size_t)kPiece4 : (size_t)cc * 2 * kPiece4) + (size_t)(j0 / 4) * kBW;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) t[i][u] = __ldcg(src + u * kBW);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (c + i >= pieces) break;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              sum[u].x += t[i][u].x;
+              sum[u].y += t[i][u].y;
+              sum[u].z += t[i][u].z;
+              sum[u].w += t[i][u].w;
             }
           }
         }
@@ -426,7 +451,7 @@ struct PairArgs {
   int64_t out_stride;
   int vec;                         // rows of out take 16-byte stores
   uint64_t wait_ns;
-  int stall;
+  int stall, overlap;
 };
 
 __device__ __forceinline__ uint32_t cta_rank() {
@@ -532,7 +557,9 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(2, 1, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (elect_one() && !a.stall) {
+    const bool leads = elect_one();
+    if (leads) pdl_wait_primary();                     // (the kernel that writes the tokens' codes)
+    if (leads && !a.stall) {
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -748,6 +775,23 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
   return p;
 }
 
+// Launch; with `overlap` the kernel may start while the one before it (which
+// allows that, and whose results it waits for by itself) still runs.
+template <typename K, typename... Args>
+static cudaError_t launch_after(K k, int grid, size_t smem, cudaStream_t st, int overlap, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
 template <bool NV>
 static int launch_pair(const CUtensorMap (&m)[4], const PairArgs& a, int grid, cudaStream_t st) {
   auto k = fp4_pair_kernel<NV>;
@@ -760,7 +804,7 @@ static int launch_pair(const CUtensorMap (&m)[4], const PairArgs& a, int grid, c
     TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_dev = dev;
   }
-  k<<<grid, kThreads, smem, st>>>(m[0], m[1], m[2], m[3], a);
+  TS_CUDA_TRY(launch_after(k, grid, smem, st, a.overlap, m[0], m[1], m[2], m[3], a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
@@ -784,7 +828,7 @@ static int launch(const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& 
     TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_dev = dev;
   }
-  k<<<grid, kThreads, smem, st>>>(wm, xm, a);
+  TS_CUDA_TRY(launch_after(k, grid, smem, st, a.overlap, wm, xm, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
@@ -813,9 +857,9 @@ extern "C" size_t ts_fp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K, 
   return paged::kCounterBytes + (!p.pair ? (size_t)p.grid * 2 * kBW * p.BT * 4 : 0);
 }
 
-extern "C" int ts_fp4_matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, const void* bias, int bias_dtype, void* out,
-                             int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
-                             void* stream) {
+static int matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, const void* bias, int bias_dtype, void* out,
+                  int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes, int overlap,
+                  void* stream) {
   int rc = check_tensor(x, "ts_fp4_matmul a");
   if (rc != TS_OK) return rc;
   rc = check_tensor(w, "ts_fp4_matmul b");
@@ -860,6 +904,7 @@ extern "C" int ts_fp4_matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, con
     a.vec = w->rows % 8 == 0 && out_row_stride % 8 == 0 && is_aligned(out, 16);
     a.wait_ns = wait_limit_ns();
     a.stall = stall;
+    a.overlap = overlap;
     CUtensorMap m[4];
     rc = encode_tmap_2d(&m[0], x->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)x->rows, row, 128, 128,
                         CU_TENSOR_MAP_SWIZZLE_128B);
@@ -892,6 +937,7 @@ extern "C" int ts_fp4_matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, con
   a.partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + paged::kCounterBytes);
   a.wait_ns = wait_limit_ns();
   a.stall = stall;
+  a.overlap = overlap;
   CUtensorMap wm, xm;
   rc = encode_tmap_2d(&wm, w->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)w->rows, row, 128, kBW,
                       CU_TENSOR_MAP_SWIZZLE_128B);
@@ -900,6 +946,12 @@ extern "C" int ts_fp4_matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, con
                       CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != TS_OK) return rc;
   return w->format == TS_NVFP4 ? launch<true>(p.BT, wm, xm, a, p.grid, st) : launch<false>(p.BT, wm, xm, a, p.grid, st);
+}
+
+extern "C" int ts_fp4_matmul(const ts_fp4_tensor* a, const ts_fp4_tensor* b, const void* bias, int bias_dtype, void* out,
+                             int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  return matmul(a, b, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, workspace_bytes, 0, stream);
 }
 
 extern "C" size_t ts_serving_counter_bytes(void) { return paged::kCounterBytes; }
@@ -959,5 +1011,5 @@ extern "C" int ts_fp4_linear(const void* x, int x_dtype, int64_t M, int64_t x_ro
   t.format = w->format;
   rc = ts_fp4_quantize(x, x_dtype, x_row_stride, &t, 0, nullptr, 0, stream);
   if (rc != TS_OK) return rc;
-  return ts_fp4_matmul(&t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, stream);
+  return matmul(&t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, 1, stream);
 }

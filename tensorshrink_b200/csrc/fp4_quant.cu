@@ -1,14 +1,14 @@
 // Quantisation to microscaled 4-bit floating point, and back.
 //
-// A warp takes 512 columns of one row: 32 groups of 16, one per lane (an
-// nvfp4 block; half an mxfp4 block, whose two lanes share their maximum). A
-// CTA's eight warps take rows 2i, 2i + 1 of the four 32-row quarters of a
-// scale tile: those rows' scales share 32-byte sectors. Rows whose addresses
-// allow it are read with 16-byte loads; the others element by element,
-// coalesced, through shared memory. Bound by DRAM traffic: x is read once
-// (twice when the tensor's scale is sought, the second time from the end, so
-// that what the first pass left in L2 is found there), 0.5625 (0.53) bytes an
-// element are written.
+// A warp takes 128 columns of the four rows that share 16-byte units of a scale
+// tile (r, r + 32, r + 64, r + 96): 16 columns per lane, an nvfp4 block or half
+// an mxfp4 block, whose two lanes share their maximum. A CTA's eight warps take
+// eight neighbouring such rows, so that its scales are whole 128-byte lines.
+// Rows that start on 32 or 16 bytes are read with loads that wide; the others
+// word by word or element by element, coalesced, through shared memory. Bound
+// by DRAM traffic: x is read once (twice when the tensor's scale is sought, the
+// second time from the end, so that what the first pass left in L2 is found
+// there), 0.5625 (0.53) bytes an element are written.
 //
 // Every rounding is spelled out (a reciprocal and products rounded to fp32,
 // two conversions to nearest even), so codes are reproducible bit for bit
@@ -16,13 +16,17 @@
 #include <algorithm>
 
 #include "fp4.cuh"
+#include "paged.cuh"
 
 namespace ts {
 namespace fp4 {
 
 constexpr int kWarps = 8;
-constexpr int kSeg = 512;          // columns of a warp's piece
-constexpr int kMaxParts = 1184;    // CTAs of the maximum pass
+constexpr int kAmaxSeg = 512;      // columns of a warp's piece of the maximum pass
+constexpr int kSeg = 128;          // columns of a warp's piece, four rows high
+constexpr int kMaxParts = 1184;    // CTAs of the maximum pass at most
+constexpr int kAmaxUnits = 2;      // pieces that a warp has in flight: maximum pass,
+constexpr int kQuantUnits = 2;     // the other passes
 
 struct QuantArgs {
   const void* x;
@@ -33,8 +37,10 @@ struct QuantArgs {
   int64_t row_bytes, kt;        // bytes of a row of codes, scale tiles along a row
   int segs;
   int reverse;                  // walk from the end
-  uint32_t* parts;              // bits of the CTAs' maxima when the scale is sought, else NULL
-  int n_parts;
+  int64_t amax_cols;            // the maximum pass takes rows without gaps as one row
+  int amax_rows, amax_segs;
+  uint32_t* parts;              // bits of the CTAs' maxima when the scale is sought
+  int* counter;                 // of CTAs that have left theirs; zero between calls
 };
 
 template <int DT>
@@ -58,76 +64,180 @@ struct Elem<TS_F32> {
   static __device__ float f(uint32_t v) { return __uint_as_float(v); }
 };
 
-// 16 elements of a row from column c0 on (zeros behind the last column).
-// ALIGNED: the row starts on a 16-byte boundary (c0 is a multiple of 16).
-// Otherwise the warp stages its 512 columns in `stage`.
-template <int DT, bool ALIGNED>
-__device__ __forceinline__ void load16(const QuantArgs& a, int64_t row, int seg, int lane, typename Elem<DT>::T* stage,
-                                       typename Elem<DT>::T (&v)[16]) {
+// 32 bytes from a 32-byte boundary.
+__device__ __forceinline__ void ld32(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// A lane's 16 elements as words (8, or 16 of fp32).
+template <int DT>
+struct Lane {
+  static constexpr int N = DT == TS_F32 ? 16 : 8;
+  uint32_t w[N];
+};
+
+// Reads the columns [first, first + 128) of the warp's four rows, row0 + 32 q
+// (zeros behind the last column and where a row does not exist). AL: the
+// alignment of rows. With 32 or 16, eight lanes read a row, 16 consecutive
+// columns each. Otherwise all 32 lanes read one row after the other, in words
+// (4) or elements, and deal() sorts them.
+template <int DT, int AL>
+__device__ __forceinline__ void load16(const void* x, int64_t rows, int64_t cols, int64_t stride, int64_t row0,
+                                       int64_t first, int lane, Lane<DT>& v) {
   using T = typename Elem<DT>::T;
-  const T* p = reinterpret_cast<const T*>(a.x) + row * a.stride;
-  const int64_t first = (int64_t)seg * kSeg;
-  if (ALIGNED) {
-    const int64_t c0 = first + lane * 16;
-    if (c0 + 16 <= a.cols) {
-      constexpr int N = 16 * sizeof(T) / 16;
-      uint4 w[N];
+  constexpr int N = Lane<DT>::N;
 #pragma unroll
-      for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint4*>(p + c0)[i];
+  for (int i = 0; i < N; ++i) v.w[i] = 0;
+  if (AL >= 16) {
+    const int64_t row = row0 + (lane >> 3) * 32, c0 = first + (lane & 7) * 16;
+    if (row >= rows) return;
+    const T* p = reinterpret_cast<const T*>(x) + row * stride;
+    if (c0 + 16 <= cols) {
+      if (AL == 32) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = reinterpret_cast<const T*>(w)[i];
+        for (int i = 0; i < N / 8; ++i) ld32(reinterpret_cast<const char*>(p + c0) + 32 * i, *reinterpret_cast<uint32_t(*)[8]>(v.w + 8 * i));
+      } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+          const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + c0) + i);
+          v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
+        }
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = c0 + i < a.cols ? p[c0 + i] : (T)0;
+      for (int i = 0; i < 16; ++i)
+        if (c0 + i < cols) {
+          if (DT == TS_F32) v.w[i % N] = (uint32_t)p[c0 + i];
+          else v.w[(i / 2) % N] |= (uint32_t)p[c0 + i] << (16 * (i & 1));
+        }
     }
-  } else {
-    T t[16];
+    return;
+  }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int64_t c = first + i * 32 + lane;
-      t[i] = c < a.cols ? p[c] : (T)0;
+  for (int i = 0; i < N; ++i) {
+    const int64_t row = row0 + i / (N / 4) * 32;
+    if (row >= rows) break;
+    const T* p = reinterpret_cast<const T*>(x) + row * stride;
+    const int word = i % (N / 4) * 32 + lane;
+    if (DT == TS_F32) {
+      if (first + word < cols) v.w[i] = (uint32_t)p[first + word];
+    } else {
+      const int64_t c = first + word * 2;   // the word of columns c, c + 1
+      if (AL == 4 && c + 1 < cols) v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(p + c));
+      else if (c < cols) v.w[i] = (uint32_t)p[c] | (c + 1 < cols ? (uint32_t)p[c + 1] << 16 : 0);
     }
-    __syncwarp();
+  }
+}
+
+// From the order that load16 read words in (AL < 16) to 16 consecutive columns
+// per lane, through the warp's 4 rows of shared memory.
+template <int DT, int AL>
+__device__ __forceinline__ void deal(uint32_t* stage, int lane, Lane<DT>& v) {
+  if (AL >= 16) return;
+  constexpr int N = Lane<DT>::N;
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) stage[i * 32 + lane] = t[i];
-    __syncwarp();
-    constexpr int N = 16 * sizeof(T) / 16;
-    uint4 w[N];
+  for (int i = 0; i < N; ++i) stage[i * 32 + lane] = v.w[i];
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint4*>(stage + lane * 16)[i];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = reinterpret_cast<const T*>(w)[i];
+  for (int i = 0; i < N / 4; ++i) {
+    const uint4 u = reinterpret_cast<const uint4*>(stage + lane * N)[i];
+    v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
   }
 }
 
 // Largest magnitude as the type's bits (a NaN or infinity: at least kInf).
 template <int DT>
-__device__ __forceinline__ uint32_t top_bits(const typename Elem<DT>::T (&v)[16]) {
-  constexpr uint32_t kAbs = DT == TS_F32 ? 0x7FFFFFFFu : 0x7FFFu;
+__device__ __forceinline__ uint32_t top_bits(const Lane<DT>& v) {
   uint32_t m = 0;
+  if constexpr (DT == TS_F32) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = max(m, (uint32_t)v[i] & kAbs);
-  return m;
+    for (int i = 0; i < Lane<DT>::N; ++i) m = max(m, v.w[i] & 0x7FFFFFFFu);
+    return m;
+  } else {
+#pragma unroll
+    for (int i = 0; i < Lane<DT>::N; ++i) m = __vmaxu2(m, v.w[i] & 0x7FFF7FFFu);
+    return max(m & 0xFFFFu, m >> 16);
+  }
 }
 
-template <int DT, bool ALIGNED>
+// Element i of a lane in fp32.
+template <int DT>
+__device__ __forceinline__ float elem(const Lane<DT>& v, int i) {
+  if (DT == TS_F32) return __uint_as_float(v.w[i % Lane<DT>::N]);
+  const uint32_t w = v.w[(i / 2) % Lane<DT>::N];
+  if (DT == TS_BF16) return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return i & 1 ? f.y : f.x;
+}
+
+// 512 columns of one row from `first` on, as words in any order (for maxima).
+template <int DT, int AL>
+__device__ __forceinline__ void load_flat(const void* x, int64_t cols, int64_t row_at, int64_t first, int lane,
+                                          Lane<DT>& v) {
+  using T = typename Elem<DT>::T;
+  constexpr int N = Lane<DT>::N;
+  const T* p = reinterpret_cast<const T*>(x) + row_at;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v.w[i] = 0;
+  if (AL >= 16 && first + kAmaxSeg <= cols) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + first) + i * 32 + lane);
+      v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int word = i * 32 + lane;
+    if (DT == TS_F32) {
+      if (first + word < cols) v.w[i] = (uint32_t)p[first + word];
+    } else {
+      const int64_t c = first + word * 2;
+      if (AL >= 4 && c + 1 < cols) v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(p + c));
+      else if (c < cols) v.w[i] = (uint32_t)p[c] | (c + 1 < cols ? (uint32_t)p[c + 1] << 16 : 0);
+    }
+  }
+}
+
+// The tensor's scale: CTAs' maxima to the workspace, the last CTA to arrive
+// takes their maximum (the order does not matter to a maximum).
+template <int DT, int AL>
 __global__ void __launch_bounds__(kWarps * 32) fp4_amax_kernel(const QuantArgs a) {
   using E = Elem<DT>;
-  __shared__ __align__(16) typename E::T stage[ALIGNED ? 1 : kWarps][ALIGNED ? 16 : kSeg];
   __shared__ uint32_t part[kWarps];
+  __shared__ int last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t units = a.rows * a.segs;
+  // a warp takes 512 columns of a row: four "rows" of 128, one behind the other
+  const int step = gridDim.x * kWarps, units = a.amax_rows * a.amax_segs;
   float m = 0.f;
-  for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < units; u += (int64_t)gridDim.x * kWarps) {
-    typename E::T v[16];
-    load16<DT, ALIGNED>(a, u / a.segs, (int)(u % a.segs), lane, stage[ALIGNED ? 0 : warp], v);
-    if (top_bits<DT>(v) < E::kInf) {
-      m = fmaxf(m, E::f((typename E::T)top_bits<DT>(v)));
-    } else {   // only finite elements count
+  for (int u = blockIdx.x * kWarps + warp; u < units; u += kAmaxUnits * step) {
+    Lane<DT> v[kAmaxUnits];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float f = fabsf(E::f(v[i]));
-        if (f < INFINITY) m = fmaxf(m, f);
+    for (int k = 0; k < kAmaxUnits; ++k) {
+      const int w = u + k * step, row = a.amax_rows == 1 ? 0 : w / a.amax_segs;
+      load_flat<DT, AL>(a.x, w < units ? a.amax_cols : 0, row * a.stride, (int64_t)(w - row * a.amax_segs) * kAmaxSeg, lane,
+                        v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kAmaxUnits; ++k) {
+      const uint32_t top = top_bits<DT>(v[k]);
+      if (top < E::kInf) {
+        m = fmaxf(m, E::f((typename E::T)top));
+      } else {   // only finite elements count
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float f = fabsf(elem<DT>(v[k], i));
+          if (f < INFINITY) m = fmaxf(m, f);
+        }
       }
     }
   }
@@ -139,72 +249,84 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_amax_kernel(const QuantArgs a
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) r = max(r, part[i]);
     a.parts[blockIdx.x] = r;
+    __threadfence();
+    last = atomicAdd(a.counter, 1) == (int)gridDim.x - 1;
+    if (last) *a.counter = 0;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
+  uint32_t r = 0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kWarps * 32) r = max(r, __ldcg(a.parts + i));
+  r = __reduce_max_sync(0xffffffffu, r);
+  __syncthreads();
+  if (lane == 0) part[warp] = r;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) r = max(r, part[i]);
+    *a.global_scale = fmaxf(__fmul_rn(__uint_as_float(r), 1.f / 2688.f), kMinScale);   // 2688 = 448 * 6
   }
 }
 
-template <int DT, bool NV, bool ALIGNED>
+template <int DT, bool NV, int AL>
 __global__ void __launch_bounds__(kWarps * 32) fp4_quantize_kernel(const QuantArgs a) {
   using E = Elem<DT>;
-  __shared__ __align__(16) typename E::T stage[ALIGNED ? 1 : kWarps][ALIGNED ? 16 : kSeg];
-  __shared__ uint32_t part[kWarps];
+  __shared__ __align__(16) uint32_t stage[AL >= 16 ? 1 : kWarps][AL >= 16 ? 4 : 32 * Lane<DT>::N];
+  pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float g = 1.f, to_scale = 0.f;
-  if (NV) {
-    if (a.parts != nullptr) {
-      uint32_t w = 0;
-      for (int i = threadIdx.x; i < a.n_parts; i += kWarps * 32) w = max(w, a.parts[i]);
-      w = __reduce_max_sync(0xffffffffu, w);
-      if (lane == 0) part[warp] = w;
-      __syncthreads();
-      w = 0;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) w = max(w, part[i]);
-      g = fmaxf(__fmul_rn(__uint_as_float(w), 1.f / 2688.f), kMinScale);   // 2688 = 448 * 6
-      if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.global_scale = g;
-    } else {
-      g = usable_scale(a.global_scale);
-    }
-    to_scale = __frcp_rn(__fmul_rn(6.f, g));
-  }
+  const float g = NV ? usable_scale(a.global_scale) : 1.f;
+  const float to_scale = NV ? __frcp_rn(__fmul_rn(6.f, g)) : 0.f;
   const int bx = a.reverse ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const int64_t row = (int64_t)(bx >> 4) * kTileRows + (bx & 15) * 2 + (warp & 1) + (warp >> 1) * 32;
-  if (row >= a.rows) return;
-  for (int s = blockIdx.y; s < a.segs; s += gridDim.y) {
-    const int seg = a.reverse ? a.segs - 1 - s : s;
-    typename E::T v[16];
-    load16<DT, ALIGNED>(a, row, seg, lane, stage[ALIGNED ? 0 : warp], v);
-    uint32_t top = top_bits<DT>(v);
-    if (!NV) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    const bool bad = top >= E::kInf;
-    const float amax = E::f((typename E::T)top);
-    float r;
-    uint32_t sc;
-    if (NV) {
-      sc = __nv_cvt_float_to_fp8(fminf(__fmul_rn(amax, to_scale), 448.f), __NV_SATFINITE, __NV_E4M3);
-      const float sf = e4m3_value((uint8_t)sc);
-      r = sf > 0.f ? __frcp_rn(__fmul_rn(sf, g)) : 0.f;
-    } else {
-      const int e = (int)(__float_as_uint(amax) >> 23) - 2;
-      sc = (uint32_t)max(e, 0);
-      r = __uint_as_float((254u - sc) << 23);
-    }
-    uint2 out = make_uint2(0, 0);
-    if (bad) {
-      sc = NV ? 0x7Fu : 0xFFu;
-    } else {
-      float f[8];
+  const int64_t row0 = (int64_t)(bx >> 2) * kTileRows + (bx & 3) * 8 + warp, row = row0 + (lane >> 3) * 32;
+  if (row0 >= a.rows) return;
+  const bool exists = row < a.rows;
+  for (int s0 = blockIdx.y; s0 < a.segs; s0 += kQuantUnits * gridDim.y) {
+    Lane<DT> vv[kQuantUnits];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = E::f(v[i]);
-      out.x = to_e2m1x8(f, r);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = E::f(v[8 + i]);
-      out.y = to_e2m1x8(f, r);
+    for (int k = 0; k < kQuantUnits; ++k) {
+      const int s = s0 + k * gridDim.y, seg = a.reverse ? a.segs - 1 - s : s;
+      load16<DT, AL>(a.x, s < a.segs ? a.rows : 0, a.cols, a.stride, row0, (int64_t)seg * kSeg, lane, vv[k]);
     }
-    const int64_t group = (int64_t)seg * 32 + lane;   // of 16 columns
-    if (group * 8 < a.row_bytes) {
-      *reinterpret_cast<uint2*>(a.codes + row * a.row_bytes + group * 8) = out;
-      if (NV) a.scales[scale_at(row, group, a.kt)] = (uint8_t)sc;
-      else if ((lane & 1) == 0) a.scales[scale_at(row, group >> 1, a.kt)] = (uint8_t)sc;
+#pragma unroll
+    for (int k = 0; k < kQuantUnits; ++k) {
+      const int s = s0 + k * gridDim.y, seg = a.reverse ? a.segs - 1 - s : s;
+      if (s >= a.segs) break;
+      Lane<DT>& v = vv[k];
+      deal<DT, AL>(stage[AL >= 16 ? 0 : warp], lane, v);
+      uint32_t top = top_bits<DT>(v);
+      if (!NV) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      const bool bad = top >= E::kInf;
+      const float amax = E::f((typename E::T)top);
+      float r;
+      uint32_t sc;
+      if (NV) {
+        sc = __nv_cvt_float_to_fp8(fminf(__fmul_rn(amax, to_scale), 448.f), __NV_SATFINITE, __NV_E4M3);
+        const float sf = e4m3_value((uint8_t)sc);
+        r = sf > 0.f ? __frcp_rn(__fmul_rn(sf, g)) : 0.f;
+      } else {
+        const int e = (int)(__float_as_uint(amax) >> 23) - 2;
+        sc = (uint32_t)max(e, 0);
+        r = __uint_as_float((254u - sc) << 23);
+      }
+      uint2 out = make_uint2(0, 0);
+      if (bad) {
+        sc = NV ? 0x7Fu : 0xFFu;
+      } else {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, i);
+        out.x = to_e2m1x8(f, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, 8 + i);
+        out.y = to_e2m1x8(f, r);
+      }
+      const int64_t group = (int64_t)seg * 8 + (lane & 7);   // of 16 columns
+      if (exists && group * 8 < a.row_bytes) {
+        *reinterpret_cast<uint2*>(a.codes + row * a.row_bytes + group * 8) = out;
+        if (NV) a.scales[scale_at(row, group, a.kt)] = (uint8_t)sc;
+        else if ((lane & 1) == 0) a.scales[scale_at(row, group >> 1, a.kt)] = (uint8_t)sc;
+      }
     }
   }
 }
@@ -218,65 +340,97 @@ struct DequantArgs {
   int segs;
 };
 
-template <int DT, bool NV, bool ALIGNED>
+template <int DT, bool NV, int AL>
 __global__ void __launch_bounds__(kWarps * 32) fp4_dequantize_kernel(const DequantArgs a) {
   using T = typename Elem<DT>::T;
-  __shared__ __align__(16) T stage[ALIGNED ? 1 : kWarps][ALIGNED ? 16 : kSeg];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int N = Lane<DT>::N;
+  __shared__ __align__(16) uint32_t stage[AL >= 16 ? 1 : kWarps][AL >= 16 ? 4 : 32 * N];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7;
   const float g = NV ? usable_scale(a.global_scale) : 1.f;
-  const int64_t row = (int64_t)(blockIdx.x >> 4) * kTileRows + (blockIdx.x & 15) * 2 + (warp & 1) + (warp >> 1) * 32;
-  if (row >= a.rows) return;
-  for (int seg = blockIdx.y; seg < a.segs; seg += gridDim.y) {
-    const int64_t group = (int64_t)seg * 32 + lane;
-    __align__(16) T v[16];
-    if (group * 8 < a.row_bytes) {
-      const uint2 w = *reinterpret_cast<const uint2*>(a.codes + row * a.row_bytes + group * 8);
-      const uint8_t sb = a.scales[scale_at(row, NV ? group : group >> 1, a.kt)];
-      const float s = NV ? __fmul_rn(e4m3_value(sb), g) : e8m0_value(sb);
+  const int64_t row0 = (int64_t)(blockIdx.x >> 2) * kTileRows + (blockIdx.x & 3) * 8 + warp, row = row0 + (lane >> 3) * 32;
+  if (row0 >= a.rows) return;
+  const bool exists = row < a.rows;
+  for (int s0 = blockIdx.y; s0 < a.segs; s0 += kQuantUnits * gridDim.y) {
+    uint2 w[kQuantUnits];
+    uint8_t sb[kQuantUnits];
+#pragma unroll
+    for (int k = 0; k < kQuantUnits; ++k) {
+      const int64_t group = (int64_t)(s0 + k * gridDim.y) * 8 + l8;
+      w[k] = make_uint2(0, 0);
+      sb[k] = 0;
+      if (exists && group * 8 < a.row_bytes) {
+        w[k] = __ldg(reinterpret_cast<const uint2*>(a.codes + row * a.row_bytes + group * 8));
+        sb[k] = __ldg(a.scales + scale_at(row, NV ? group : group >> 1, a.kt));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kQuantUnits; ++k) {
+      const int seg = s0 + k * gridDim.y;
+      if (seg >= a.segs) break;
+      const float s = NV ? __fmul_rn(e4m3_value(sb[k]), g) : e8m0_value(sb[k]);
       uint32_t h[8];
-      uint32_t (&h0)[4] = *reinterpret_cast<uint32_t(*)[4]>(h);
-      uint32_t (&h1)[4] = *reinterpret_cast<uint32_t(*)[4]>(h + 4);
-      from_e2m1x8(w.x, h0);
-      from_e2m1x8(w.y, h1);
+      from_e2m1x8(w[k].x, *reinterpret_cast<uint32_t(*)[4]>(h));
+      from_e2m1x8(w[k].y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
+      __align__(16) uint32_t v[N];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
         const float y0 = __fmul_rn(f.x, s), y1 = __fmul_rn(f.y, s);
         if (DT == TS_F32) {
-          v[2 * i] = (T)__float_as_uint(y0);
-          v[2 * i + 1] = (T)__float_as_uint(y1);
+          v[(2 * i) % N] = __float_as_uint(y0);
+          v[(2 * i + 1) % N] = __float_as_uint(y1);
         } else if (DT == TS_BF16) {
-          v[2 * i] = (T)__bfloat16_as_ushort(__float2bfloat16_rn(y0));
-          v[2 * i + 1] = (T)__bfloat16_as_ushort(__float2bfloat16_rn(y1));
+          const __nv_bfloat162 b2 = __floats2bfloat162_rn(y0, y1);
+          v[i] = *reinterpret_cast<const uint32_t*>(&b2);
         } else {
-          v[2 * i] = (T)__half_as_ushort(__float2half_rn(y0));
-          v[2 * i + 1] = (T)__half_as_ushort(__float2half_rn(y1));
+          const __half2 b2 = __floats2half2_rn(y0, y1);
+          v[i] = *reinterpret_cast<const uint32_t*>(&b2);
         }
       }
-    }
-    T* p = reinterpret_cast<T*>(a.out) + row * a.out_stride;
-    const int64_t c0 = group * 16;
-    if (ALIGNED) {
-      if (c0 + 16 <= a.cols) {
+      T* p = reinterpret_cast<T*>(a.out) + row * a.out_stride;
+      const int64_t first = (int64_t)seg * kSeg, c0 = first + l8 * 16;
+      if (AL >= 16) {
+        if (!exists) continue;
+        if (c0 + 16 <= a.cols) {
+          if (AL == 32) {
 #pragma unroll
-        for (int i = 0; i < (int)(16 * sizeof(T) / 16); ++i)
-          reinterpret_cast<uint4*>(p + c0)[i] = reinterpret_cast<const uint4*>(v)[i];
-      } else {
+            for (int i = 0; i < N / 8; ++i) st32(reinterpret_cast<char*>(p + c0) + 32 * i, v + 8 * i);
+          } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (c0 + i < a.cols) p[c0 + i] = v[i];
+            for (int i = 0; i < N / 4; ++i)
+              reinterpret_cast<uint4*>(p + c0)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c0 + i < a.cols) p[c0 + i] = DT == TS_F32 ? (T)v[i % N] : (T)(v[(i / 2) % N] >> (16 * (i & 1)));
+        }
+        continue;
       }
-    } else {
-      T* st = stage[warp];
+      uint32_t* st = stage[warp];
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < (int)(16 * sizeof(T) / 16); ++i)
-        reinterpret_cast<uint4*>(st + lane * 16)[i] = reinterpret_cast<const uint4*>(v)[i];
+      for (int i = 0; i < N / 4; ++i)
+        reinterpret_cast<uint4*>(st + lane * N)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int64_t c = (int64_t)seg * kSeg + i * 32 + lane;
-        if (c < a.cols) p[c] = st[i * 32 + lane];
+      for (int i = 0; i < N; ++i) {
+        const int64_t r = row0 + i / (N / 4) * 32;
+        if (r >= a.rows) break;
+        T* q = reinterpret_cast<T*>(a.out) + r * a.out_stride;
+        const int word = i % (N / 4) * 32 + lane;
+        const uint32_t x = st[i * 32 + lane];
+        if (DT == TS_F32) {
+          if (first + word < a.cols) q[first + word] = (T)x;
+        } else {
+          const int64_t c = first + word * 2;
+          if (AL == 4 && c + 1 < a.cols) {
+            *reinterpret_cast<uint32_t*>(q + c) = x;
+          } else {
+            if (c < a.cols) q[c] = (T)x;
+            if (c + 1 < a.cols) q[c + 1] = (T)(x >> 16);
+          }
+        }
       }
     }
   }
@@ -292,34 +446,69 @@ int check_tensor(const ts_fp4_tensor* t, const char* what) {
   return TS_OK;
 }
 
-// Grid of the row-tile kernels: 16 CTAs per 128 rows, enough along the
-// columns to give every SM eight CTAs.
+// Grid of the row-tile kernels: 4 CTAs per 128 rows (fewer for few rows), enough
+// along the columns to give every SM sixteen CTAs.
 static dim3 tile_grid(int64_t rows, int segs) {
-  const int64_t gx = (rows + kTileRows - 1) / kTileRows * 16;
+  const int64_t gx = rows <= 8 ? 1 : (rows + kTileRows - 1) / kTileRows * 4;
   const int64_t want = ((int64_t)sm_count() * 16 + gx - 1) / gx;
   return dim3((unsigned)gx, (unsigned)std::min<int64_t>(segs, std::max<int64_t>(1, std::min<int64_t>(want, 65535))));
 }
 
-template <int DT, bool AL>
+template <int DT, int AL>
+static int launch_amax(const QuantArgs& a, cudaStream_t st) {
+  const int64_t units = (int64_t)a.amax_rows * a.amax_segs;
+  const int grid = (int)std::min<int64_t>(std::min(kMaxParts, sm_count() * 8), (units + kWarps - 1) / kWarps);
+  fp4_amax_kernel<DT, AL><<<grid, kWarps * 32, 0, st>>>(a);
+  TS_LAUNCH_CHECK();
+  return TS_OK;
+}
+
+template <int DT, int AL>
 static int launch_quantize(const QuantArgs& a, bool nv, cudaStream_t st) {
   const dim3 grid = tile_grid(a.rows, a.segs);
-  if (a.parts != nullptr) {
-    fp4_amax_kernel<DT, AL><<<a.n_parts, kWarps * 32, 0, st>>>(a);
-    TS_LAUNCH_CHECK();
-  }
   if (nv) fp4_quantize_kernel<DT, true, AL><<<grid, kWarps * 32, 0, st>>>(a);
   else fp4_quantize_kernel<DT, false, AL><<<grid, kWarps * 32, 0, st>>>(a);
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
 
-template <int DT, bool AL>
+template <int DT>
+static int launch_quantize(const QuantArgs& a, int al, int amax_al, bool nv, bool find, cudaStream_t st) {
+  if (find) {
+    int rc;
+    if (amax_al >= 16) rc = launch_amax<DT, 16>(a, st);
+    else if (amax_al == 4 && DT != TS_F32) rc = launch_amax<DT, 4>(a, st);
+    else rc = launch_amax<DT, 1>(a, st);
+    if (rc != TS_OK) return rc;
+  }
+  if (al == 32) return launch_quantize<DT, 32>(a, nv, st);
+  if (al == 16) return launch_quantize<DT, 16>(a, nv, st);
+  if (al == 4 && DT != TS_F32) return launch_quantize<DT, 4>(a, nv, st);
+  return launch_quantize<DT, 1>(a, nv, st);
+}
+
+template <int DT, int AL>
 static int launch_dequantize(const DequantArgs& a, bool nv, cudaStream_t st) {
   const dim3 grid = tile_grid(a.rows, a.segs);
   if (nv) fp4_dequantize_kernel<DT, true, AL><<<grid, kWarps * 32, 0, st>>>(a);
   else fp4_dequantize_kernel<DT, false, AL><<<grid, kWarps * 32, 0, st>>>(a);
   TS_LAUNCH_CHECK();
   return TS_OK;
+}
+
+template <int DT>
+static int launch_dequantize(const DequantArgs& a, int al, bool nv, cudaStream_t st) {
+  if (al == 32) return launch_dequantize<DT, 32>(a, nv, st);
+  if (al == 16) return launch_dequantize<DT, 16>(a, nv, st);
+  if (al == 4 && DT != TS_F32) return launch_dequantize<DT, 4>(a, nv, st);
+  return launch_dequantize<DT, 1>(a, nv, st);
+}
+
+// Alignment of rows that the kernels use: 32, 16 or 4 bytes, or the element's.
+static int row_alignment(const void* p, int64_t stride, int es) {
+  for (int al : {32, 16, 4})
+    if (is_aligned(p, al) && (stride * es) % al == 0) return al;
+  return 1;
 }
 
 }  // namespace fp4
@@ -333,7 +522,7 @@ extern "C" size_t ts_fp4_scales_bytes(int64_t rows, int64_t cols, int format) {
   return (size_t)((rows + kTileRows - 1) / kTileRows) * scale_tiles(cols, format) * kTileBytes;
 }
 
-extern "C" size_t ts_fp4_quantize_workspace_size(void) { return (size_t)kMaxParts * 4; }
+extern "C" size_t ts_fp4_quantize_workspace_size(void) { return paged::kCounterBytes + (size_t)kMaxParts * 4; }
 
 extern "C" int ts_fp4_quantize(const void* x, int x_dtype, int64_t x_row_stride, const ts_fp4_tensor* t, int find_scale,
                                void* workspace, size_t workspace_bytes, void* stream) {
@@ -360,15 +549,21 @@ extern "C" int ts_fp4_quantize(const void* x, int x_dtype, int64_t x_row_stride,
   a.kt = scale_tiles(t->cols, t->format);
   a.segs = (int)((padded_cols(t->cols) + kSeg - 1) / kSeg);
   a.reverse = find_scale ? 1 : 0;
-  a.parts = find_scale ? reinterpret_cast<uint32_t*>(workspace) : nullptr;
-  a.n_parts = (int)std::min<int64_t>(std::min(kMaxParts, sm_count() * 4), (a.rows * a.segs + kWarps - 1) / kWarps);
-  const int es = x_dtype == TS_F32 ? 4 : 2;
-  const bool al = is_aligned(x, 16) && (x_row_stride * es) % 16 == 0;
+  a.parts = find_scale ? reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(workspace) + paged::kCounterBytes) : nullptr;
+  a.counter = reinterpret_cast<int*>(workspace);
+  const bool flat = x_row_stride == t->cols || t->rows == 1;
+  a.amax_rows = flat ? 1 : (int)t->rows;
+  a.amax_cols = flat ? t->rows * t->cols : t->cols;
+  const int64_t amax_segs = (a.amax_cols + kAmaxSeg - 1) / kAmaxSeg;
+  TS_UNSUPPORTED(!find_scale || a.amax_rows * amax_segs < ((int64_t)1 << 31) - (1 << 24), "tensor too large to find its scale");
+  a.amax_segs = (int)amax_segs;
+  const int es = x_dtype == TS_F32 ? 4 : 2, al = row_alignment(x, x_row_stride, es);
+  const int amax_al = flat ? row_alignment(x, 0, es) : al;
+  const bool find = find_scale != 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (x_dtype == TS_F16) return al ? launch_quantize<TS_F16, true>(a, nv, st) : launch_quantize<TS_F16, false>(a, nv, st);
-  if (x_dtype == TS_BF16)
-    return al ? launch_quantize<TS_BF16, true>(a, nv, st) : launch_quantize<TS_BF16, false>(a, nv, st);
-  return al ? launch_quantize<TS_F32, true>(a, nv, st) : launch_quantize<TS_F32, false>(a, nv, st);
+  if (x_dtype == TS_F16) return launch_quantize<TS_F16>(a, al, amax_al, nv, find, st);
+  if (x_dtype == TS_BF16) return launch_quantize<TS_BF16>(a, al, amax_al, nv, find, st);
+  return launch_quantize<TS_F32>(a, al, amax_al, nv, find, st);
 }
 
 extern "C" int ts_fp4_dequantize(const ts_fp4_tensor* t, void* out, int out_dtype, int64_t out_row_stride,
@@ -391,12 +586,9 @@ extern "C" int ts_fp4_dequantize(const ts_fp4_tensor* t, void* out, int out_dtyp
   a.out = out;
   a.segs = (int)((t->cols + kSeg - 1) / kSeg);
   const bool nv = t->format == TS_NVFP4;
-  const int es = out_dtype == TS_F32 ? 4 : 2;
-  const bool al = is_aligned(out, 16) && (out_row_stride * es) % 16 == 0;
+  const int al = row_alignment(out, out_row_stride, out_dtype == TS_F32 ? 4 : 2);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (out_dtype == TS_F16)
-    return al ? launch_dequantize<TS_F16, true>(a, nv, st) : launch_dequantize<TS_F16, false>(a, nv, st);
-  if (out_dtype == TS_BF16)
-    return al ? launch_dequantize<TS_BF16, true>(a, nv, st) : launch_dequantize<TS_BF16, false>(a, nv, st);
-  return al ? launch_dequantize<TS_F32, true>(a, nv, st) : launch_dequantize<TS_F32, false>(a, nv, st);
+  if (out_dtype == TS_F16) return launch_dequantize<TS_F16>(a, al, nv, st);
+  if (out_dtype == TS_BF16) return launch_dequantize<TS_BF16>(a, al, nv, st);
+  return launch_dequantize<TS_F32>(a, al, nv, st);
 }

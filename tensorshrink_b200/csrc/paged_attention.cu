@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
   __shared__ uint64_t warp_sums[kWarps];
   __shared__ int warp_most[kWarps];
   __shared__ int is_last;
+  pdl_launch_dependents();                             // the weights' kernel may take its place in the queue
   const Cache& c = a.c;
   int* lens = prefix + c.batch + 1;                                                        // [batch]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -675,23 +676,57 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
   }
 }
 
-// score[slot] (+)= sum over the group of exp2(logit - lse2): one thread per
-// slot of a kv head. Reads 4 bytes per slot and query head, next to the
-// 4 D bytes per slot that the attention read.
+// score[slot] += sum over the group of 2^(logit - lse2): a thread takes W
+// neighbouring slots of a kv head, W = 4 where pages hold a multiple of four.
+// Reads 4 bytes per slot and query head, next to the 4 D bytes per slot that
+// the attention read.
+template <int W>
 __global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a) {
+  pdl_wait_primary();
   const Cache& c = a.c;
   const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv;
   const int len = c.seq_lens[b];
-  if (units_of(a, len) == 0 || !takes(a, b, len, a.positions != nullptr ? a.positions[b] : 0)) return;
-  for (int slot = blockIdx.x * blockDim.x + threadIdx.x; slot <= len; slot += gridDim.x * blockDim.x) {
-    const int page = page_of(c, b, slot);
-    if (page < 0) continue;
-    float w = 0.f;
-    for (int g = 0; g < a.group; ++g) {
-      const int64_t q = (int64_t)b * a.n_q + h * a.group + g;
-      w += ex2(__ldcs(a.logits + q * a.logit_stride + slot) - a.lse2[q]);
+  if (units_of(a, len) == 0) return;
+  const bool ok = takes(a, b, len, a.positions != nullptr ? a.positions[b] : 0);
+  const int64_t q = (int64_t)b * a.n_q + h * a.group;
+  for (int slot0 = (blockIdx.x * blockDim.x + threadIdx.x) * W; slot0 <= len; slot0 += gridDim.x * blockDim.x * W) {
+    // everything that is read is on its way before the first of it is needed
+    int pg, off;
+    split_slot(a, slot0, &pg, &off);
+    const int page = c.table[b * c.table_stride + pg];
+    const float* lg = a.logits + q * a.logit_stride + slot0;
+    float w[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = 0.f;
+    for (int g0 = 0; g0 < a.group; g0 += 8) {
+      float v[8][W], lse[8];
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        if (g0 + g >= a.group) break;
+        lse[g] = a.lse2[q + g0 + g];
+        const float* src = lg + (g0 + g) * a.logit_stride;
+        if (W == 4) {
+          const float4 f = __ldcs(reinterpret_cast<const float4*>(src));
+          v[g][0] = f.x; v[g][1 % W] = f.y; v[g][2 % W] = f.z; v[g][3 % W] = f.w;
+        } else {
+          v[g][0] = __ldcs(src);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        if (g0 + g >= a.group) break;
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] += ex2(v[g][i] - lse[g]);
+      }
     }
-    c.scores[stat_at(c, page, h, slot % c.page_size)] += w;   // the attention has set the new slot's to 0
+    if (!ok || (unsigned)page >= (unsigned)c.num_pages) continue;
+    float* s = c.scores + stat_at(c, page, h, off);    // (the attention has set the new slot's to 0)
+    float old[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) old[i] = slot0 + i <= len ? s[i] : 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (slot0 + i <= len) s[i] = old[i] + w[i];
   }
 }
 
@@ -716,25 +751,27 @@ struct AppendArgs {
   int64_t sb, sh, st;
 };
 
-template <bool BF>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
+template <bool BF, bool ROPE>
+__global__ void __launch_bounds__(256, ROPE ? 2 : 4) paged_append_kernel(const AppendArgs a) {
   const Cache& c = a.c;
   const int lane = threadIdx.x & 31;
   const int D = c.head_dim, chunks = D / 8, half = chunks / 2;
-  const int b = blockIdx.z, len = c.seq_lens[b];
+  const int b = blockIdx.y, len = c.seq_lens[b];
   const int tokens = a.n_new != nullptr ? min(a.tokens, a.n_new[b]) : a.tokens;
-  if (len < 0) return;
-  // a warp takes kTok tokens of one head, so that their loads overlap
-  const int h = blockIdx.y;
+  if (len < 0 || tokens <= 0) return;
   const int64_t first = a.first != nullptr ? a.first[b] : len;
-  for (int t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kTok; t0 < tokens; t0 += gridDim.x * 8 * kTok) {
+  // neighbouring warps take neighbouring heads of the same kTok tokens: both
+  // the tokens' rows and the pages are touched in runs
+  const int items = (tokens + kTok - 1) / kTok * c.n_kv;
+  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < items; i += gridDim.x * 8) {
+    const int h = i % c.n_kv, t0 = i / c.n_kv * kTok;
     int64_t at[kTok];
     bool ok[kTok];
     for (int ch = lane; ch < 2 * chunks; ch += 32) {
       const bool is_v = ch >= chunks;
       const int cc = is_v ? ch - chunks : ch;
       const bool hi = cc >= half;
-      const bool turn = !is_v && a.cos_t != nullptr;
+      const bool turn = ROPE && !is_v;
       const uint16_t* src = is_v ? a.v + b * a.vb + h * a.vh : a.k + b * a.kb + h * a.kh;
       const int64_t step = is_v ? a.vt : a.kt;
       // the rows are on their way while the pages are looked up
@@ -750,7 +787,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
 #pragma unroll
         for (int i = 0; i < kTok; ++i) {
           const int64_t slot = (int64_t)len + t0 + i, pos = first + t0 + i;
-          ok[i] = t0 + i < tokens && slot < capacity(c) && (a.cos_t == nullptr || (pos >= 0 && pos < a.rope_rows));
+          ok[i] = t0 + i < tokens && slot < capacity(c) && (!ROPE || (pos >= 0 && pos < a.rope_rows));
           at[i] = 0;
           const int page = ok[i] ? page_of(c, b, (int)slot) : -1;
           ok[i] = page >= 0;
@@ -928,9 +965,21 @@ extern "C" int ts_paged_decode_attention(const void* qkv, int64_t qkv_row_stride
   const int r = cache->dtype == TS_BF16 ? launch_attention<true>(a, grid, st) : launch_attention<false>(a, grid, st);
   if (r != TS_OK || !accumulate) return r;
   const int rows = a.c.batch * a.c.n_kv;
+  TS_UNSUPPORTED(rows <= 65535, "too many heads in one call");
   const int64_t cap = (int64_t)a.c.max_pages * a.c.page_size;
-  const int per_row = (int)std::max<int64_t>(1, std::min<int64_t>((cap + 255) / 256, (4 * sm_count() + rows - 1) / rows));
-  paged_weights_kernel<<<dim3(per_row, rows), 256, 0, st>>>(a);
+  const int per = a.c.page_size % 4 == 0 ? 4 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>((cap + 256 * per - 1) / (256 * per), (16 * sm_count() + rows - 1) / rows),
+                     (unsigned)rows);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];                         // (it waits for the attention by itself)
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TS_CUDA_TRY(per == 4 ? cudaLaunchKernelEx(&cfg, paged_weights_kernel<4>, a)
+                       : cudaLaunchKernelEx(&cfg, paged_weights_kernel<1>, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
@@ -964,13 +1013,19 @@ extern "C" int ts_paged_append(const void* k, const int64_t* k_strides, const vo
   a.sb = scores ? score_strides[0] : 0;
   a.sh = scores ? score_strides[1] : 0;
   a.st = scores ? score_strides[2] : 0;
-  TS_UNSUPPORTED(a.c.batch <= 65535 && a.c.n_kv <= 65535, "too many sequences or heads in one call");
-  const int rows = a.c.batch * a.c.n_kv;
-  const dim3 grid((unsigned)std::max(1, std::min((tokens + 8 * kTok - 1) / (8 * kTok), (16 * sm_count() + rows - 1) / rows)),
-                  (unsigned)a.c.n_kv, (unsigned)a.c.batch);
+  const int64_t items = (int64_t)((tokens + kTok - 1) / kTok) * a.c.n_kv;
+  TS_UNSUPPORTED(a.c.batch <= 65535 && items < (int64_t)1 << 30, "too many sequences or tokens in one call");
+  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 7) / 8, (16 * sm_count() + a.c.batch - 1) / a.c.batch)),
+                  (unsigned)a.c.batch);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (cache->dtype == TS_BF16) paged_append_kernel<true><<<grid, 256, 0, st>>>(a);
-  else paged_append_kernel<false><<<grid, 256, 0, st>>>(a);
+  const bool rope = rope_cos != nullptr;
+  if (cache->dtype == TS_BF16) {
+    if (rope) paged_append_kernel<true, true><<<grid, 256, 0, st>>>(a);
+    else paged_append_kernel<true, false><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (rope) paged_append_kernel<false, true><<<grid, 256, 0, st>>>(a);
+    else paged_append_kernel<false, false><<<grid, 256, 0, st>>>(a);
+  }
   TS_LAUNCH_CHECK();
   return TS_OK;
 }

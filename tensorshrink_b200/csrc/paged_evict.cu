@@ -28,6 +28,8 @@ namespace paged {
 constexpr int kSelThreads = 1024;
 constexpr int kBins = 2048;
 constexpr int kMoveWarps = 8;
+constexpr int kMoves = 4;              // slots that a warp moves at a time
+constexpr int kSmemKeys = 24 * 1024;   // slots of a select CTA in shared memory
 
 struct EvictArgs {
   Cache c;
@@ -36,9 +38,10 @@ struct EvictArgs {
   int32_t* holes;         // [batch * n_kv][list]
   int32_t* movers;
   int list;
-  uint32_t* keys;         // [batch * n_kv][cap] when they do not fit shared memory, else NULL
+  uint32_t* keys;         // [batch * n_kv][2][cap]: keys and positions that do not fit shared memory
   int64_t cap;
-  int smem_keys;          // keys that fit shared memory
+  int smem_keys;          // slots whose keys and positions fit shared memory
+  int page_shift;         // log2(page_size), or -1
 };
 
 // Monotone key: larger scores have larger keys, -0 equals +0, NaN counts as -inf.
@@ -80,6 +83,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
   __shared__ int hist[kBins];
   __shared__ int warp_tot[33];
   __shared__ int s_newest, s_digit, s_left;
+  pdl_launch_dependents();
   const Cache& c = a.c;
   const int row = blockIdx.x, b = row / c.n_kv, h = row - b * c.n_kv, tid = threadIdx.x;
   const int n = (int)min((int64_t)max(c.seq_lens[b], 0), capacity(c));
@@ -87,28 +91,45 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     if (tid == 0) a.n_move[row] = 0;
     return;
   }
-  uint32_t* keys = n <= a.smem_keys ? skeys : a.keys + (int64_t)row * a.cap;
+  uint32_t* keys = n <= a.smem_keys ? skeys : a.keys + (int64_t)row * a.cap * 2;
+  int32_t* pos = reinterpret_cast<int32_t*>(keys + (n <= a.smem_keys ? a.smem_keys : a.cap));
 
+  // keys and positions, four slots of a thread in flight; the newest position
   if (tid == 0) s_newest = INT_MIN;
   __syncthreads();
   int newest = INT_MIN;
-  for (int i = tid; i < n; i += kSelThreads) {
-    const int page = page_of(c, b, i);
-    if (page >= 0) newest = max(newest, c.slot_pos[stat_at(c, page, h, i % c.page_size)]);
+  for (int i0 = tid; i0 < n; i0 += 4 * kSelThreads) {
+    int64_t at[4];
+    float sc[4];
+    int po[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * kSelThreads, pg = a.page_shift >= 0 ? i >> a.page_shift : i / c.page_size;
+      const int page = i < n ? c.table[b * c.table_stride + pg] : -1;
+      at[k] = (unsigned)page < (unsigned)c.num_pages ? stat_at(c, page, h, i - pg * c.page_size) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (at[k] >= 0) {
+        sc[k] = c.scores[at[k]];
+        po[k] = c.slot_pos[at[k]];
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * kSelThreads;
+      if (i >= n) break;
+      // a slot without memory: key 0, below every score's, and never recent
+      keys[i] = at[k] >= 0 ? key_of(sc[k]) : 0;
+      pos[i] = at[k] >= 0 ? po[k] : INT_MIN;
+      if (at[k] >= 0) newest = max(newest, po[k]);
+    }
   }
   newest = __reduce_max_sync(0xffffffffu, newest);
   if ((tid & 31) == 0) atomicMax(&s_newest, newest);
   __syncthreads();
   const int64_t limit = (int64_t)s_newest - a.recent;
-  for (int i = tid; i < n; i += kSelThreads) {
-    const int page = page_of(c, b, i);
-    uint32_t k = 0;
-    if (page >= 0) {
-      const int64_t at = stat_at(c, page, h, i % c.page_size);
-      k = (int64_t)c.slot_pos[at] > limit ? 0xFF800000u : key_of(c.scores[at]);   // the key of +inf
-    }
-    keys[i] = k;
-  }
+  for (int i = tid; i < n; i += kSelThreads)
+    if ((int64_t)pos[i] > limit && keys[i] != 0) keys[i] = 0xFF800000u;   // recent: the key of +inf
 
   // radix selection of the budget-th largest key
   uint32_t prefix = 0, mask = 0;
@@ -179,26 +200,44 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
 }
 
 __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictArgs a) {
+  pdl_wait_primary();
   const Cache& c = a.c;
   const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv, lane = threadIdx.x & 31;
   const int n = a.n_move[row], chunks = c.head_dim / 8;
   const int32_t* lh = a.holes + (int64_t)row * a.list;
   const int32_t* lm = a.movers + (int64_t)row * a.list;
-  for (int i = blockIdx.x * kMoveWarps + (threadIdx.x >> 5); i < n; i += gridDim.x * kMoveWarps) {
-    const int to = lh[i], from = lm[i];
-    const int pt = page_of(c, b, to), pf = page_of(c, b, from);
-    if (pt < 0 || pf < 0) continue;
-    const int ot = to % c.page_size, of = from % c.page_size;
-    const int64_t rt = row_at(c, pt, h, ot) * 2, rf = row_at(c, pf, h, of) * 2;
-    for (int ch = lane; ch < 2 * chunks; ch += 32) {
-      char* base = ch < chunks ? c.k : c.v;
-      const int64_t e = (ch < chunks ? ch : ch - chunks) * 16;
-      *reinterpret_cast<uint4*>(base + rt + e) = *reinterpret_cast<const uint4*>(base + rf + e);
+  for (int i0 = (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoves; i0 < n; i0 += gridDim.x * kMoveWarps * kMoves) {
+    // lane k looks up target k, lane k + 16 source k
+    int64_t row_off = -1, stat = 0;
+    if ((lane & 15) < kMoves && i0 + (lane & 15) < n) {
+      const int slot = (lane < 16 ? lh : lm)[i0 + (lane & 15)];
+      const int page = page_of(c, b, slot), off = slot % c.page_size;
+      if (page >= 0) {
+        row_off = row_at(c, page, h, off) * 2;
+        stat = stat_at(c, page, h, off);
+      }
     }
-    if (lane == 0) {
-      const int64_t st = stat_at(c, pt, h, ot), sf = stat_at(c, pf, h, of);
-      c.scores[st] = c.scores[sf];
-      c.slot_pos[st] = c.slot_pos[sf];
+    int64_t to[kMoves], from[kMoves];
+#pragma unroll
+    for (int k = 0; k < kMoves; ++k) {
+      to[k] = __shfl_sync(0xffffffffu, row_off, k);
+      from[k] = __shfl_sync(0xffffffffu, row_off, k + 16);
+    }
+    const int64_t src_stat = __shfl_down_sync(0xffffffffu, stat, 16);
+    const int64_t src_off = __shfl_down_sync(0xffffffffu, row_off, 16);
+    if (lane < kMoves && row_off >= 0 && src_off >= 0) {
+      c.scores[stat] = c.scores[src_stat];
+      c.slot_pos[stat] = c.slot_pos[src_stat];
+    }
+    for (int ch = lane; ch < 2 * chunks; ch += 32) {
+      char* base = (ch < chunks ? c.k : c.v) + (ch < chunks ? ch : ch - chunks) * 16;
+      uint4 w[kMoves];
+#pragma unroll
+      for (int k = 0; k < kMoves; ++k)
+        if (to[k] >= 0 && from[k] >= 0) w[k] = *reinterpret_cast<const uint4*>(base + from[k]);
+#pragma unroll
+      for (int k = 0; k < kMoves; ++k)
+        if (to[k] >= 0 && from[k] >= 0) *reinterpret_cast<uint4*>(base + to[k]) = w[k];
     }
   }
   // nothing in this kernel reads the lengths, so they can be set here
@@ -215,12 +254,12 @@ static EvictLayout evict_layout(const ts_paged_cache& p, int budget) {
   EvictLayout L;
   const int64_t cap = (int64_t)p.max_pages * p.page_size, rows = (int64_t)p.batch * p.n_kv;
   L.list = std::max<int64_t>(1, std::min<int64_t>(budget, cap - budget));
-  L.smem_keys = (int)std::min<int64_t>(cap, 48 * 1024);
+  L.smem_keys = (int)std::min<int64_t>(cap, kSmemKeys);
   L.n_move = kCounterBytes;
   L.holes = align_up(L.n_move + rows * 4, 256);
   L.movers = align_up(L.holes + rows * L.list * 4, 256);
   L.keys = align_up(L.movers + rows * L.list * 4, 256);
-  L.bytes = L.keys + (cap > L.smem_keys ? (size_t)rows * cap * 4 : 0);
+  L.bytes = L.keys + (cap > L.smem_keys ? (size_t)rows * cap * 8 : 0);
   return L;
 }
 
@@ -261,22 +300,34 @@ extern "C" int ts_paged_evict(const ts_paged_cache* cache, int budget, int recen
   a.keys = reinterpret_cast<uint32_t*>(ws + L.keys);
   a.cap = cap;
   a.smem_keys = L.smem_keys;
+  a.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (a.c.page_size == 1 << i) a.page_shift = i;
   const int rows = a.c.batch * a.c.n_kv;
   TS_UNSUPPORTED(rows <= 65535, "too many heads in one call");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const size_t smem = (size_t)L.smem_keys * 4;
+  const size_t smem = (size_t)L.smem_keys * 8;
   static thread_local int configured_dev = -1;
   int dev = 0;
   TS_CUDA_TRY(cudaGetDevice(&dev));
   if (configured_dev != dev) {
-    TS_CUDA_TRY(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 48 * 1024 * 4));
+    TS_CUDA_TRY(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemKeys * 8));
     configured_dev = dev;
   }
   evict_select_kernel<<<rows, kSelThreads, smem, st>>>(a);
   TS_LAUNCH_CHECK();
   const int per_row = (int)std::max<int64_t>(
-      1, std::min<int64_t>((L.list + kMoveWarps * 4 - 1) / (kMoveWarps * 4), (8 * sm_count() + rows - 1) / rows));
-  evict_move_kernel<<<dim3(per_row, rows), kMoveWarps * 32, 0, st>>>(a);
+      1, std::min<int64_t>((L.list + kMoveWarps * kMoves - 1) / (kMoveWarps * kMoves), (16 * sm_count() + rows - 1) / rows));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)per_row, (unsigned)rows);
+  cfg.blockDim = dim3(kMoveWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];                         // (it waits for the selection by itself)
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TS_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_move_kernel, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }

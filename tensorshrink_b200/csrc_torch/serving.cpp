@@ -124,12 +124,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_quantize(const at::Tensor& x_
   at::Tensor scales = at::empty({(int64_t)ts_fp4_scales_bytes(rows, cols, (int)format)}, bytes);
   const ts_fp4_tensor t = fp4_view(codes, scales, g.defined() ? OptTensor(g) : c10::nullopt, rows, cols, format, "fp4_quantize");
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-  // the partial maxima lie behind the workspace's counters
-  const size_t at_ = (size_t)ts_serving_counter_bytes(), need = ts_fp4_quantize_workspace_size();
   at::Tensor ws;
-  if (find) ws = workspace(dev, s, at_ + need);
-  done(ts_fp4_quantize(x.data_ptr(), dt, x.stride(0), &t, find, find ? static_cast<char*>(ws.data_ptr()) + at_ : nullptr,
-                       need, s), "fp4_quantize");
+  if (find) ws = workspace(dev, s, ts_fp4_quantize_workspace_size());
+  done(ts_fp4_quantize(x.data_ptr(), dt, x.stride(0), &t, find, find ? ws.data_ptr() : nullptr,
+                       find ? (size_t)ws.numel() : 0, s), "fp4_quantize");
   return {codes, scales, g};
 }
 
