@@ -771,7 +771,13 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
   p.wblocks = (int)((N + kBW - 1) / kBW);
   p.tblocks = (int)((M + p.BT - 1) / p.BT);
   p.ntiles = p.wblocks * p.tblocks;
-  p.grid = (int)std::min<int64_t>((int64_t)p.ntiles * p.kblocks, sms);
+  // Equal shares of all stages for every SM, or, where that occupies two
+  // thirds of them, whole parts of tiles: 1 / parts of a tile's stages per CTA
+  // has fewer pieces to join (1 x 14336 x 4096: 112 whole tiles; 33 x 4096 x
+  // 14336: 32 tiles in 4 parts).
+  const int parts = std::min(p.kblocks, sms / p.ntiles);
+  if (parts >= 1 && p.ntiles * parts * 3 >= sms * 2) p.grid = p.ntiles * parts;
+  else p.grid = (int)std::min<int64_t>((int64_t)p.ntiles * p.kblocks, sms);
   return p;
 }
 

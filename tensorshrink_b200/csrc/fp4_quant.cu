@@ -25,7 +25,7 @@ constexpr int kWarps = 8;
 constexpr int kAmaxSeg = 512;      // columns of a warp's piece of the maximum pass
 constexpr int kSeg = 128;          // columns of a warp's piece, four rows high
 constexpr int kMaxParts = 1184;    // CTAs of the maximum pass at most
-constexpr int kAmaxUnits = 2;      // pieces that a warp has in flight: maximum pass,
+constexpr int kAmaxUnits = 4;      // pieces that a warp has in flight: maximum pass,
 constexpr int kQuantUnits = 2;     // the other passes
 
 struct QuantArgs {
@@ -120,6 +120,14 @@ __device__ __forceinline__ void load16(const void* x, int64_t rows, int64_t cols
     }
     return;
   }
+  if (first + kSeg <= cols && (DT == TS_F32 || AL == 4) && row0 + 96 < rows) {   // whole words of four rows
+    const char* p = reinterpret_cast<const char*>(reinterpret_cast<const T*>(x) + row0 * stride + first) + lane * 4;
+    const int64_t step = stride * 32 * (int64_t)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(p + i / (N / 4) * step + i % (N / 4) * 128));
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int64_t row = row0 + i / (N / 4) * 32;
@@ -140,7 +148,7 @@ __device__ __forceinline__ void load16(const void* x, int64_t rows, int64_t cols
 // per lane, through the warp's 4 rows of shared memory.
 template <int DT, int AL>
 __device__ __forceinline__ void deal(uint32_t* stage, int lane, Lane<DT>& v) {
-  if (AL >= 16) return;
+  if constexpr (AL >= 16) return;
   constexpr int N = Lane<DT>::N;
   __syncwarp();
 #pragma unroll
@@ -413,6 +421,14 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_dequantize_kernel(const Dequa
       for (int i = 0; i < N / 4; ++i)
         reinterpret_cast<uint4*>(st + lane * N)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       __syncwarp();
+      if (first + kSeg <= a.cols && (DT == TS_F32 || AL == 4) && row0 + 96 < a.rows) {   // whole words of four rows
+        char* q = reinterpret_cast<char*>(reinterpret_cast<T*>(a.out) + row0 * a.out_stride + first) + lane * 4;
+        const int64_t step = a.out_stride * 32 * (int64_t)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          *reinterpret_cast<uint32_t*>(q + i / (N / 4) * step + i % (N / 4) * 128) = st[i * 32 + lane];
+        continue;
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int64_t r = row0 + i / (N / 4) * 32;
@@ -457,7 +473,7 @@ static dim3 tile_grid(int64_t rows, int segs) {
 template <int DT, int AL>
 static int launch_amax(const QuantArgs& a, cudaStream_t st) {
   const int64_t units = (int64_t)a.amax_rows * a.amax_segs;
-  const int grid = (int)std::min<int64_t>(std::min(kMaxParts, sm_count() * 8), (units + kWarps - 1) / kWarps);
+  const int grid = (int)std::min<int64_t>(std::min(kMaxParts, sm_count() * 3), (units + kWarps - 1) / kWarps);
   fp4_amax_kernel<DT, AL><<<grid, kWarps * 32, 0, st>>>(a);
   TS_LAUNCH_CHECK();
   return TS_OK;

@@ -25,6 +25,7 @@ struct Cache {
 
 // Checks the description of a cache and fills the device view.
 int make_cache(const ts_paged_cache* c, Cache* out);
+int log2_of(int v);   // -1 of anything but a power of two
 
 __device__ __forceinline__ int64_t capacity(const Cache& c) { return (int64_t)c.max_pages * c.page_size; }
 

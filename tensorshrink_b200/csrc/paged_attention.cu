@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
 // Reads 4 bytes per slot and query head, next to the 4 D bytes per slot that
 // the attention read.
 template <int W>
-__global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256, 6) paged_weights_kernel(const AttnArgs a) {
   pdl_wait_primary();
   const Cache& c = a.c;
   const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv;
@@ -698,10 +698,10 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a) {
     float w[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) w[i] = 0.f;
-    for (int g0 = 0; g0 < a.group; g0 += 8) {
-      float v[8][W], lse[8];
+    for (int g0 = 0; g0 < a.group; g0 += 4) {
+      float v[4][W], lse[4];
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
+      for (int g = 0; g < 4; ++g) {
         if (g0 + g >= a.group) break;
         lse[g] = a.lse2[q + g0 + g];
         const float* src = lg + (g0 + g) * a.logit_stride;
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a) {
         }
       }
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
+      for (int g = 0; g < 4; ++g) {
         if (g0 + g >= a.group) break;
 #pragma unroll
         for (int i = 0; i < W; ++i) w[i] += ex2(v[g][i] - lse[g]);
@@ -749,6 +749,7 @@ struct AppendArgs {
   int64_t rope_rows;
   const float* scores;
   int64_t sb, sh, st;
+  int page_shift;       // log2(page_size), or -1
 };
 
 template <bool BF, bool ROPE>
@@ -766,8 +767,8 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) paged_append_kernel(const A
   for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < items; i += gridDim.x * 8) {
     const int h = i % c.n_kv, t0 = i / c.n_kv * kTok;
     int64_t at[kTok];
-    bool ok[kTok];
-    for (int ch = lane; ch < 2 * chunks; ch += 32) {
+    const int ch0 = lane;
+    for (int ch = ch0; ch < 2 * chunks || ch == ch0; ch += 32) {   // (every lane comes by once, for the look-up)
       const bool is_v = ch >= chunks;
       const int cc = is_v ? ch - chunks : ch;
       const bool hi = cc >= half;
@@ -778,34 +779,33 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) paged_append_kernel(const A
       uint4 w[kTok], p[kTok];
 #pragma unroll
       for (int i = 0; i < kTok; ++i)
-        if (t0 + i < tokens) {
+        if (t0 + i < tokens && ch < 2 * chunks) {
           const uint16_t* r = src + (t0 + i) * step;
           w[i] = *reinterpret_cast<const uint4*>(r + cc * 8);
           if (turn) p[i] = *reinterpret_cast<const uint4*>(r + (hi ? cc - half : cc + half) * 8);
         }
-      if (ch == lane) {
-#pragma unroll
-        for (int i = 0; i < kTok; ++i) {
-          const int64_t slot = (int64_t)len + t0 + i, pos = first + t0 + i;
-          ok[i] = t0 + i < tokens && slot < capacity(c) && (!ROPE || (pos >= 0 && pos < a.rope_rows));
-          at[i] = 0;
-          const int page = ok[i] ? page_of(c, b, (int)slot) : -1;
-          ok[i] = page >= 0;
-          if (ok[i]) {
-            const int off = (int)slot % c.page_size;
-            at[i] = row_at(c, page, h, off);
-            if (lane == 0) {
-              const int64_t sa = stat_at(c, page, h, off);
-              if (c.scores != nullptr)
-                c.scores[sa] = a.scores != nullptr ? a.scores[b * a.sb + h * a.sh + (t0 + i) * a.st] : 0.f;
-              if (c.slot_pos != nullptr) c.slot_pos[sa] = (int32_t)pos;
-            }
+      if (ch == ch0) {
+        // lane i (< kTok) looks token i up
+        const int t = t0 + lane;
+        const int64_t slot = (int64_t)len + t, pos = first + t;
+        int64_t mine = -1;
+        if (lane < kTok && t < tokens && slot < capacity(c) && (!ROPE || (pos >= 0 && pos < a.rope_rows))) {
+          const int pg = a.page_shift >= 0 ? (int)slot >> a.page_shift : (int)slot / c.page_size;
+          const int page = c.table[b * c.table_stride + pg], off = (int)slot - pg * c.page_size;
+          if ((unsigned)page < (unsigned)c.num_pages) {
+            mine = row_at(c, page, h, off);
+            const int64_t sa = stat_at(c, page, h, off);
+            if (c.scores != nullptr) c.scores[sa] = a.scores != nullptr ? a.scores[b * a.sb + h * a.sh + t * a.st] : 0.f;
+            if (c.slot_pos != nullptr) c.slot_pos[sa] = (int32_t)pos;
           }
         }
+#pragma unroll
+        for (int i = 0; i < kTok; ++i) at[i] = __shfl_sync(0xffffffffu, mine, i);
       }
+      if (ch >= 2 * chunks) break;
 #pragma unroll
       for (int i = 0; i < kTok; ++i) {
-        if (!ok[i]) continue;
+        if (at[i] < 0) continue;
         if (turn) {
           const int64_t j = (first + t0 + i) * (D / 2) + (hi ? cc - half : cc) * 8;
           const float* cs = a.cos_t + j;
@@ -855,6 +855,13 @@ int make_cache(const ts_paged_cache* p, Cache* o) {
   o->num_pages = p->num_pages;
   o->max_pages = p->max_pages;
   return TS_OK;
+}
+
+// log2 of a power of two, -1 of anything else.
+int log2_of(int v) {
+  for (int i = 0; i < 31; ++i)
+    if (v == 1 << i) return i;
+  return -1;
 }
 
 static size_t grid_of(int head_dim) { return (size_t)sm_count() * (head_dim > 128 ? 1 : head_dim > 64 ? 2 : 3); }
@@ -956,9 +963,7 @@ extern "C" int ts_paged_decode_attention(const void* qkv, int64_t qkv_row_stride
   a.lse2 = accumulate ? reinterpret_cast<float*>(ws + L.lse) : nullptr;
   a.logits = accumulate ? reinterpret_cast<float*>(ws + L.logits) : nullptr;
   a.logit_stride = L.logit_stride;
-  a.page_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if (a.c.page_size == 1 << i) a.page_shift = i;
+  a.page_shift = log2_of(a.c.page_size);
   a.one_page = a.c.page_size % kRows == 0 ? 1 : 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int grid = (int)grid_of(a.c.head_dim);
@@ -1013,6 +1018,7 @@ extern "C" int ts_paged_append(const void* k, const int64_t* k_strides, const vo
   a.sb = scores ? score_strides[0] : 0;
   a.sh = scores ? score_strides[1] : 0;
   a.st = scores ? score_strides[2] : 0;
+  a.page_shift = log2_of(a.c.page_size);
   const int64_t items = (int64_t)((tokens + kTok - 1) / kTok) * a.c.n_kv;
   TS_UNSUPPORTED(a.c.batch <= 65535 && items < (int64_t)1 << 30, "too many sequences or tokens in one call");
   const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 7) / 8, (16 * sm_count() + a.c.batch - 1) / a.c.batch)),

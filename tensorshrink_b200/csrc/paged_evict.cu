@@ -28,7 +28,7 @@ namespace paged {
 constexpr int kSelThreads = 1024;
 constexpr int kBins = 2048;
 constexpr int kMoveWarps = 8;
-constexpr int kMoves = 4;              // slots that a warp moves at a time
+constexpr int kMoves = 8;              // slots that a warp moves at a time
 constexpr int kSmemKeys = 24 * 1024;   // slots of a select CTA in shared memory
 
 struct EvictArgs {
@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
 }
 
 __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictArgs a) {
+  __shared__ int64_t where[kMoveWarps][2 * kMoves];
   pdl_wait_primary();
   const Cache& c = a.c;
   const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv, lane = threadIdx.x & 31;
@@ -217,28 +218,28 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const Evict
         stat = stat_at(c, page, h, off);
       }
     }
-    int64_t to[kMoves], from[kMoves];
-#pragma unroll
-    for (int k = 0; k < kMoves; ++k) {
-      to[k] = __shfl_sync(0xffffffffu, row_off, k);
-      from[k] = __shfl_sync(0xffffffffu, row_off, k + 16);
-    }
     const int64_t src_stat = __shfl_down_sync(0xffffffffu, stat, 16);
     const int64_t src_off = __shfl_down_sync(0xffffffffu, row_off, 16);
     if (lane < kMoves && row_off >= 0 && src_off >= 0) {
       c.scores[stat] = c.scores[src_stat];
       c.slot_pos[stat] = c.slot_pos[src_stat];
     }
+    const unsigned moves = __ballot_sync(0xffffffffu, lane < kMoves && row_off >= 0 && src_off >= 0);
+    // the rows' places, read back by every lane
+    int64_t* to = where[threadIdx.x >> 5], *from = to + kMoves;
+    if ((lane & 15) < kMoves) to[(lane >> 4) * kMoves + (lane & 15)] = row_off;
+    __syncwarp();
     for (int ch = lane; ch < 2 * chunks; ch += 32) {
       char* base = (ch < chunks ? c.k : c.v) + (ch < chunks ? ch : ch - chunks) * 16;
       uint4 w[kMoves];
 #pragma unroll
       for (int k = 0; k < kMoves; ++k)
-        if (to[k] >= 0 && from[k] >= 0) w[k] = *reinterpret_cast<const uint4*>(base + from[k]);
+        if ((moves >> k) & 1) w[k] = *reinterpret_cast<const uint4*>(base + from[k]);
 #pragma unroll
       for (int k = 0; k < kMoves; ++k)
-        if (to[k] >= 0 && from[k] >= 0) *reinterpret_cast<uint4*>(base + to[k]) = w[k];
+        if ((moves >> k) & 1) *reinterpret_cast<uint4*>(base + to[k]) = w[k];
     }
+    __syncwarp();
   }
   // nothing in this kernel reads the lengths, so they can be set here
   if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0 && c.seq_lens[b] > a.budget) c.seq_lens[b] = a.budget;
@@ -300,9 +301,7 @@ extern "C" int ts_paged_evict(const ts_paged_cache* cache, int budget, int recen
   a.keys = reinterpret_cast<uint32_t*>(ws + L.keys);
   a.cap = cap;
   a.smem_keys = L.smem_keys;
-  a.page_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if (a.c.page_size == 1 << i) a.page_shift = i;
+  a.page_shift = log2_of(a.c.page_size);
   const int rows = a.c.batch * a.c.n_kv;
   TS_UNSUPPORTED(rows <= 65535, "too many heads in one call");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
