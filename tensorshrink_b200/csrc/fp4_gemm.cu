@@ -363,29 +363,30 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
       if (r == 0) a.counters[x.tile] = 0;
       if (!valid) continue;
       // the tile's beginning lies in its CTA's second slot, the other pieces
-      // in their CTAs' first; 16 tokens of 4 pieces in flight
+      // in their CTAs' first; kRun tokens of 4 pieces in flight
       constexpr int kPiece4 = BT * kBW / 4;
       const float4* base = reinterpret_cast<const float4*>(a.partials) + (size_t)c_first * 2 * kPiece4 + r;
       const int pieces = c_last - c_first + 1;
-      for (int j0 = 0; j0 < jn_all; j0 += 16) {
-        float4 sum[4];
+      constexpr int kRun = BT < 32 ? BT : 32, kRun4 = kRun / 4;   // tokens of a round
+      for (int j0 = 0; j0 < jn_all; j0 += kRun) {
+        float4 sum[kRun4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int u = 0; u < kRun4; ++u) sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int c = 0; c < pieces; c += 4) {
           // (tokens behind the last one were not written: read, never stored)
-          float4 t[4][4];
+          float4 t[4][kRun4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int cc = min(c + i, pieces - 1);
             const float4* src = base + (cc == 0 ? (size_t)kPiece4 : (size_t)cc * 2 * kPiece4) + (size_t)(j0 / 4) * kBW;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) t[i][u] = __ldcg(src + u * kBW);
+            for (int u = 0; u < kRun4; ++u) t[i][u] = __ldcg(src + u * kBW);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (c + i >= pieces) break;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < kRun4; ++u) {
               sum[u].x += t[i][u].x;
               sum[u].y += t[i][u].y;
               sum[u].z += t[i][u].z;
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
         }
         const float* f = reinterpret_cast<const float*>(sum);
 #pragma unroll
-        for (int u = 0; u < 16; ++u)
+        for (int u = 0; u < kRun; ++u)
           if (j0 + u < jn_all)
             store_f(a.out, a.out_dtype, (m0 + j0 + u) * a.out_stride + n, fmaf(f[u], alpha, bias));
       }
@@ -421,7 +422,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
 // and MMAs for both; commits release the stage in both. Tokens are the
 // accumulator's lanes, so that a thread stores runs of its token's outputs.
 
-constexpr int BN = 256;
+constexpr int BN = 256, kHalf = BN / 2;
+constexpr int kPairEpi = 8, kPairThreads = (2 + kPairEpi) * 32;
 
 template <bool NV>
 struct Pair {
@@ -453,6 +455,34 @@ struct PairArgs {
   uint64_t wait_ns;
   int stall, overlap;
 };
+
+// 64 consecutive fp32 columns of this warp's TMEM lane quadrant, both halves in flight.
+__device__ __forceinline__ void tmem_ld32x2(uint32_t taddr, float (&a)[32], float (&b)[32]) {
+  uint32_t r[64];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t* q = r + 32 * h;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
+          "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]),
+          "=r"(q[15]), "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]),
+          "=r"(q[22]), "=r"(q[23]), "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]),
+          "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
+        : "r"(taddr + 32 * h));
+  }
+  // the registers are written when the wait returns: it takes and gives them
+  // back, so that no use moves before it
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(r[i]));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    a[i] = __uint_as_float(r[i]);
+    b[i] = __uint_as_float(r[32 + i]);
+  }
+}
 
 __device__ __forceinline__ uint32_t cta_rank() {
   uint32_t r;
@@ -506,7 +536,7 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
 }
 
 template <bool NV>
-__global__ void __launch_bounds__(kThreads) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
     fp4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                     const __grid_constant__ CUtensorMap asmap, const __grid_constant__ CUtensorMap bsmap,
                     const PairArgs a) {
@@ -540,7 +570,7 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(2, 1, 1)
       mbar_init(empty + i, 1);
     }
     mbar_init(tfull, 1);
-    mbar_init(tempty, 2 * kEpiWarps);
+    mbar_init(tempty, 2 * kPairEpi);
     mbar_init(drain, 1);
     fence_barrier_init();
   }
@@ -656,25 +686,26 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(2, 1, 1)
       mbar_wait_hint(drain, 0, nullptr, 0, a.wait_ns);
     }
   } else {
-    const int quad = warp & 3;
+    // two warps per quadrant of TMEM lanes, each with half of the columns
+    const int quad = warp & 3, half = (warp - 2) >> 2;
     const float alpha = usable_scale(a.wg) * usable_scale(a.xg);
-    const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf;
     const uint32_t free_bar = map_cta(smem_u32(tempty), 0);
     int n = 0;
     for (int tile = pair; tile < ntiles; tile += pairs, ++n) {
       const int64_t m = (int64_t)(tile % a.mblocks) * 256 + rank * 128 + quad * 32 + lane;
-      const int64_t n0 = (int64_t)(tile / a.mblocks) * BN;
-      const int cols = (int)min((int64_t)BN, a.N - n0);
+      const int64_t n0 = (int64_t)(tile / a.mblocks) * BN + half * kHalf;
+      const int cols = (int)max((int64_t)0, min((int64_t)kHalf, a.N - n0));
       const bool got = mbar_wait_hint(tfull, n & 1, &g_err, 34, a.wait_ns);
       if (!__all_sync(0xffffffffu, got)) break;
       tc_fence_after();
       if (a.out_dtype == TS_F32) {
         float* row = reinterpret_cast<float*>(a.out) + m * a.out_stride + n0;
 #pragma unroll 1
-        for (int c = 0; c < BN / 32; ++c) {
+        for (int c = 0; c < kHalf / 32; ++c) {
           float v[32];
           tmem_ld32(acc + c * 32, v);
-          if (c == BN / 32 - 1) {
+          if (c == kHalf / 32 - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_cluster(free_bar);
@@ -690,11 +721,12 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(2, 1, 1)
       }
       // 16-bit outputs wait in registers, so that the accumulator is free
       // again before the first of them is stored
-      uint32_t w[BN / 2];
+      uint32_t w[kHalf / 2];
+      float vv[2][32];
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c) {
-        float v[32];
-        tmem_ld32(acc + c * 32, v);
+      for (int c = 0; c < kHalf / 32; ++c) {
+        float (&v)[32] = vv[c & 1];
+        if ((c & 1) == 0) tmem_ld32x2(acc + c * 32, vv[0], vv[1]);   // two loads in flight
         if (a.bias != nullptr) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -723,12 +755,12 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(2, 1, 1)
       uint16_t* row = reinterpret_cast<uint16_t*>(a.out) + m * a.out_stride + n0;
       if (a.vec) {
 #pragma unroll
-        for (int i = 0; i < BN / 8; ++i)
+        for (int i = 0; i < kHalf / 8; ++i)
           if (i * 8 < cols)   // N is a multiple of 8 here
             *reinterpret_cast<uint4*>(row + i * 8) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       } else {
 #pragma unroll
-        for (int i = 0; i < BN / 2; ++i) {
+        for (int i = 0; i < kHalf / 2; ++i) {
           if (2 * i < cols) row[2 * i] = (uint16_t)w[i];
           if (2 * i + 1 < cols) row[2 * i + 1] = (uint16_t)(w[i] >> 16);
         }
@@ -784,10 +816,10 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
 // Launch; with `overlap` the kernel may start while the one before it (which
 // allows that, and whose results it waits for by itself) still runs.
 template <typename K, typename... Args>
-static cudaError_t launch_after(K k, int grid, size_t smem, cudaStream_t st, int overlap, const Args&... args) {
+static cudaError_t launch_after(K k, int grid, int threads, size_t smem, cudaStream_t st, int overlap, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -810,7 +842,7 @@ static int launch_pair(const CUtensorMap (&m)[4], const PairArgs& a, int grid, c
     TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_dev = dev;
   }
-  TS_CUDA_TRY(launch_after(k, grid, smem, st, a.overlap, m[0], m[1], m[2], m[3], a));
+  TS_CUDA_TRY(launch_after(k, grid, kPairThreads, smem, st, a.overlap, m[0], m[1], m[2], m[3], a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
@@ -834,7 +866,7 @@ static int launch(const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& 
     TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_dev = dev;
   }
-  TS_CUDA_TRY(launch_after(k, grid, smem, st, a.overlap, wm, xm, a));
+  TS_CUDA_TRY(launch_after(k, grid, kThreads, smem, st, a.overlap, wm, xm, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }

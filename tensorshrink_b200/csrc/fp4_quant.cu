@@ -5,10 +5,10 @@
 // an mxfp4 block, whose two lanes share their maximum. A CTA's eight warps take
 // eight neighbouring such rows, so that its scales are whole 128-byte lines.
 // Rows that start on 32 or 16 bytes are read with loads that wide; the others
-// word by word or element by element, coalesced, through shared memory. Bound
-// by DRAM traffic: x is read once (twice when the tensor's scale is sought, the
-// second time from the end, so that what the first pass left in L2 is found
-// there), 0.5625 (0.53) bytes an element are written.
+// word by word, coalesced, through shared memory. Bound by DRAM traffic: x is
+// read once (twice when the tensor's scale is sought, the second time from the
+// end, so that what the first pass left in L2 is found there), 0.5625 (0.53)
+// bytes an element are written.
 //
 // Every rounding is spelled out (a reciprocal and products rounded to fp32,
 // two conversions to nearest even), so codes are reproducible bit for bit
@@ -25,8 +25,7 @@ constexpr int kWarps = 8;
 constexpr int kAmaxSeg = 512;      // columns of a warp's piece of the maximum pass
 constexpr int kSeg = 128;          // columns of a warp's piece, four rows high
 constexpr int kMaxParts = 1184;    // CTAs of the maximum pass at most
-constexpr int kAmaxUnits = 4;      // pieces that a warp has in flight: maximum pass,
-constexpr int kQuantUnits = 2;     // the other passes
+constexpr int kAmaxUnits = 4;      // pieces that a warp of the maximum pass has in flight
 
 struct QuantArgs {
   const void* x;
@@ -76,70 +75,98 @@ __device__ __forceinline__ void st32(void* p, const uint32_t* w) {
                : "memory");
 }
 
-// A lane's 16 elements as words (8, or 16 of fp32).
+// A lane's 16 elements as words (8, or 16 of fp32); of rows that start in the
+// middle of a word, also the first element of row `lane` (lanes 0 to 3).
 template <int DT>
 struct Lane {
   static constexpr int N = DT == TS_F32 ? 16 : 8;
   uint32_t w[N];
+  uint32_t e;
 };
 
-// Reads the columns [first, first + 128) of the warp's four rows, row0 + 32 q
-// (zeros behind the last column and where a row does not exist). AL: the
-// alignment of rows. With 32 or 16, eight lanes read a row, 16 consecutive
-// columns each. Otherwise all 32 lanes read one row after the other, in words
-// (4) or elements, and deal() sorts them.
+// Where a lane reads (or writes) its share of a warp's four rows, row0 + 32 q.
+// AL: the alignment of rows. With 32 or 16, eight lanes take a row, 16
+// consecutive columns each. With 4, all 32 lanes take one row after the other
+// in words, and deal() sorts them. With 2 (16-bit elements) the four rows may
+// start in the middle of a word: the words are then those behind the first
+// element.
 template <int DT, int AL>
-__device__ __forceinline__ void load16(const void* x, int64_t rows, int64_t cols, int64_t stride, int64_t row0,
-                                       int64_t first, int lane, Lane<DT>& v) {
+struct Place {
+  using T = typename Elem<DT>::T;
+  const char* p;     // this lane's place in columns 0 .. 127
+  int64_t step;      // bytes from one of the four rows to the next (AL < 16)
+  int rows;          // of the four, how many exist (AL >= 16: whether this lane's does)
+  int mid;           // the rows start in the middle of a word
+  __device__ __forceinline__ Place(const void* x, int64_t n_rows, int64_t stride, int64_t row0, int lane) {
+    const T* t = reinterpret_cast<const T*>(x);
+    const int64_t left = n_rows - row0;
+    mid = 0;
+    if (AL >= 16) {
+      p = reinterpret_cast<const char*>(t + (row0 + (lane >> 3) * 32) * stride + (lane & 7) * 16);
+      rows = left > (lane >> 3) * 32;
+    } else {
+      const T* r = t + row0 * stride;
+      if (AL == 2) mid = (int)(reinterpret_cast<uintptr_t>(r) >> 1) & 1;
+      p = reinterpret_cast<const char*>(r + mid) + lane * 4;
+      rows = left > 96 ? 4 : left > 64 ? 3 : left > 32 ? 2 : left > 0 ? 1 : 0;
+    }
+    step = stride * 32 * (int64_t)sizeof(T);
+  }
+};
+
+// Reads columns [first, first + 128), of which `left` exist (zeros for the
+// others and for rows that do not exist).
+template <int DT, int AL>
+__device__ __forceinline__ void load16(const Place<DT, AL>& w, int64_t first, int64_t left64, int lane, Lane<DT>& v) {
   using T = typename Elem<DT>::T;
   constexpr int N = Lane<DT>::N;
+  const int left = (int)min((int64_t)kSeg + 1, left64);
+  const char* p = w.p + first * (int)sizeof(T);
+  v.e = 0;
+  if (AL == 2 && w.mid && lane < w.rows && left > 0)
+    v.e = *reinterpret_cast<const T*>(p - lane * 4 - 2 + lane * w.step);
+  if (left >= kSeg + w.mid && (AL >= 16 ? w.rows : w.rows == 4)) {
+    if constexpr (AL == 32) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v.w[i] = 0;
-  if (AL >= 16) {
-    const int64_t row = row0 + (lane >> 3) * 32, c0 = first + (lane & 7) * 16;
-    if (row >= rows) return;
-    const T* p = reinterpret_cast<const T*>(x) + row * stride;
-    if (c0 + 16 <= cols) {
-      if (AL == 32) {
+      for (int i = 0; i < N / 8; ++i) ld32(p + 32 * i, *reinterpret_cast<uint32_t(*)[8]>(v.w + 8 * i));
+    } else if constexpr (AL == 16) {
 #pragma unroll
-        for (int i = 0; i < N / 8; ++i) ld32(reinterpret_cast<const char*>(p + c0) + 32 * i, *reinterpret_cast<uint32_t(*)[8]>(v.w + 8 * i));
-      } else {
-#pragma unroll
-        for (int i = 0; i < N / 4; ++i) {
-          const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + c0) + i);
-          v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
-        }
+      for (int i = 0; i < N / 4; ++i) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (c0 + i < cols) {
-          if (DT == TS_F32) v.w[i % N] = (uint32_t)p[c0 + i];
-          else v.w[(i / 2) % N] |= (uint32_t)p[c0 + i] << (16 * (i & 1));
-        }
+      for (int i = 0; i < N; ++i)
+        v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(p + i / (N / 4) * w.step + i % (N / 4) * 128));
     }
     return;
   }
-  if (first + kSeg <= cols && (DT == TS_F32 || AL == 4) && row0 + 96 < rows) {   // whole words of four rows
-    const char* p = reinterpret_cast<const char*>(reinterpret_cast<const T*>(x) + row0 * stride + first) + lane * 4;
-    const int64_t step = stride * 32 * (int64_t)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(p + i / (N / 4) * step + i % (N / 4) * 128));
-    return;
-  }
+  for (int i = 0; i < N; ++i) v.w[i] = 0;
+  if constexpr (AL >= 16) {
+    if (!w.rows) return;
+    const T* t = reinterpret_cast<const T*>(p);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t row = row0 + i / (N / 4) * 32;
-    if (row >= rows) break;
-    const T* p = reinterpret_cast<const T*>(x) + row * stride;
-    const int word = i % (N / 4) * 32 + lane;
-    if (DT == TS_F32) {
-      if (first + word < cols) v.w[i] = (uint32_t)p[first + word];
-    } else {
-      const int64_t c = first + word * 2;   // the word of columns c, c + 1
-      if (AL == 4 && c + 1 < cols) v.w[i] = __ldg(reinterpret_cast<const uint32_t*>(p + c));
-      else if (c < cols) v.w[i] = (uint32_t)p[c] | (c + 1 < cols ? (uint32_t)p[c + 1] << 16 : 0);
+    for (int i = 0; i < 16; ++i)
+      if ((lane & 7) * 16 + i < left) {
+        if (DT == TS_F32) v.w[i % N] = (uint32_t)t[i];
+        else v.w[(i / 2) % N] |= (uint32_t)t[i] << (16 * (i & 1));
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i / (N / 4) >= w.rows) break;
+      const char* q = p + i / (N / 4) * w.step + i % (N / 4) * 128;
+      const int word = i % (N / 4) * 32 + lane;
+      if (DT == TS_F32) {
+        if (word < left) v.w[i] = *reinterpret_cast<const uint32_t*>(q);
+      } else {
+        const T* t = reinterpret_cast<const T*>(q);
+        const int c = 2 * word + w.mid;               // the word's columns: c, c + 1
+        if (c < left) v.w[i] = (uint32_t)t[0];
+        if (c + 1 < left) v.w[i] |= (uint32_t)t[1] << 16;
+      }
     }
   }
 }
@@ -147,12 +174,23 @@ __device__ __forceinline__ void load16(const void* x, int64_t rows, int64_t cols
 // From the order that load16 read words in (AL < 16) to 16 consecutive columns
 // per lane, through the warp's 4 rows of shared memory.
 template <int DT, int AL>
-__device__ __forceinline__ void deal(uint32_t* stage, int lane, Lane<DT>& v) {
+__device__ __forceinline__ void deal(const Place<DT, AL>& place, uint32_t* stage, int lane, Lane<DT>& v) {
   if constexpr (AL >= 16) return;
   constexpr int N = Lane<DT>::N;
   __syncwarp();
+  if (AL == 2 && place.mid) {
+    uint16_t* s = reinterpret_cast<uint16_t*>(stage);
 #pragma unroll
-  for (int i = 0; i < N; ++i) stage[i * 32 + lane] = v.w[i];
+    for (int i = 0; i < N; ++i) {
+      const int c = 2 * (i % (N / 4) * 32 + lane) + 1, r = i / (N / 4) * kSeg;
+      s[r + c] = (uint16_t)v.w[i];
+      if (c + 1 < kSeg) s[r + c + 1] = (uint16_t)(v.w[i] >> 16);
+    }
+    if (lane < 4) s[lane * kSeg] = (uint16_t)v.e;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) stage[i * 32 + lane] = v.w[i];
+  }
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < N / 4; ++i) {
@@ -278,7 +316,7 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_amax_kernel(const QuantArgs a
 }
 
 template <int DT, bool NV, int AL>
-__global__ void __launch_bounds__(kWarps * 32) fp4_quantize_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, DT == TS_F32 ? 6 : 7) fp4_quantize_kernel(const QuantArgs a) {
   using E = Elem<DT>;
   __shared__ __align__(16) uint32_t stage[AL >= 16 ? 1 : kWarps][AL >= 16 ? 4 : 32 * Lane<DT>::N];
   pdl_launch_dependents();
@@ -289,52 +327,46 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_quantize_kernel(const QuantAr
   const int64_t row0 = (int64_t)(bx >> 2) * kTileRows + (bx & 3) * 8 + warp, row = row0 + (lane >> 3) * 32;
   if (row0 >= a.rows) return;
   const bool exists = row < a.rows;
-  for (int s0 = blockIdx.y; s0 < a.segs; s0 += kQuantUnits * gridDim.y) {
-    Lane<DT> vv[kQuantUnits];
-#pragma unroll
-    for (int k = 0; k < kQuantUnits; ++k) {
-      const int s = s0 + k * gridDim.y, seg = a.reverse ? a.segs - 1 - s : s;
-      load16<DT, AL>(a.x, s < a.segs ? a.rows : 0, a.cols, a.stride, row0, (int64_t)seg * kSeg, lane, vv[k]);
+  const Place<DT, AL> src(a.x, a.rows, a.stride, row0, lane);
+  uint8_t* codes = a.codes + row * a.row_bytes + (lane & 7) * 8;
+  uint8_t* scales = a.scales + scale_at(row, NV ? lane & 7 : (lane & 7) >> 1, a.kt);
+  const int groups = (int)(a.row_bytes / 8);             // of 16 columns
+  for (int s = blockIdx.y; s < a.segs; s += gridDim.y) {
+    const int seg = a.reverse ? a.segs - 1 - s : s;
+    Lane<DT> v;
+    load16<DT, AL>(src, (int64_t)seg * kSeg, a.cols - (int64_t)seg * kSeg, lane, v);
+    deal<DT, AL>(src, stage[AL >= 16 ? 0 : warp], lane, v);
+    uint32_t top = top_bits<DT>(v);
+    if (!NV) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const bool bad = top >= E::kInf;
+    const float amax = E::f((typename E::T)top);
+    float r;
+    uint32_t sc;
+    if (NV) {
+      sc = __nv_cvt_float_to_fp8(fminf(__fmul_rn(amax, to_scale), 448.f), __NV_SATFINITE, __NV_E4M3);
+      const float sf = e4m3_value((uint8_t)sc);
+      r = sf > 0.f ? __frcp_rn(__fmul_rn(sf, g)) : 0.f;
+    } else {
+      const int e = (int)(__float_as_uint(amax) >> 23) - 2;
+      sc = (uint32_t)max(e, 0);
+      r = __uint_as_float((254u - sc) << 23);
     }
+    uint2 out = make_uint2(0, 0);
+    if (bad) {
+      sc = NV ? 0x7Fu : 0xFFu;
+    } else {
+      float f[8];
 #pragma unroll
-    for (int k = 0; k < kQuantUnits; ++k) {
-      const int s = s0 + k * gridDim.y, seg = a.reverse ? a.segs - 1 - s : s;
-      if (s >= a.segs) break;
-      Lane<DT>& v = vv[k];
-      deal<DT, AL>(stage[AL >= 16 ? 0 : warp], lane, v);
-      uint32_t top = top_bits<DT>(v);
-      if (!NV) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      const bool bad = top >= E::kInf;
-      const float amax = E::f((typename E::T)top);
-      float r;
-      uint32_t sc;
-      if (NV) {
-        sc = __nv_cvt_float_to_fp8(fminf(__fmul_rn(amax, to_scale), 448.f), __NV_SATFINITE, __NV_E4M3);
-        const float sf = e4m3_value((uint8_t)sc);
-        r = sf > 0.f ? __frcp_rn(__fmul_rn(sf, g)) : 0.f;
-      } else {
-        const int e = (int)(__float_as_uint(amax) >> 23) - 2;
-        sc = (uint32_t)max(e, 0);
-        r = __uint_as_float((254u - sc) << 23);
-      }
-      uint2 out = make_uint2(0, 0);
-      if (bad) {
-        sc = NV ? 0x7Fu : 0xFFu;
-      } else {
-        float f[8];
+      for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, i);
+      out.x = to_e2m1x8(f, r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, i);
-        out.x = to_e2m1x8(f, r);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, 8 + i);
-        out.y = to_e2m1x8(f, r);
-      }
-      const int64_t group = (int64_t)seg * 8 + (lane & 7);   // of 16 columns
-      if (exists && group * 8 < a.row_bytes) {
-        *reinterpret_cast<uint2*>(a.codes + row * a.row_bytes + group * 8) = out;
-        if (NV) a.scales[scale_at(row, group, a.kt)] = (uint8_t)sc;
-        else if ((lane & 1) == 0) a.scales[scale_at(row, group >> 1, a.kt)] = (uint8_t)sc;
-      }
+      for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, 8 + i);
+      out.y = to_e2m1x8(f, r);
+    }
+    if (exists && seg * 8 + (lane & 7) < groups) {
+      *reinterpret_cast<uint2*>(codes + (int64_t)seg * 64) = out;
+      // 128 columns are two scale tiles of nvfp4, one of mxfp4
+      if (NV || (lane & 1) == 0) scales[(int64_t)seg * (NV ? 2 : 1) * kTileBytes] = (uint8_t)sc;
     }
   }
 }
@@ -349,7 +381,7 @@ struct DequantArgs {
 };
 
 template <int DT, bool NV, int AL>
-__global__ void __launch_bounds__(kWarps * 32) fp4_dequantize_kernel(const DequantArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, 7) fp4_dequantize_kernel(const DequantArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int N = Lane<DT>::N;
   __shared__ __align__(16) uint32_t stage[AL >= 16 ? 1 : kWarps][AL >= 16 ? 4 : 32 * N];
@@ -358,94 +390,91 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_dequantize_kernel(const Dequa
   const int64_t row0 = (int64_t)(blockIdx.x >> 2) * kTileRows + (blockIdx.x & 3) * 8 + warp, row = row0 + (lane >> 3) * 32;
   if (row0 >= a.rows) return;
   const bool exists = row < a.rows;
-  for (int s0 = blockIdx.y; s0 < a.segs; s0 += kQuantUnits * gridDim.y) {
-    uint2 w[kQuantUnits];
-    uint8_t sb[kQuantUnits];
+  const Place<DT, AL> dst(a.out, a.rows, a.out_stride, row0, lane);
+  const uint8_t* codes = a.codes + row * a.row_bytes + l8 * 8;
+  const uint8_t* scales = a.scales + scale_at(row, NV ? l8 : l8 >> 1, a.kt);
+  const int groups = (int)(a.row_bytes / 8);             // of 16 columns
+  for (int seg = blockIdx.y; seg < a.segs; seg += gridDim.y) {
+    uint2 w = make_uint2(0, 0);
+    uint8_t sb = 0;
+    if (exists && seg * 8 + l8 < groups) {
+      w = __ldg(reinterpret_cast<const uint2*>(codes + (int64_t)seg * 64));
+      sb = __ldg(scales + (int64_t)seg * (NV ? 2 : 1) * kTileBytes);
+    }
+    const float s = NV ? __fmul_rn(e4m3_value(sb), g) : e8m0_value(sb);
+    uint32_t h[8];
+    from_e2m1x8(w.x, *reinterpret_cast<uint32_t(*)[4]>(h));
+    from_e2m1x8(w.y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
+    __align__(16) uint32_t v[N];
 #pragma unroll
-    for (int k = 0; k < kQuantUnits; ++k) {
-      const int64_t group = (int64_t)(s0 + k * gridDim.y) * 8 + l8;
-      w[k] = make_uint2(0, 0);
-      sb[k] = 0;
-      if (exists && group * 8 < a.row_bytes) {
-        w[k] = __ldg(reinterpret_cast<const uint2*>(a.codes + row * a.row_bytes + group * 8));
-        sb[k] = __ldg(a.scales + scale_at(row, NV ? group : group >> 1, a.kt));
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+      const float y0 = __fmul_rn(f.x, s), y1 = __fmul_rn(f.y, s);
+      if (DT == TS_F32) {
+        v[(2 * i) % N] = __float_as_uint(y0);
+        v[(2 * i + 1) % N] = __float_as_uint(y1);
+      } else if (DT == TS_BF16) {
+        const __nv_bfloat162 b2 = __floats2bfloat162_rn(y0, y1);
+        v[i] = *reinterpret_cast<const uint32_t*>(&b2);
+      } else {
+        const __half2 b2 = __floats2half2_rn(y0, y1);
+        v[i] = *reinterpret_cast<const uint32_t*>(&b2);
       }
     }
+    const int64_t first = (int64_t)seg * kSeg;
+    const int left = (int)min((int64_t)kSeg, a.cols - first);
+    char* p = const_cast<char*>(dst.p) + first * (int)sizeof(T);
+    if constexpr (AL >= 16) {
+      if (!dst.rows) continue;
+      if (left == kSeg) {
+        if constexpr (AL == 32) {
 #pragma unroll
-    for (int k = 0; k < kQuantUnits; ++k) {
-      const int seg = s0 + k * gridDim.y;
-      if (seg >= a.segs) break;
-      const float s = NV ? __fmul_rn(e4m3_value(sb[k]), g) : e8m0_value(sb[k]);
-      uint32_t h[8];
-      from_e2m1x8(w[k].x, *reinterpret_cast<uint32_t(*)[4]>(h));
-      from_e2m1x8(w[k].y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
-      __align__(16) uint32_t v[N];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-        const float y0 = __fmul_rn(f.x, s), y1 = __fmul_rn(f.y, s);
-        if (DT == TS_F32) {
-          v[(2 * i) % N] = __float_as_uint(y0);
-          v[(2 * i + 1) % N] = __float_as_uint(y1);
-        } else if (DT == TS_BF16) {
-          const __nv_bfloat162 b2 = __floats2bfloat162_rn(y0, y1);
-          v[i] = *reinterpret_cast<const uint32_t*>(&b2);
-        } else {
-          const __half2 b2 = __floats2half2_rn(y0, y1);
-          v[i] = *reinterpret_cast<const uint32_t*>(&b2);
-        }
-      }
-      T* p = reinterpret_cast<T*>(a.out) + row * a.out_stride;
-      const int64_t first = (int64_t)seg * kSeg, c0 = first + l8 * 16;
-      if (AL >= 16) {
-        if (!exists) continue;
-        if (c0 + 16 <= a.cols) {
-          if (AL == 32) {
-#pragma unroll
-            for (int i = 0; i < N / 8; ++i) st32(reinterpret_cast<char*>(p + c0) + 32 * i, v + 8 * i);
-          } else {
-#pragma unroll
-            for (int i = 0; i < N / 4; ++i)
-              reinterpret_cast<uint4*>(p + c0)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          }
+          for (int i = 0; i < N / 8; ++i) st32(p + 32 * i, v + 8 * i);
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c0 + i < a.cols) p[c0 + i] = DT == TS_F32 ? (T)v[i % N] : (T)(v[(i / 2) % N] >> (16 * (i & 1)));
+          for (int i = 0; i < N / 4; ++i)
+            reinterpret_cast<uint4*>(p)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         }
-        continue;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (l8 * 16 + i < left)
+            reinterpret_cast<T*>(p)[i] = DT == TS_F32 ? (T)v[i % N] : (T)(v[(i / 2) % N] >> (16 * (i & 1)));
       }
+    } else {
       uint32_t* st = stage[warp];
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < N / 4; ++i)
         reinterpret_cast<uint4*>(st + lane * N)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       __syncwarp();
-      if (first + kSeg <= a.cols && (DT == TS_F32 || AL == 4) && row0 + 96 < a.rows) {   // whole words of four rows
-        char* q = reinterpret_cast<char*>(reinterpret_cast<T*>(a.out) + row0 * a.out_stride + first) + lane * 4;
-        const int64_t step = a.out_stride * 32 * (int64_t)sizeof(T);
+      if (AL == 2 && dst.mid) {
+        // the first element of row `lane`, then the words behind it
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(st);
+        if (lane < dst.rows) *reinterpret_cast<T*>(p - lane * 4 - 2 + lane * dst.step) = (T)h[lane * kSeg];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          *reinterpret_cast<uint32_t*>(q + i / (N / 4) * step + i % (N / 4) * 128) = st[i * 32 + lane];
+        for (int i = 0; i < N; ++i) {
+          if (i / (N / 4) >= dst.rows) break;
+          char* q = p + i / (N / 4) * dst.step + i % (N / 4) * 128;
+          const int c = 2 * (i % (N / 4) * 32 + lane) + 1, r = i / (N / 4) * kSeg;
+          if (c + 1 < min(left, kSeg)) *reinterpret_cast<uint32_t*>(q) = (uint32_t)h[r + c] | ((uint32_t)h[r + c + 1] << 16);
+          else if (c < left) *reinterpret_cast<T*>(q) = (T)h[r + c];
+        }
         continue;
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int64_t r = row0 + i / (N / 4) * 32;
-        if (r >= a.rows) break;
-        T* q = reinterpret_cast<T*>(a.out) + r * a.out_stride;
-        const int word = i % (N / 4) * 32 + lane;
+        if (i / (N / 4) >= dst.rows) break;
+        char* q = p + i / (N / 4) * dst.step + i % (N / 4) * 128;
         const uint32_t x = st[i * 32 + lane];
-        if (DT == TS_F32) {
-          if (first + word < a.cols) q[first + word] = (T)x;
+        const int word = i % (N / 4) * 32 + lane;
+        if (left == kSeg) {
+          *reinterpret_cast<uint32_t*>(q) = x;
+        } else if (DT == TS_F32) {
+          if (word < left) *reinterpret_cast<uint32_t*>(q) = x;
         } else {
-          const int64_t c = first + word * 2;
-          if (AL == 4 && c + 1 < a.cols) {
-            *reinterpret_cast<uint32_t*>(q + c) = x;
-          } else {
-            if (c < a.cols) q[c] = (T)x;
-            if (c + 1 < a.cols) q[c + 1] = (T)(x >> 16);
-          }
+          if (2 * word < left) reinterpret_cast<T*>(q)[0] = (T)x;
+          if (2 * word + 1 < left) reinterpret_cast<T*>(q)[1] = (T)(x >> 16);
         }
       }
     }
@@ -462,12 +491,14 @@ int check_tensor(const ts_fp4_tensor* t, const char* what) {
   return TS_OK;
 }
 
-// Grid of the row-tile kernels: 4 CTAs per 128 rows (fewer for few rows), enough
-// along the columns to give every SM sixteen CTAs.
+// Grid of the row-tile kernels: 4 CTAs per 128 rows (one for up to 8) and
+// enough along the columns for four waves of eight CTAs per SM. (Many short
+// CTAs at full occupancy measured better than fewer with several pieces in
+// flight each: 2047 x 14330, 18.6 against 20 to 32 us.)
 static dim3 tile_grid(int64_t rows, int segs) {
   const int64_t gx = rows <= 8 ? 1 : (rows + kTileRows - 1) / kTileRows * 4;
-  const int64_t want = ((int64_t)sm_count() * 16 + gx - 1) / gx;
-  return dim3((unsigned)gx, (unsigned)std::min<int64_t>(segs, std::max<int64_t>(1, std::min<int64_t>(want, 65535))));
+  const int64_t want = ((int64_t)sm_count() * 32 + gx - 1) / gx;
+  return dim3((unsigned)gx, (unsigned)std::min<int64_t>(segs, std::min<int64_t>(want, 65535)));
 }
 
 template <int DT, int AL>
@@ -493,14 +524,14 @@ static int launch_quantize(const QuantArgs& a, int al, int amax_al, bool nv, boo
   if (find) {
     int rc;
     if (amax_al >= 16) rc = launch_amax<DT, 16>(a, st);
-    else if (amax_al == 4 && DT != TS_F32) rc = launch_amax<DT, 4>(a, st);
-    else rc = launch_amax<DT, 1>(a, st);
+    else if (amax_al == 4 || DT == TS_F32) rc = launch_amax<DT, 4>(a, st);
+    else rc = launch_amax<DT, DT == TS_F32 ? 4 : 2>(a, st);
     if (rc != TS_OK) return rc;
   }
   if (al == 32) return launch_quantize<DT, 32>(a, nv, st);
   if (al == 16) return launch_quantize<DT, 16>(a, nv, st);
-  if (al == 4 && DT != TS_F32) return launch_quantize<DT, 4>(a, nv, st);
-  return launch_quantize<DT, 1>(a, nv, st);
+  if (al == 4 || DT == TS_F32) return launch_quantize<DT, 4>(a, nv, st);
+  return launch_quantize<DT, DT == TS_F32 ? 4 : 2>(a, nv, st);
 }
 
 template <int DT, int AL>
@@ -516,15 +547,15 @@ template <int DT>
 static int launch_dequantize(const DequantArgs& a, int al, bool nv, cudaStream_t st) {
   if (al == 32) return launch_dequantize<DT, 32>(a, nv, st);
   if (al == 16) return launch_dequantize<DT, 16>(a, nv, st);
-  if (al == 4 && DT != TS_F32) return launch_dequantize<DT, 4>(a, nv, st);
-  return launch_dequantize<DT, 1>(a, nv, st);
+  if (al == 4 || DT == TS_F32) return launch_dequantize<DT, 4>(a, nv, st);
+  return launch_dequantize<DT, DT == TS_F32 ? 4 : 2>(a, nv, st);
 }
 
-// Alignment of rows that the kernels use: 32, 16 or 4 bytes, or the element's.
+// Alignment of rows that the kernels use: 32, 16, 4 or 2 bytes.
 static int row_alignment(const void* p, int64_t stride, int es) {
   for (int al : {32, 16, 4})
     if (is_aligned(p, al) && (stride * es) % al == 0) return al;
-  return 1;
+  return 2;
 }
 
 }  // namespace fp4

@@ -14,7 +14,9 @@
 // select: one CTA per (sequence, kv head) finds the budget-th largest key by
 // radix selection over monotone 32-bit keys (three digits of 11, 11 and 10
 // bits, histograms in shared memory) and lists holes and movers by block
-// scans. move: a warp per moved slot copies both rows, 16 bytes per lane.
+// scans. move: a warp copies eight slots at a time, 16 bytes per lane and row.
+// Where a head can have only few movers (a token in, a token out), the select
+// CTA moves them itself and there is no second kernel.
 // What bounds them: select reads 8 bytes per slot and is latency-bound at one
 // CTA per head; move is DRAM traffic of the moved slots only.
 #include <algorithm>
@@ -28,6 +30,7 @@ namespace paged {
 constexpr int kSelThreads = 1024;
 constexpr int kBins = 2048;
 constexpr int kMoveWarps = 8;
+constexpr int kInline = 64;            // moves that a select CTA does itself
 constexpr int kMoves = 8;              // slots that a warp moves at a time
 constexpr int kSmemKeys = 24 * 1024;   // slots of a select CTA in shared memory
 
@@ -42,6 +45,8 @@ struct EvictArgs {
   int64_t cap;
   int smem_keys;          // slots whose keys and positions fit shared memory
   int page_shift;         // log2(page_size), or -1
+  int* counters;          // [batch] heads of a sequence that are done (moves in the select CTA)
+  int inline_moves;       // at most kInline moves a head: the select CTA does them itself
 };
 
 // Monotone key: larger scores have larger keys, -0 equals +0, NaN counts as -inf.
@@ -78,16 +83,58 @@ __device__ __forceinline__ int block_scan(int v, int* sum, int* warp_tot) {
   return warp_tot[warp] + inc - v;
 }
 
+// Moves first .. n - 1 of a head's list, kMoves of them per step, by one warp;
+// `to` is the warp's place for 2 kMoves offsets.
+__device__ __forceinline__ void move_slots(const Cache& c, int b, int h, const int32_t* lh, const int32_t* lm, int first,
+                                           int n, int step, int64_t* to) {
+  const int lane = threadIdx.x & 31, chunks = c.head_dim / 8;
+  for (int i0 = first; i0 < n; i0 += step) {
+    // lane k looks up target k, lane k + 16 source k
+    int64_t row_off = -1, stat = 0;
+    if ((lane & 15) < kMoves && i0 + (lane & 15) < n) {
+      const int slot = (lane < 16 ? lh : lm)[i0 + (lane & 15)];
+      const int page = page_of(c, b, slot), off = slot % c.page_size;
+      if (page >= 0) {
+        row_off = row_at(c, page, h, off) * 2;
+        stat = stat_at(c, page, h, off);
+      }
+    }
+    const int64_t src_stat = __shfl_down_sync(0xffffffffu, stat, 16);
+    const int64_t src_off = __shfl_down_sync(0xffffffffu, row_off, 16);
+    if (lane < kMoves && row_off >= 0 && src_off >= 0) {
+      c.scores[stat] = c.scores[src_stat];
+      c.slot_pos[stat] = c.slot_pos[src_stat];
+    }
+    const unsigned moves = __ballot_sync(0xffffffffu, lane < kMoves && row_off >= 0 && src_off >= 0);
+    // the rows' places, read back by every lane
+    int64_t* from = to + kMoves;
+    if ((lane & 15) < kMoves) to[(lane >> 4) * kMoves + (lane & 15)] = row_off;
+    __syncwarp();
+    for (int ch = lane; ch < 2 * chunks; ch += 32) {
+      char* base = (ch < chunks ? c.k : c.v) + (ch < chunks ? ch : ch - chunks) * 16;
+      uint4 w[kMoves];
+#pragma unroll
+      for (int k = 0; k < kMoves; ++k)
+        if ((moves >> k) & 1) w[k] = *reinterpret_cast<const uint4*>(base + from[k]);
+#pragma unroll
+      for (int k = 0; k < kMoves; ++k)
+        if ((moves >> k) & 1) *reinterpret_cast<uint4*>(base + to[k]) = w[k];
+    }
+    __syncwarp();
+  }
+}
+
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
   extern __shared__ uint32_t skeys[];
-  __shared__ int hist[kBins];
+  __shared__ __align__(16) int hist[kBins];
+  static_assert(kSelThreads / 32 * 2 * kMoves * 8 <= sizeof(int) * kBins, "the moves' offsets lie over the histogram");
   __shared__ int warp_tot[33];
   __shared__ int s_newest, s_digit, s_left;
   pdl_launch_dependents();
   const Cache& c = a.c;
   const int row = blockIdx.x, b = row / c.n_kv, h = row - b * c.n_kv, tid = threadIdx.x;
   const int n = (int)min((int64_t)max(c.seq_lens[b], 0), capacity(c));
-  if (n <= a.budget) {
+  if (n <= a.budget) {   // (so are the sequence's other heads)
     if (tid == 0) a.n_move[row] = 0;
     return;
   }
@@ -196,51 +243,30 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
       lm[at_m++] = i;
     }
   }
-  if (tid == 0) a.n_move[row] = n_movers;   // == n_holes
+  if (!a.inline_moves) {
+    if (tid == 0) a.n_move[row] = n_movers;   // == n_holes
+    return;
+  }
+  __syncthreads();                            // the lists are written, the keys have been read
+  move_slots(c, b, h, lh, lm, (tid >> 5) * kMoves, n_movers, kSelThreads / 32 * kMoves,
+             reinterpret_cast<int64_t*>(hist) + (tid >> 5) * 2 * kMoves);
+  // the last head of the sequence sets its length, which every head has read
+  if (tid == 0 && atomicAdd(a.counters + b, 1) == c.n_kv - 1) {
+    a.counters[b] = 0;
+    c.seq_lens[b] = a.budget;
+  }
 }
 
 __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictArgs a) {
   __shared__ int64_t where[kMoveWarps][2 * kMoves];
   pdl_wait_primary();
   const Cache& c = a.c;
-  const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv, lane = threadIdx.x & 31;
-  const int n = a.n_move[row], chunks = c.head_dim / 8;
+  const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv;
+  const int n = a.n_move[row];
   const int32_t* lh = a.holes + (int64_t)row * a.list;
   const int32_t* lm = a.movers + (int64_t)row * a.list;
-  for (int i0 = (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoves; i0 < n; i0 += gridDim.x * kMoveWarps * kMoves) {
-    // lane k looks up target k, lane k + 16 source k
-    int64_t row_off = -1, stat = 0;
-    if ((lane & 15) < kMoves && i0 + (lane & 15) < n) {
-      const int slot = (lane < 16 ? lh : lm)[i0 + (lane & 15)];
-      const int page = page_of(c, b, slot), off = slot % c.page_size;
-      if (page >= 0) {
-        row_off = row_at(c, page, h, off) * 2;
-        stat = stat_at(c, page, h, off);
-      }
-    }
-    const int64_t src_stat = __shfl_down_sync(0xffffffffu, stat, 16);
-    const int64_t src_off = __shfl_down_sync(0xffffffffu, row_off, 16);
-    if (lane < kMoves && row_off >= 0 && src_off >= 0) {
-      c.scores[stat] = c.scores[src_stat];
-      c.slot_pos[stat] = c.slot_pos[src_stat];
-    }
-    const unsigned moves = __ballot_sync(0xffffffffu, lane < kMoves && row_off >= 0 && src_off >= 0);
-    // the rows' places, read back by every lane
-    int64_t* to = where[threadIdx.x >> 5], *from = to + kMoves;
-    if ((lane & 15) < kMoves) to[(lane >> 4) * kMoves + (lane & 15)] = row_off;
-    __syncwarp();
-    for (int ch = lane; ch < 2 * chunks; ch += 32) {
-      char* base = (ch < chunks ? c.k : c.v) + (ch < chunks ? ch : ch - chunks) * 16;
-      uint4 w[kMoves];
-#pragma unroll
-      for (int k = 0; k < kMoves; ++k)
-        if ((moves >> k) & 1) w[k] = *reinterpret_cast<const uint4*>(base + from[k]);
-#pragma unroll
-      for (int k = 0; k < kMoves; ++k)
-        if ((moves >> k) & 1) *reinterpret_cast<uint4*>(base + to[k]) = w[k];
-    }
-    __syncwarp();
-  }
+  move_slots(c, b, h, lh, lm, (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoves, n, gridDim.x * kMoveWarps * kMoves,
+             where[threadIdx.x >> 5]);
   // nothing in this kernel reads the lengths, so they can be set here
   if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0 && c.seq_lens[b] > a.budget) c.seq_lens[b] = a.budget;
 }
@@ -302,6 +328,8 @@ extern "C" int ts_paged_evict(const ts_paged_cache* cache, int budget, int recen
   a.cap = cap;
   a.smem_keys = L.smem_keys;
   a.page_shift = log2_of(a.c.page_size);
+  a.counters = reinterpret_cast<int*>(ws);
+  a.inline_moves = L.list <= kInline && a.c.batch <= (int)kCounters ? 1 : 0;
   const int rows = a.c.batch * a.c.n_kv;
   TS_UNSUPPORTED(rows <= 65535, "too many heads in one call");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -315,6 +343,7 @@ extern "C" int ts_paged_evict(const ts_paged_cache* cache, int budget, int recen
   }
   evict_select_kernel<<<rows, kSelThreads, smem, st>>>(a);
   TS_LAUNCH_CHECK();
+  if (a.inline_moves) return TS_OK;
   const int per_row = (int)std::max<int64_t>(
       1, std::min<int64_t>((L.list + kMoveWarps * kMoves - 1) / (kMoveWarps * kMoves), (16 * sm_count() + rows - 1) / rows));
   cudaLaunchConfig_t cfg = {};
