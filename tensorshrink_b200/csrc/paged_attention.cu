@@ -21,9 +21,10 @@
 // loop). Scores and outputs use mma.m16n8k16 with the group's heads as the 16
 // rows: padding a small group to 16 rows costs tensor-core time that the
 // kernel has to spare, and P passes from the score accumulators to the second
-// product without leaving registers. Softmax statistics and sums are fp32; P
-// is rounded to the cache's type for its product, as wide as v itself: the
-// rounding errors of a row's weights average out in the sum over slots.
+// product without leaving registers. Softmax statistics and sums are fp32. P
+// enters its product as two terms of the cache's type (16 bits of it): one
+// alone would add as large an error as the rounding of the output does, and
+// the second product costs nothing that the loads do not hide.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -60,7 +61,7 @@ struct AttnArgs {
   int one_page;          // page_size % 16 == 0: a warp's 16 slots share a page
 };
 
-constexpr int kMaxPieces = 64;   // CTAs that share a kv head's units at most
+constexpr int kMaxPieces = 96;   // CTAs that share a kv head's units at most
 
 // s / page_size and s % page_size.
 __device__ __forceinline__ void split_slot(const AttnArgs& a, int s, int* page, int* off) {
@@ -523,8 +524,15 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
         for (int e = 0; e < 4; ++e) sc[n][e] = ex2(fmaf(sc[n][e], a.scale2, -base[e >> 1]));
       l[0] += (sc[0][0] + sc[0][1]) + (sc[1][0] + sc[1][1]);
       l[1] += (sc[0][2] + sc[0][3]) + (sc[1][2] + sc[1][3]);
-      const uint32_t pf[4] = {pack2<BF>(sc[0][0], sc[0][1]), pack2<BF>(sc[0][2], sc[0][3]),
-                              pack2<BF>(sc[1][0], sc[1][1]), pack2<BF>(sc[1][2], sc[1][3])};
+      // P in two terms of the cache's type
+      uint32_t pf[4], pr[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = sc[i >> 1][2 * (i & 1)], y = sc[i >> 1][2 * (i & 1) + 1];
+        pf[i] = pack2<BF>(x, y);
+        const float2 h = unpack2<BF>(pf[i]);
+        pr[i] = pack2<BF>(x - h.x, y - h.y);
+      }
       const int vrow = lane & 15;
       const uint32_t v_addr = (vb + vrow * kPitch) | (((lane >> 4) ^ r7) << 4);
 #pragma unroll
@@ -534,6 +542,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
         ldsm4t(v_addr ^ (s << 5), vf);
         mma<BF>(o[2 * s], pf, vf[0], vf[1]);
         mma<BF>(o[2 * s + 1], pf, vf[2], vf[3]);
+        mma<BF>(o[2 * s], pr, vf[0], vf[1]);
+        mma<BF>(o[2 * s + 1], pr, vf[2], vf[3]);
       }
       __syncwarp();   // the stage is refilled at the top of the next round
     }

@@ -1,0 +1,142 @@
+"""A Llama-shaped decoder served from 4-bit floating-point projections and a
+paged key-value cache: `fp4_linear`, `paged_append`, `paged_decode_attention`
+and `paged_evict` as a serving program strings them together.
+
+`decoder.QuantDecoder` decodes a batch whose sequences all stand at one
+position of a dense cache. Here every sequence has its own length, and with a
+`budget` the cache stops growing: after each step every kv head keeps the
+newest tokens and those that drew the most attention (the reference serves its
+models through `CUDAGraphQuantModel`, modules.py:1589-1691, and leaves the
+cache to them). Weights are random, as in `QuantDecoder`.
+
+    model = PagedDecoder(DecoderConfig(...), "cuda", max_batch=8, max_len=4096, budget=1024, recent=128)
+    token = model.prefill(prompts)          # list of 1-D token tensors, one per sequence
+    for _ in range(n):
+        token = model.decode_step(token)    # may be captured in a CUDA graph
+"""
+
+from __future__ import annotations
+
+from typing import List, Optional, Sequence
+
+import torch
+import torch.nn.functional as F
+from torch import nn
+
+from .decoder import DecoderConfig, _rms_norm, student_t_weight
+from .fp4 import Fp4Linear, fp4_quantize
+from .paged import PagedKVCache, paged_append, paged_decode_attention, paged_evict
+
+
+class PagedDecoderLayer(nn.Module):
+    """One layer's projections (q/k/v and gate/up fused by rows) and norms."""
+
+    def __init__(self, cfg: DecoderConfig, layer_idx: int, format: str, device):
+        super().__init__()
+        H, D = cfg.hidden, cfg.head_dim
+        shapes = {"qkv": ((cfg.n_heads + 2 * cfg.n_kv_heads) * D, H), "o": (H, cfg.n_heads * D),
+                  "gate_up": (2 * cfg.intermediate, H), "down": (H, cfg.intermediate)}
+        for j, (name, shape) in enumerate(shapes.items()):
+            w = student_t_weight(shape, seed=cfg.seed * 100003 + layer_idx * 16 + j, device=device)
+            setattr(self, name, Fp4Linear(fp4_quantize(w, format)))
+        self.input_norm = nn.Parameter(torch.ones(H, dtype=torch.float32, device=device), requires_grad=False)
+        self.post_norm = nn.Parameter(torch.ones(H, dtype=torch.float32, device=device), requires_grad=False)
+
+    def projections(self) -> List[Fp4Linear]:
+        return [self.qkv, self.o, self.gate_up, self.down]
+
+
+class PagedDecoder(nn.Module):
+    """See the module documentation. budget: tokens that each sequence's cache
+    is cut back to after a step (None: it grows up to max_len); recent: how many of
+    them are the newest whatever their weight. With a budget the caches keep
+    each slot's accumulated attention weight and position."""
+
+    def __init__(self, cfg: DecoderConfig, device, format: str = "nvfp4", max_batch: int = 1, max_len: int = 2048,
+                 page_size: int = 64, max_position: Optional[int] = None, budget: Optional[int] = None, recent: int = 0):
+        super().__init__()
+        self.cfg, self.device = cfg, torch.device(device)
+        self.budget, self.recent = budget, recent
+        if budget is not None and not 0 <= recent <= budget < max_len:
+            raise ValueError(f"recent <= budget < max_len is needed, got {recent}, {budget}, {max_len}")
+        H, D = cfg.hidden, cfg.head_dim
+        g = torch.Generator(device=self.device).manual_seed(cfg.seed + 7)
+        self.embed = (torch.randn(cfg.vocab, H, generator=g, device=self.device) * 0.02).to(torch.bfloat16)
+        self.lm_head = (torch.randn(cfg.vocab, H, generator=g, device=self.device) * 0.02).to(torch.bfloat16)
+        self.final_norm = torch.ones(H, dtype=torch.float32, device=self.device)
+        self.layers = nn.ModuleList(PagedDecoderLayer(cfg, i, format, self.device) for i in range(cfg.n_layers))
+        positions = max_position or max_len
+        inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, D, 2, device=self.device, dtype=torch.float32) / D))
+        ang = torch.outer(torch.arange(positions, device=self.device, dtype=torch.float32), inv)
+        self.rope_cos, self.rope_sin = ang.cos(), ang.sin()
+        self.caches = [PagedKVCache.allocate(max_batch, cfg.n_kv_heads, D, max_len, page_size, device=self.device,
+                                             track=budget is not None) for _ in range(cfg.n_layers)]
+        self.positions = torch.zeros(max_batch, dtype=torch.int64, device=self.device)   # of the next token
+
+    def packed_nbytes(self) -> int:
+        """Bytes of the projections' weights."""
+        return sum(p.weight().nbytes() for layer in self.layers for p in layer.projections())
+
+    def _evict(self, cache: PagedKVCache) -> None:
+        if self.budget is not None:
+            paged_evict(cache, self.budget, self.recent)
+
+    def _mlp(self, layer: PagedDecoderLayer, h: torch.Tensor) -> torch.Tensor:
+        gate, up = layer.gate_up(_rms_norm(h, layer.post_norm, self.cfg.rms_eps)).chunk(2, dim=-1)
+        return h + layer.down(F.silu(gate) * up)
+
+    def _logits(self, h: torch.Tensor) -> torch.Tensor:
+        return F.linear(_rms_norm(h, self.final_norm, self.cfg.rms_eps), self.lm_head).float()
+
+    @torch.no_grad()
+    def prefill(self, prompts: Sequence[torch.Tensor], return_logits: bool = False) -> torch.Tensor:
+        """Run one prompt per sequence (1-D token tensors, of any lengths up to
+        max_len; max_batch of them) from position 0 and fill the caches. Returns the greedy
+        next tokens [batch], or the logits [batch, vocab]."""
+        cfg, D = self.cfg, self.cfg.head_dim
+        B, lens = len(prompts), [len(p) for p in prompts]
+        if B != self.positions.shape[0] or min(lens) < 1 or max(lens) > self.caches[0].capacity:
+            raise ValueError(f"{self.positions.shape[0]} prompts of 1 to {self.caches[0].capacity} tokens are needed")
+        T = max(lens)
+        tokens = torch.zeros(B, T, dtype=torch.long, device=self.device)
+        for i, p in enumerate(prompts):
+            tokens[i, :lens[i]] = p.to(self.device)
+        n_new = torch.tensor(lens, dtype=torch.int32, device=self.device)
+        self.positions.zero_()
+        h = self.embed[tokens].float()
+        cos, sin = self.rope_cos[:T, None], self.rope_sin[:T, None]
+
+        def rope(x):
+            x1, x2 = x.float().chunk(2, dim=-1)
+            return torch.cat([x1 * cos - x2 * sin, x1 * sin + x2 * cos], dim=-1).to(x.dtype)
+
+        for layer, cache in zip(self.layers, self.caches):
+            x = _rms_norm(h, layer.input_norm, cfg.rms_eps)
+            q, k, v = layer.qkv(x).view(B, T, -1, D).split([cfg.n_heads, cfg.n_kv_heads, cfg.n_kv_heads], dim=2)
+            cache.seq_lens.zero_()
+            paged_append(k, v, cache, self.positions, self.rope_cos, self.rope_sin, n_new=n_new)
+            cache.seq_lens.copy_(n_new)
+            self._evict(cache)
+            # padding stands behind a prompt's tokens: causal attention never looks at it
+            a = F.scaled_dot_product_attention(rope(q).transpose(1, 2), rope(k).transpose(1, 2), v.transpose(1, 2),
+                                               is_causal=True, enable_gqa=True)
+            h = self._mlp(layer, h + layer.o(a.transpose(1, 2).reshape(B, T, -1)))
+        self.positions.copy_(n_new)
+        logits = self._logits(h[torch.arange(B, device=self.device), n_new.long() - 1])
+        return logits if return_logits else logits.argmax(dim=-1)
+
+    @torch.no_grad()
+    def decode_step(self, tokens: torch.Tensor, return_logits: bool = False) -> torch.Tensor:
+        """One token per sequence at its own position. Returns the greedy next
+        tokens [batch], or the logits [batch, vocab]."""
+        h = self.embed[tokens].float()
+        for layer, cache in zip(self.layers, self.caches):
+            qkv = layer.qkv(_rms_norm(h, layer.input_norm, self.cfg.rms_eps))
+            a = paged_decode_attention(qkv, self.cfg.n_heads, cache, self.positions, self.rope_cos, self.rope_sin,
+                                       accumulate=self.budget is not None)
+            cache.advance()
+            self._evict(cache)
+            h = self._mlp(layer, h + layer.o(a))
+        self.positions.add_(1)
+        logits = self._logits(h)
+        return logits if return_logits else logits.argmax(dim=-1)
