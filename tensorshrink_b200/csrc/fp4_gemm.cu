@@ -126,6 +126,30 @@ __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint
         : "memory");
 }
 
+// Stores alpha * v + bias for `jn` tokens from m on, of output feature n (one
+// per lane: the lanes of a warp store neighbours).
+template <int R>
+__device__ __forceinline__ void store_tokens(const GemmArgs& a, int64_t m, int64_t n, int jn, const float* v, float alpha,
+                                             float bias) {
+  const int64_t at = m * a.out_stride + n, step = a.out_stride;
+  if (a.out_dtype == TS_F32) {
+    float* p = reinterpret_cast<float*>(a.out) + at;
+#pragma unroll
+    for (int j = 0; j < R; ++j, p += step)
+      if (j < jn) *p = fmaf(v[j], alpha, bias);
+  } else if (a.out_dtype == TS_BF16) {
+    __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.out) + at;
+#pragma unroll
+    for (int j = 0; j < R; ++j, p += step)
+      if (j < jn) *p = __float2bfloat16_rn(fmaf(v[j], alpha, bias));
+  } else {
+    __half* p = reinterpret_cast<__half*>(a.out) + at;
+#pragma unroll
+    for (int j = 0; j < R; ++j, p += step)
+      if (j < jn) *p = __float2half_rn(fmaf(v[j], alpha, bias));
+  }
+}
+
 // Work items of a CTA: a tile and the stages [k0, k1) of it that are its own.
 struct Item {
   int tile, k0, k1;
@@ -334,11 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
           continue;
         }
         if (!valid) continue;
-        const int64_t mb = m0 + c * CW;
-        const int jn = (int)min((int64_t)CW, a.M - mb);
-#pragma unroll
-        for (int j = 0; j < CW; ++j)
-          if (j < jn) store_f(a.out, a.out_dtype, (mb + j) * a.out_stride + n, fmaf(v[j], alpha, bias));
+        store_tokens<CW>(a, m0 + c * CW, n, min(CW, jn_all - c * CW), v, alpha, bias);
       }
       if (++buf == P::kAcc) {
         buf = 0;
@@ -394,11 +414,15 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
             }
           }
         }
-        const float* f = reinterpret_cast<const float*>(sum);
+        float f[kRun];
 #pragma unroll
-        for (int u = 0; u < kRun; ++u)
-          if (j0 + u < jn_all)
-            store_f(a.out, a.out_dtype, (m0 + j0 + u) * a.out_stride + n, fmaf(f[u], alpha, bias));
+        for (int u = 0; u < kRun4; ++u) {
+          f[4 * u] = sum[u].x;
+          f[4 * u + 1] = sum[u].y;
+          f[4 * u + 2] = sum[u].z;
+          f[4 * u + 3] = sum[u].w;
+        }
+        store_tokens<kRun>(a, m0 + j0, n, min(kRun, jn_all - j0), f, alpha, bias);
       }
     }
   }
@@ -424,6 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
 
 constexpr int BN = 256, kHalf = BN / 2;
 constexpr int kPairEpi = 8, kPairThreads = (2 + kPairEpi) * 32;
+constexpr int kOutWords = 32 * 17;         // an epilogue warp's staging: 32 rows of 16 words, one word apart
 
 template <bool NV>
 struct Pair {
@@ -435,9 +460,11 @@ struct Pair {
   static constexpr int kStage = kABytes + kBBytes + kSfA + kSfB;
   static constexpr int kSfCols = 4 * kTiles * (1 + kRowTiles);
   static constexpr int kFitTmem = (kTmemCols - BN) / kSfCols;
-  static constexpr int kFitSmem = (227 * 1024 - 2048) / kStage;
+  static constexpr int kEpi = 128 + kPairEpi * (kHalf + kOutWords) * 4;   // barriers, then the epilogue warps' words
+  static constexpr int kFitSmem = (227 * 1024 - 1024 - kEpi) / kStage;
   static constexpr int S = kFitTmem < kFitSmem ? kFitTmem : kFitSmem;
-  static constexpr size_t kSmem = 1024 + (size_t)S * kStage + (2 * S + 3) * 8 + 16;
+  static_assert((2 * S + 3) * 8 + 4 <= 128, "barriers");
+  static constexpr size_t kSmem = 1024 + (size_t)S * kStage + kEpi;
 };
 
 struct PairArgs {
@@ -456,11 +483,10 @@ struct PairArgs {
   int stall, overlap;
 };
 
-// 64 consecutive fp32 columns of this warp's TMEM lane quadrant, both halves in flight.
-__device__ __forceinline__ void tmem_ld32x2(uint32_t taddr, float (&a)[32], float (&b)[32]) {
-  uint32_t r[64];
+// 128 consecutive fp32 columns of this warp's TMEM lane quadrant, four loads in flight.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < 4; ++h) {
     uint32_t* q = r + 32 * h;
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -472,16 +498,10 @@ __device__ __forceinline__ void tmem_ld32x2(uint32_t taddr, float (&a)[32], floa
           "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
         : "r"(taddr + 32 * h));
   }
-  // the registers are written when the wait returns: it takes and gives them
-  // back, so that no use moves before it
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  // the registers hold the values from here on: no use moves before the wait
 #pragma unroll
-  for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(r[i]));
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    a[i] = __uint_as_float(r[i]);
-    b[i] = __uint_as_float(r[32 + i]);
-  }
+  for (int i = 0; i < 128; ++i) asm volatile("" : "+r"(r[i]));
 }
 
 __device__ __forceinline__ uint32_t cta_rank() {
@@ -555,6 +575,7 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
   uint64_t* tempty = tfull + 1;
   uint64_t* drain = tempty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  char* s_epi = reinterpret_cast<char*>(full) + 128;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
@@ -692,77 +713,103 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
     const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf;
     const uint32_t free_bar = map_cta(smem_u32(tempty), 0);
     int n = 0;
+    float* s_bias = reinterpret_cast<float*>(s_epi) + (warp - 2) * (kHalf + kOutWords);   // [128]
+    uint32_t* s_out = reinterpret_cast<uint32_t*>(s_bias + kHalf);                         // [32 rows][17 words]
     for (int tile = pair; tile < ntiles; tile += pairs, ++n) {
-      const int64_t m = (int64_t)(tile % a.mblocks) * 256 + rank * 128 + quad * 32 + lane;
+      const int64_t m0 = (int64_t)(tile % a.mblocks) * 256 + rank * 128 + quad * 32;
       const int64_t n0 = (int64_t)(tile / a.mblocks) * BN + half * kHalf;
       const int cols = (int)max((int64_t)0, min((int64_t)kHalf, a.N - n0));
+      const int rows = (int)max((int64_t)0, min((int64_t)32, a.M - m0));
+      __syncwarp();                                    // (the last tile's biases have been used)
+#pragma unroll
+      for (int i = 0; i < kHalf / 32; ++i) {
+        const int col = i * 32 + lane;
+        s_bias[col] = a.bias != nullptr && col < cols ? load_f(a.bias, a.bias_dtype, n0 + col) : 0.f;
+      }
+      __syncwarp();
       const bool got = mbar_wait_hint(tfull, n & 1, &g_err, 34, a.wait_ns);
       if (!__all_sync(0xffffffffu, got)) break;
       tc_fence_after();
-      if (a.out_dtype == TS_F32) {
-        float* row = reinterpret_cast<float*>(a.out) + m * a.out_stride + n0;
-#pragma unroll 1
-        for (int c = 0; c < kHalf / 32; ++c) {
-          float v[32];
-          tmem_ld32(acc + c * 32, v);
-          if (c == kHalf / 32 - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_cluster(free_bar);
-          }
-          if (m >= a.M) continue;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int col = c * 32 + j;
-            if (col < cols) row[col] = fmaf(v[j], alpha, a.bias ? load_f(a.bias, a.bias_dtype, n0 + col) : 0.f);
-          }
-        }
-        continue;
-      }
-      // 16-bit outputs wait in registers, so that the accumulator is free
-      // again before the first of them is stored
-      uint32_t w[kHalf / 2];
-      float vv[2][32];
-#pragma unroll
-      for (int c = 0; c < kHalf / 32; ++c) {
-        float (&v)[32] = vv[c & 1];
-        if ((c & 1) == 0) tmem_ld32x2(acc + c * 32, vv[0], vv[1]);   // two loads in flight
-        if (a.bias != nullptr) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int col = c * 32 + j;
-            v[j] = fmaf(v[j], alpha, col < cols ? load_f(a.bias, a.bias_dtype, n0 + col) : 0.f);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= alpha;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (a.out_dtype == TS_BF16) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-            w[c * 16 + j] = *reinterpret_cast<const uint32_t*>(&h);
-          } else {
-            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-            w[c * 16 + j] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-        }
-      }
+      // the sums wait in registers, so that the accumulator is free again
+      // before the first of them is stored
+      uint32_t v[kHalf];
+      tmem_ld128(acc, v);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(free_bar);
-      if (m >= a.M) continue;
-      uint16_t* row = reinterpret_cast<uint16_t*>(a.out) + m * a.out_stride + n0;
-      if (a.vec) {
+      if (rows == 0) continue;
+#pragma unroll
+      for (int i = 0; i < kHalf; i += 4) {
+        const float4 bs = *reinterpret_cast<const float4*>(s_bias + i);
+        v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), alpha, bs.x));
+        v[i + 1] = __float_as_uint(fmaf(__uint_as_float(v[i + 1]), alpha, bs.y));
+        v[i + 2] = __float_as_uint(fmaf(__uint_as_float(v[i + 2]), alpha, bs.z));
+        v[i + 3] = __float_as_uint(fmaf(__uint_as_float(v[i + 3]), alpha, bs.w));
+      }
+      if (a.out_dtype == TS_F32) {
+        float* out = reinterpret_cast<float*>(a.out) + m0 * a.out_stride + n0;
+        if (a.vec) {                                   // N is a multiple of 4
+          float* row = out + lane * a.out_stride;
+#pragma unroll
+          for (int i = 0; i < kHalf; i += 4)
+            if (lane < rows && i < cols) *reinterpret_cast<uint4*>(row + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          continue;
+        }
+        // 16 columns of the warp's rows at a time through shared memory, two
+        // rows of them per store
+#pragma unroll
+        for (int c = 0; c < kHalf; c += 16) {
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s_out[lane * 17 + j] = v[c + j];
+          __syncwarp();
+          const int col = c + (lane & 15);
+          for (int r = lane >> 4; r < rows; r += 2)
+            if (col < cols) out[r * a.out_stride + col] = __uint_as_float(s_out[r * 17 + (lane & 15)]);
+        }
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i < kHalf / 2; ++i) {
+        const float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
+        if (a.out_dtype == TS_BF16) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+          v[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __half2 h = __floats2half2_rn(x, y);
+          v[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + m0 * a.out_stride + n0;
+      if (a.vec) {                                     // N is a multiple of 8
+        uint16_t* row = out + lane * a.out_stride;
 #pragma unroll
         for (int i = 0; i < kHalf / 8; ++i)
-          if (i * 8 < cols)   // N is a multiple of 8 here
-            *reinterpret_cast<uint4*>(row + i * 8) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-      } else {
+          if (lane < rows && i * 8 < cols)
+            *reinterpret_cast<uint4*>(row + i * 8) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        continue;
+      }
+      // 32 columns of the warp's rows at a time through shared memory: two rows
+      // per store where rows start on words, one row of elements otherwise
+      const bool words = (reinterpret_cast<uintptr_t>(a.out) & 3) == 0 && (a.out_stride & 1) == 0;
 #pragma unroll
-        for (int i = 0; i < kHalf / 2; ++i) {
-          if (2 * i < cols) row[2 * i] = (uint16_t)w[i];
-          if (2 * i + 1 < cols) row[2 * i + 1] = (uint16_t)(w[i] >> 16);
+      for (int c = 0; c < kHalf / 2; c += 16) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s_out[lane * 17 + j] = v[c + j];
+        __syncwarp();
+        if (words) {
+          const int col = 2 * (c + (lane & 15));
+          for (int r = lane >> 4; r < rows; r += 2) {
+            const uint32_t x = s_out[r * 17 + (lane & 15)];
+            uint16_t* dst = out + r * a.out_stride + col;
+            if (col + 1 < cols) *reinterpret_cast<uint32_t*>(dst) = x;
+            else if (col < cols) *dst = (uint16_t)x;
+          }
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(s_out);
+          for (int r = 0; r < rows; ++r)
+            if (2 * c + lane < cols) out[r * a.out_stride + 2 * c + lane] = h[r * 34 + lane];
         }
       }
     }
@@ -786,30 +833,48 @@ struct Plan {
   int BT, tblocks, wblocks, kblocks, ntiles, grid;
 };
 
+// Cycles that a call takes at least, as measured: a stage of a pair's tile 620
+// and the change from tile to tile 2000; a stage of a lone CTA's tile 550, or what
+// its bytes take at DRAM's rate; a join of up to four pieces 3000 and 2500 per
+// 32 tokens; the start 4000. Only their order matters.
 static Plan plan(int64_t M, int64_t N, int64_t K) {
   Plan p{};
-  const int sms = sm_count(), pairs = sms / 2;
+  const int sms = std::max(2, sm_count()), pairs = sms / 2;
   p.kblocks = (int)((padded_cols(K) + kBK - 1) / kBK);
+  p.BT = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  p.wblocks = (int)((N + kBW - 1) / kBW);
+  p.tblocks = (int)((M + p.BT - 1) / p.BT);
+  const int64_t ntiles = (int64_t)p.wblocks * p.tblocks, units = ntiles * p.kblocks;
+  const int rounds = (int)(std::min<int64_t>(M, p.BT) + 31) / 32;
+  const double stream = (double)units * (kABytes + 2048) / 3300;   // the weight's bytes, at DRAM's bytes per cycle
+  auto cost = [&](int64_t grid, int pieces) {
+    const double own = (double)((units + grid - 1) / grid) * 550;
+    return std::max(own, stream) + (pieces > 1 ? 3000 + 2500.0 * rounds * ((pieces + 3) / 4) : 0) +
+           (double)((ntiles + grid - 1) / grid) * rounds * 400;
+  };
+  // whole tiles, or whole parts of them, where the SMs hold them all at once;
+  // else, or if that is better, equal shares of all stages
+  const int64_t all = std::min<int64_t>(units, sms);
+  p.grid = (int)all;
+  double best = cost(all, (int)std::min<int64_t>(p.kblocks, all / std::max<int64_t>(1, ntiles) + 2));
+  for (int parts = 1; parts <= p.kblocks && ntiles * parts <= sms; ++parts) {
+    const double c = cost(ntiles * parts, parts);
+    if (c < best) {
+      best = c;
+      p.grid = (int)(ntiles * parts);
+    }
+  }
+  p.ntiles = (int)std::min<int64_t>(ntiles, INT32_MAX);
+  if (M <= 128) return p;
   const int64_t mb = (M + 255) / 256, nb = (N + BN - 1) / BN;
-  if (M > 128 && mb * nb * 2 >= pairs) {
+  const double pair = (double)((mb * nb + pairs - 1) / pairs) * (620.0 * p.kblocks + 2000);
+  if (pair <= best || ntiles > (int64_t)paged::kCounters) {
     p.pair = true;
     p.tblocks = (int)mb;
     p.wblocks = (int)nb;
     p.ntiles = (int)(mb * nb);
     p.grid = 2 * (int)std::min<int64_t>(mb * nb, pairs);
-    return p;
   }
-  p.BT = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  p.wblocks = (int)((N + kBW - 1) / kBW);
-  p.tblocks = (int)((M + p.BT - 1) / p.BT);
-  p.ntiles = p.wblocks * p.tblocks;
-  // Equal shares of all stages for every SM, or, where that occupies two
-  // thirds of them, whole parts of tiles: 1 / parts of a tile's stages per CTA
-  // has fewer pieces to join (1 x 14336 x 4096: 112 whole tiles; 33 x 4096 x
-  // 14336: 32 tiles in 4 parts).
-  const int parts = std::min(p.kblocks, sms / p.ntiles);
-  if (parts >= 1 && p.ntiles * parts * 3 >= sms * 2) p.grid = p.ntiles * parts;
-  else p.grid = (int)std::min<int64_t>((int64_t)p.ntiles * p.kblocks, sms);
   return p;
 }
 
@@ -939,7 +1004,8 @@ static int matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, const void* bi
     a.out = out;
     a.out_dtype = out_dtype;
     a.out_stride = out_row_stride;
-    a.vec = w->rows % 8 == 0 && out_row_stride % 8 == 0 && is_aligned(out, 16);
+    const int per = out_dtype == TS_F32 ? 4 : 8;     // values of a 16-byte store
+    a.vec = w->rows % per == 0 && out_row_stride % per == 0 && is_aligned(out, 16);
     a.wait_ns = wait_limit_ns();
     a.stall = stall;
     a.overlap = overlap;
