@@ -129,6 +129,45 @@ struct Shares {
   }
 };
 
+// How the rows' units (a row: a kv head's, or 16 of its query heads) are dealt
+// out to CTAs.
+struct Deal {
+  int front;          // see below
+  unsigned n_cta;
+};
+
+// Cycles, as measured: a unit 1100 where CTAs have little to do; a row's start
+// and its warps' join 6000; the join of pieces 3000, and for each eight query
+// heads 1200 and 800 for each eight pieces.
+__device__ __forceinline__ Deal choose_deal(unsigned units, unsigned rows, int longest, unsigned grid, int heads) {
+  if (rows == 0) return {0, 0};
+  const unsigned turns = (heads + 2 * kWarps - 1) / (2 * kWarps);
+  auto join = [&](unsigned pieces) { return pieces > 1 ? 3000 + turns * (1200 + (pieces + 7) / 8 * 800) : 0; };
+  // Equal shares of all units laid end to end, each row with a few units in
+  // front of its own for its start, so that a CTA of many short rows gets
+  // fewer units than one of few long ones. No row in more than kMaxPieces + 1.
+  const bool full = units >= kFullUnits * grid || rows > grid;
+  Deal d;
+  d.front = full ? kRowCost : 0;
+  const unsigned total = units + rows * d.front;
+  const unsigned least = max((unsigned)d.front + 1, (longest + d.front + kMaxPieces - 1) / kMaxPieces);
+  d.n_cta = max(1u, min(grid, total / least));
+  if (full) return d;
+  // Where a launch has few units: each row in equal parts of CTAs of its own,
+  // if that lets the last of them finish sooner.
+  const unsigned share = (units + d.n_cta - 1) / d.n_cta;
+  unsigned best = share * 1100 + (rows > 1 ? 6000 : 0) + join((longest + share - 1) / share + 1);
+  for (unsigned p = 1; p <= (unsigned)min(longest, kMaxPieces) && rows * p <= grid; p = p < 8 ? p + 1 : p * 2) {
+    const unsigned q = (longest + p - 1) / p, cost = q * 1100 + join(p);
+    if (cost < best) {
+      best = cost;
+      d.front = -(int)(q * p);
+      d.n_cta = rows * p;
+    }
+  }
+  return d;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -170,7 +209,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
   const int D = c.head_dim, chunks = D / 8, steps = D / 16, rows_per_b = c.n_kv * a.head_tiles;
 
   // prefix sums of the sequences' units; every thread takes a run of sequences
-  int longest = 0, front = 0;
+  int longest = 0;
+  Deal deal;
   {
     const int per = (c.batch + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
@@ -201,16 +241,17 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
       if (w < warp) at += warp_sums[w];
       all += warp_sums[w];
     }
-    // With units enough for every CTA, a row counts kRowCost units in front of
-    // its own, so that a CTA of many short rows gets fewer units than one of
-    // few long ones.
-    front = (uint64_t)(uint32_t)all * rows_per_b >= (uint64_t)kFullUnits * gridDim.x ? kRowCost : 0;
-    longest += front;
-    int v = (int)(uint32_t)at + front * (int)(at >> 32);
+    // How the units are dealt out (`deal`): a row of n units counts n + front,
+    // or, with front < 0, -front whatever n is.
+    const unsigned units = (unsigned)(uint32_t)all * rows_per_b, rows = (unsigned)(all >> 32) * rows_per_b;
+    deal = choose_deal(units, rows, longest, gridDim.x, min(a.group, kHeads));
+    int v = 0;
+    if (deal.front >= 0) v = (int)(uint32_t)at + deal.front * (int)(at >> 32);
+    else v = -deal.front * (int)(at >> 32);
     for (int b = b0; b < b1; ++b) {
       prefix[b] = v;
       const int n = units_of(a, lens[b]);
-      v += n > 0 ? n + front : 0;
+      v += n > 0 ? (deal.front >= 0 ? n + deal.front : -deal.front) : 0;
     }
     if (b1 == c.batch && b0 < b1) prefix[c.batch] = v;
   }
@@ -224,10 +265,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
 
   const unsigned total = (unsigned)prefix[c.batch] * rows_per_b;   // (the host keeps it below 2^31)
   if (total == 0) return;
-  // as many CTAs as get a whole unit each, but none with less than 1 / kMaxPieces
-  // of the longest row: a row is then cut into at most kMaxPieces + 1 pieces
-  const unsigned least = max(front + 1, (longest + kMaxPieces - 1) / kMaxPieces);
-  const unsigned n_cta = max(1u, min(gridDim.x, total / least));
+  const unsigned n_cta = min(deal.n_cta, total);
   if (blockIdx.x >= n_cta) return;
   const Shares shares(total, n_cta);
   const unsigned u1 = shares.begin(blockIdx.x + 1);
@@ -250,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
       row = 0;
       do ++b; while (prefix[b + 1] == prefix[b]);
     }
-    const int cost = prefix[b + 1] - prefix[b], nt = cost - front;
+    const int cost = prefix[b + 1] - prefix[b], nt = units_of(a, lens[b]), front = cost - nt;
     const unsigned row_u = (unsigned)prefix[b] * rows_per_b + (unsigned)(row * cost);
     const int v0 = (int)(u - row_u), v1 = (int)min((unsigned)cost, v0 + (u1 - u));
     u += v1 - v0;
@@ -261,23 +299,59 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
     const int head0 = h * a.group + ht * kHeads;       // first query head of the tile
     const int len = lens[b];
     const int32_t* table = c.table + b * c.table_stride;
-    int64_t pos = a.positions != nullptr ? a.positions[b] : 0;
-    const bool ok = takes(a, b, len, pos);             // (a sequence that cannot take its token answers with zeros)
-    if (!ok) pos = 0;
     const uint16_t* new_row = a.qkv + b * a.qkv_stride;
     const bool turn = a.cos_t != nullptr;
 
-    // A warp's share of unit t: slots t * 64 + warp * 16 + r. It copies the
-    // rows of cached slots and zeros for the others; `live` is a bit per row
-    // that has a cached token, queued until the stage is consumed.
-    const int cl = lane % kRowChunks, rl = lane / kRowChunks;   // this lane's 16-byte column and first row
-    const bool col = cl < chunks;
+    // What the segment needs first is loaded before any of it is used: the
+    // position, the new token's page, the first stages' pages, the query heads
+    // (kQ pairs of a thread at a time; behind the copies they would wait).
+    constexpr int kQ = 4;
+    const int64_t pos_in = a.positions != nullptr ? a.positions[b] : 0;
+    int pg_new, off_new;
+    split_slot(a, len, &pg_new, &off_new);
+    const int page_new = table[pg_new];
     auto page_at = [&](int t) {                        // (one_page) the page of unit t's rows
       const int slot0 = t * kUnit + warp * kRows;
       int pg, off;
       split_slot(a, slot0, &pg, &off);
       return t < t1 && slot0 < len ? table[pg] : -1;
     };
+    int pages[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) pages[s] = a.one_page ? page_at(t0 + s) : -1;
+    uint32_t qx[kQ];
+    float2 rot[kQ];
+    const int pairs = heads * (D / 2);
+    auto load_q = [&](int i0) {
+#pragma unroll
+      for (int k = 0; k < kQ; ++k) {
+        const int i = i0 + k * kThreads, g = i / (D / 2), j = i - g * (D / 2);
+        if (i < pairs) {
+          const uint16_t* qr = new_row + (int64_t)(head0 + g) * D + j;
+          qx[k] = (uint32_t)qr[0] | ((uint32_t)qr[D / 2] << 16);
+        }
+      }
+    };
+    load_q(tid);
+    // a sequence that cannot take its token answers with zeros
+    const bool ok = (unsigned)page_new < (unsigned)c.num_pages && (!turn || (pos_in >= 0 && pos_in < a.rope_rows));
+    const int64_t pos = ok ? pos_in : 0;
+    const float* cs = a.cos_t + pos * (D / 2);
+    const float* sn = a.sin_t + pos * (D / 2);
+    auto load_rot = [&](int i0) {
+#pragma unroll
+      for (int k = 0; k < kQ; ++k) {
+        const int i = i0 + k * kThreads, j = i % (D / 2);
+        if (turn && i < pairs) rot[k] = make_float2(cs[j], sn[j]);
+      }
+    };
+    load_rot(tid);
+
+    // A warp's share of unit t: slots t * 64 + warp * 16 + r. It copies the
+    // rows of cached slots and zeros for the others; `live` is a bit per row
+    // that has a cached token, queued until the stage is consumed.
+    const int cl = lane % kRowChunks, rl = lane / kRowChunks;   // this lane's 16-byte column and first row
+    const bool col = cl < chunks;
     auto issue = [&](int t, int stage, int page) -> uint32_t {
       uint32_t live = 0;
       if (t < t1) {
@@ -343,41 +417,21 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
       cp_commit();
       return live;
     };
-    // The rotated query heads of the tile, kQ pairs of a thread at a time; the
-    // first are loaded before the copies, which would hold them up.
-    constexpr int kQ = 4;
-    const float* cs = a.cos_t + pos * (D / 2);
-    const float* sn = a.sin_t + pos * (D / 2);
-    uint32_t qx[kQ];
-    float2 rot[kQ];
-    auto load_q = [&](int i0) {
-#pragma unroll
-      for (int k = 0; k < kQ; ++k) {
-        const int i = i0 + k * kThreads, g = i / (D / 2), j = i - g * (D / 2);
-        if (i < heads * (D / 2)) {
-          const uint16_t* qr = new_row + (int64_t)(head0 + g) * D + j;
-          qx[k] = (uint32_t)qr[0] | ((uint32_t)qr[D / 2] << 16);
-          if (turn) rot[k] = make_float2(cs[j], sn[j]);
-        }
-      }
-    };
-    load_q(tid);
     uint64_t live_q = 0;
-    int page_next;
-    {
-      int pages[S];
 #pragma unroll
-      for (int s = 0; s < S; ++s) pages[s] = a.one_page ? page_at(t0 + s) : -1;
-#pragma unroll
-      for (int s = 0; s < S - 1; ++s) live_q |= (uint64_t)issue(t0 + s, s, pages[s]) << (16 * s);
-      page_next = pages[S - 1];
-    }
-    for (int i0 = tid; i0 < heads * (D / 2); i0 += kQ * kThreads) {
-      if (i0 != tid) load_q(i0);
+    for (int s = 0; s < S - 1; ++s) live_q |= (uint64_t)issue(t0 + s, s, pages[s]) << (16 * s);
+    int page_next = pages[S - 1];
+
+    // the rotated query heads of the tile
+    for (int i0 = tid; i0 < pairs; i0 += kQ * kThreads) {
+      if (i0 != tid) {
+        load_q(i0);
+        load_rot(i0);
+      }
 #pragma unroll
       for (int k = 0; k < kQ; ++k) {
         const int i = i0 + k * kThreads, g = i / (D / 2), j = i - g * (D / 2);
-        if (i >= heads * (D / 2)) continue;
+        if (i >= pairs) continue;
         if (turn) {
           const float2 f = unpack2<BF>(qx[k]);
           const float2 y = rotate(f.x, f.y, rot[k].x, rot[k].y);
@@ -421,8 +475,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
         const int r = len - slot0;
         live |= 1u << r;
         char* st = ring + (kb - ring_u);
-        const int page = page_of(c, b, len);
-        const int64_t at = row_at(c, page, h, len % c.page_size);
+        const int64_t at = row_at(c, page_new, h, off_new);
         uint16_t* kc = reinterpret_cast<uint16_t*>(c.k) + at;
         uint16_t* vc = reinterpret_cast<uint16_t*>(c.v) + at;
         const uint16_t* kr = new_row + (int64_t)(a.n_q + h) * D;
@@ -451,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
           }
         }
         if (lane == 0 && ht == 0) {
-          const int64_t sa = stat_at(c, page, h, len % c.page_size);
+          const int64_t sa = stat_at(c, page_new, h, off_new);
           if (c.scores != nullptr) c.scores[sa] = 0.f;
           if (c.slot_pos != nullptr) c.slot_pos[sa] = (int32_t)pos;
         }
@@ -558,8 +611,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
     // join the warps through shared memory (over the drained rings)
     constexpr int kJoin = DP + 4;                    // floats of a row: its sums, max, sum
     float* jo = reinterpret_cast<float*>(smem);      // [kWarps][16][kJoin]
-    static_assert((size_t)kWarps * kHeads * (kJoin + 2) * 4 <= ring_bytes<DP>() &&
-                      (size_t)kHeads * (2 * (kMaxPieces + 4) + 1) * 4 <= ring_bytes<DP>(), "join areas");
+    static_assert((size_t)kWarps * kHeads * (kJoin + 2) * 4 <= ring_bytes<DP>(), "join area");
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float* r = jo + (warp * kHeads + (lane >> 2) + 8 * e) * kJoin;
@@ -638,47 +690,70 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
         const float* begun = a.partials + ((int64_t)cta0 * 2 + 1) * prow;
         const float* others = a.partials + (int64_t)cta0 * 2 * prow;
         auto piece = [&](int i) { return i == 0 ? begun : others + (int64_t)i * 2 * prow; };
-        float2* ml = reinterpret_cast<float2*>(jo);  // [pieces][16]: (max, sum), then (factor, -)
-        float* inv_l = jo + 2 * kHeads * (kMaxPieces + 4);
-        for (int i = tid; i < pieces * kHeads; i += kThreads) {
-          const int pc = i / kHeads, g = i % kHeads;
-          if (g < heads) ml[i] = __ldcg(reinterpret_cast<const float2*>(piece(pc) + kHeads * D) + g);
-        }
-        __syncthreads();
-        for (int g = warp; g < heads; g += kWarps) {
-          float mm = -INFINITY;
-          for (int i = lane; i < pieces; i += 32) mm = fmaxf(mm, ml[i * kHeads + g].x);
+        // two heads per warp, which needs no other: the pieces' factors
+        // 2^(m_piece - m), lane i those of pieces i, i + 32, ..., then the sums, four
+        // values a lane
+        constexpr int kML = (kMaxPieces + 1 + 31) / 32;
+        for (int g0 = warp; g0 < heads; g0 += 2 * kWarps) {
+          float f[2][kML], inv[2];
+          {
+            float2 v[2][kML];
 #pragma unroll
-          for (int o2 = 16; o2 > 0; o2 >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o2));
-          const float bs = mm == -INFINITY ? 0.f : mm;
-          float ll = 0.f;
-          for (int i = lane; i < pieces; i += 32) {
-            const float f = ex2(ml[i * kHeads + g].x - bs);
-            ll = fmaf(f, ml[i * kHeads + g].y, ll);
-            ml[i * kHeads + g].x = f;
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int k = 0; k < kML; ++k) {
+                const int i = lane + 32 * k, g = g0 + e * kWarps;
+                v[e][k] = i < pieces && g < heads ? __ldcg(reinterpret_cast<const float2*>(piece(i) + kHeads * D) + g)
+                                                  : make_float2(-INFINITY, 0.f);
+              }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+              for (int k = 0; k < kML; ++k) mm = fmaxf(mm, v[e][k].x);
+#pragma unroll
+              for (int o2 = 16; o2 > 0; o2 >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o2));
+              const float bs = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+              for (int k = 0; k < kML; ++k) {
+                f[e][k] = ex2(v[e][k].x - bs);
+                ll = fmaf(f[e][k], v[e][k].y, ll);
+              }
+              ll = warp_sum(ll);
+              inv[e] = 1.f / ll;
+              if (lane == 0 && a.lse2 != nullptr && g0 + e * kWarps < heads)
+                a.lse2[b * a.n_q + head0 + g0 + e * kWarps] = bs + log2f(ll);
+            }
           }
-          ll = warp_sum(ll);
-          if (lane == 0) {
-            inv_l[g] = 1.f / ll;
-            if (a.lse2 != nullptr) a.lse2[b * a.n_q + head0 + g] = bs + log2f(ll);
+          const int second = g0 + kWarps < heads ? kWarps * D : 0;   // (an odd head is summed twice)
+          for (int d = 4 * lane; d - 4 * lane < D; d += 128) {
+            const bool mine = d < D;
+            const int at = g0 * D + (mine ? d : 0);
+            float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+            for (int k = 0; k < kML; ++k) {
+#pragma unroll 4
+              for (int i = 32 * k; i < min(pieces, 32 * k + 32); ++i) {
+                const float* src = piece(i) + at;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float w = __shfl_sync(0xffffffffu, f[e][k], i - 32 * k);
+                  const float4 v = __ldcg(reinterpret_cast<const float4*>(src + e * second));
+                  acc[e].x = fmaf(w, v.x, acc[e].x);
+                  acc[e].y = fmaf(w, v.y, acc[e].y);
+                  acc[e].z = fmaf(w, v.z, acc[e].z);
+                  acc[e].w = fmaf(w, v.w, acc[e].w);
+                }
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (!mine || (e == 1 && second == 0)) continue;
+              uint32_t* dst = reinterpret_cast<uint32_t*>(out + (g0 + e * kWarps) * D + d);
+              dst[0] = ok ? pack2<BF>(acc[e].x * inv[e], acc[e].y * inv[e]) : 0;
+              dst[1] = ok ? pack2<BF>(acc[e].z * inv[e], acc[e].w * inv[e]) : 0;
+            }
           }
-        }
-        __syncthreads();
-        for (int i = tid; i < heads * (D / 4); i += kThreads) {
-          const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int p = 0; p < pieces; ++p) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(p) + g * D + d));
-            const float f = ml[p * kHeads + g].x;
-            acc.x = fmaf(f, v.x, acc.x);
-            acc.y = fmaf(f, v.y, acc.y);
-            acc.z = fmaf(f, v.z, acc.z);
-            acc.w = fmaf(f, v.w, acc.w);
-          }
-          uint32_t* dst = reinterpret_cast<uint32_t*>(out + g * D + d);
-          dst[0] = ok ? pack2<BF>(acc.x * inv_l[g], acc.y * inv_l[g]) : 0;
-          dst[1] = ok ? pack2<BF>(acc.z * inv_l[g], acc.w * inv_l[g]) : 0;
         }
       }
     }
