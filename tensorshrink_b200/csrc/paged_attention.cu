@@ -136,13 +136,13 @@ struct Deal {
   unsigned n_cta;
 };
 
-// Cycles, as measured: a unit 1100 where CTAs have little to do; a row's start
+// Cycles, as measured where CTAs have little to do: a unit 1800; a row's start
 // and its warps' join 6000; the join of pieces 3000, and for each eight query
-// heads 1200 and 800 for each eight pieces.
+// heads 2500 and 1200 for each eight pieces. (A whole warp calls it.)
 __device__ __forceinline__ Deal choose_deal(unsigned units, unsigned rows, int longest, unsigned grid, int heads) {
   if (rows == 0) return {0, 0};
   const unsigned turns = (heads + 2 * kWarps - 1) / (2 * kWarps);
-  auto join = [&](unsigned pieces) { return pieces > 1 ? 3000 + turns * (1200 + (pieces + 7) / 8 * 800) : 0; };
+  auto join = [&](unsigned pieces) { return pieces > 1 ? 3000 + turns * (2500 + (pieces + 7) / 8 * 1200) : 0; };
   // Equal shares of all units laid end to end, each row with a few units in
   // front of its own for its start, so that a CTA of many short rows gets
   // fewer units than one of few long ones. No row in more than kMaxPieces + 1.
@@ -156,14 +156,20 @@ __device__ __forceinline__ Deal choose_deal(unsigned units, unsigned rows, int l
   // Where a launch has few units: each row in equal parts of CTAs of its own,
   // if that lets the last of them finish sooner.
   const unsigned share = (units + d.n_cta - 1) / d.n_cta;
-  unsigned best = share * 1100 + (rows > 1 ? 6000 : 0) + join((longest + share - 1) / share + 1);
-  for (unsigned p = 1; p <= (unsigned)min(longest, kMaxPieces) && rows * p <= grid; p = p < 8 ? p + 1 : p * 2) {
-    const unsigned q = (longest + p - 1) / p, cost = q * 1100 + join(p);
-    if (cost < best) {
-      best = cost;
-      d.front = -(int)(q * p);
-      d.n_cta = rows * p;
-    }
+  const unsigned shares_cost = share * 1800 + (rows > 1 ? 6000 : 0) + join((longest + share - 1) / share + 1);
+  // lane i looks at i + 1 and at 34 + 2 i parts
+  unsigned best = 0xFFFFFFFFu;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const unsigned p = k == 0 ? (threadIdx.x & 31) + 1 : 34 + 2 * (threadIdx.x & 31);
+    const unsigned q = (longest + p - 1) / p;
+    if (p <= (unsigned)min(longest, kMaxPieces) && rows * p <= grid) best = min(best, (q * 1800 + join(p)) << 7 | p);
+  }
+  best = __reduce_min_sync(0xffffffffu, best);
+  if (best >> 7 < shares_cost) {
+    const unsigned p = best & 127;
+    d.front = -(int)((longest + p - 1) / p * p);
+    d.n_cta = rows * p;
   }
   return d;
 }
@@ -304,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
 
     // What the segment needs first is loaded before any of it is used: the
     // position, the new token's page, the first stages' pages, the query heads
-    // (kQ pairs of a thread at a time; behind the copies they would wait).
+    // (kQ of a thread at a time; behind the copies they would wait).
     constexpr int kQ = 4;
     const int64_t pos_in = a.positions != nullptr ? a.positions[b] : 0;
     int pg_new, off_new;
@@ -319,33 +325,27 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
     int pages[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) pages[s] = a.one_page ? page_at(t0 + s) : -1;
+    const int qj = tid % (DP / 2), q_first = tid / (DP / 2);   // this thread's column pair and first head
+    constexpr int kQStep = kThreads / (DP / 2);                 // heads that the threads cover at once
     uint32_t qx[kQ];
-    float2 rot[kQ];
-    const int pairs = heads * (D / 2);
-    auto load_q = [&](int i0) {
+    auto load_q = [&](int g0) {
 #pragma unroll
       for (int k = 0; k < kQ; ++k) {
-        const int i = i0 + k * kThreads, g = i / (D / 2), j = i - g * (D / 2);
-        if (i < pairs) {
-          const uint16_t* qr = new_row + (int64_t)(head0 + g) * D + j;
+        const int g = g0 + k * kQStep;
+        if (qj < D / 2 && g < heads) {
+          const uint16_t* qr = new_row + (int64_t)(head0 + g) * D + qj;
           qx[k] = (uint32_t)qr[0] | ((uint32_t)qr[D / 2] << 16);
         }
       }
     };
-    load_q(tid);
+    load_q(q_first);
     // a sequence that cannot take its token answers with zeros
     const bool ok = (unsigned)page_new < (unsigned)c.num_pages && (!turn || (pos_in >= 0 && pos_in < a.rope_rows));
     const int64_t pos = ok ? pos_in : 0;
     const float* cs = a.cos_t + pos * (D / 2);
     const float* sn = a.sin_t + pos * (D / 2);
-    auto load_rot = [&](int i0) {
-#pragma unroll
-      for (int k = 0; k < kQ; ++k) {
-        const int i = i0 + k * kThreads, j = i % (D / 2);
-        if (turn && i < pairs) rot[k] = make_float2(cs[j], sn[j]);
-      }
-    };
-    load_rot(tid);
+    float2 rot = make_float2(1.f, 0.f);
+    if (turn && qj < D / 2) rot = make_float2(cs[qj], sn[qj]);
 
     // A warp's share of unit t: slots t * 64 + warp * 16 + r. It copies the
     // rows of cached slots and zeros for the others; `live` is a bit per row
@@ -423,22 +423,19 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
     int page_next = pages[S - 1];
 
     // the rotated query heads of the tile
-    for (int i0 = tid; i0 < pairs; i0 += kQ * kThreads) {
-      if (i0 != tid) {
-        load_q(i0);
-        load_rot(i0);
-      }
+    for (int g0 = q_first; g0 < heads; g0 += kQ * kQStep) {
+      if (g0 != q_first) load_q(g0);
 #pragma unroll
       for (int k = 0; k < kQ; ++k) {
-        const int i = i0 + k * kThreads, g = i / (D / 2), j = i - g * (D / 2);
-        if (i >= pairs) continue;
+        const int g = g0 + k * kQStep;
+        if (qj >= D / 2 || g >= heads) continue;
         if (turn) {
           const float2 f = unpack2<BF>(qx[k]);
-          const float2 y = rotate(f.x, f.y, rot[k].x, rot[k].y);
+          const float2 y = rotate(f.x, f.y, rot.x, rot.y);
           qx[k] = pack2<BF>(y.x, y.y);
         }
-        qs[g * (DP + 8) + j] = (uint16_t)qx[k];
-        qs[g * (DP + 8) + j + D / 2] = (uint16_t)(qx[k] >> 16);
+        qs[g * (DP + 8) + qj] = (uint16_t)qx[k];
+        qs[g * (DP + 8) + qj + D / 2] = (uint16_t)(qx[k] >> 16);
       }
     }
     __syncthreads();
@@ -678,10 +675,12 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
       int* cnt = a.counters + b * rows_per_b + row;
       __syncthreads();
       if (tid == 0) {
-        __threadfence();                             // the CTA's piece, before its arrival
-        is_last = atomicAdd(cnt, 1) == cta1 - cta0;
+        // releases the CTA's piece (ordered before by the barrier) and acquires
+        // the others'
+        int seen;
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(seen) : "l"(cnt) : "memory");
+        is_last = seen == cta1 - cta0;
         if (is_last) *cnt = 0;                       // zero for the next call
-        __threadfence();
       }
       __syncthreads();
       if (is_last) {
@@ -690,34 +689,45 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
         const float* begun = a.partials + ((int64_t)cta0 * 2 + 1) * prow;
         const float* others = a.partials + (int64_t)cta0 * 2 * prow;
         auto piece = [&](int i) { return i == 0 ? begun : others + (int64_t)i * 2 * prow; };
-        // two heads per warp, which needs no other: the pieces' factors
-        // 2^(m_piece - m), lane i those of pieces i, i + 32, ..., then the sums, four
-        // values a lane
-        constexpr int kML = (kMaxPieces + 1 + 31) / 32;
+        // Two heads per warp, which needs no other: the pieces' factors
+        // 2^(m_piece - m), lane i those of pieces i, i + 32, ..., and their sums, four
+        // values a lane, eight pieces in flight ahead of their use.
+        constexpr int kML = (kMaxPieces + 1 + 31) / 32, kAhead = 8;
         for (int g0 = warp; g0 < heads; g0 += 2 * kWarps) {
+          const int second = g0 + kWarps < heads ? kWarps * D : 0;   // (an odd head is summed twice)
+          float4 v[kAhead][2];
+          auto load = [&](int i0, int d) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+              const float* src = piece(min(i0 + i, pieces - 1)) + g0 * D + (d < D ? d : 0);
+              v[i][0] = __ldcg(reinterpret_cast<const float4*>(src));
+              v[i][1] = __ldcg(reinterpret_cast<const float4*>(src + second));
+            }
+          };
+          load(0, 4 * lane);
           float f[2][kML], inv[2];
           {
-            float2 v[2][kML];
+            float2 ml[2][kML];
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
               for (int k = 0; k < kML; ++k) {
                 const int i = lane + 32 * k, g = g0 + e * kWarps;
-                v[e][k] = i < pieces && g < heads ? __ldcg(reinterpret_cast<const float2*>(piece(i) + kHeads * D) + g)
-                                                  : make_float2(-INFINITY, 0.f);
+                ml[e][k] = i < pieces && g < heads ? __ldcg(reinterpret_cast<const float2*>(piece(i) + kHeads * D) + g)
+                                                   : make_float2(-INFINITY, 0.f);
               }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-              for (int k = 0; k < kML; ++k) mm = fmaxf(mm, v[e][k].x);
+              for (int k = 0; k < kML; ++k) mm = fmaxf(mm, ml[e][k].x);
 #pragma unroll
               for (int o2 = 16; o2 > 0; o2 >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o2));
               const float bs = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
               for (int k = 0; k < kML; ++k) {
-                f[e][k] = ex2(v[e][k].x - bs);
-                ll = fmaf(f[e][k], v[e][k].y, ll);
+                f[e][k] = ex2(ml[e][k].x - bs);
+                ll = fmaf(f[e][k], ml[e][k].y, ll);
               }
               ll = warp_sum(ll);
               inv[e] = 1.f / ll;
@@ -725,30 +735,31 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
                 a.lse2[b * a.n_q + head0 + g0 + e * kWarps] = bs + log2f(ll);
             }
           }
-          const int second = g0 + kWarps < heads ? kWarps * D : 0;   // (an odd head is summed twice)
           for (int d = 4 * lane; d - 4 * lane < D; d += 128) {
-            const bool mine = d < D;
-            const int at = g0 * D + (mine ? d : 0);
+            if (d != 4 * lane) load(0, d);
             float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+            for (int i0 = 0; i0 < pieces; i0 += kAhead) {
 #pragma unroll
-            for (int k = 0; k < kML; ++k) {
-#pragma unroll 4
-              for (int i = 32 * k; i < min(pieces, 32 * k + 32); ++i) {
-                const float* src = piece(i) + at;
+              for (int i = 0; i < kAhead; ++i) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const float w = __shfl_sync(0xffffffffu, f[e][k], i - 32 * k);
-                  const float4 v = __ldcg(reinterpret_cast<const float4*>(src + e * second));
-                  acc[e].x = fmaf(w, v.x, acc[e].x);
-                  acc[e].y = fmaf(w, v.y, acc[e].y);
-                  acc[e].z = fmaf(w, v.z, acc[e].z);
-                  acc[e].w = fmaf(w, v.w, acc[e].w);
+                  // the factor of piece i0 + i, 0 behind the last
+                  float w = f[e][0];
+#pragma unroll
+                  for (int k = 1; k < kML; ++k) w = i0 >= 32 * k ? f[e][k] : w;
+                  w = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
+                  if (i0 + i >= pieces) w = 0.f;
+                  acc[e].x = fmaf(w, v[i][e].x, acc[e].x);
+                  acc[e].y = fmaf(w, v[i][e].y, acc[e].y);
+                  acc[e].z = fmaf(w, v[i][e].z, acc[e].z);
+                  acc[e].w = fmaf(w, v[i][e].w, acc[e].w);
                 }
               }
+              if (i0 + kAhead < pieces) load(i0 + kAhead, d);
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              if (!mine || (e == 1 && second == 0)) continue;
+              if (d >= D || (e == 1 && second == 0)) continue;
               uint32_t* dst = reinterpret_cast<uint32_t*>(out + (g0 + e * kWarps) * D + d);
               dst[0] = ok ? pack2<BF>(acc[e].x * inv[e], acc[e].y * inv[e]) : 0;
               dst[1] = ok ? pack2<BF>(acc[e].z * inv[e], acc[e].w * inv[e]) : 0;
