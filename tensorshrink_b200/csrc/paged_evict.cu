@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
   __syncthreads();
   const int64_t limit = (int64_t)s_newest - a.recent;
   for (int i = tid; i < n; i += kSelThreads)
-    if ((int64_t)pos[i] > limit && keys[i] != 0) keys[i] = 0xFF800000u;   // recent: the key of +inf
+    if ((int64_t)pos[i] > limit && keys[i] != 0) keys[i] = 0xFFFFFFFFu;   // recent: above any score
 
   // radix selection of the budget-th largest key
   uint32_t prefix = 0, mask = 0;

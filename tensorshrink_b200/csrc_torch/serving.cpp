@@ -4,9 +4,8 @@
 // As for qlinear, each call is one dispatcher call with no Python-side
 // workspace lookup or struct packing. Arguments are checked here (ValueError
 // and NotImplementedError as the Python wrappers document them); launches go
-// to the current stream of the tensors' device. One zero-filled workspace per
-// (device, stream) serves all of them; buffers are kept for the life of the
-// process, since a captured graph may still point at one.
+// to the current stream of the tensors' device. One workspace per (device,
+// stream) serves all of them, and one per graph while the stream is captured.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -24,18 +23,32 @@ namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
 
-std::mutex g_mu;
-std::map<std::pair<int, cudaStream_t>, at::Tensor> g_ws;
-std::vector<at::Tensor> g_old;   // superseded buffers
+struct Workspace {
+  at::Tensor t;
+  unsigned long long capture = 0;   // of the graph that it belongs to
+};
 
+std::mutex g_mu;
+std::map<std::pair<int, cudaStream_t>, Workspace> g_ws, g_captured;
+
+// A workspace of at least `bytes`, its counters zero. A captured stream has
+// its own, from the graph's memory, and the graph zeroes it: neither the
+// graph's replays on another stream nor calls outside of it meet the other's
+// counters, and no warm-up has to come before the capture. Buffers are used on
+// the stream that they were allocated on, so a superseded one can be freed.
 at::Tensor workspace(const at::Device& dev, cudaStream_t s, size_t bytes) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(s, &status, &id) != cudaSuccess) (void)cudaGetLastError();
+  const bool captured = status == cudaStreamCaptureStatusActive;
   std::lock_guard<std::mutex> lk(g_mu);
-  auto& w = g_ws[{dev.index(), s}];
-  if (!w.defined() || (size_t)w.numel() < bytes) {
-    if (w.defined()) g_old.push_back(w);
-    w = at::zeros({(int64_t)std::max<size_t>(bytes, 1 << 20)}, at::TensorOptions().dtype(at::kByte).device(dev));
+  Workspace& w = (captured ? g_captured : g_ws)[{dev.index(), s}];
+  if (!w.t.defined() || (captured && w.capture != id) || (size_t)w.t.numel() < bytes) {
+    w.t = at::empty({(int64_t)std::max<size_t>(bytes, 1 << 20)}, at::TensorOptions().dtype(at::kByte).device(dev));
+    w.t.slice(0, 0, (int64_t)ts_serving_counter_bytes()).zero_();
+    w.capture = id;
   }
-  return w;
+  return w.t;
 }
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
@@ -367,12 +380,10 @@ void serving_status(int64_t device, bool clear) {
   const int rc = ts_fp4_status(nullptr, 0, clear ? 1 : 0, s);
   if (rc == TS_OK) return;
   if (clear) {
-    // counters that CTAs which gave up may have left non-zero
+    // counters that CTAs which gave up may have left non-zero (a graph zeroes its own)
     std::lock_guard<std::mutex> lk(g_mu);
     for (auto& kv : g_ws)
-      if (kv.first.first == device) kv.second.slice(0, 0, (int64_t)ts_serving_counter_bytes()).zero_();
-    for (auto& w : g_old)
-      if (w.device().index() == device) w.slice(0, 0, (int64_t)ts_serving_counter_bytes()).zero_();
+      if (kv.first.first == device) kv.second.t.slice(0, 0, (int64_t)ts_serving_counter_bytes()).zero_();
   }
   done(rc, "ts_fp4_status");
 }

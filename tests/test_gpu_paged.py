@@ -412,6 +412,40 @@ def test_captured_in_a_graph(ts):
         assert torch.equal(getattr(c, name), getattr(eager, name)), name
 
 
+def test_captured_without_a_warm_up(ts):
+    """Graphs of one stream do not depend on calls outside of them, nor on one another's order."""
+    c = make(ts, [300, 30], 2, 64, 16, torch.bfloat16, 15, room=8)
+    qkv = [torch.randn(2, 12 * 64, device="cuda").to(torch.bfloat16) for _ in range(2)]
+    want = [ts.paged_decode_attention(q, 8, clone(ts, c), c.seq_lens.long()) for q in qkv]
+    pos = c.seq_lens.long()
+    s = torch.cuda.Stream()
+    graphs, got = [], []
+    for q in qkv:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            got.append(ts.paged_decode_attention(q, 8, c, pos))
+    with torch.cuda.stream(s):
+        outside = ts.paged_decode_attention(qkv[0], 8, c, pos)
+    torch.cuda.synchronize()
+    assert torch.equal(outside, want[0])
+    for i in (1, 0, 1):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[i], want[i]), i
+
+
+def test_evict_keeps_recent_slots_beside_infinite_scores(ts):
+    c = make(ts, [90], 1, 64, 16, torch.bfloat16, 16)
+    t = c.page_table.long()[0]
+    c.scores[t[:5]] = float("inf")                               # 80 slots, more than the budget
+    for i in range(90):
+        c.slot_pos[t[i // 16], 0, i % 16] = i
+    newest = set(range(86, 90))
+    ts.paged_evict(c, 33, 4)
+    pos = [int(c.slot_pos[t[i // 16], 0, i % 16]) for i in range(33)]
+    assert newest <= set(pos) and len(set(pos)) == 33
+
+
 def test_refusals(ts):
     c = make(ts, [5, 9], 2, 64, 16, torch.bfloat16, 1)
     plain = make(ts, [5, 9], 2, 64, 16, torch.bfloat16, 1, track=False)
