@@ -953,29 +953,26 @@ static int launch(int BT, const CUtensorMap& wm, const CUtensorMap& xm, const Ge
 using namespace ts;
 using namespace ts::fp4;
 
-extern "C" size_t ts_fp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int format) {
-  (void)format;
-  if (M <= 0 || N <= 0 || K <= 0) return paged::kCounterBytes;
-  const Plan p = plan(M, N, K);
+// Bytes of a plan's workspace: counters, then partial sums.
+static size_t plan_bytes(const Plan& p) {
   return paged::kCounterBytes + (!p.pair ? (size_t)p.grid * 2 * kBW * p.BT * 4 : 0);
 }
 
-static int matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, const void* bias, int bias_dtype, void* out,
+extern "C" size_t ts_fp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int format) {
+  (void)format;
+  if (M <= 0 || N <= 0 || K <= 0) return paged::kCounterBytes;
+  return plan_bytes(plan(M, N, K));
+}
+
+static int matmul(const Plan& p, const ts_fp4_tensor* x, const ts_fp4_tensor* w, const void* bias, int bias_dtype, void* out,
                   int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes, int overlap,
                   void* stream) {
-  int rc = check_tensor(x, "ts_fp4_matmul a");
-  if (rc != TS_OK) return rc;
-  rc = check_tensor(w, "ts_fp4_matmul b");
-  if (rc != TS_OK) return rc;
-  TS_REQUIRE(x->format == w->format, "both operands must have one format");
-  TS_REQUIRE(x->cols == w->cols, "a has %lld columns, b %lld", (long long)x->cols, (long long)w->cols);
+  int rc;
   TS_UNSUPPORTED(out_dtype == TS_F16 || out_dtype == TS_BF16 || out_dtype == TS_F32, "unknown output type %d", out_dtype);
   TS_UNSUPPORTED(!bias || bias_dtype == TS_F16 || bias_dtype == TS_BF16 || bias_dtype == TS_F32, "unknown bias type %d",
                  bias_dtype);
-  if (x->rows == 0 || w->rows == 0) return TS_OK;
   TS_REQUIRE(out, "NULL pointer");
-  const Plan p = plan(x->rows, w->rows, w->cols);
-  const size_t need = ts_fp4_matmul_workspace_size(x->rows, w->rows, w->cols, w->format);
+  const size_t need = plan_bytes(p);
   if (!p.pair && (workspace == nullptr || workspace_bytes < need)) {
     set_error("workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return TS_ERR_WORKSPACE;
@@ -1055,7 +1052,15 @@ static int matmul(const ts_fp4_tensor* x, const ts_fp4_tensor* w, const void* bi
 extern "C" int ts_fp4_matmul(const ts_fp4_tensor* a, const ts_fp4_tensor* b, const void* bias, int bias_dtype, void* out,
                              int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
                              void* stream) {
-  return matmul(a, b, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, workspace_bytes, 0, stream);
+  int rc = check_tensor(a, "ts_fp4_matmul a");
+  if (rc != TS_OK) return rc;
+  rc = check_tensor(b, "ts_fp4_matmul b");
+  if (rc != TS_OK) return rc;
+  TS_REQUIRE(a->format == b->format, "both operands must have one format");
+  TS_REQUIRE(a->cols == b->cols, "a has %lld columns, b %lld", (long long)a->cols, (long long)b->cols);
+  if (a->rows == 0 || b->rows == 0) return TS_OK;
+  return matmul(plan(a->rows, b->rows, b->cols), a, b, bias, bias_dtype, out, out_dtype, out_row_stride, workspace,
+                workspace_bytes, 0, stream);
 }
 
 extern "C" size_t ts_serving_counter_bytes(void) { return paged::kCounterBytes; }
@@ -1098,14 +1103,14 @@ extern "C" int ts_fp4_linear(const void* x, int x_dtype, int64_t M, int64_t x_ro
   if (rc != TS_OK) return rc;
   TS_REQUIRE(M >= 0, "bad shape");
   if (M == 0 || w->rows == 0) return TS_OK;
-  const size_t need = ts_fp4_linear_workspace_size(M, w->rows, w->cols, w->format);
+  const Plan p = plan(M, w->rows, w->cols);
+  // the activations' codes and scales lie behind the product's scratch
+  const size_t at = align_up(plan_bytes(p), 256), need = at + linear_act_bytes(M, w->cols, w->format);
   if (workspace == nullptr || workspace_bytes < need) {
     set_error("workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return TS_ERR_WORKSPACE;
   }
   TS_REQUIRE(is_aligned(workspace, 16), "workspace must be 16-byte aligned");
-  // the activations' codes and scales lie behind the product's scratch
-  const size_t at = align_up(ts_fp4_matmul_workspace_size(M, w->rows, w->cols, w->format), 256);
   ts_fp4_tensor t{};
   t.codes = reinterpret_cast<uint8_t*>(workspace) + at;
   t.scales = t.codes + align_up((size_t)M * (size_t)(padded_cols(w->cols) / 2), 256);
@@ -1115,5 +1120,5 @@ extern "C" int ts_fp4_linear(const void* x, int x_dtype, int64_t M, int64_t x_ro
   t.format = w->format;
   rc = ts_fp4_quantize(x, x_dtype, x_row_stride, &t, 0, nullptr, 0, stream);
   if (rc != TS_OK) return rc;
-  return matmul(&t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, 1, stream);
+  return matmul(p, &t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, 1, stream);
 }

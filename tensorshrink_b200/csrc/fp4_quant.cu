@@ -24,7 +24,6 @@ namespace fp4 {
 constexpr int kWarps = 8;
 constexpr int kAmaxSeg = 512;      // columns of a warp's piece of the maximum pass
 constexpr int kSeg = 128;          // columns of a warp's piece, four rows high
-constexpr int kMaxParts = 1184;    // CTAs of the maximum pass at most
 constexpr int kAmaxUnits = 4;      // pieces that a warp of the maximum pass has in flight
 
 struct QuantArgs {
@@ -38,8 +37,7 @@ struct QuantArgs {
   int reverse;                  // walk from the end
   int64_t amax_cols;            // the maximum pass takes rows without gaps as one row
   int amax_rows, amax_segs;
-  uint32_t* parts;              // bits of the CTAs' maxima when the scale is sought
-  int* counter;                 // of CTAs that have left theirs; zero between calls
+  int* counters;                // CTAs that have left their maximum, the maximum's bits; zero between calls
 };
 
 template <int DT>
@@ -254,13 +252,13 @@ __device__ __forceinline__ void load_flat(const void* x, int64_t cols, int64_t r
   }
 }
 
-// The tensor's scale: CTAs' maxima to the workspace, the last CTA to arrive
-// takes their maximum (the order does not matter to a maximum).
+// The tensor's scale. CTAs take the maximum in the workspace (its order does
+// not matter); the last to arrive finishes it. 14336 x 4096 fp16: 23 us, 5.1 TB/s
+// (28 us with a maximum per CTA that the last one gathers behind fences).
 template <int DT, int AL>
 __global__ void __launch_bounds__(kWarps * 32) fp4_amax_kernel(const QuantArgs a) {
   using E = Elem<DT>;
   __shared__ uint32_t part[kWarps];
-  __shared__ int last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // a warp takes 512 columns of a row: four "rows" of 128, one behind the other
   const int step = gridDim.x * kWarps, units = a.amax_rows * a.amax_segs;
@@ -294,24 +292,14 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_amax_kernel(const QuantArgs a
     uint32_t r = 0;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) r = max(r, part[i]);
-    a.parts[blockIdx.x] = r;
-    __threadfence();
-    last = atomicAdd(a.counter, 1) == (int)gridDim.x - 1;
-    if (last) *a.counter = 0;
-    __threadfence();
-  }
-  __syncthreads();
-  if (!last) return;
-  uint32_t r = 0;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += kWarps * 32) r = max(r, __ldcg(a.parts + i));
-  r = __reduce_max_sync(0xffffffffu, r);
-  __syncthreads();
-  if (lane == 0) part[warp] = r;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) r = max(r, part[i]);
-    *a.global_scale = fmaxf(__fmul_rn(__uint_as_float(r), 1.f / 2688.f), kMinScale);   // 2688 = 448 * 6
+    asm volatile("red.relaxed.gpu.global.max.u32 [%0], %1;" ::"l"(a.counters + 1), "r"(r) : "memory");
+    int seen;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(seen) : "l"(a.counters) : "memory");
+    if (seen == (int)gridDim.x - 1) {
+      const float top = __uint_as_float((uint32_t)__ldcg(a.counters + 1));
+      a.counters[0] = a.counters[1] = 0;
+      *a.global_scale = fmaxf(__fmul_rn(top, 1.f / 2688.f), kMinScale);   // 2688 = 448 * 6
+    }
   }
 }
 
@@ -504,7 +492,7 @@ static dim3 tile_grid(int64_t rows, int segs) {
 template <int DT, int AL>
 static int launch_amax(const QuantArgs& a, cudaStream_t st) {
   const int64_t units = (int64_t)a.amax_rows * a.amax_segs;
-  const int grid = (int)std::min<int64_t>(std::min(kMaxParts, sm_count() * 3), (units + kWarps - 1) / kWarps);
+  const int grid = (int)std::min<int64_t>(sm_count() * 3, (units + kWarps - 1) / kWarps);
   fp4_amax_kernel<DT, AL><<<grid, kWarps * 32, 0, st>>>(a);
   TS_LAUNCH_CHECK();
   return TS_OK;
@@ -569,7 +557,7 @@ extern "C" size_t ts_fp4_scales_bytes(int64_t rows, int64_t cols, int format) {
   return (size_t)((rows + kTileRows - 1) / kTileRows) * scale_tiles(cols, format) * kTileBytes;
 }
 
-extern "C" size_t ts_fp4_quantize_workspace_size(void) { return paged::kCounterBytes + (size_t)kMaxParts * 4; }
+extern "C" size_t ts_fp4_quantize_workspace_size(void) { return paged::kCounterBytes; }
 
 extern "C" int ts_fp4_quantize(const void* x, int x_dtype, int64_t x_row_stride, const ts_fp4_tensor* t, int find_scale,
                                void* workspace, size_t workspace_bytes, void* stream) {
@@ -596,8 +584,7 @@ extern "C" int ts_fp4_quantize(const void* x, int x_dtype, int64_t x_row_stride,
   a.kt = scale_tiles(t->cols, t->format);
   a.segs = (int)((padded_cols(t->cols) + kSeg - 1) / kSeg);
   a.reverse = find_scale ? 1 : 0;
-  a.parts = find_scale ? reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(workspace) + paged::kCounterBytes) : nullptr;
-  a.counter = reinterpret_cast<int*>(workspace);
+  a.counters = reinterpret_cast<int*>(workspace);
   const bool flat = x_row_stride == t->cols || t->rows == 1;
   a.amax_rows = flat ? 1 : (int)t->rows;
   a.amax_cols = flat ? t->rows * t->cols : t->cols;

@@ -8,6 +8,7 @@
 // stream) serves all of them, and one per graph while the stream is captured.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -54,6 +55,11 @@ at::Tensor workspace(const at::Device& dev, cudaStream_t s, size_t bytes) {
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 template <typename T = void>
 T* ptr(const OptTensor& t) { return has(t) ? static_cast<T*>(t->data_ptr()) : nullptr; }
+
+// An uninitialised tensor on the current device, without a dispatcher call.
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Device& dev) {
+  return at::Tensor(at::detail::empty_cuda(shape, type, dev, c10::nullopt));
+}
 
 bool known(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16 || t == at::kFloat; }
 
@@ -129,12 +135,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_quantize(const at::Tensor& x_
   const at::Tensor x = x_in.stride(1) == 1 || x_in.size(1) == 1 ? x_in : x_in.contiguous();
   const int64_t rows = x.size(0), cols = x.size(1), kb = padded(cols) / 2;
   const bool find = format == TS_NVFP4 && !has(scale);
-  const auto bytes = at::TensorOptions().dtype(at::kByte).device(dev);
   at::Tensor g;
-  if (find) g = rows ? at::empty({1}, bytes.dtype(at::kFloat)) : at::ones({1}, bytes.dtype(at::kFloat));
+  if (find) g = rows ? fresh({1}, at::kFloat, dev) : at::ones({1}, at::TensorOptions().dtype(at::kFloat).device(dev));
   else if (has(scale)) g = *scale;
-  at::Tensor codes = at::empty({rows, kb}, bytes);
-  at::Tensor scales = at::empty({(int64_t)ts_fp4_scales_bytes(rows, cols, (int)format)}, bytes);
+  at::Tensor codes = fresh({rows, kb}, at::kByte, dev);
+  at::Tensor scales = fresh({(int64_t)ts_fp4_scales_bytes(rows, cols, (int)format)}, at::kByte, dev);
   const ts_fp4_tensor t = fp4_view(codes, scales, g.defined() ? OptTensor(g) : c10::nullopt, rows, cols, format, "fp4_quantize");
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   at::Tensor ws;
@@ -149,7 +154,7 @@ at::Tensor fp4_dequantize(const at::Tensor& codes, const at::Tensor& scales, con
   const ts_fp4_tensor t = fp4_view(codes, scales, g, rows, cols, format, "fp4_dequantize");
   const int dt = code_of(dtype, "fp4_dequantize");
   c10::cuda::CUDAGuard guard(codes.device());
-  at::Tensor out = at::empty({rows, cols}, codes.options().dtype(dtype));
+  at::Tensor out = fresh({rows, cols}, dtype, codes.device());
   done(ts_fp4_dequantize(&t, out.data_ptr(), dt, cols, at::cuda::getCurrentCUDAStream(codes.device().index()).stream()),
        "fp4_dequantize");
   return out;
@@ -172,7 +177,7 @@ at::Tensor fp4_matmul(const at::Tensor& ac, const at::Tensor& as, const OptTenso
   on(bc, dev, "b");
   c10::cuda::CUDAGuard guard(dev);
   const int bdt = check_bias(bias, n, dev, "fp4_matmul"), dt = code_of(out_dtype, "fp4_matmul");
-  at::Tensor out = at::empty({m, n}, ac.options().dtype(out_dtype));
+  at::Tensor out = fresh({m, n}, out_dtype, dev);
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   at::Tensor ws = workspace(dev, s, ts_fp4_matmul_workspace_size(m, n, cols, (int)format));
   done(ts_fp4_matmul(&a, &b, ptr(bias), bdt, out.data_ptr(), dt, n, ws.data_ptr(), (size_t)ws.numel(), s), "fp4_matmul");
@@ -201,7 +206,7 @@ at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& codes, const at::Te
   if (x2d.stride(1) != 1 && cols != 1) x2d = x2d.contiguous();
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = rows;
-  at::Tensor out = at::empty(shape, x.options().dtype(odt));
+  at::Tensor out = fresh(shape, odt, dev);
   const int64_t m = x2d.size(0);
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   at::Tensor ws = workspace(dev, s, ts_fp4_linear_workspace_size(m, rows, cols, (int)format));
@@ -348,7 +353,7 @@ at::Tensor paged_decode_attention(const at::Tensor& qkv, int64_t n_q, const at::
                           out.scalar_type() == qkv.scalar_type() && out.stride(1) == 1,
                       "out must be [batch, n_q head_dim] of qkv's type with contiguous rows");
   } else {
-    out = at::empty({c.batch, owidth}, qkv.options());
+    out = fresh({c.batch, owidth}, qkv.scalar_type(), dev);
   }
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   at::Tensor ws = workspace(dev, s, ts_paged_attention_workspace_size(&c, (int)n_q, accumulate));
