@@ -413,8 +413,8 @@ TS_API int ts_fp4_matmul(const ts_fp4_tensor* a, const ts_fp4_tensor* b, const v
 
 /*
  * out[M, N] = x . w^T (+ bias): ts_fp4_quantize of x [M, cols] (with the given
- * device scale x_scale for TS_NVFP4, NULL: 1) into the workspace, then
- * ts_fp4_matmul.
+ * device scale x_scale for TS_NVFP4, NULL: 1), then ts_fp4_matmul, bit for
+ * bit; a few tokens in one kernel, more by way of the workspace.
  */
 TS_API size_t ts_fp4_linear_workspace_size(int64_t M, int64_t N, int64_t K, int format);
 TS_API int ts_fp4_linear(const void* x, int x_dtype, int64_t M, int64_t x_row_stride, float* x_scale,

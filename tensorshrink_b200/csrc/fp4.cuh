@@ -66,6 +66,94 @@ __device__ __forceinline__ void from_e2m1x8(uint32_t d, uint32_t (&h)[4]) {
       : "r"(d));
 }
 
+// Element types of what is quantised.
+template <int DT>
+struct Elem;
+template <>
+struct Elem<TS_F16> {
+  using T = uint16_t;
+  static constexpr uint32_t kInf = 0x7C00u;
+  static __device__ float f(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+};
+template <>
+struct Elem<TS_BF16> {
+  using T = uint16_t;
+  static constexpr uint32_t kInf = 0x7F80u;
+  static __device__ float f(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+};
+template <>
+struct Elem<TS_F32> {
+  using T = uint32_t;
+  static constexpr uint32_t kInf = 0x7F800000u;
+  static __device__ float f(uint32_t v) { return __uint_as_float(v); }
+};
+
+// A lane's 16 elements as words (8, or 16 of fp32); of rows that start in the
+// middle of a word, also the first element of row `lane` (lanes 0 to 3).
+template <int DT>
+struct Lane {
+  static constexpr int N = DT == TS_F32 ? 16 : 8;
+  uint32_t w[N];
+  uint32_t e;
+};
+
+// Largest magnitude as the type's bits (a NaN or infinity: at least kInf).
+template <int DT>
+__device__ __forceinline__ uint32_t top_bits(const Lane<DT>& v) {
+  uint32_t m = 0;
+  if constexpr (DT == TS_F32) {
+#pragma unroll
+    for (int i = 0; i < Lane<DT>::N; ++i) m = max(m, v.w[i] & 0x7FFFFFFFu);
+    return m;
+  } else {
+#pragma unroll
+    for (int i = 0; i < Lane<DT>::N; ++i) m = __vmaxu2(m, v.w[i] & 0x7FFF7FFFu);
+    return max(m & 0xFFFFu, m >> 16);
+  }
+}
+
+// Element i of a lane in fp32.
+template <int DT>
+__device__ __forceinline__ float elem(const Lane<DT>& v, int i) {
+  if (DT == TS_F32) return __uint_as_float(v.w[i % Lane<DT>::N]);
+  const uint32_t w = v.w[(i / 2) % Lane<DT>::N];
+  if (DT == TS_BF16) return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return i & 1 ? f.y : f.x;
+}
+
+// Codes (`out`) and scale (returned) of a lane's 16 columns: a block of nvfp4,
+// whose tensor scale is g and to_scale = 1 / (6 g); half a block of mxfp4, the
+// neighbouring lane having the other. A whole warp calls it.
+template <int DT, bool NV>
+__device__ __forceinline__ uint32_t quantise16(const Lane<DT>& v, float g, float to_scale, uint2& out) {
+  using E = Elem<DT>;
+  uint32_t top = top_bits<DT>(v);
+  if (!NV) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  out = make_uint2(0, 0);
+  if (top >= E::kInf) return NV ? 0x7Fu : 0xFFu;
+  const float amax = E::f((typename E::T)top);
+  float r;
+  uint32_t sc;
+  if (NV) {
+    sc = __nv_cvt_float_to_fp8(fminf(__fmul_rn(amax, to_scale), 448.f), __NV_SATFINITE, __NV_E4M3);
+    const float sf = e4m3_value((uint8_t)sc);
+    r = sf > 0.f ? __frcp_rn(__fmul_rn(sf, g)) : 0.f;
+  } else {
+    const int e = (int)(__float_as_uint(amax) >> 23) - 2;
+    sc = (uint32_t)max(e, 0);
+    r = __uint_as_float((254u - sc) << 23);
+  }
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, i);
+  out.x = to_e2m1x8(f, r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, 8 + i);
+  out.y = to_e2m1x8(f, r);
+  return sc;
+}
+
 // Checks a tensor's description (`what` names it in messages).
 int check_tensor(const ts_fp4_tensor* t, const char* what);
 

@@ -22,6 +22,8 @@
 //               stage's columns are rewritten only after the MMAs that read
 //               them have released the stage.
 //   warps 2-5   epilogue: tcgen05.ld, tensor scales, bias, stores
+//   warps 6-13  (kernels of few tokens that come unquantised) quantise the
+//               stage's tokens into shared memory, a stage per warp in turn
 // Bound by the weight's bytes. The tiles are few, so their stages are laid end
 // to end and each CTA takes an equal share (split along K); partial sums are
 // added by the last CTA of a tile to arrive, in CTA order.
@@ -40,6 +42,13 @@ constexpr int kBW = 128;                 // weight rows of a tile = TMEM lanes
 constexpr int kBK = 256;                 // columns of a stage = one 128-byte row
 constexpr int kEpiWarps = 4;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
+constexpr int kQuantWarps = 8;
+
+// Up to this many tokens the kernel quantises them itself, every CTA those of
+// its stages; more come from a quantiser in front, which the kernel's start
+// overlaps. nvfp4, 14336 x 4096, back to back in a graph: 1 token 11.3 us by
+// itself, 8 tokens 12.4, 16 tokens 15.5; 9 to 16 tokens behind a quantiser 14.1.
+constexpr int kOwnTokens = 8;
 constexpr int kTmemCols = 512;
 constexpr int kABytes = kBW * 128;
 
@@ -63,6 +72,9 @@ struct GemmArgs {
   uint64_t wait_ns;
   int stall;                       // test hook: the producer issues nothing
   int overlap;                     // launched while the quantisation of x may still run
+  const void* x;                   // tokens to be quantised by the kernel itself
+  int x_dtype, x_aligned;          // x_aligned: rows start on 16 bytes
+  int64_t x_stride, K;
 };
 
 template <bool NV, int BT>
@@ -170,11 +182,69 @@ __device__ __forceinline__ bool items_next(const GemmArgs& a, ItemIter& it, Item
   return true;
 }
 
-template <bool NV, int BT>
-__global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_constant__ CUtensorMap wmap,
+// A lane's 16 columns of a row of tokens from p on, of which `left` exist.
+template <int DT>
+__device__ __forceinline__ void load_run(const typename Elem<DT>::T* p, int left, bool aligned, Lane<DT>& v) {
+  constexpr int N = Lane<DT>::N;
+  if (aligned && left >= 16) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v.w[i] = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < left) {
+      if (DT == TS_F32) v.w[i % N] = (uint32_t)p[i];
+      else v.w[(i / 2) % N] |= (uint32_t)p[i] << (16 * (i & 1));
+    }
+}
+
+// Quantises columns [256 kb, 256 kb + 256) of all tokens into a stage: codes as
+// TMA would swizzle them, scales as a scale tile lays them. The loads are on
+// their way while the warp waits for the stage (`ready`). By a whole warp, 16
+// lanes a row.
+template <bool NV, int DT, typename Ready>
+__device__ __forceinline__ bool quantise_stage(const GemmArgs& a, int kb, char* sx, char* ssx, float g, float to_scale,
+                                               Ready ready) {
+  using T = typename Elem<DT>::T;
+  constexpr int kAhead = 4;                        // rows of a lane in flight
+  const int lane = threadIdx.x & 31, j = lane & 15, M = (int)a.M;
+  const int64_t c0 = (int64_t)kb * kBK + j * 16;
+  const int left = (int)max((int64_t)0, min((int64_t)16, a.K - c0));
+  const int block = NV ? j : j >> 1;               // of the stage
+  for (int r0 = 0; r0 < M; r0 += 2 * kAhead) {
+    Lane<DT> v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int r = r0 + 2 * k + (lane >> 4);
+      load_run<DT>(reinterpret_cast<const T*>(a.x) + (r < M ? r * a.x_stride + c0 : 0), r < M ? left : 0, a.x_aligned, v[k]);
+    }
+    if (r0 == 0 && !ready()) return false;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (r0 + 2 * k >= M) break;
+      const int r = r0 + 2 * k + (lane >> 4);
+      uint2 codes;
+      const uint32_t sc = quantise16<DT, NV>(v[k], g, to_scale, codes);
+      if (r >= M) continue;
+      *reinterpret_cast<uint2*>(sx + r * 128 + (((j >> 1) ^ (r & 7)) << 4) + (j & 1) * 8) = codes;
+      if (NV || (j & 1) == 0) ssx[(block >> 2) * kTileBytes + r * 16 + (block & 3)] = (char)sc;
+    }
+  }
+  return true;
+}
+
+template <bool NV, int BT, bool Q>
+__global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_gemm_kernel(const __grid_constant__ CUtensorMap wmap,
                                                             const __grid_constant__ CUtensorMap xmap,
                                                             const GemmArgs a) {
   using P = Shape<NV, BT>;
+  static_assert(!Q || BT <= 32, "the tokens' scales lie in a tile's first 32 rows");
   constexpr int S = P::S;
   extern __shared__ char smem_raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -194,9 +264,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
   const int ntiles = a.wblocks * a.tblocks;
   if (warp == 0 && lane == 0) {
     prefetch_tensormap(&wmap);
-    prefetch_tensormap(&xmap);
+    if (!Q) prefetch_tensormap(&xmap);
     for (int i = 0; i < S; ++i) {
-      mbar_init(full + i, 1);
+      mbar_init(full + i, Q ? 2 : 1);
       mbar_init(empty + i, 1);
     }
     for (int i = 0; i < P::kAcc; ++i) {
@@ -220,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
       auto load_w = [&](const Item& x, int kb, int s) {
         const int wb = x.tile / a.tblocks, t0 = kb * P::kTiles;
         const uint32_t sf_bytes = min(P::kTiles, a.kt - t0) * kTileBytes;
-        mbar_arrive_expect_tx(full + s, kABytes + P::kXBytes + 2 * sf_bytes);
+        mbar_arrive_expect_tx(full + s, Q ? kABytes + sf_bytes : kABytes + P::kXBytes + 2 * sf_bytes);
         tma_load_2d(s_w + s * kABytes, &wmap, kb * 128, wb * kBW, full + s);
         bulk_load(s_sw + s * P::kSf, a.wscales + ((int64_t)wb * a.kt + t0) * kTileBytes, sf_bytes, full + s);
       };
@@ -253,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
             }
             load_w(x, kb, s);
           }
-          load_x(x, kb, s);
+          if (!Q) load_x(x, kb, s);
           ++issued;
           if (++s == S) {
             s = 0;
@@ -319,6 +389,30 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_gemm_kernel(const __grid_cons
       // every MMA issued has finished before the TMEM is freed
       umma_commit(drain);
       mbar_wait_hint(drain, 0, nullptr, 0, a.wait_ns);
+    }
+  } else if (Q && warp >= 2 + kEpiWarps) {
+    const float g = usable_scale(a.xg), to_scale = NV ? __frcp_rn(__fmul_rn(6.f, g)) : 0.f;
+    int n = 0;                                         // of the CTA's stages
+    bool ok = true;
+    ItemIter it = items_begin(a, ntiles);
+    Item x;
+    while (ok && items_next(a, it, x)) {
+      for (int kb = x.k0; kb < x.k1; ++kb, ++n) {
+        if (n % kQuantWarps != warp - (2 + kEpiWarps)) continue;
+        const int s = n % S;
+        auto ready = [&] {
+          return __all_sync(0xffffffffu, mbar_wait_hint(empty + s, (uint32_t)(n / S & 1) ^ 1, &g_err, 25, a.wait_ns));
+        };
+        char* sx = s_x + s * P::kXBytes;
+        char* ssx = s_sx + s * P::kSf;
+        if (a.x_dtype == TS_BF16) ok = quantise_stage<NV, TS_BF16>(a, kb, sx, ssx, g, to_scale, ready);
+        else if (a.x_dtype == TS_F16) ok = quantise_stage<NV, TS_F16>(a, kb, sx, ssx, g, to_scale, ready);
+        else ok = quantise_stage<NV, TS_F32>(a, kb, sx, ssx, g, to_scale, ready);
+        if (!ok) break;
+        fence_proxy_async_smem();                      // the tensor cores read what was written
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + s);
+      }
     }
   } else {
     const int quad = warp & 3;
@@ -919,9 +1013,9 @@ static int scale_map(CUtensorMap* map, const ts_fp4_tensor& t) {
                         kBK / block_of(t.format) / 4, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <bool NV, int BT>
+template <bool NV, int BT, bool Q>
 static int launch(const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& a, int grid, cudaStream_t st) {
-  auto k = fp4_gemm_kernel<NV, BT>;
+  auto k = fp4_gemm_kernel<NV, BT, Q>;
   constexpr size_t smem = Shape<NV, BT>::kSmem;
   static_assert(smem <= 227 * 1024, "shared memory");
   static thread_local int configured_dev = -1;
@@ -931,18 +1025,20 @@ static int launch(const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& 
     TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_dev = dev;
   }
-  TS_CUDA_TRY(launch_after(k, grid, kThreads, smem, st, a.overlap, wm, xm, a));
+  TS_CUDA_TRY(launch_after(k, grid, kThreads + (Q ? kQuantWarps * 32 : 0), smem, st, a.overlap, wm, xm, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
 
 template <bool NV>
 static int launch(int BT, const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& a, int grid, cudaStream_t st) {
+  static_assert(kOwnTokens <= 16, "tokens of the kernel that quantises them");
+  if (a.x != nullptr) return launch<NV, 16, true>(wm, xm, a, grid, st);
   switch (BT) {
-    case 16: return launch<NV, 16>(wm, xm, a, grid, st);
-    case 32: return launch<NV, 32>(wm, xm, a, grid, st);
-    case 64: return launch<NV, 64>(wm, xm, a, grid, st);
-    default: return launch<NV, 128>(wm, xm, a, grid, st);
+    case 16: return launch<NV, 16, false>(wm, xm, a, grid, st);
+    case 32: return launch<NV, 32, false>(wm, xm, a, grid, st);
+    case 64: return launch<NV, 64, false>(wm, xm, a, grid, st);
+    default: return launch<NV, 128, false>(wm, xm, a, grid, st);
   }
 }
 
@@ -964,9 +1060,16 @@ extern "C" size_t ts_fp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K, 
   return plan_bytes(plan(M, N, K));
 }
 
+// Tokens that the product quantises itself.
+struct Tokens {
+  const void* x;
+  int dtype;
+  int64_t stride;
+};
+
 static int matmul(const Plan& p, const ts_fp4_tensor* x, const ts_fp4_tensor* w, const void* bias, int bias_dtype, void* out,
                   int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes, int overlap,
-                  void* stream) {
+                  const Tokens* own, void* stream) {
   int rc;
   TS_UNSUPPORTED(out_dtype == TS_F16 || out_dtype == TS_BF16 || out_dtype == TS_F32, "unknown output type %d", out_dtype);
   TS_UNSUPPORTED(!bias || bias_dtype == TS_F16 || bias_dtype == TS_BF16 || bias_dtype == TS_F32, "unknown bias type %d",
@@ -1039,11 +1142,17 @@ static int matmul(const Plan& p, const ts_fp4_tensor* x, const ts_fp4_tensor* w,
   a.wait_ns = wait_limit_ns();
   a.stall = stall;
   a.overlap = overlap;
+  a.x = own ? own->x : nullptr;
+  a.x_dtype = own ? own->dtype : 0;
+  a.x_stride = own ? own->stride : 0;
+  a.x_aligned = own && is_aligned(own->x, 16) && own->stride * (own->dtype == TS_F32 ? 4 : 2) % 16 == 0;
+  a.K = w->cols;
   CUtensorMap wm, xm;
   rc = encode_tmap_2d(&wm, w->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)w->rows, row, 128, kBW,
                       CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != TS_OK) return rc;
-  rc = encode_tmap_2d(&xm, x->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)x->rows, row, 128, p.BT,
+  if (own) xm = wm;                                    // (not used)
+  else rc = encode_tmap_2d(&xm, x->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)x->rows, row, 128, p.BT,
                       CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != TS_OK) return rc;
   return w->format == TS_NVFP4 ? launch<true>(p.BT, wm, xm, a, p.grid, st) : launch<false>(p.BT, wm, xm, a, p.grid, st);
@@ -1060,7 +1169,7 @@ extern "C" int ts_fp4_matmul(const ts_fp4_tensor* a, const ts_fp4_tensor* b, con
   TS_REQUIRE(a->cols == b->cols, "a has %lld columns, b %lld", (long long)a->cols, (long long)b->cols);
   if (a->rows == 0 || b->rows == 0) return TS_OK;
   return matmul(plan(a->rows, b->rows, b->cols), a, b, bias, bias_dtype, out, out_dtype, out_row_stride, workspace,
-                workspace_bytes, 0, stream);
+                workspace_bytes, 0, nullptr, stream);
 }
 
 extern "C" size_t ts_serving_counter_bytes(void) { return paged::kCounterBytes; }
@@ -1118,7 +1227,13 @@ extern "C" int ts_fp4_linear(const void* x, int x_dtype, int64_t M, int64_t x_ro
   t.rows = M;
   t.cols = w->cols;
   t.format = w->format;
+  if (M <= kOwnTokens) {
+    TS_UNSUPPORTED(x_dtype == TS_F16 || x_dtype == TS_BF16 || x_dtype == TS_F32, "unknown element type %d", x_dtype);
+    TS_REQUIRE(x, "NULL pointer");
+    const Tokens own = {x, x_dtype, x_row_stride};
+    return matmul(p, &t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, 0, &own, stream);
+  }
   rc = ts_fp4_quantize(x, x_dtype, x_row_stride, &t, 0, nullptr, 0, stream);
   if (rc != TS_OK) return rc;
-  return matmul(p, &t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, 1, stream);
+  return matmul(p, &t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, 1, nullptr, stream);
 }

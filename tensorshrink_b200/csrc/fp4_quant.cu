@@ -40,27 +40,6 @@ struct QuantArgs {
   int* counters;                // CTAs that have left their maximum, the maximum's bits; zero between calls
 };
 
-template <int DT>
-struct Elem;
-template <>
-struct Elem<TS_F16> {
-  using T = uint16_t;
-  static constexpr uint32_t kInf = 0x7C00u;
-  static __device__ float f(uint16_t v) { return __half2float(__ushort_as_half(v)); }
-};
-template <>
-struct Elem<TS_BF16> {
-  using T = uint16_t;
-  static constexpr uint32_t kInf = 0x7F80u;
-  static __device__ float f(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
-};
-template <>
-struct Elem<TS_F32> {
-  using T = uint32_t;
-  static constexpr uint32_t kInf = 0x7F800000u;
-  static __device__ float f(uint32_t v) { return __uint_as_float(v); }
-};
-
 // 32 bytes from a 32-byte boundary.
 __device__ __forceinline__ void ld32(const void* p, uint32_t (&w)[8]) {
   asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -72,15 +51,6 @@ __device__ __forceinline__ void st32(void* p, const uint32_t* w) {
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
-
-// A lane's 16 elements as words (8, or 16 of fp32); of rows that start in the
-// middle of a word, also the first element of row `lane` (lanes 0 to 3).
-template <int DT>
-struct Lane {
-  static constexpr int N = DT == TS_F32 ? 16 : 8;
-  uint32_t w[N];
-  uint32_t e;
-};
 
 // Where a lane reads (or writes) its share of a warp's four rows, row0 + 32 q.
 // AL: the alignment of rows. With 32 or 16, eight lanes take a row, 16
@@ -197,31 +167,6 @@ __device__ __forceinline__ void deal(const Place<DT, AL>& place, uint32_t* stage
   }
 }
 
-// Largest magnitude as the type's bits (a NaN or infinity: at least kInf).
-template <int DT>
-__device__ __forceinline__ uint32_t top_bits(const Lane<DT>& v) {
-  uint32_t m = 0;
-  if constexpr (DT == TS_F32) {
-#pragma unroll
-    for (int i = 0; i < Lane<DT>::N; ++i) m = max(m, v.w[i] & 0x7FFFFFFFu);
-    return m;
-  } else {
-#pragma unroll
-    for (int i = 0; i < Lane<DT>::N; ++i) m = __vmaxu2(m, v.w[i] & 0x7FFF7FFFu);
-    return max(m & 0xFFFFu, m >> 16);
-  }
-}
-
-// Element i of a lane in fp32.
-template <int DT>
-__device__ __forceinline__ float elem(const Lane<DT>& v, int i) {
-  if (DT == TS_F32) return __uint_as_float(v.w[i % Lane<DT>::N]);
-  const uint32_t w = v.w[(i / 2) % Lane<DT>::N];
-  if (DT == TS_BF16) return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return i & 1 ? f.y : f.x;
-}
-
 // 512 columns of one row from `first` on, as words in any order (for maxima).
 template <int DT, int AL>
 __device__ __forceinline__ void load_flat(const void* x, int64_t cols, int64_t row_at, int64_t first, int lane,
@@ -305,7 +250,6 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_amax_kernel(const QuantArgs a
 
 template <int DT, bool NV, int AL>
 __global__ void __launch_bounds__(kWarps * 32, DT == TS_F32 ? 6 : 7) fp4_quantize_kernel(const QuantArgs a) {
-  using E = Elem<DT>;
   __shared__ __align__(16) uint32_t stage[AL >= 16 ? 1 : kWarps][AL >= 16 ? 4 : 32 * Lane<DT>::N];
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -324,33 +268,8 @@ __global__ void __launch_bounds__(kWarps * 32, DT == TS_F32 ? 6 : 7) fp4_quantiz
     Lane<DT> v;
     load16<DT, AL>(src, (int64_t)seg * kSeg, a.cols - (int64_t)seg * kSeg, lane, v);
     deal<DT, AL>(src, stage[AL >= 16 ? 0 : warp], lane, v);
-    uint32_t top = top_bits<DT>(v);
-    if (!NV) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    const bool bad = top >= E::kInf;
-    const float amax = E::f((typename E::T)top);
-    float r;
-    uint32_t sc;
-    if (NV) {
-      sc = __nv_cvt_float_to_fp8(fminf(__fmul_rn(amax, to_scale), 448.f), __NV_SATFINITE, __NV_E4M3);
-      const float sf = e4m3_value((uint8_t)sc);
-      r = sf > 0.f ? __frcp_rn(__fmul_rn(sf, g)) : 0.f;
-    } else {
-      const int e = (int)(__float_as_uint(amax) >> 23) - 2;
-      sc = (uint32_t)max(e, 0);
-      r = __uint_as_float((254u - sc) << 23);
-    }
-    uint2 out = make_uint2(0, 0);
-    if (bad) {
-      sc = NV ? 0x7Fu : 0xFFu;
-    } else {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, i);
-      out.x = to_e2m1x8(f, r);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = elem<DT>(v, 8 + i);
-      out.y = to_e2m1x8(f, r);
-    }
+    uint2 out;
+    const uint32_t sc = quantise16<DT, NV>(v, g, to_scale, out);
     if (exists && seg * 8 + (lane & 7) < groups) {
       *reinterpret_cast<uint2*>(codes + (int64_t)seg * 64) = out;
       // 128 columns are two scale tiles of nvfp4, one of mxfp4

@@ -252,6 +252,31 @@ def test_linear_is_quantise_then_product(ts, fmt, shape, n, k):
         check_product(y.reshape(-1, n), values64(a), values64(w), bias, k)
 
 
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(1, 130, 17), (2, 300, 64), (3, 128, 250), (5, 1000, 5001), (8, 4096, 4096), (8, 200, 8200),
+                                   (9, 130, 515)])
+def test_linear_of_few_tokens(ts, fmt, dtype, m, n, k):
+    """Tokens that the product may quantise itself: the bits of a quantisation
+    in front, for any stride and alignment, with blocks that are not finite."""
+    w = ts.fp4_quantize(data(n, k, torch.bfloat16, 20), fmt)
+    wide = data(m, k + 21, dtype, 21)
+    g = torch.full((1,), 0.01, device="cuda") if fmt == "nvfp4" else None
+    for x in (wide[:, :k].contiguous(), wide[:, 8:8 + k], wide[:, 1:1 + k], wide[:1, 3:3 + k].expand(m, k)):
+        y = ts.fp4_linear(x, w, input_scale=g, out_dtype=torch.float32)
+        assert torch.equal(y, ts.fp4_matmul(ts.fp4_quantize(x, fmt, g), w, out_dtype=torch.float32))
+    x = wide[:, :k].clone()
+    x[0, k // 2] = float("inf")
+    x[m - 1, 0] = float("nan")
+    x[m // 2, k - 1] = 0.0
+    y = ts.fp4_linear(x, w, input_scale=g, out_dtype=torch.float32)
+    want = ts.fp4_matmul(ts.fp4_quantize(x, fmt, g), w, out_dtype=torch.float32)
+    assert torch.equal(y.nan_to_num(), want.nan_to_num()) and torch.equal(y.isnan(), want.isnan())
+    bad = torch.zeros(m, dtype=torch.bool, device="cuda")
+    bad[0] = bad[m - 1] = True
+    assert torch.equal(y.isnan().all(1), bad)
+
+
 def test_results_repeat_and_do_not_depend_on_earlier_calls(ts):
     """Split sums are added in a fixed order, and a call leaves the workspace
     as the next one of another shape needs it."""
