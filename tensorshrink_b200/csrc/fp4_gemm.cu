@@ -24,9 +24,11 @@
 //   warps 2-5   epilogue: tcgen05.ld, tensor scales, bias, stores
 //   warps 6-13  (kernels of few tokens that come unquantised) quantise the
 //               stage's tokens into shared memory, a stage per warp in turn
-// Bound by the weight's bytes. The tiles are few, so their stages are laid end
-// to end and each CTA takes an equal share (split along K); partial sums are
-// added by the last CTA of a tile to arrive, in CTA order.
+// Bound by the weight's bytes. The tiles are few, so they are split along K:
+// into whole parts, whose CTAs are a cluster and add their sums through
+// distributed shared memory, or, where clusters do not fit the tiles, into
+// equal shares of all stages laid end to end, whose sums the last CTA of a
+// tile to arrive adds from the workspace. Either way in CTA order.
 //
 // Every wait is bounded in wall-clock time: a role whose wait runs out records
 // a code and unwinds; the TMEM is freed at the end in any case.
@@ -51,6 +53,7 @@ constexpr int kQuantWarps = 8;
 constexpr int kOwnTokens = 8;
 constexpr int kTmemCols = 512;
 constexpr int kABytes = kBW * 128;
+constexpr int kMaxCluster = 8;           // CTAs of a cluster that share a tile
 
 __device__ int g_err;
 
@@ -75,6 +78,8 @@ struct GemmArgs {
   const void* x;                   // tokens to be quantised by the kernel itself
   int x_dtype, x_aligned;          // x_aligned: rows start on 16 bytes
   int64_t x_stride, K;
+  int cluster;                     // CTAs that share a tile as a cluster, or 0
+  int out_vec;                     // rows of out take stores of four values
 };
 
 template <bool NV, int BT>
@@ -160,6 +165,59 @@ __device__ __forceinline__ void store_tokens(const GemmArgs& a, int64_t m, int64
     for (int j = 0; j < R; ++j, p += step)
       if (j < jn) *p = __float2half_rn(fmaf(v[j], alpha, bias));
   }
+}
+
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address of the same shared-memory location in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Stores alpha * v + bias as output features n .. n + 3 of token m.
+__device__ __forceinline__ void store_four(const GemmArgs& a, int64_t m, int64_t n, const float4& v, float alpha) {
+  float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = fmaf(f[i], alpha, a.bias && n + i < a.N ? load_f(a.bias, a.bias_dtype, n + i) : 0.f);
+  const int64_t at = m * a.out_stride + n;
+  if (a.out_dtype == TS_F32) {
+    float* p = reinterpret_cast<float*>(a.out) + at;
+    if (a.out_vec && n + 3 < a.N) {
+      *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) p[i] = f[i];
+    return;
+  }
+  uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + at;
+  uint2 w;
+  if (a.out_dtype == TS_BF16) {
+    w = make_uint2(paged::pack2<true>(f[0], f[1]), paged::pack2<true>(f[2], f[3]));
+  } else {
+    w = make_uint2(paged::pack2<false>(f[0], f[1]), paged::pack2<false>(f[2], f[3]));
+  }
+  if (a.out_vec && n + 3 < a.N) {
+    *reinterpret_cast<uint2*>(p) = w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < a.N) p[i] = (uint16_t)((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
 }
 
 // Work items of a CTA: a tile and the stages [k0, k1) of it that are its own.
@@ -443,6 +501,14 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
           tc_fence_before();
           mbar_arrive(tempty + buf);
         }
+        if (a.cluster) {
+          // to shared memory, over the stages (all used): [BT tokens][128 rows]
+          float* dst = reinterpret_cast<float*>(s_w) + c * CW * kBW + r;
+#pragma unroll
+          for (int j = 0; j < CW; ++j)
+            if (c * CW + j < jn_all) dst[j * kBW] = v[j];
+          continue;
+        }
         if (!whole) {
           // a piece: [BT / 4 tokens][128 rows][4 tokens], coalesced both ways
           float4* dst = reinterpret_cast<float4*>(pp) + (size_t)(c * CW / 4) * kBW + r;
@@ -458,7 +524,7 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
         buf = 0;
         bph ^= 1;
       }
-      if (whole) continue;
+      if (whole || a.cluster) continue;
       // a tile split over several CTAs: the last to arrive adds the pieces
       named_bar_sync(3, kEpiWarps * 32);
       if (r == 0) {
@@ -526,6 +592,34 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
+  }
+  if (a.cluster) {
+    // every CTA of the tile has its sums in shared memory: a warp adds a
+    // token's, four neighbouring features per lane
+    static_assert((size_t)BT * kBW * 4 <= (size_t)S * kABytes, "the sums lie over the stages");
+    constexpr int kWarpsAll = kThreads / 32 + (Q ? kQuantWarps : 0);
+    cluster_sync();
+    const int rank = (int)cta_rank(), tile = blockIdx.x / a.cluster;
+    const int64_t m0 = (int64_t)(tile % a.tblocks) * BT, n = (int64_t)(tile / a.tblocks) * kBW + 4 * lane;
+    const int jn = (int)min((int64_t)BT, a.M - m0);
+    const float alpha = usable_scale(a.wg) * usable_scale(a.xg);
+    for (int j = rank + a.cluster * warp; j < jn; j += a.cluster * kWarpsAll) {
+      const uint32_t at = smem_u32(s_w) + (uint32_t)(j * kBW + 4 * lane) * 4;
+      float4 v[kMaxCluster];
+#pragma unroll
+      for (int p = 0; p < kMaxCluster; ++p)
+        if (p < a.cluster) v[p] = ld_cluster(map_cta(at, p));
+#pragma unroll
+      for (int p = 1; p < kMaxCluster; ++p)
+        if (p < a.cluster) {
+          v[0].x += v[p].x;
+          v[0].y += v[p].y;
+          v[0].z += v[p].z;
+          v[0].w += v[p].w;
+        }
+      if (n < a.N) store_four(a, m0 + j, n, v[0], alpha);
+    }
+    cluster_sync();                                    // nobody leaves while its sums may be read
   }
 }
 
@@ -598,20 +692,6 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
   for (int i = 0; i < 128; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-__device__ __forceinline__ uint32_t cta_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// The address of the same shared-memory location in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_cta(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-}
 // TMA tile load into this CTA's shared memory, completing on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
@@ -925,12 +1005,48 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
 struct Plan {
   bool pair;        // CTA pairs on tiles of 256 tokens x 256 weight rows
   int BT, tblocks, wblocks, kblocks, ntiles, grid;
+  int cluster;      // CTAs that share a tile as a cluster, or 0
 };
+
+// Clusters of `size` CTAs, one per SM, that the device holds at once.
+static int max_clusters(int size) {
+  static thread_local int known[kMaxCluster + 1], known_dev = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  if (dev != known_dev) {
+    for (int i = 0; i <= kMaxCluster; ++i) known[i] = -1;
+    known_dev = dev;
+  }
+  if (known[size] < 0) {
+    auto k = fp4_gemm_kernel<true, 128, false>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(sm_count() / size * size));
+    cfg.blockDim = dim3((unsigned)kThreads);
+    cfg.dynamicSmemBytes = Shape<true, 128>::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    known[size] = n;
+  }
+  return known[size];
+}
 
 // Cycles that a call takes at least, as measured: a stage of a pair's tile 620
 // and the change from tile to tile 2000; a stage of a lone CTA's tile 550, or what
 // its bytes take at DRAM's rate; a join of up to four pieces 3000 and 2500 per
-// 32 tokens; the start 4000. Only their order matters.
+// 32 tokens, of a cluster 1500 and 600. Only their order matters.
 static Plan plan(int64_t M, int64_t N, int64_t K) {
   Plan p{};
   const int sms = std::max(2, sm_count()), pairs = sms / 2;
@@ -952,10 +1068,12 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
   p.grid = (int)all;
   double best = cost(all, (int)std::min<int64_t>(p.kblocks, all / std::max<int64_t>(1, ntiles) + 2));
   for (int parts = 1; parts <= p.kblocks && ntiles * parts <= sms; ++parts) {
-    const double c = cost(ntiles * parts, parts);
+    const bool fits = parts > 1 && parts <= kMaxCluster && max_clusters(parts) >= ntiles;
+    const double c = fits ? cost(ntiles * parts, 1) + 1500 + 600.0 * rounds : cost(ntiles * parts, parts);
     if (c < best) {
       best = c;
       p.grid = (int)(ntiles * parts);
+      p.cluster = fits ? parts : 0;
     }
   }
   p.ntiles = (int)std::min<int64_t>(ntiles, INT32_MAX);
@@ -964,6 +1082,7 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
   const double pair = (double)((mb * nb + pairs - 1) / pairs) * (620.0 * p.kblocks + 2000);
   if (pair <= best || ntiles > (int64_t)paged::kCounters) {
     p.pair = true;
+    p.cluster = 0;
     p.tblocks = (int)mb;
     p.wblocks = (int)nb;
     p.ntiles = (int)(mb * nb);
@@ -975,17 +1094,25 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
 // Launch; with `overlap` the kernel may start while the one before it (which
 // allows that, and whose results it waits for by itself) still runs.
 template <typename K, typename... Args>
-static cudaError_t launch_after(K k, int grid, int threads, size_t smem, cudaStream_t st, int overlap, const Args&... args) {
+static cudaError_t launch_after(K k, int grid, int threads, size_t smem, cudaStream_t st, int overlap, int cluster,
+                                const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = overlap ? 1 : 0;
+  if (overlap) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
   return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
@@ -1001,7 +1128,7 @@ static int launch_pair(const CUtensorMap (&m)[4], const PairArgs& a, int grid, c
     TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_dev = dev;
   }
-  TS_CUDA_TRY(launch_after(k, grid, kPairThreads, smem, st, a.overlap, m[0], m[1], m[2], m[3], a));
+  TS_CUDA_TRY(launch_after(k, grid, kPairThreads, smem, st, a.overlap, 0, m[0], m[1], m[2], m[3], a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
@@ -1025,7 +1152,7 @@ static int launch(const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& 
     TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_dev = dev;
   }
-  TS_CUDA_TRY(launch_after(k, grid, kThreads + (Q ? kQuantWarps * 32 : 0), smem, st, a.overlap, wm, xm, a));
+  TS_CUDA_TRY(launch_after(k, grid, kThreads + (Q ? kQuantWarps * 32 : 0), smem, st, a.overlap, a.cluster, wm, xm, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
@@ -1051,7 +1178,7 @@ using namespace ts::fp4;
 
 // Bytes of a plan's workspace: counters, then partial sums.
 static size_t plan_bytes(const Plan& p) {
-  return paged::kCounterBytes + (!p.pair ? (size_t)p.grid * 2 * kBW * p.BT * 4 : 0);
+  return paged::kCounterBytes + (!p.pair && !p.cluster ? (size_t)p.grid * 2 * kBW * p.BT * 4 : 0);
 }
 
 extern "C" size_t ts_fp4_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int format) {
@@ -1147,6 +1274,9 @@ static int matmul(const Plan& p, const ts_fp4_tensor* x, const ts_fp4_tensor* w,
   a.x_stride = own ? own->stride : 0;
   a.x_aligned = own && is_aligned(own->x, 16) && own->stride * (own->dtype == TS_F32 ? 4 : 2) % 16 == 0;
   a.K = w->cols;
+  a.cluster = p.cluster;
+  const int wide = out_dtype == TS_F32 ? 16 : 8;       // bytes of four values
+  a.out_vec = is_aligned(out, wide) && out_row_stride % 4 == 0;
   CUtensorMap wm, xm;
   rc = encode_tmap_2d(&wm, w->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, row, (uint64_t)w->rows, row, 128, kBW,
                       CU_TENSOR_MAP_SWIZZLE_128B);

@@ -202,6 +202,26 @@ def test_product(ts, fmt, m, n, k):
                   bias.to(torch.bfloat16), k)
 
 
+# few tiles of many columns: tiles split over CTAs, as whole parts and as equal shares, few and many of them
+SPLITS = [(1, 128, 14336), (100, 120, 9000), (40, 10300, 4160), (3, 1023, 4160), (33, 640, 9000), (128, 257, 12173),
+          (7, 3136, 2000), (64, 9000, 3000), (190, 700, 6000), (16, 2300, 1100), (1, 18800, 8192)]
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m,n,k", SPLITS)
+def test_product_split_along_its_columns(ts, fmt, m, n, k):
+    a = ts.fp4_quantize(data(m, k, torch.bfloat16, m + k), fmt)
+    b = ts.fp4_quantize(data(n, k, torch.bfloat16, n), fmt)
+    bias = torch.randn(n, device="cuda").to(torch.bfloat16)
+    va, vb = values64(a), values64(b)
+    first = {}
+    for _ in range(2):
+        for dt in (torch.float32, torch.bfloat16):
+            y = ts.fp4_matmul(a, b, bias=bias, out_dtype=dt)
+            check_product(y, va, vb, bias, k)
+            assert torch.equal(y, first.setdefault(dt, y))
+
+
 # enough tiles for CTA pairs, with edges in every direction
 PAIRS = [(200, 9500, 320), (257, 5000, 1088), (1000, 2561, 576), (129, 19000, 64), (600, 3200, 2000),
          (130, 16576, 256), (512, 8288, 640), (400, 8100, 1344), (256, 16500, 832)]
