@@ -778,22 +778,29 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
 // the attention read.
 template <int W>
 __global__ void __launch_bounds__(256, 6) paged_weights_kernel(const AttnArgs a) {
-  pdl_wait_primary();
   const Cache& c = a.c;
   const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv;
   const int len = c.seq_lens[b];
   if (units_of(a, len) == 0) return;
   const bool ok = takes(a, b, len, a.positions != nullptr ? a.positions[b] : 0);
   const int64_t q = (int64_t)b * a.n_q + h * a.group;
+  bool waits = true;
   for (int slot0 = (blockIdx.x * blockDim.x + threadIdx.x) * W; slot0 <= len; slot0 += gridDim.x * blockDim.x * W) {
-    // everything that is read is on its way before the first of it is needed
+    // what the attention does not write is read while it may still run
     int pg, off;
     split_slot(a, slot0, &pg, &off);
     const int page = c.table[b * c.table_stride + pg];
-    const float* lg = a.logits + q * a.logit_stride + slot0;
+    const bool has = ok && (unsigned)page < (unsigned)c.num_pages;
+    float* s = c.scores + (has ? stat_at(c, page, h, off) : 0);
     float w[W];
 #pragma unroll
-    for (int i = 0; i < W; ++i) w[i] = 0.f;
+    for (int i = 0; i < W; ++i) w[i] = has && slot0 + i < len ? s[i] : 0.f;
+    if (waits) pdl_wait_primary();
+    waits = false;
+    const float* lg = a.logits + q * a.logit_stride + slot0;
+    float sum[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) sum[i] = 0.f;
     for (int g0 = 0; g0 < a.group; g0 += 4) {
       float v[4][W], lse[4];
 #pragma unroll
@@ -812,17 +819,13 @@ __global__ void __launch_bounds__(256, 6) paged_weights_kernel(const AttnArgs a)
       for (int g = 0; g < 4; ++g) {
         if (g0 + g >= a.group) break;
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i] += ex2(v[g][i] - lse[g]);
+        for (int i = 0; i < W; ++i) sum[i] += ex2(v[g][i] - lse[g]);
       }
     }
-    if (!ok || (unsigned)page >= (unsigned)c.num_pages) continue;
-    float* s = c.scores + stat_at(c, page, h, off);    // (the attention has set the new slot's to 0)
-    float old[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) old[i] = slot0 + i <= len ? s[i] : 0.f;
+    if (!has) continue;
 #pragma unroll
     for (int i = 0; i < W; ++i)
-      if (slot0 + i <= len) s[i] = old[i] + w[i];
+      if (slot0 + i <= len) s[i] = w[i] + sum[i];
   }
 }
 
