@@ -74,11 +74,12 @@ __device__ __forceinline__ void split_slot(const AttnArgs& a, int s, int* page, 
   }
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes), "l"(policy)
+               : "memory");
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -276,6 +277,10 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
   const Shares shares(total, n_cta);
   const unsigned u1 = shares.begin(blockIdx.x + 1);
 
+  // with scores to accumulate, the logits shall stay in L2, not the cache
+  uint64_t policy;
+  if (a.logits != nullptr) asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  else asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
   char* ring = smem + (size_t)warp * S * kStage;
   const uint32_t ring_u = smem_u32(ring);
   const uint32_t qs_u = smem_u32(qs);
@@ -374,8 +379,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
 #pragma unroll
               for (int i = 0; i < kRows / kRowsPer; ++i) {
                 const uint32_t d = dst + i * kRowsPer * kPitch + (x0 ^ (((i * kRowsPer) & 7) << 4));
-                cp16(d, kp);
-                cp16(d + kRows * kPitch, kp + kv);
+                cp16(d, kp, policy);
+                cp16(d + kRows * kPitch, kp + kv, policy);
                 kp += step;
               }
             }
@@ -384,8 +389,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
             for (int i = 0; i < kRows / kRowsPer; ++i) {
               const int ok = i * kRowsPer + rl < rows;
               const uint32_t d = dst + i * kRowsPer * kPitch + (x0 ^ (((i * kRowsPer) & 7) << 4));
-              cp16(d, ok ? kp : c.k, ok * 16);
-              cp16(d + kRows * kPitch, ok ? kp + kv : c.v, ok * 16);
+              cp16(d, ok ? kp : c.k, ok * 16, policy);
+              cp16(d + kRows * kPitch, ok ? kp + kv : c.v, ok * 16, policy);
               if (ok) kp += step;
             }
           }
@@ -408,8 +413,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
             const int64_t e = ok ? (ro + cl * 8) * 2 : 0;
             const uint32_t d = dst + i * kRowsPer * kPitch + ((cl ^ (r & 7)) << 4);
             if (col) {
-              cp16(d, c.k + e, ok * 16);
-              cp16(d + kRows * kPitch, c.v + e, ok * 16);
+              cp16(d, c.k + e, ok * 16, policy);
+              cp16(d + kRows * kPitch, c.v + e, ok * 16, policy);
             }
           }
         }
