@@ -28,7 +28,11 @@
 // into whole parts, whose CTAs are a cluster and add their sums through
 // distributed shared memory, or, where clusters do not fit the tiles, into
 // equal shares of all stages laid end to end, whose sums the last CTA of a
-// tile to arrive adds from the workspace. Either way in CTA order.
+// tile to arrive adds from the workspace. Either way in CTA order. Measured, back
+// to back in a graph: 14336 x 4096 nvfp4, 1 token 11.8 us, 128 tokens 14.4 (33 MB,
+// 5.1 us at the copy bandwidth: 6.2 TB/s while the weight streams, the rest is
+// start, first loads and epilogue); 4096 x 14336, four CTAs a tile, 33 tokens
+// 13.8 us (15.8 by way of the workspace), 128 tokens 15.9 (19.0).
 //
 // Every wait is bounded in wall-clock time: a role whose wait runs out records
 // a code and unwinds; the TMEM is freed at the end in any case.
@@ -619,6 +623,10 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
 // complete on the leader's barrier; the leader's thread issues scale copies
 // and MMAs for both; commits release the stage in both. Tokens are the
 // accumulator's lanes, so that a thread stores runs of its token's outputs.
+// Measured: 8192 x 28672 x 8192 nvfp4, 720 to 760 us, 5.1 to 5.3 PFLOP/s at the
+// power limit (a lone CTA's tiles of 128 x 128: 1284 us); 2047 x 14336 x 4096,
+// 62 us, 3.9 PFLOP/s, in seven rounds of tiles where six hold all but four.
+// Bound by the loads into each SM (about 52 of 64 bytes a clock).
 
 constexpr int BN = 256, kHalf = BN / 2;
 constexpr int kPairEpi = 8, kPairThreads = (2 + kPairEpi) * 32;

@@ -8,7 +8,10 @@
 // word by word, coalesced, through shared memory. Bound by DRAM traffic: x is
 // read once (twice when the tensor's scale is sought, the second time from the
 // end, so that what the first pass left in L2 is found there), 0.5625 (0.53)
-// bytes an element are written.
+// bytes an element are written. Measured: 14336 x 4096 fp16, 27 us behind the
+// maximum pass and 26 us back, 5.7 TB/s; 2047 x 14330 bf16 (rows that start in
+// the middle of a word), 19 us and 15 us, 3.9 and 4.8 TB/s, bound by the words'
+// way through shared memory; 1 x 4096, 2.0 us each.
 //
 // Every rounding is spelled out (a reciprocal and products rounded to fp32,
 // two conversions to nearest even), so codes are reproducible bit for bit

@@ -25,6 +25,12 @@
 // enters its product as two terms of the cache's type (16 bits of it): one
 // alone would add as large an error as the rounding of the output does, and
 // the second product costs nothing that the loads do not hide.
+//
+// Measured (bf16, 128 columns, 8 kv heads of 4 query heads): 64 sequences of up to
+// 8191 slots, 177 us, 6.1 TB/s, 94% of the copy bandwidth; 4 of 32768, 88 us, with
+// the logits kept 90 us (98 us with the cache read at the same L2 priority as
+// the logits are written); one of 512, 10.0 us, a chain of latencies (lengths,
+// pages, rows, the warps' and the CTAs' joins).
 #include <algorithm>
 
 #include "paged.cuh"
@@ -780,7 +786,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : DP == 128 ? 2 : 1) pa
 // score[slot] += sum over the group of 2^(logit - lse2): a thread takes W
 // neighbouring slots of a kv head, W = 4 where pages hold a multiple of four.
 // Reads 4 bytes per slot and query head, next to the 4 D bytes per slot that
-// the attention read.
+// the attention read, from L2: 8 us behind the attention of 4 x 32768 slots of 8
+// kv heads of 4.
 template <int W>
 __global__ void __launch_bounds__(256, 6) paged_weights_kernel(const AttnArgs a) {
   const Cache& c = a.c;
@@ -837,7 +844,8 @@ __global__ void __launch_bounds__(256, 6) paged_weights_kernel(const AttnArgs a)
 // Stores tokens behind a sequence's cached ones: slot len + t of every kv
 // head gets k (rotated when tables are given) and v; scores and positions
 // are set. A warp takes four tokens of a head at a time, 16 bytes per lane
-// and token. Bound by DRAM traffic: every row is read and written once.
+// and token. Bound by DRAM traffic: every row is read and written once. 16 x 4096
+// tokens of 8 kv heads of 128 columns: 86 us, 6.2 TB/s; one token: 2.5 us.
 constexpr int kTok = 4;
 
 struct AppendArgs {

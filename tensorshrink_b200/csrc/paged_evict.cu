@@ -18,7 +18,9 @@
 // Where a head can have only few movers (a token in, a token out), the select
 // CTA moves them itself and there is no second kernel.
 // What bounds them: select reads 8 bytes per slot and is latency-bound at one
-// CTA per head; move is DRAM traffic of the moved slots only.
+// CTA per head (1025 slots 9.6 us with its one move, 8192 slots 15 us); move is
+// DRAM traffic of the moved slots only (16 sequences cut from 8192 to 4096 slots
+// of 8 heads of 128 columns: 25 us, lists and pages looked up on the way).
 #include <algorithm>
 #include <climits>
 
