@@ -1030,7 +1030,7 @@ static int max_clusters(int size) {
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess) {
       (void)cudaGetLastError();
-      n = 0;
+      return 0;
     }
     known[size] = n;
   }
