@@ -147,27 +147,42 @@ __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint
         : "memory");
 }
 
+// Both tensor scales on a sum: as their product or, where that is no number of
+// good precision, one after the other (the one that keeps clear of the range's end
+// first), so that a result within the range is right for any pair of scales.
+struct Alpha {
+  float a, b;
+  __device__ __forceinline__ Alpha(float x, float y) : a(x * y), b(1.f) {
+    const bool high = a > 1.329227995784916e36f, low = a < 7.52316384526264e-37f;   // 2^120, 2^-120
+    if (high || low) {
+      a = high ? fminf(x, y) : fmaxf(x, y);
+      b = high ? fmaxf(x, y) : fminf(x, y);
+    }
+  }
+  __device__ __forceinline__ float operator()(float v, float bias) const { return fmaf(__fmul_rn(v, a), b, bias); }
+};
+
 // Stores alpha * v + bias for `jn` tokens from m on, of output feature n (one
 // per lane: the lanes of a warp store neighbours).
 template <int R>
-__device__ __forceinline__ void store_tokens(const GemmArgs& a, int64_t m, int64_t n, int jn, const float* v, float alpha,
+__device__ __forceinline__ void store_tokens(const GemmArgs& a, int64_t m, int64_t n, int jn, const float* v, const Alpha& alpha,
                                              float bias) {
   const int64_t at = m * a.out_stride + n, step = a.out_stride;
   if (a.out_dtype == TS_F32) {
     float* p = reinterpret_cast<float*>(a.out) + at;
 #pragma unroll
     for (int j = 0; j < R; ++j, p += step)
-      if (j < jn) *p = fmaf(v[j], alpha, bias);
+      if (j < jn) *p = alpha(v[j], bias);
   } else if (a.out_dtype == TS_BF16) {
     __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.out) + at;
 #pragma unroll
     for (int j = 0; j < R; ++j, p += step)
-      if (j < jn) *p = __float2bfloat16_rn(fmaf(v[j], alpha, bias));
+      if (j < jn) *p = __float2bfloat16_rn(alpha(v[j], bias));
   } else {
     __half* p = reinterpret_cast<__half*>(a.out) + at;
 #pragma unroll
     for (int j = 0; j < R; ++j, p += step)
-      if (j < jn) *p = __float2half_rn(fmaf(v[j], alpha, bias));
+      if (j < jn) *p = __float2half_rn(alpha(v[j], bias));
   }
 }
 
@@ -178,10 +193,10 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
 }
 
 // Stores alpha * v + bias as output features n .. n + 3 of token m.
-__device__ __forceinline__ void store_four(const GemmArgs& a, int64_t m, int64_t n, const float4& v, float alpha) {
+__device__ __forceinline__ void store_four(const GemmArgs& a, int64_t m, int64_t n, const float4& v, const Alpha& alpha) {
   float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = fmaf(f[i], alpha, a.bias && n + i < a.N ? load_f(a.bias, a.bias_dtype, n + i) : 0.f);
+  for (int i = 0; i < 4; ++i) f[i] = alpha(f[i], a.bias && n + i < a.N ? load_f(a.bias, a.bias_dtype, n + i) : 0.f);
   const int64_t at = m * a.out_stride + n;
   if (a.out_dtype == TS_F32) {
     float* p = reinterpret_cast<float*>(a.out) + at;
@@ -465,7 +480,7 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
   } else {
     const int quad = warp & 3;
     const int r = quad * 32 + lane;                  // this thread's row of the tile
-    const float alpha = usable_scale(a.wg) * usable_scale(a.xg);
+    const Alpha alpha(usable_scale(a.wg), usable_scale(a.xg));
     constexpr int CW = BT < 32 ? 16 : 32;
     int buf = 0;
     uint32_t bph = 0;
@@ -592,7 +607,7 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
     const int rank = (int)cta_rank(), tile = blockIdx.x / a.cluster;
     const int64_t m0 = (int64_t)(tile % a.tblocks) * BT, n = (int64_t)(tile / a.tblocks) * kBW + 4 * lane;
     const int jn = (int)min((int64_t)BT, a.M - m0);
-    const float alpha = usable_scale(a.wg) * usable_scale(a.xg);
+    const Alpha alpha(usable_scale(a.wg), usable_scale(a.xg));
     for (int j = rank + a.cluster * warp; j < jn; j += a.cluster * kWarpsAll) {
       const uint32_t at = smem_u32(s_w) + (uint32_t)(j * kBW + 4 * lane) * 4;
       float4 v[kMaxCluster];
@@ -877,7 +892,7 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
   } else {
     // two warps per quadrant of TMEM lanes, each with half of the columns
     const int quad = warp & 3, half = (warp - 2) >> 2;
-    const float alpha = usable_scale(a.wg) * usable_scale(a.xg);
+    const Alpha alpha(usable_scale(a.wg), usable_scale(a.xg));
     const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf;
     const uint32_t free_bar = map_cta(smem_u32(tempty), 0);
     int n = 0;
@@ -909,10 +924,10 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
 #pragma unroll
       for (int i = 0; i < kHalf; i += 4) {
         const float4 bs = *reinterpret_cast<const float4*>(s_bias + i);
-        v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), alpha, bs.x));
-        v[i + 1] = __float_as_uint(fmaf(__uint_as_float(v[i + 1]), alpha, bs.y));
-        v[i + 2] = __float_as_uint(fmaf(__uint_as_float(v[i + 2]), alpha, bs.z));
-        v[i + 3] = __float_as_uint(fmaf(__uint_as_float(v[i + 3]), alpha, bs.w));
+        v[i] = __float_as_uint(alpha(__uint_as_float(v[i]), bs.x));
+        v[i + 1] = __float_as_uint(alpha(__uint_as_float(v[i + 1]), bs.y));
+        v[i + 2] = __float_as_uint(alpha(__uint_as_float(v[i + 2]), bs.z));
+        v[i + 3] = __float_as_uint(alpha(__uint_as_float(v[i + 3]), bs.w));
       }
       if (a.out_dtype == TS_F32) {
         float* out = reinterpret_cast<float*>(a.out) + m0 * a.out_stride + n0;

@@ -245,6 +245,26 @@ def test_product_of_large_shapes(ts, m, n, k):
     check_product(ts.fp4_matmul(a, b, out_dtype=torch.float32), values64(a), values64(b), None, k)
 
 
+@pytest.mark.parametrize("m", [3, 40, 2000])
+@pytest.mark.parametrize("ga,gb", [(-70, -65), (-100, -40), (118, -100), (-90, 118), (100, 21), (61, 60), (-3, 5)])
+def test_product_of_extreme_tensor_scales(ts, m, ga, gb):
+    """Scales whose product leaves fp32's normal range on the way to sums that do not."""
+    n, k = (300, 500) if m < 100 else (4800, 500)
+    def tensor(rows, seed, e):
+        t = ts.fp4_quantize(data(rows, k, torch.bfloat16, seed), "nvfp4")
+        return ts.Fp4Tensor(t.codes, t.scales, torch.full((1,), 2.0 ** e, device="cuda"), rows, k, "nvfp4")
+    a, b = tensor(m, 1, ga), tensor(n, 2, gb)
+    if ga + gb > 90:                                     # sums of up to 2^39 would leave the range
+        for t in (a, b):
+            t.scales.copy_(torch.where(t.scales > 8, t.scales // 16, t.scales))
+    a.codes[0] = 0
+    va, vb = values64(a), values64(b)
+    y = ts.fp4_matmul(a, b, out_dtype=torch.float32).double()
+    want, mag = va @ vb.t(), va.abs() @ vb.abs().t()
+    assert mag.max() < 2.0 ** 127 and (y[0] == 0).all()
+    assert ((y - want).abs() <= (k / 64 + 8) * 2.0 ** -22 * mag + 2.0 ** -149).all()
+
+
 def test_nan_blocks_reach_their_rows_only(ts):
     x, w = data(20, 256, torch.bfloat16, 3), data(140, 256, torch.bfloat16, 4)
     x[7, 100] = float("nan")
