@@ -497,6 +497,20 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
       float* pp = whole ? nullptr : a.partials + ((size_t)blockIdx.x * 2 + (x.k0 > 0 ? 0 : 1)) * (BT * kBW);
       const float bias = a.bias && valid ? load_f(a.bias, a.bias_dtype, n) : 0.f;
       const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * P::kAccCols;
+      if (a.cluster) {
+        // to shared memory, over the stages (all used): [BT tokens][128 rows]
+        // (the CTA's only item: nobody waits for the accumulator)
+#pragma unroll 1
+        for (int c = 0; c < BT / CW && c * CW < jn_all; ++c) {
+          float v[CW];
+          if constexpr (CW == 32) tmem_ld32(acc + c * CW, v);
+          else tmem_ld16(acc + c * CW, v);
+          float* dst = reinterpret_cast<float*>(s_w) + c * CW * kBW + r;
+#pragma unroll
+          for (int j = 0; j < CW; ++j) dst[j * kBW] = v[j];
+        }
+        break;
+      }
 #pragma unroll 1
       for (int c = 0; c < BT / CW; ++c) {
         float v[CW];
@@ -505,14 +519,6 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
         if (c == BT / CW - 1) {
           tc_fence_before();
           mbar_arrive(tempty + buf);
-        }
-        if (a.cluster) {
-          // to shared memory, over the stages (all used): [BT tokens][128 rows]
-          float* dst = reinterpret_cast<float*>(s_w) + c * CW * kBW + r;
-#pragma unroll
-          for (int j = 0; j < CW; ++j)
-            if (c * CW + j < jn_all) dst[j * kBW] = v[j];
-          continue;
         }
         if (!whole) {
           // a piece: [BT / 4 tokens][128 rows][4 tokens], coalesced both ways
@@ -529,7 +535,7 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
         buf = 0;
         bph ^= 1;
       }
-      if (whole || a.cluster) continue;
+      if (whole) continue;
       // a tile split over several CTAs: the last to arrive adds the pieces
       named_bar_sync(3, kEpiWarps * 32);
       if (r == 0) {
