@@ -793,7 +793,13 @@ __global__ void __launch_bounds__(256, 6) paged_weights_kernel(const AttnArgs a)
   const Cache& c = a.c;
   const int row = blockIdx.y, b = row / c.n_kv, h = row - b * c.n_kv;
   const int len = c.seq_lens[b];
-  if (units_of(a, len) == 0) return;
+  if (units_of(a, len) == 0) {
+    // Every thread waits for the attention before it ends, those without a
+    // slot too: where no sequence takes part nobody else would, and whatever
+    // follows this kernel would not find the attention's zeros in `out`.
+    pdl_wait_primary();
+    return;
+  }
   const bool ok = takes(a, b, len, a.positions != nullptr ? a.positions[b] : 0);
   const int64_t q = (int64_t)b * a.n_q + h * a.group;
   bool waits = true;
@@ -839,6 +845,7 @@ __global__ void __launch_bounds__(256, 6) paged_weights_kernel(const AttnArgs a)
     for (int i = 0; i < W; ++i)
       if (slot0 + i <= len) s[i] = w[i] + sum[i];
   }
+  if (waits) pdl_wait_primary();
 }
 
 // Stores tokens behind a sequence's cached ones: slot len + t of every kv
