@@ -1004,16 +1004,21 @@ template <bool BF, int DP>
 static int launch_attention(const AttnArgs& a, int grid, cudaStream_t st) {
   auto k = paged_attention_kernel<BF, DP>;
   const size_t smem = attn_smem<DP>(a.c.batch);
-  TS_UNSUPPORTED(smem <= (size_t)max_smem_optin(), "batch too large for the kernel's tables");
+  // The attribute is the function's on the device, whoever sets it: always the
+  // same value, what a block can have next to its static shared memory, so that
+  // no thread lowers it under another's larger batch.
   static thread_local int configured_dev = -1;
-  static thread_local size_t configured_smem = 0;
+  static thread_local size_t most = 0;
   int dev = 0;
   TS_CUDA_TRY(cudaGetDevice(&dev));
-  if (configured_dev != dev || configured_smem < smem) {
-    TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (configured_dev != dev) {
+    cudaFuncAttributes attr;
+    TS_CUDA_TRY(cudaFuncGetAttributes(&attr, k));
+    most = (size_t)max_smem_optin() - attr.sharedSizeBytes;
+    TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
     configured_dev = dev;
-    configured_smem = smem;
   }
+  TS_UNSUPPORTED(smem <= most, "batch too large for the kernel's tables");
   k<<<grid, kThreads, smem, st>>>(a);
   TS_LAUNCH_CHECK();
   return TS_OK;

@@ -49,3 +49,39 @@ def test_zeros_of_sequences_that_take_no_part_are_there_for_the_next_kernel(ts, 
         seen.append(out.clone())
     assert all((o == 0).all() for o in seen)
     assert all(torch.equal(x, y) for x, y in zip(before, (c.k_pages, c.v_pages, c.scores, c.slot_pos)))
+
+
+def run_in_thread(f):
+    import threading
+    out = []
+    t = threading.Thread(target=lambda: out.append(f()))
+    t.start()
+    t.join()
+    return out[0]
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_small_batch_of_another_thread_leaves_room_for_a_large_one(ts, d):
+    """The kernel's shared memory grows with the batch; how much it may have is
+    one setting for all threads."""
+    def attend(batch):
+        c = filled_cache(ts, [30] * batch, d=d, track=False)
+        qkv = torch.ones(batch, 8 * d, dtype=torch.bfloat16, device="cuda")
+        return ts.paged_decode_attention(qkv, 4, c)
+    want = attend(300)
+    assert run_in_thread(lambda: attend(1).shape) == (1, 4 * d)
+    assert torch.equal(attend(300), want)
+
+
+def test_batches_at_the_kernels_limit(ts):
+    """A block has 227 KB: 1 KB for the kernel's own variables, 98304 + 4352 bytes for
+    stages and queries of 128 columns, 8 for a sequence and 4 more. That is room for
+    16095 sequences; without the variables it would be 16223."""
+    c = ts.PagedKVCache.allocate(16223, 1, 128, 1, 1)
+    qkv = torch.randn(16223, 3 * 128, device="cuda").to(torch.bfloat16)
+    with pytest.raises(NotImplementedError, match="batch too large"):
+        ts.paged_decode_attention(qkv, 1, c)
+    n = 16095
+    fit = ts.PagedKVCache(c.k_pages, c.v_pages, c.page_table[:n], c.seq_lens[:n])
+    assert torch.equal(ts.paged_decode_attention(qkv[:n], 1, fit), qkv[:n, 256:])
+    assert torch.equal(c.v_pages[:n].view(n, 128), qkv[:n, 256:])
