@@ -336,7 +336,9 @@ TS_API int ts_paged_append(const void* k, const int64_t* k_strides, const void* 
  * seq_lens is not changed. qkv, out as in ts_decode_attention, in the
  * cache's type. workspace: zero-filled once; its first
  * ts_serving_counter_bytes() are zero again after every call and the rest is scratch (one workspace may serve all
- * ts_paged_* and ts_fp4_* calls of a stream).
+ * ts_paged_* and ts_fp4_* calls of a stream). A call's kernels pass data to
+ * one another through it: host threads that launch on one stream need a
+ * workspace each, or a lock around each call.
  */
 TS_API size_t ts_paged_attention_workspace_size(const ts_paged_cache* cache, int n_q, int accumulate);
 TS_API int ts_paged_decode_attention(const void* qkv, int64_t qkv_row_stride, int n_q, const ts_paged_cache* cache,

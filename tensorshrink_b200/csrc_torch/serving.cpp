@@ -5,7 +5,8 @@
 // workspace lookup or struct packing. Arguments are checked here (ValueError
 // and NotImplementedError as the Python wrappers document them); launches go
 // to the current stream of the tensors' device. One workspace per (device,
-// stream) serves all of them, and one per graph while the stream is captured.
+// stream) serves all of them, and one per graph while the stream is captured;
+// calls of several host threads take turns at it.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -25,31 +26,49 @@ namespace {
 using OptTensor = c10::optional<at::Tensor>;
 
 struct Workspace {
+  std::mutex mu;                    // see Scratch
   at::Tensor t;
   unsigned long long capture = 0;   // of the graph that it belongs to
 };
 
-std::mutex g_mu;
+std::mutex g_mu;                    // of the maps; entries stay where they are
 std::map<std::pair<int, cudaStream_t>, Workspace> g_ws, g_captured;
+
+// A stream's workspace in the hands of one call. Kernels of a call pass data to
+// one another through it, so the call holds it from before its first launch to
+// behind its last: another host thread's launches on the same stream come
+// before or behind them, never between.
+struct Scratch {
+  std::unique_lock<std::mutex> held;
+  at::Tensor t;
+  void* data() const { return t.defined() ? t.data_ptr() : nullptr; }
+  size_t bytes() const { return t.defined() ? (size_t)t.numel() : 0; }
+};
 
 // A workspace of at least `bytes`, its counters zero. A captured stream has
 // its own, from the graph's memory, and the graph zeroes it: neither the
 // graph's replays on another stream nor calls outside of it meet the other's
 // counters, and no warm-up has to come before the capture. Buffers are used on
 // the stream that they were allocated on, so a superseded one can be freed.
-at::Tensor workspace(const at::Device& dev, cudaStream_t s, size_t bytes) {
+Scratch workspace(const at::Device& dev, cudaStream_t s, size_t bytes) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   unsigned long long id = 0;
   if (cudaStreamGetCaptureInfo(s, &status, &id) != cudaSuccess) (void)cudaGetLastError();
   const bool captured = status == cudaStreamCaptureStatusActive;
-  std::lock_guard<std::mutex> lk(g_mu);
-  Workspace& w = (captured ? g_captured : g_ws)[{dev.index(), s}];
-  if (!w.t.defined() || (captured && w.capture != id) || (size_t)w.t.numel() < bytes) {
-    w.t = at::empty({(int64_t)std::max<size_t>(bytes, 1 << 20)}, at::TensorOptions().dtype(at::kByte).device(dev));
-    w.t.slice(0, 0, (int64_t)ts_serving_counter_bytes()).zero_();
-    w.capture = id;
+  Workspace* w;
+  {
+    std::lock_guard<std::mutex> lk(g_mu);
+    w = &(captured ? g_captured : g_ws)[{dev.index(), s}];
   }
-  return w.t;
+  Scratch r;
+  r.held = std::unique_lock<std::mutex>(w->mu);
+  if (!w->t.defined() || (captured && w->capture != id) || (size_t)w->t.numel() < bytes) {
+    w->t = at::empty({(int64_t)std::max<size_t>(bytes, 1 << 20)}, at::TensorOptions().dtype(at::kByte).device(dev));
+    w->t.slice(0, 0, (int64_t)ts_serving_counter_bytes()).zero_();
+    w->capture = id;
+  }
+  r.t = w->t;
+  return r;
 }
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
@@ -142,10 +161,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_quantize(const at::Tensor& x_
   at::Tensor scales = fresh({(int64_t)ts_fp4_scales_bytes(rows, cols, (int)format)}, at::kByte, dev);
   const ts_fp4_tensor t = fp4_view(codes, scales, g.defined() ? OptTensor(g) : c10::nullopt, rows, cols, format, "fp4_quantize");
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-  at::Tensor ws;
+  Scratch ws;
   if (find) ws = workspace(dev, s, ts_fp4_quantize_workspace_size());
-  done(ts_fp4_quantize(x.data_ptr(), dt, x.stride(0), &t, find, find ? ws.data_ptr() : nullptr,
-                       find ? (size_t)ws.numel() : 0, s), "fp4_quantize");
+  done(ts_fp4_quantize(x.data_ptr(), dt, x.stride(0), &t, find, ws.data(), ws.bytes(), s), "fp4_quantize");
   return {codes, scales, g};
 }
 
@@ -179,8 +197,8 @@ at::Tensor fp4_matmul(const at::Tensor& ac, const at::Tensor& as, const OptTenso
   const int bdt = check_bias(bias, n, dev, "fp4_matmul"), dt = code_of(out_dtype, "fp4_matmul");
   at::Tensor out = fresh({m, n}, out_dtype, dev);
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-  at::Tensor ws = workspace(dev, s, ts_fp4_matmul_workspace_size(m, n, cols, (int)format));
-  done(ts_fp4_matmul(&a, &b, ptr(bias), bdt, out.data_ptr(), dt, n, ws.data_ptr(), (size_t)ws.numel(), s), "fp4_matmul");
+  const Scratch ws = workspace(dev, s, ts_fp4_matmul_workspace_size(m, n, cols, (int)format));
+  done(ts_fp4_matmul(&a, &b, ptr(bias), bdt, out.data_ptr(), dt, n, ws.data(), ws.bytes(), s), "fp4_matmul");
   return out;
 }
 
@@ -209,9 +227,9 @@ at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& codes, const at::Te
   at::Tensor out = fresh(shape, odt, dev);
   const int64_t m = x2d.size(0);
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-  at::Tensor ws = workspace(dev, s, ts_fp4_linear_workspace_size(m, rows, cols, (int)format));
+  const Scratch ws = workspace(dev, s, ts_fp4_linear_workspace_size(m, rows, cols, (int)format));
   done(ts_fp4_linear(x2d.data_ptr(), xdt, m, x2d.stride(0), ptr<float>(input_scale), &w, ptr(bias), bdt, out.data_ptr(), dt,
-                     rows, ws.data_ptr(), (size_t)ws.numel(), s), "fp4_linear");
+                     rows, ws.data(), ws.bytes(), s), "fp4_linear");
   return out;
 }
 
@@ -356,11 +374,11 @@ at::Tensor paged_decode_attention(const at::Tensor& qkv, int64_t n_q, const at::
     out = fresh({c.batch, owidth}, qkv.scalar_type(), dev);
   }
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-  at::Tensor ws = workspace(dev, s, ts_paged_attention_workspace_size(&c, (int)n_q, accumulate));
+  const Scratch ws = workspace(dev, s, ts_paged_attention_workspace_size(&c, (int)n_q, accumulate));
   const float sc = scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)c.head_dim);
   done(ts_paged_decode_attention(qkv.data_ptr(), qkv.stride(0), (int)n_q, &c, ptr<int64_t>(positions), ptr<float>(cos),
-                                 ptr<float>(sin), rows, sc, accumulate, out.data_ptr(), out.stride(0), ws.data_ptr(),
-                                 (size_t)ws.numel(), s), "paged_decode_attention");
+                                 ptr<float>(sin), rows, sc, accumulate, out.data_ptr(), out.stride(0), ws.data(),
+                                 ws.bytes(), s), "paged_decode_attention");
   return out;
 }
 
@@ -373,8 +391,8 @@ void paged_evict(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& t
   const at::Device dev = kp.device();
   c10::cuda::CUDAGuard guard(dev);
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-  at::Tensor ws = workspace(dev, s, ts_paged_evict_workspace_size(&c, (int)budget));
-  done(ts_paged_evict(&c, (int)budget, (int)recent, ws.data_ptr(), (size_t)ws.numel(), s), "paged_evict");
+  const Scratch ws = workspace(dev, s, ts_paged_evict_workspace_size(&c, (int)budget));
+  done(ts_paged_evict(&c, (int)budget, (int)recent, ws.data(), ws.bytes(), s), "paged_evict");
 }
 
 // ts_fp4_status over the device's workspaces: raises if a bounded wait in a

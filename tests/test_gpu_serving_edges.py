@@ -85,3 +85,73 @@ def test_batches_at_the_kernels_limit(ts):
     fit = ts.PagedKVCache(c.k_pages, c.v_pages, c.page_table[:n], c.seq_lens[:n])
     assert torch.equal(ts.paged_decode_attention(qkv[:n], 1, fit), qkv[:n, 256:])
     assert torch.equal(c.v_pages[:n].view(n, 128), qkv[:n, 256:])
+def in_threads(jobs, rounds):
+    """Runs every job `rounds` times, each in a thread of its own, all on the
+    default stream; returns the lists of their results."""
+    import threading
+    results, errors = [[] for _ in jobs], []
+    start = threading.Barrier(len(jobs))
+
+    def work(i):
+        try:
+            start.wait()
+            for _ in range(rounds):
+                results[i].append(jobs[i]())
+        except Exception as e:                               # (an assertion here would be lost in the thread)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    torch.cuda.synchronize()
+    return results
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_threads_on_one_stream_multiply_their_own_tokens(ts, fmt):
+    """More tokens than the product quantises itself: quantiser and product are
+    two launches with the tokens' codes between them."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = ts.fp4_quantize(torch.randn(640, 1024, generator=g, device="cuda"), fmt)
+    xs = [torch.randn(40, 1024, generator=g, device="cuda").to(torch.bfloat16) for _ in range(3)]
+    want = [ts.fp4_linear(x, w) for x in xs]
+    got = in_threads([lambda x=x: ts.fp4_linear(x, w) for x in xs], 300)
+    for y, ys in zip(want, got):
+        assert all(torch.equal(y, z) for z in ys)
+
+
+def test_threads_on_one_stream_accumulate_their_own_weights(ts):
+    """Attention leaves logits and sums for the kernel that adds up the weights."""
+    pos = torch.tensor([300, 20], device="cuda")
+    caches = [filled_cache(ts, [300, 20], seed=i) for i in range(3)]
+    qkv = [torch.randn(2, 12 * 64, device="cuda").to(torch.bfloat16) for _ in range(3)]
+    before = [c.scores.clone() for c in caches]
+
+    def step(c, q):
+        return ts.paged_decode_attention(q, 8, c, pos, accumulate=True), c.scores.clone()
+
+    serial = [[step(c, q) for _ in range(200)] for c, q in zip(caches, qkv)]
+    for c, s in zip(caches, before):
+        c.scores.copy_(s)
+    got = in_threads([lambda c=c, q=q: step(c, q) for c, q in zip(caches, qkv)], 200)
+    for want, have in zip(serial, got):
+        assert all(torch.equal(a, b) and torch.equal(s, t) for (a, s), (b, t) in zip(want, have))
+
+
+def test_threads_on_one_stream_evict_from_their_own_caches(ts):
+    """The selection leaves lists for the kernel that moves the slots."""
+    def build(seed):
+        return [filled_cache(ts, [600, 500], d=32, seed=seed * 100 + i) for i in range(40)]
+
+    serial, threaded = [build(i) for i in range(3)], [build(i) for i in range(3)]
+    for caches in serial:
+        for c in caches:
+            ts.paged_evict(c, 200, 10)
+    todo = [list(caches) for caches in threaded]
+    in_threads([lambda q=q: ts.paged_evict(q.pop(), 200, 10) for q in todo], 40)
+    for a, b in zip(serial, threaded):
+        for x, y in zip(a, b):
+            for name in ("k_pages", "v_pages", "scores", "slot_pos", "seq_lens"):
+                assert torch.equal(getattr(x, name), getattr(y, name)), name
