@@ -428,7 +428,9 @@ TS_API int ts_fp4_linear(const void* x, int x_dtype, int64_t M, int64_t x_row_st
 TS_API size_t ts_serving_counter_bytes(void);
 
 /* ts_qlinear_status for the fp4 product (a per-device flag); with clear the
- * counters at the workspace's start are zeroed too (workspace may be NULL). */
+ * counters at the workspace's start are zeroed too (workspace may be NULL): no
+ * call that uses it may be in flight on another stream then. Waits for
+ * `stream`; covers its calls and those that other streams have finished. */
 TS_API int ts_fp4_status(void* workspace, size_t workspace_bytes, int clear, void* stream);
 
 /* Dense reconstruction W[rows, cols] in `out_dtype`.

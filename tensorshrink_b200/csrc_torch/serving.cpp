@@ -395,18 +395,26 @@ void paged_evict(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& t
   done(ts_paged_evict(&c, (int)budget, (int)recent, ws.data(), ws.bytes(), s), "paged_evict");
 }
 
-// ts_fp4_status over the device's workspaces: raises if a bounded wait in a
-// kernel ran out since the last check.
+// Raises if a bounded wait in a kernel ran out since the last check: of the
+// current stream, which is waited for, and of what other streams have finished.
+// With `clear`, after such a failure, the whole device is waited for, so that
+// no kernel of any stream is on its way, and nobody launches until the flag
+// and the counters that CTAs which gave up may have left non-zero are zero
+// again (a graph zeroes its own).
 void serving_status(int64_t device, bool clear) {
   c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   cudaStream_t s = at::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
-  const int rc = ts_fp4_status(nullptr, 0, clear ? 1 : 0, s);
-  if (rc == TS_OK) return;
-  if (clear) {
-    // counters that CTAs which gave up may have left non-zero (a graph zeroes its own)
+  int rc = ts_fp4_status(nullptr, 0, 0, s);
+  if (rc == TS_ERR_TIMEOUT && clear) {
     std::lock_guard<std::mutex> lk(g_mu);
+    std::vector<std::unique_lock<std::mutex>> held;
     for (auto& kv : g_ws)
-      if (kv.first.first == device) kv.second.t.slice(0, 0, (int64_t)ts_serving_counter_bytes()).zero_();
+      if (kv.first.first == device) held.emplace_back(kv.second.mu);
+    C10_CUDA_CHECK(cudaDeviceSynchronize());
+    for (auto& kv : g_ws)
+      if (kv.first.first == device && kv.second.t.defined())
+        C10_CUDA_CHECK(cudaMemsetAsync(kv.second.t.data_ptr(), 0, ts_serving_counter_bytes(), s));
+    rc = ts_fp4_status(nullptr, 0, 1, s);   // waits for the stream
   }
   done(rc, "ts_fp4_status");
 }

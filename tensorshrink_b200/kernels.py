@@ -168,9 +168,12 @@ _WORKSPACES = _Workspaces()
 def device_status(device: Optional[torch.device] = None, clear: bool = True) -> None:
     """Raise RuntimeError if a bounded wait inside a qlinear kernel ran out
     on `device` since the last check (`ts_qlinear_status` over every cached
-    workspace of the device). The call synchronizes the current stream; with
-    `clear` the flags and the workspaces' counters are reset, so later calls
-    run normally. A timed-out call's outputs are not valid."""
+    workspace of the device), or one inside the fp4 product
+    (`ts_fp4_status`). The call synchronizes the current stream; with `clear`
+    the flags and the workspaces' counters are reset, so later calls run
+    normally (after a failure of the fp4 product the whole device is
+    synchronized first). A timed-out call's outputs are not valid; a call of
+    another stream that is still running is covered by the next check."""
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     lib = _C.load()
     with torch.cuda.device(dev):

@@ -155,3 +155,47 @@ def test_threads_on_one_stream_evict_from_their_own_caches(ts):
         for x, y in zip(a, b):
             for name in ("k_pages", "v_pages", "scores", "slot_pos", "seq_lens"):
                 assert torch.equal(getattr(x, name), getattr(y, name)), name
+
+
+def test_status_of_a_stalled_product_leaves_other_streams_alone(ts):
+    """Attention on a side stream, joined through arrival counters, is on its way
+    while a product that stalled is reported and cleared."""
+    from tensorshrink_b200 import _C, kernels
+    a = ts.fp4_quantize(torch.randn(1, 1024, device="cuda").to(torch.bfloat16))
+    b = ts.fp4_quantize(torch.randn(9500, 1024, device="cuda"))
+    c = filled_cache(ts, [9000, 40], n_kv=4, d=128, page=64, track=False)
+    qkv = torch.randn(2, 24 * 128, device="cuda").to(torch.bfloat16)
+    product, want = ts.fp4_matmul(a, b), ts.paged_decode_attention(qkv, 16, c)
+    side = torch.cuda.Stream()
+    kernels.device_status()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            early = [ts.paged_decode_attention(qkv, 16, c) for _ in range(600)]
+        assert _C.load().ts_test_inject_stall(1_000_000) == 0
+        ts.fp4_matmul(a, b)
+        with pytest.raises(RuntimeError, match="ts_fp4_status"):
+            kernels.device_status()
+        with torch.cuda.stream(side):
+            late = [ts.paged_decode_attention(qkv, 16, c) for _ in range(50)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for x in early + late)
+        kernels.device_status()
+        assert torch.equal(ts.fp4_matmul(a, b), product)
+
+
+def test_status_of_a_workspace_made_in_inference_mode(ts):
+    from tensorshrink_b200 import _C, kernels
+    side = torch.cuda.Stream()
+    a, b = (ts.fp4_quantize(torch.randn(n, 1024, device="cuda")) for n in (1, 9500))
+    want = ts.fp4_matmul(a, b)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        with torch.inference_mode():
+            ts.fp4_matmul(a, b)
+        assert _C.load().ts_test_inject_stall(1_000_000) == 0
+        ts.fp4_matmul(a, b)
+        with pytest.raises(RuntimeError, match="ts_fp4_status"):
+            kernels.device_status()
+        kernels.device_status()
+        assert torch.equal(ts.fp4_matmul(a, b), want)
