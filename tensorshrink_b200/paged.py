@@ -13,7 +13,7 @@ captured in a graph.
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -78,9 +78,11 @@ class PagedKVCache:
         """Slots that a sequence's row of the page table can name."""
         return self.page_table.shape[1] * self.page_size
 
-    def advance(self, n: int = 1) -> None:
-        """Count `n` appended tokens as cached. (A negative count, of a
-        sequence that takes no part, has to be put back by the caller.)"""
+    def advance(self, n: Union[int, torch.Tensor] = 1) -> None:
+        """Count `n` appended tokens as cached, or n[b] of sequence b (int32
+        [batch]). (A negative count, of a sequence that takes no part, has to
+        be put back by the caller, and a token that found no slot is not to be
+        counted.)"""
         self.seq_lens.add_(n)
 
     def _args(self):

@@ -11,8 +11,14 @@ cache to them). Weights are random, as in `QuantDecoder`.
 
     model = PagedDecoder(DecoderConfig(...), "cuda", max_batch=8, max_len=4096, budget=1024, recent=128)
     token = model.prefill(prompts)          # list of 1-D token tensors, one per sequence
-    for _ in range(n):
+    for _ in range(min(n, model.steps_left)):
         token = model.decode_step(token)    # may be captured in a CUDA graph
+
+A step that a sequence has no rotary row or no slot for raises; the others go
+on once that one is taken out (`drop`). Replays of a captured step run without
+the host: the program counts them with `count_steps`, which raises for them.
+Without that, a sequence past its limit keeps its cache as it is, and its
+logits mean nothing.
 """
 
 from __future__ import annotations
@@ -50,7 +56,12 @@ class PagedDecoder(nn.Module):
     """See the module documentation. budget: tokens that each sequence's cache
     is cut back to after a step (None: it grows up to max_len); recent: how many of
     them are the newest whatever their weight. With a budget the caches keep
-    each slot's accumulated attention weight and position."""
+    each slot's accumulated attention weight and position. max_position: the
+    rotary tables' rows, tokens that a sequence can have in all; max_len by
+    default, and LONG (33 MB of tables for heads of 128) with a budget, under
+    which sequences go on beyond max_len."""
+
+    LONG = 65536
 
     def __init__(self, cfg: DecoderConfig, device, format: str = "nvfp4", max_batch: int = 1, max_len: int = 2048,
                  page_size: int = 64, max_position: Optional[int] = None, budget: Optional[int] = None, recent: int = 0):
@@ -65,17 +76,46 @@ class PagedDecoder(nn.Module):
         self.lm_head = (torch.randn(cfg.vocab, H, generator=g, device=self.device) * 0.02).to(torch.bfloat16)
         self.final_norm = torch.ones(H, dtype=torch.float32, device=self.device)
         self.layers = nn.ModuleList(PagedDecoderLayer(cfg, i, format, self.device) for i in range(cfg.n_layers))
-        positions = max_position or max_len
+        positions = max_position or (max_len if budget is None else max(max_len, self.LONG))
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, D, 2, device=self.device, dtype=torch.float32) / D))
         ang = torch.outer(torch.arange(positions, device=self.device, dtype=torch.float32), inv)
         self.rope_cos, self.rope_sin = ang.cos(), ang.sin()
         self.caches = [PagedKVCache.allocate(max_batch, cfg.n_kv_heads, D, max_len, page_size, device=self.device,
                                              track=budget is not None) for _ in range(cfg.n_layers)]
         self.positions = torch.zeros(max_batch, dtype=torch.int64, device=self.device)   # of the next token
+        self._tokens: List[Optional[int]] = [0] * max_batch   # the same as the host counts them; None: dropped
 
     def packed_nbytes(self) -> int:
         """Bytes of the projections' weights."""
         return sum(p.weight().nbytes() for layer in self.layers for p in layer.projections())
+
+    @property
+    def longest_sequence(self) -> int:
+        """Tokens that a sequence can have: rotary rows and, without a budget, slots."""
+        rows = self.rope_cos.shape[0]
+        return rows if self.budget is not None else min(rows, self.caches[0].capacity)
+
+    @property
+    def steps_left(self) -> int:
+        """Decode steps until a sequence has no place for its token."""
+        return self.longest_sequence - max((n for n in self._tokens if n is not None), default=0)
+
+    def count_steps(self, n: int = 1) -> None:
+        """Count n decode steps (negative: steps that the program took back);
+        raises if fewer are left. `decode_step` does it by itself, except while
+        it is captured: a program that replays a captured step counts each replay."""
+        if n > self.steps_left:
+            raise RuntimeError(f"{n} decode steps, but a sequence has {self.longest_sequence - self.steps_left} of "
+                               f"{self.longest_sequence} tokens (see max_position, max_len and drop)")
+        self._tokens = [None if t is None else t + n for t in self._tokens]
+
+    def drop(self, sequence: int) -> None:
+        """Take a sequence out of the steps that follow, until the next
+        prefill: it no longer counts, its cache is empty and its logits mean
+        nothing."""
+        self._tokens[sequence] = None
+        for cache in self.caches:
+            cache.seq_lens[sequence] = -1
 
     def _evict(self, cache: PagedKVCache) -> None:
         if self.budget is not None:
@@ -95,9 +135,11 @@ class PagedDecoder(nn.Module):
         next tokens [batch], or the logits [batch, vocab]."""
         cfg, D = self.cfg, self.cfg.head_dim
         B, lens = len(prompts), [len(p) for p in prompts]
-        if B != self.positions.shape[0] or min(lens) < 1 or max(lens) > self.caches[0].capacity:
-            raise ValueError(f"{self.positions.shape[0]} prompts of 1 to {self.caches[0].capacity} tokens are needed")
+        most = min(self.caches[0].capacity, self.rope_cos.shape[0])
+        if B != self.positions.shape[0] or min(lens) < 1 or max(lens) > most:
+            raise ValueError(f"{self.positions.shape[0]} prompts of 1 to {most} tokens are needed")
         T = max(lens)
+        self._tokens = list(lens)
         tokens = torch.zeros(B, T, dtype=torch.long, device=self.device)
         for i, p in enumerate(prompts):
             tokens[i, :lens[i]] = p.to(self.device)
@@ -128,13 +170,19 @@ class PagedDecoder(nn.Module):
     @torch.no_grad()
     def decode_step(self, tokens: torch.Tensor, return_logits: bool = False) -> torch.Tensor:
         """One token per sequence at its own position. Returns the greedy next
-        tokens [batch], or the logits [batch, vocab]."""
+        tokens [batch], or the logits [batch, vocab]. Raises if a sequence has
+        no place for its token (`steps_left`)."""
+        self.count_steps(1)
+        if torch.cuda.is_current_stream_capturing():
+            self.count_steps(-1)                         # nothing runs yet
+        # which sequences' caches take the token: all but the dropped ones, and those of uncounted replays
+        taken = ((self.positions < self.longest_sequence) & (self.caches[0].seq_lens >= 0)).to(torch.int32)
         h = self.embed[tokens].float()
         for layer, cache in zip(self.layers, self.caches):
             qkv = layer.qkv(_rms_norm(h, layer.input_norm, self.cfg.rms_eps))
             a = paged_decode_attention(qkv, self.cfg.n_heads, cache, self.positions, self.rope_cos, self.rope_sin,
                                        accumulate=self.budget is not None)
-            cache.advance()
+            cache.advance(taken)
             self._evict(cache)
             h = self._mlp(layer, h + layer.o(a))
         self.positions.add_(1)
