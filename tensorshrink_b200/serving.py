@@ -34,6 +34,32 @@ from .fp4 import Fp4Linear, fp4_quantize
 from .paged import PagedKVCache, paged_append, paged_decode_attention, paged_evict
 
 
+def _prompt_weights(q: torch.Tensor, k: torch.Tensor, lens: Sequence[int], most: int = 1 << 26) -> torch.Tensor:
+    """The weight that each prompt token draws from its own prompt: [batch,
+    n_kv, tokens], fp32, summed over the prompt's queries and each kv head's query
+    heads, as `paged_decode_attention` accumulates it step by step. q [batch,
+    tokens, n_heads, D] and k [batch, tokens, n_kv, D] are rotated; lens[b] tokens
+    of sequence b count. Scores and softmax are fp32, in blocks of queries of at
+    most `most` scores. (4 prompts of 4096 tokens, 32 heads over 8 of 128 columns:
+    see the figure at `PagedDecoder.prefill`.)"""
+    B, T, H, D = q.shape
+    n_kv = k.shape[2]
+    q = q.view(B, T, n_kv, H // n_kv, D).transpose(1, 2)                     # a token's query heads side by side
+    k = k.permute(0, 2, 3, 1)
+    total = torch.zeros(B, n_kv, T, dtype=torch.float32, device=q.device)
+    none = total.new_zeros(())
+    for b, n in enumerate(lens):
+        rows = max(1, most // (H * n))
+        for i in range(0, n, rows):
+            j = min(n, i + rows)                                              # queries i .. j - 1 see keys 0 .. j - 1
+            s = torch.baddbmm(none.expand(n_kv, (j - i) * (H // n_kv), j), q[b, :, i:j].reshape(n_kv, -1, D), k[b, :, :, :j],
+                              beta=0, alpha=D ** -0.5, out_dtype=torch.float32)
+            late = torch.ones(j - i, j - i, dtype=torch.bool, device=q.device).triu(1)
+            s.view(n_kv, j - i, -1, j)[..., i:].masked_fill_(late[:, None], float("-inf"))
+            total[b, :, :j] += s.softmax(dim=-1).sum(dim=1)
+    return total
+
+
 class PagedDecoderLayer(nn.Module):
     """One layer's projections (q/k/v and gate/up fused by rows) and norms."""
 
@@ -155,12 +181,14 @@ class PagedDecoder(nn.Module):
         for layer, cache in zip(self.layers, self.caches):
             x = _rms_norm(h, layer.input_norm, cfg.rms_eps)
             q, k, v = layer.qkv(x).view(B, T, -1, D).split([cfg.n_heads, cfg.n_kv_heads, cfg.n_kv_heads], dim=2)
+            rq, rk = rope(q), rope(k)
             cache.seq_lens.zero_()
-            paged_append(k, v, cache, self.positions, self.rope_cos, self.rope_sin, n_new=n_new)
+            paged_append(k, v, cache, self.positions, self.rope_cos, self.rope_sin, n_new=n_new,
+                         scores=_prompt_weights(rq, rk, lens) if self.budget is not None else None)
             cache.seq_lens.copy_(n_new)
             self._evict(cache)
             # padding stands behind a prompt's tokens: causal attention never looks at it
-            a = F.scaled_dot_product_attention(rope(q).transpose(1, 2), rope(k).transpose(1, 2), v.transpose(1, 2),
+            a = F.scaled_dot_product_attention(rq.transpose(1, 2), rk.transpose(1, 2), v.transpose(1, 2),
                                                is_causal=True, enable_gqa=True)
             h = self._mlp(layer, h + layer.o(a.transpose(1, 2).reshape(B, T, -1)))
         self.positions.copy_(n_new)

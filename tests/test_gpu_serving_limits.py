@@ -115,3 +115,76 @@ def test_a_dropped_sequence_lets_the_others_go_on():
     assert torch.equal(before, m.caches[0].k_pages[m.caches[0].page_table[1].long()])
     m.prefill(ps)
     assert m.steps_left == 1 and m.caches[0].seq_lens.tolist() == [7, 31]
+
+
+def prompt_weights64(q, k):
+    """Weight that each key of one prompt draws, [tokens, n_kv] in 64 bits, and
+    a bound on the error that fp32 scores make of it, as a part of the weight:
+    a score is off by (D + 2) 2^-24 of sum |q||k| at most, a weight by twice
+    that (numerator and denominator), and 2^-18 more from exponentials and sums."""
+    n, heads, d = q.shape
+    n_kv = k.shape[1]
+    q = q.double().view(n, n_kv, heads // n_kv, d)
+    s = torch.einsum("ihgd,jhd->hgij", q, k.double()) * d ** -0.5
+    size = torch.einsum("ihgd,jhd->hgij", q.abs(), k.double().abs()).max().item() * d ** -0.5
+    s = s.masked_fill(torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1), -float("inf"))
+    return s.softmax(-1).sum((1, 2)).t(), 2 * (d + 2) * 2.0 ** -24 * size + 2.0 ** -18
+
+
+@pytest.mark.parametrize("most", [None, 4000])
+def test_prompts_are_cut_back_to_the_tokens_that_drew_attention(monkeypatch, most):
+    """Against column sums in 64 bits of the first layer's own queries and keys."""
+    import tensorshrink_b200.serving as serving
+    if most is not None:                                     # many blocks of queries
+        whole = serving._prompt_weights
+        monkeypatch.setattr(serving, "_prompt_weights", lambda q, k, n: whole(q, k, n, most))
+    lens, budget, recent = [90, 5, 41, 64], 40, 8
+    m, full = build(batch=4, max_len=96, budget=budget, recent=recent), build(batch=4, max_len=96)
+    for x in (m, full):                                      # six times the queries and keys: a few tokens draw most of it
+        x.layers[0].qkv.global_scale.mul_(6)
+    seen = []
+    hook = full.layers[0].qkv.register_forward_hook(lambda _, x, y: seen.append(y))
+    ps = prompts(lens, seed=9)
+    m.prefill(ps)
+    full.prefill(ps)
+    hook.remove()
+    qkv = seen[0].view(4, max(lens), 8, 64)
+    c, f = m.caches[0], full.caches[0]
+    middle = 0
+    for b, n in enumerate(lens):
+        cos, sin = full.rope_cos[:n, None], full.rope_sin[:n, None]
+        x1, x2 = qkv[b, :n, :4].float().chunk(2, dim=-1)
+        q = torch.cat([x1 * cos - x2 * sin, x1 * sin + x2 * cos], dim=-1).to(qkv.dtype)
+        t = torch.arange(n, device="cuda")
+        k = f.k_pages[f.page_table[b, t // 16].long(), :, t % 16]
+        want, off = prompt_weights64(q, k)
+        s = torch.arange(min(n, budget), device="cuda")
+        page = c.page_table[b, s // 16].long()
+        pos, have = c.slot_pos[page, :, s % 16].long(), c.scores[page, :, s % 16].double()
+        for h in range(2):
+            kept = pos[:, h]
+            assert len(set(kept.tolist())) == len(s)
+            assert ((have[:, h] - want[kept, h]).abs() <= off * want[kept, h]).all()
+            if n <= budget:
+                continue
+            gone = torch.ones(n, dtype=torch.bool, device="cuda")
+            gone[kept] = False
+            assert not gone[n - recent:].any()
+            least = want[kept[kept < n - recent], h].min()
+            assert least >= want[gone, h].max() * (1 - 2 * off)
+            middle += int(((kept >= budget) & (kept < n - recent)).sum())
+    assert middle > 0                                        # the first slots alone would not have done
+
+
+def test_decoding_starts_from_the_prompts_weights():
+    """A step adds its weights to the prompt's: kept scores sum up to one per
+    query, of the prompt and of the step, and per query head of the kv head."""
+    m = build(batch=2, max_len=96, budget=80, recent=4)
+    token = m.prefill(prompts([30, 50]))
+    for step in range(1, 4):
+        token = m.decode_step(token)
+        for c in m.caches:
+            for b, n in enumerate((30 + step, 50 + step)):
+                s = torch.arange(n, device="cuda")
+                total = c.scores[c.page_table[b, s // 16].long(), :, s % 16].double().sum(0)
+                assert ((total - 2 * n).abs() <= 2.0 ** -16 * 2 * n).all()
