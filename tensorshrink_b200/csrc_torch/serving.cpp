@@ -111,9 +111,9 @@ void done(int rc, const char* what) {
 
 int64_t padded(int64_t cols) { return (cols + 63) / 64 * 64; }
 
-ts_fp4_tensor fp4_view(const at::Tensor& codes, const at::Tensor& scales, const OptTensor& g, int64_t rows, int64_t cols,
-                       int64_t format, const char* what) {
-  TORCH_CHECK(codes.is_cuda(), what, ": tensorshrink_b200 runs on CUDA tensors only (got ", codes.device(), ")");
+// What can be said of a tensor's description without its memory.
+void fp4_fits(const at::Tensor& codes, const at::Tensor& scales, const OptTensor& g, int64_t rows, int64_t cols,
+              int64_t format, const char* what) {
   TORCH_CHECK_NOT_IMPLEMENTED(format == TS_NVFP4 || format == TS_MXFP4, what, ": unknown format");
   TORCH_CHECK_VALUE(rows >= 0 && cols > 0, what, ": bad shape [", rows, ", ", cols, "]");
   TORCH_CHECK_VALUE(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && codes.is_contiguous() &&
@@ -129,6 +129,12 @@ ts_fp4_tensor fp4_view(const at::Tensor& codes, const at::Tensor& scales, const 
     TORCH_CHECK_VALUE(g->scalar_type() == at::kFloat && g->numel() == 1, what, ": the tensor scale must be one fp32 value");
     on(*g, codes.device(), "the tensor scale");
   }
+}
+
+ts_fp4_tensor fp4_view(const at::Tensor& codes, const at::Tensor& scales, const OptTensor& g, int64_t rows, int64_t cols,
+                       int64_t format, const char* what) {
+  TORCH_CHECK(codes.is_cuda(), what, ": tensorshrink_b200 runs on CUDA tensors only (got ", codes.device(), ")");
+  fp4_fits(codes, scales, g, rows, cols, format, what);
   ts_fp4_tensor t{};
   t.codes = static_cast<uint8_t*>(codes.data_ptr());
   t.scales = static_cast<uint8_t*>(scales.data_ptr());
@@ -144,8 +150,8 @@ void fp4_check(const at::Tensor& codes, const at::Tensor& scales, const OptTenso
   fp4_view(codes, scales, g, rows, cols, format, "Fp4Tensor");
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_quantize(const at::Tensor& x_in, int64_t format,
-                                                            const OptTensor& scale) {
+// Codes, scales and the tensor scale where it was found (a given one is the caller's).
+std::tuple<at::Tensor, at::Tensor, OptTensor> fp4_quantize(const at::Tensor& x_in, int64_t format, const OptTensor& scale) {
   TORCH_CHECK(x_in.is_cuda(), "fp4_quantize: tensorshrink_b200 runs on CUDA tensors only (got ", x_in.device(), ")");
   const at::Device dev = x_in.device();
   c10::cuda::CUDAGuard guard(dev);
@@ -164,7 +170,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_quantize(const at::Tensor& x_
   Scratch ws;
   if (find) ws = workspace(dev, s, ts_fp4_quantize_workspace_size());
   done(ts_fp4_quantize(x.data_ptr(), dt, x.stride(0), &t, find, ws.data(), ws.bytes(), s), "fp4_quantize");
-  return {codes, scales, g};
+  return {codes, scales, find ? OptTensor(g) : c10::nullopt};
 }
 
 at::Tensor fp4_dequantize(const at::Tensor& codes, const at::Tensor& scales, const OptTensor& g, int64_t rows,
@@ -235,9 +241,9 @@ at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& codes, const at::Te
 
 // ---- paged cache ------------------------------------------------------------------
 
-ts_paged_cache cache_view(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lens,
-                          const OptTensor& scores, const OptTensor& slot_pos) {
-  TORCH_CHECK(k.is_cuda(), "PagedKVCache: tensorshrink_b200 runs on CUDA tensors only (got ", k.device(), ")");
+// What can be said of a cache without its memory.
+void cache_fits(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lens,
+                const OptTensor& scores, const OptTensor& slot_pos) {
   const at::Device dev = k.device();
   TORCH_CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes(),
                     "k_pages and v_pages must both be [num_pages, n_kv, page_size, head_dim]");
@@ -260,6 +266,12 @@ ts_paged_cache cache_view(const at::Tensor& k, const at::Tensor& v, const at::Te
     TORCH_CHECK_VALUE((*t)->scalar_type() == type && (*t)->sizes() == k.sizes().slice(0, 3) && (*t)->is_contiguous(), name,
                       " must be contiguous ", type, " [num_pages, n_kv, page_size]");
   }
+}
+
+ts_paged_cache cache_view(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lens,
+                          const OptTensor& scores, const OptTensor& slot_pos) {
+  TORCH_CHECK(k.is_cuda(), "PagedKVCache: tensorshrink_b200 runs on CUDA tensors only (got ", k.device(), ")");
+  cache_fits(k, v, table, lens, scores, slot_pos);
   ts_paged_cache c{};
   c.k_pages = k.data_ptr();
   c.v_pages = v.data_ptr();
@@ -345,10 +357,10 @@ void paged_append(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tens
                        at::cuda::getCurrentCUDAStream(dev.index()).stream()), "paged_append");
 }
 
-at::Tensor paged_decode_attention(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, const at::Tensor& vp,
-                                  const at::Tensor& table, const at::Tensor& lens, const OptTensor& scores,
-                                  const OptTensor& slot_pos, const OptTensor& positions, const OptTensor& cos,
-                                  const OptTensor& sin, c10::optional<double> scale, bool accumulate, const OptTensor& out_) {
+at::Tensor attend(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& table,
+                  const at::Tensor& lens, const OptTensor& scores, const OptTensor& slot_pos, const OptTensor& positions,
+                  const OptTensor& cos, const OptTensor& sin, c10::optional<double> scale, bool accumulate,
+                  const OptTensor& out_) {
   const ts_paged_cache c = cache_view(kp, vp, table, lens, scores, slot_pos);
   const at::Device dev = kp.device();
   c10::cuda::CUDAGuard guard(dev);
@@ -379,6 +391,20 @@ at::Tensor paged_decode_attention(const at::Tensor& qkv, int64_t n_q, const at::
   done(ts_paged_decode_attention(qkv.data_ptr(), qkv.stride(0), (int)n_q, &c, ptr<int64_t>(positions), ptr<float>(cos),
                                  ptr<float>(sin), rows, sc, accumulate, out.data_ptr(), out.stride(0), ws.data(),
                                  ws.bytes(), s), "paged_decode_attention");
+  return out;
+}
+
+at::Tensor paged_decode_attention(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, const at::Tensor& vp,
+                                  const at::Tensor& table, const at::Tensor& lens, const OptTensor& scores,
+                                  const OptTensor& slot_pos, const OptTensor& positions, const OptTensor& cos,
+                                  const OptTensor& sin, c10::optional<double> scale, bool accumulate) {
+  return attend(qkv, n_q, kp, vp, table, lens, scores, slot_pos, positions, cos, sin, scale, accumulate, c10::nullopt);
+}
+at::Tensor& paged_decode_attention_out(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, const at::Tensor& vp,
+                                       const at::Tensor& table, const at::Tensor& lens, const OptTensor& scores,
+                                       const OptTensor& slot_pos, const OptTensor& positions, const OptTensor& cos,
+                                       const OptTensor& sin, c10::optional<double> scale, bool accumulate, at::Tensor& out) {
+  attend(qkv, n_q, kp, vp, table, lens, scores, slot_pos, positions, cos, sin, scale, accumulate, out);
   return out;
 }
 
@@ -419,26 +445,142 @@ void serving_status(int64_t device, bool clear) {
   done(rc, "ts_fp4_status");
 }
 
+// ---- shapes for tracing -------------------------------------------------------
+//
+// The operators on tensors without memory: the outputs' shapes and types, after
+// those checks that do not need numbers a tracer may not have.
+
+using c10::SymInt;
+
+SymInt padded(const SymInt& cols) { return (cols + 63) / 64 * 64; }
+
+void fp4_check_meta(const at::Tensor& codes, const at::Tensor& scales, const OptTensor& g, int64_t rows, int64_t cols,
+                    int64_t format) {
+  fp4_fits(codes, scales, g, rows, cols, format, "Fp4Tensor");
+}
+
+std::tuple<at::Tensor, at::Tensor, OptTensor> fp4_quantize_meta(const at::Tensor& x, int64_t format, const OptTensor& scale) {
+  TORCH_CHECK_VALUE(x.dim() == 2, "fp4_quantize takes a [rows, cols] tensor, got ", x.dim(), " dimensions");
+  code_of(x.scalar_type(), "fp4_quantize");
+  TORCH_CHECK_NOT_IMPLEMENTED(format == TS_NVFP4 || format == TS_MXFP4, "fp4_quantize: unknown format");
+  TORCH_CHECK_VALUE(!has(scale) || format == TS_NVFP4, "fp4_quantize: only nvfp4 has a tensor scale");
+  const SymInt rows = x.sym_size(0), cols = padded(x.sym_size(1));
+  const SymInt tiles = (rows + 127) / 128 * ((cols / (format == TS_NVFP4 ? 16 : 32) + 3) / 4);
+  const auto bytes = x.options().dtype(at::kByte);
+  return {at::empty_symint({rows, cols / 2}, bytes), at::empty_symint({tiles * 512}, bytes),
+          format == TS_NVFP4 && !has(scale) ? OptTensor(at::empty({1}, x.options().dtype(at::kFloat))) : c10::nullopt};
+}
+
+at::Tensor fp4_dequantize_meta(const at::Tensor& codes, const at::Tensor& scales, const OptTensor& g, int64_t rows,
+                               int64_t cols, int64_t format, at::ScalarType dtype) {
+  fp4_fits(codes, scales, g, rows, cols, format, "fp4_dequantize");
+  code_of(dtype, "fp4_dequantize");
+  return at::empty({rows, cols}, codes.options().dtype(dtype));
+}
+
+at::Tensor fp4_matmul_meta(const at::Tensor& ac, const at::Tensor& as, const OptTensor& ag, int64_t m, const at::Tensor& bc,
+                           const at::Tensor& bs, const OptTensor& bg, int64_t n, int64_t cols, int64_t format,
+                           const OptTensor& bias, at::ScalarType out_dtype) {
+  fp4_fits(ac, as, ag, m, cols, format, "fp4_matmul");
+  fp4_fits(bc, bs, bg, n, cols, format, "fp4_matmul");
+  check_bias(bias, n, bc.device(), "fp4_matmul");
+  code_of(out_dtype, "fp4_matmul");
+  return at::empty({m, n}, ac.options().dtype(out_dtype));
+}
+
+at::Tensor fp4_linear_meta(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales, const OptTensor& g,
+                           int64_t rows, int64_t cols, int64_t format, const OptTensor& bias, const OptTensor& input_scale,
+                           c10::optional<at::ScalarType> out_dtype) {
+  fp4_fits(codes, scales, g, rows, cols, format, "fp4_linear");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.sym_size(-1) == cols, "fp4_linear: x has ", x.dim() ? x.sym_size(-1) : SymInt(0),
+                    " features, the weight ", cols);
+  TORCH_CHECK_VALUE(!has(input_scale) || format == TS_NVFP4, "fp4_linear: only nvfp4 has an input_scale");
+  check_bias(bias, rows, codes.device(), "fp4_linear");
+  code_of(x.scalar_type(), "fp4_linear");
+  const at::ScalarType odt = out_dtype.value_or(x.scalar_type());
+  code_of(odt, "fp4_linear");
+  c10::SymDimVector shape(x.sym_sizes().begin(), x.sym_sizes().end());
+  shape.back() = rows;
+  return at::empty_symint(shape, x.options().dtype(odt));
+}
+
+void paged_check_meta(const at::Tensor& k, const at::Tensor& v, const at::Tensor&, const at::Tensor&, const OptTensor&,
+                      const OptTensor&) {
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.dim() == 4, "k_pages and v_pages must both be [num_pages, n_kv, page_size, head_dim]");
+  TORCH_CHECK_NOT_IMPLEMENTED(k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16,
+                              "the cache holds fp16 or bf16");
+}
+
+void paged_append_meta(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kp, const at::Tensor&, const at::Tensor&,
+                       const at::Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+                       const OptTensor&, const OptTensor&, const OptTensor&) {
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.dim() == 4, "k and v must be [batch, tokens, n_kv, head_dim]");
+  TORCH_CHECK_VALUE(k.scalar_type() == kp.scalar_type() && v.scalar_type() == kp.scalar_type(),
+                    "k and v must have the cache's type");
+}
+
+at::Tensor paged_decode_attention_meta(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, const at::Tensor&,
+                                       const at::Tensor&, const at::Tensor&, const OptTensor& scores, const OptTensor&,
+                                       const OptTensor&, const OptTensor&, const OptTensor&, c10::optional<double>,
+                                       bool accumulate) {
+  TORCH_CHECK_VALUE(n_q > 0 && qkv.dim() == 2 && kp.dim() == 4 && qkv.scalar_type() == kp.scalar_type(),
+                    "qkv must be [batch, (n_q + 2 n_kv) head_dim] of the cache's type");
+  TORCH_CHECK_VALUE(!accumulate || has(scores), "the cache has no scores to accumulate into");
+  return at::empty_symint({qkv.sym_size(0), kp.sym_size(3) * n_q}, qkv.options());
+}
+at::Tensor& paged_decode_attention_out_meta(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, const at::Tensor& vp,
+                                            const at::Tensor& table, const at::Tensor& lens, const OptTensor& scores,
+                                            const OptTensor& slot_pos, const OptTensor& positions, const OptTensor& cos,
+                                            const OptTensor& sin, c10::optional<double> scale, bool accumulate,
+                                            at::Tensor& out) {
+  paged_decode_attention_meta(qkv, n_q, kp, vp, table, lens, scores, slot_pos, positions, cos, sin, scale, accumulate);
+  return out;
+}
+
+void paged_evict_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor& scores,
+                      const OptTensor& slot_pos, int64_t, int64_t) {
+  TORCH_CHECK_VALUE(has(scores) && has(slot_pos), "eviction needs the cache's scores and slot_pos");
+}
+
 }  // namespace
 
-#define TS_CACHE "Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor(c!) seq_lens, " \
-                 "Tensor(d!)? scores, Tensor(e!)? slot_pos"
+#define TS_CACHE(lens) "Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, " lens " seq_lens, " \
+                       "Tensor(d!)? scores, Tensor(e!)? slot_pos"
+#define TS_ATTEND "Tensor qkv, int n_q, " TS_CACHE("Tensor") ", Tensor? positions, Tensor? rope_cos, Tensor? rope_sin, " \
+                  "float? scale, bool accumulate"
 
 TORCH_LIBRARY_FRAGMENT(tensorshrink, m) {
   m.def("serving_status(int device, bool clear=True) -> ()", &serving_status);
-  m.def("fp4_check(Tensor codes, Tensor scales, Tensor? global_scale, int rows, int cols, int format) -> ()", &fp4_check);
-  m.def("fp4_quantize(Tensor x, int format, Tensor? global_scale) -> (Tensor, Tensor, Tensor)", &fp4_quantize);
+  m.def("fp4_check(Tensor codes, Tensor scales, Tensor? global_scale, int rows, int cols, int format) -> ()");
+  m.def("fp4_quantize(Tensor x, int format, Tensor? global_scale) -> (Tensor, Tensor, Tensor?)");
   m.def("fp4_dequantize(Tensor codes, Tensor scales, Tensor? global_scale, int rows, int cols, int format, "
-        "ScalarType dtype) -> Tensor", &fp4_dequantize);
+        "ScalarType dtype) -> Tensor");
   m.def("fp4_matmul(Tensor a_codes, Tensor a_scales, Tensor? a_scale, int m, Tensor b_codes, Tensor b_scales, "
-        "Tensor? b_scale, int n, int cols, int format, Tensor? bias, ScalarType out_dtype) -> Tensor", &fp4_matmul);
+        "Tensor? b_scale, int n, int cols, int format, Tensor? bias, ScalarType out_dtype) -> Tensor");
   m.def("fp4_linear(Tensor x, Tensor codes, Tensor scales, Tensor? global_scale, int rows, int cols, int format, "
-        "Tensor? bias, Tensor? input_scale, ScalarType? out_dtype=None) -> Tensor", &fp4_linear);
+        "Tensor? bias, Tensor? input_scale, ScalarType? out_dtype=None) -> Tensor");
   m.def("paged_check(Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor seq_lens, Tensor? scores, "
-        "Tensor? slot_pos) -> ()", &paged_check);
-  m.def("paged_append(Tensor k, Tensor v, " TS_CACHE ", Tensor? positions, Tensor? rope_cos, Tensor? rope_sin, "
-        "Tensor? n_new, Tensor? new_scores) -> ()", &paged_append);
-  m.def("paged_decode_attention(Tensor qkv, int n_q, " TS_CACHE ", Tensor? positions, Tensor? rope_cos, "
-        "Tensor? rope_sin, float? scale, bool accumulate, Tensor? out) -> Tensor", &paged_decode_attention);
-  m.def("paged_evict(" TS_CACHE ", int budget, int recent) -> ()", &paged_evict);
+        "Tensor? slot_pos) -> ()");
+  m.def("paged_append(Tensor k, Tensor v, " TS_CACHE("Tensor") ", Tensor? positions, Tensor? rope_cos, Tensor? rope_sin, "
+        "Tensor? n_new, Tensor? new_scores) -> ()");
+  m.def("paged_decode_attention(" TS_ATTEND ") -> Tensor");
+  m.def("paged_decode_attention.out(" TS_ATTEND ", *, Tensor(f!) out) -> Tensor(f!)");
+  m.def("paged_evict(" TS_CACHE("Tensor(c!)") ", int budget, int recent) -> ()");
 }
+
+// (On the CPU the operators say that they do not run there.)
+#define TS_IMPL(m, suffix)                                                     \
+  m.impl("fp4_check", &fp4_check##suffix);                                     \
+  m.impl("fp4_quantize", &fp4_quantize##suffix);                               \
+  m.impl("fp4_dequantize", &fp4_dequantize##suffix);                           \
+  m.impl("fp4_matmul", &fp4_matmul##suffix);                                   \
+  m.impl("fp4_linear", &fp4_linear##suffix);                                   \
+  m.impl("paged_check", &paged_check##suffix);                                 \
+  m.impl("paged_append", &paged_append##suffix);                               \
+  m.impl("paged_decode_attention", &paged_decode_attention##suffix);           \
+  m.impl("paged_decode_attention.out", &paged_decode_attention_out##suffix);   \
+  m.impl("paged_evict", &paged_evict##suffix);
+
+TORCH_LIBRARY_IMPL(tensorshrink, CUDA, m) { TS_IMPL(m, ) }
+TORCH_LIBRARY_IMPL(tensorshrink, CPU, m) { TS_IMPL(m, ) }
+TORCH_LIBRARY_IMPL(tensorshrink, Meta, m) { TS_IMPL(m, _meta) }

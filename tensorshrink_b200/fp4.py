@@ -33,11 +33,11 @@ BLOCK = {"nvfp4": 16, "mxfp4": 32}
 _ops = {}
 
 
-def _op(name: str):
-    """The overload `torch.ops.tensorshrink.<name>`, looked up once."""
-    f = _ops.get(name)
+def _op(name: str, overload: str = "default"):
+    """The operator `torch.ops.tensorshrink.<name>.<overload>`, looked up once."""
+    f = _ops.get((name, overload))
     if f is None:
-        f = _ops[name] = getattr(_C.serving_ops(), name).default
+        f = _ops[name, overload] = getattr(getattr(_C.serving_ops(), name), overload)
     return f
 
 
@@ -99,7 +99,8 @@ def fp4_quantize(x: torch.Tensor, format: str = "nvfp4", global_scale: Optional[
     NaN."""
     t = Fp4Tensor.__new__(Fp4Tensor)
     t.format, t._code = format, _format(format)
-    t.codes, t.scales, t.global_scale = _op("fp4_quantize")(x, t._code, global_scale)
+    t.codes, t.scales, found = _op("fp4_quantize")(x, t._code, global_scale)
+    t.global_scale = global_scale if found is None else found
     t.rows, t.cols = x.shape
     return t
 

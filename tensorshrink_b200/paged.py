@@ -118,7 +118,10 @@ def paged_decode_attention(qkv: torch.Tensor, n_q: int, cache: PagedKVCache, pos
     seq_lens, no page left, a position without a rotary row) answers with
     zeros and stores nothing. Returns [batch, n_q head_dim] in qkv's type.
     seq_lens is not changed (see `PagedKVCache.advance`)."""
-    return _op("paged_decode_attention")(qkv, n_q, *cache._args(), positions, rope_cos, rope_sin, scale, accumulate, out)
+    args = (qkv, n_q, *cache._args(), positions, rope_cos, rope_sin, scale, accumulate)
+    if out is not None:
+        return _op("paged_decode_attention", "out")(*args, out=out)
+    return _op("paged_decode_attention")(*args)
 
 
 def paged_evict(cache: PagedKVCache, budget: int, recent: int = 0) -> None:

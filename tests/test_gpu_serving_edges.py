@@ -199,3 +199,39 @@ def test_status_of_a_workspace_made_in_inference_mode(ts):
             kernels.device_status()
         kernels.device_status()
         assert torch.equal(ts.fp4_matmul(a, b), want)
+
+
+def test_operators_keep_their_schemas(ts):
+    """What an operator writes and returns is what its schema says, and fake tensors get the same shapes."""
+    from torch.library import opcheck
+    ops = torch.ops.tensorshrink
+    x, one = torch.randn(40, 200, device="cuda").to(torch.bfloat16), torch.full((1,), 0.01, device="cuda")
+    c = filled_cache(ts, [30, 20], room=20)
+    pos = c.seq_lens.long()
+    kv, qkv = torch.randn(2, 3, 2, 64, device="cuda").to(torch.bfloat16), torch.randn(2, 8 * 64, device="cuda").to(torch.bfloat16)
+    cache = (c.k_pages, c.v_pages, c.page_table, c.seq_lens, c.scores, c.slot_pos)
+    tests = ("test_schema", "test_faketensor")
+    for fmt in (0, 1):
+        for g in ((None, one) if fmt == 0 else (None,)):
+            codes, scales, found = ops.fp4_quantize(x, fmt, g)
+            opcheck(ops.fp4_quantize.default, (x, fmt, g), test_utils=tests)
+        g = found if g is None else g
+        opcheck(ops.fp4_dequantize.default, (codes, scales, g, 40, 200, fmt, torch.float32), test_utils=tests)
+        opcheck(ops.fp4_matmul.default, (codes, scales, g, 40, codes, scales, g, 40, 200, fmt, None, torch.float16), test_utils=tests)
+        opcheck(ops.fp4_linear.default, (x, codes, scales, g, 40, 200, fmt, None, None, None), test_utils=tests)
+    opcheck(ops.paged_append.default, (kv, kv, *cache, pos, None, None, None, None), test_utils=tests)
+    attend = (qkv, 4, *cache, pos, None, None, None, True)
+    opcheck(ops.paged_decode_attention.default, attend, test_utils=tests)
+    opcheck(ops.paged_decode_attention.out, attend, dict(out=torch.empty(2, 256, device="cuda", dtype=torch.bfloat16)),
+            test_utils=tests)
+    opcheck(ops.paged_evict.default, (*cache, 16, 2), test_utils=tests)
+
+
+def test_a_compiled_module_runs_the_operator(ts):
+    w = ts.fp4_quantize(torch.randn(128, 256, device="cuda"))
+    layer = ts.Fp4Linear(w, torch.randn(128, device="cuda"))
+    f = torch.compile(lambda x: torch.nn.functional.silu(layer(x)), backend="aot_eager", fullgraph=True, dynamic=True)
+    for m in (3, 40, 41):
+        x = torch.randn(m, 256, device="cuda").to(torch.bfloat16)
+        with torch.no_grad():
+            assert torch.equal(f(x), torch.nn.functional.silu(layer(x)))

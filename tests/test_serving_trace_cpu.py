@@ -1,0 +1,120 @@
+"""The serving operators under tracing, without a GPU: fake tensors get shapes
+and types and never reach the launch code, and the schemas say what is written."""
+
+from __future__ import annotations
+
+import warnings
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import tensorshrink_b200 as ts
+from tensorshrink_b200 import _C, fp4
+
+DEVICE = "cuda"
+
+
+@pytest.fixture
+def fake():
+    """Fake CUDA tensors; a kernel that touches their memory warns, which is an error here."""
+    with warnings.catch_warnings(), FakeTensorMode() as mode:
+        warnings.simplefilter("error")
+        yield mode
+
+
+def weight(n, k, fmt, device=DEVICE):
+    g = torch.ones(1, device=device) if fmt == "nvfp4" else None
+    codes = torch.empty(n, fp4.padded_cols(k) // 2, dtype=torch.uint8, device=device)
+    scales = torch.empty(fp4.scales_nbytes(n, k, fmt), dtype=torch.uint8, device=device)
+    return ts.Fp4Tensor(codes, scales, g, n, k, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 64), (129, 200), (300, 4099)])
+def test_quantise_and_back(fake, fmt, rows, cols):
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEVICE)
+    t = ts.fp4_quantize(x, fmt)
+    assert t.codes.shape == (rows, fp4.padded_cols(cols) // 2) and t.codes.dtype == torch.uint8
+    assert t.scales.shape == (fp4.scales_nbytes(rows, cols, fmt),)
+    assert (t.global_scale is not None) == (fmt == "nvfp4")
+    y = ts.fp4_dequantize(t, torch.float16)
+    assert y.shape == x.shape and y.dtype == torch.float16 and y.device.type == "cuda"
+    if fmt == "nvfp4":
+        g = torch.ones(1, device=DEVICE)
+        assert ts.fp4_quantize(x, fmt, global_scale=g).global_scale is g
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_products(fake, fmt):
+    w = weight(300, 520, fmt)
+    for shape in ((520,), (1, 520), (40, 520), (2, 5, 520)):
+        x = torch.empty(shape, dtype=torch.float16, device=DEVICE)
+        y = ts.fp4_linear(x, w, bias=torch.empty(300, device=DEVICE))
+        assert y.shape == (*shape[:-1], 300) and y.dtype == torch.float16 and y.device.type == "cuda"
+        assert ts.fp4_linear(x, w, out_dtype=torch.float32).dtype == torch.float32
+    a = weight(7, 520, fmt)
+    y = ts.fp4_matmul(a, w)
+    assert y.shape == (7, 300) and y.dtype == torch.bfloat16
+    with pytest.raises(ValueError):
+        ts.fp4_linear(torch.empty(4, 519, device=DEVICE), w)
+
+
+def test_module_traces_to_one_operator(fake):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    layer = ts.Fp4Linear(weight(128, 256, "nvfp4"), torch.empty(128, device=DEVICE))
+    graph = make_fx(layer)(torch.empty(3, 256, dtype=torch.bfloat16, device=DEVICE))
+    calls = [n.target for n in graph.graph.nodes if n.op == "call_function"]
+    assert calls == [torch.ops.tensorshrink.fp4_linear.default]
+
+
+def test_dynamic_token_counts():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    w = weight(128, 256, "mxfp4", "meta")
+    x = torch.empty(9, 256, dtype=torch.bfloat16, device="meta")
+    graph = make_fx(lambda x: ts.fp4_linear(x, w), tracing_mode="symbolic", _allow_non_fake_inputs=True)(x)
+    out = next(n for n in graph.graph.nodes if n.op == "output").args[0]
+    assert not isinstance(out.meta["val"].shape[0], int) and out.meta["val"].shape[1] == 128
+
+
+@pytest.mark.parametrize("track", [False, True])
+def test_cache(fake, track):
+    c = ts.PagedKVCache.allocate(3, 2, 64, 100, 16, device=DEVICE, track=track)
+    pos = torch.zeros(3, dtype=torch.int64, device=DEVICE)
+    cos, sin = torch.empty(200, 32, device=DEVICE), torch.empty(200, 32, device=DEVICE)
+    kv = torch.empty(3, 9, 2, 64, dtype=torch.bfloat16, device=DEVICE)
+    assert ts.paged_append(kv, kv, c, pos, cos, sin) is None
+    qkv = torch.empty(3, 12 * 64, dtype=torch.bfloat16, device=DEVICE)
+    y = ts.paged_decode_attention(qkv, 8, c, pos, cos, sin, accumulate=track)
+    assert y.shape == (3, 8 * 64) and y.dtype == torch.bfloat16 and y.device.type == "cuda"
+    out = torch.empty(3, 8 * 64, dtype=torch.bfloat16, device=DEVICE)
+    assert ts.paged_decode_attention(qkv, 8, c, pos, cos, sin, out=out) is out
+    if track:
+        assert ts.paged_evict(c, 50, 4) is None
+    else:
+        with pytest.raises(ValueError):
+            ts.paged_evict(c, 50, 4)
+
+
+def test_schemas_name_what_is_written_and_returned():
+    ops = _C.serving_ops()
+
+    def written(overload):
+        return {a.name for a in overload._schema.arguments if a.alias_info is not None and a.alias_info.is_write}
+    pool = {"k_pages", "v_pages", "scores", "slot_pos"}
+    assert written(ops.paged_append.default) == pool
+    assert written(ops.paged_decode_attention.default) == pool
+    assert written(ops.paged_decode_attention.out) == pool | {"out"}
+    assert written(ops.paged_evict.default) == pool | {"seq_lens"}
+    assert ops.paged_decode_attention.out._schema.returns[0].alias_info.is_write
+    for op in (ops.fp4_quantize, ops.fp4_dequantize, ops.fp4_matmul, ops.fp4_linear, ops.paged_decode_attention):
+        assert all(r.alias_info is None for r in op.default._schema.returns)
+
+
+def test_the_cpu_is_refused_by_name():
+    x = torch.randn(4, 64)
+    for call in (lambda: ts.fp4_quantize(x), lambda: _C.serving_ops().paged_evict(
+            torch.zeros(1, 1, 16, 64), torch.zeros(1, 1, 16, 64), torch.zeros(1, 1, dtype=torch.int32),
+            torch.zeros(1, dtype=torch.int32), None, None, 4, 0)):
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            call()
