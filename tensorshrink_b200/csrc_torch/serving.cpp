@@ -11,6 +11,9 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <map>
@@ -99,6 +102,23 @@ void on(const OptTensor& t, const at::Device& dev, const char* name) {
   if (has(t)) on(*t, dev, name);
 }
 
+// The operators compute no gradients. A floating-point result of inputs that want
+// them says so when a backward pass reaches it, instead of ending it silently;
+// the forward pass is the same. (Codes are integers, and what is written into a
+// cache or into a given result is held without its history.)
+const at::Tensor* in(const OptTensor& t) { return has(t) ? &*t : nullptr; }
+at::Tensor forward_only(at::Tensor y, const char* name, std::initializer_list<const at::Tensor*> of) {
+  if (!at::GradMode::is_enabled()) return y;
+  std::vector<at::Tensor> in;
+  for (const at::Tensor* t : of)
+    if (t != nullptr && t->requires_grad()) in.push_back(*t);
+  if (!in.empty())
+    torch::autograd::set_history(
+        y, std::make_shared<torch::autograd::NotImplemented>(std::string("tensorshrink::") + name,
+                                                             torch::autograd::collect_next_edges(in)));
+  return y;
+}
+
 // Raises the exception that the library's status stands for.
 void done(int rc, const char* what) {
   if (rc == TS_OK) return;
@@ -181,7 +201,7 @@ at::Tensor fp4_dequantize(const at::Tensor& codes, const at::Tensor& scales, con
   at::Tensor out = fresh({rows, cols}, dtype, codes.device());
   done(ts_fp4_dequantize(&t, out.data_ptr(), dt, cols, at::cuda::getCurrentCUDAStream(codes.device().index()).stream()),
        "fp4_dequantize");
-  return out;
+  return forward_only(std::move(out), "fp4_dequantize", {in(g)});
 }
 
 int check_bias(const OptTensor& bias, int64_t n, const at::Device& dev, const char* what) {
@@ -205,7 +225,7 @@ at::Tensor fp4_matmul(const at::Tensor& ac, const at::Tensor& as, const OptTenso
   cudaStream_t s = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   const Scratch ws = workspace(dev, s, ts_fp4_matmul_workspace_size(m, n, cols, (int)format));
   done(ts_fp4_matmul(&a, &b, ptr(bias), bdt, out.data_ptr(), dt, n, ws.data(), ws.bytes(), s), "fp4_matmul");
-  return out;
+  return forward_only(std::move(out), "fp4_matmul", {in(ag), in(bg), in(bias)});
 }
 
 at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales, const OptTensor& g,
@@ -236,7 +256,7 @@ at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& codes, const at::Te
   const Scratch ws = workspace(dev, s, ts_fp4_linear_workspace_size(m, rows, cols, (int)format));
   done(ts_fp4_linear(x2d.data_ptr(), xdt, m, x2d.stride(0), ptr<float>(input_scale), &w, ptr(bias), bdt, out.data_ptr(), dt,
                      rows, ws.data(), ws.bytes(), s), "fp4_linear");
-  return out;
+  return forward_only(std::move(out), "fp4_linear", {&x, in(g), in(bias), in(input_scale)});
 }
 
 // ---- paged cache ------------------------------------------------------------------
@@ -398,7 +418,8 @@ at::Tensor paged_decode_attention(const at::Tensor& qkv, int64_t n_q, const at::
                                   const at::Tensor& table, const at::Tensor& lens, const OptTensor& scores,
                                   const OptTensor& slot_pos, const OptTensor& positions, const OptTensor& cos,
                                   const OptTensor& sin, c10::optional<double> scale, bool accumulate) {
-  return attend(qkv, n_q, kp, vp, table, lens, scores, slot_pos, positions, cos, sin, scale, accumulate, c10::nullopt);
+  return forward_only(attend(qkv, n_q, kp, vp, table, lens, scores, slot_pos, positions, cos, sin, scale, accumulate,
+                             c10::nullopt), "paged_decode_attention", {&qkv});
 }
 at::Tensor& paged_decode_attention_out(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, const at::Tensor& vp,
                                        const at::Tensor& table, const at::Tensor& lens, const OptTensor& scores,
@@ -475,7 +496,7 @@ at::Tensor fp4_dequantize_meta(const at::Tensor& codes, const at::Tensor& scales
                                int64_t cols, int64_t format, at::ScalarType dtype) {
   fp4_fits(codes, scales, g, rows, cols, format, "fp4_dequantize");
   code_of(dtype, "fp4_dequantize");
-  return at::empty({rows, cols}, codes.options().dtype(dtype));
+  return forward_only(at::empty({rows, cols}, codes.options().dtype(dtype)), "fp4_dequantize", {in(g)});
 }
 
 at::Tensor fp4_matmul_meta(const at::Tensor& ac, const at::Tensor& as, const OptTensor& ag, int64_t m, const at::Tensor& bc,
@@ -485,7 +506,7 @@ at::Tensor fp4_matmul_meta(const at::Tensor& ac, const at::Tensor& as, const Opt
   fp4_fits(bc, bs, bg, n, cols, format, "fp4_matmul");
   check_bias(bias, n, bc.device(), "fp4_matmul");
   code_of(out_dtype, "fp4_matmul");
-  return at::empty({m, n}, ac.options().dtype(out_dtype));
+  return forward_only(at::empty({m, n}, ac.options().dtype(out_dtype)), "fp4_matmul", {in(ag), in(bg), in(bias)});
 }
 
 at::Tensor fp4_linear_meta(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales, const OptTensor& g,
@@ -501,7 +522,7 @@ at::Tensor fp4_linear_meta(const at::Tensor& x, const at::Tensor& codes, const a
   code_of(odt, "fp4_linear");
   c10::SymDimVector shape(x.sym_sizes().begin(), x.sym_sizes().end());
   shape.back() = rows;
-  return at::empty_symint(shape, x.options().dtype(odt));
+  return forward_only(at::empty_symint(shape, x.options().dtype(odt)), "fp4_linear", {&x, in(g), in(bias), in(input_scale)});
 }
 
 void paged_check_meta(const at::Tensor& k, const at::Tensor& v, const at::Tensor&, const at::Tensor&, const OptTensor&,
@@ -526,7 +547,8 @@ at::Tensor paged_decode_attention_meta(const at::Tensor& qkv, int64_t n_q, const
   TORCH_CHECK_VALUE(n_q > 0 && qkv.dim() == 2 && kp.dim() == 4 && qkv.scalar_type() == kp.scalar_type(),
                     "qkv must be [batch, (n_q + 2 n_kv) head_dim] of the cache's type");
   TORCH_CHECK_VALUE(!accumulate || has(scores), "the cache has no scores to accumulate into");
-  return at::empty_symint({qkv.sym_size(0), kp.sym_size(3) * n_q}, qkv.options());
+  return forward_only(at::empty_symint({qkv.sym_size(0), kp.sym_size(3) * n_q}, qkv.options()), "paged_decode_attention",
+                      {&qkv});
 }
 at::Tensor& paged_decode_attention_out_meta(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, const at::Tensor& vp,
                                             const at::Tensor& table, const at::Tensor& lens, const OptTensor& scores,
@@ -584,3 +606,9 @@ TORCH_LIBRARY_FRAGMENT(tensorshrink, m) {
 TORCH_LIBRARY_IMPL(tensorshrink, CUDA, m) { TS_IMPL(m, ) }
 TORCH_LIBRARY_IMPL(tensorshrink, CPU, m) { TS_IMPL(m, ) }
 TORCH_LIBRARY_IMPL(tensorshrink, Meta, m) { TS_IMPL(m, _meta) }
+// (See forward_only: the dispatcher has nothing to do for gradients.)
+TORCH_LIBRARY_IMPL(tensorshrink, Autograd, m) {
+  for (const char* name : {"fp4_check", "fp4_quantize", "fp4_dequantize", "fp4_matmul", "fp4_linear", "paged_check",
+                           "paged_append", "paged_decode_attention", "paged_decode_attention.out", "paged_evict"})
+    m.impl(name, torch::CppFunction::makeFallthrough());
+}

@@ -15,7 +15,8 @@ The reference has neither (its 4-bit codes are integers, codec.py:102-151).
 The functions are thin layers over `torch.ops.tensorshrink.fp4_*`, which check
 their arguments and launch on the current stream of the tensors' device;
 nothing synchronises, so calls can be captured in a graph. They take CUDA
-tensors only and compute no gradients.
+tensors only and compute no gradients: a backward pass that reaches one of their
+results raises. (Codes are integers, so that none reaches `fp4_quantize`.)
 """
 
 from __future__ import annotations

@@ -235,3 +235,13 @@ def test_a_compiled_module_runs_the_operator(ts):
         x = torch.randn(m, 256, device="cuda").to(torch.bfloat16)
         with torch.no_grad():
             assert torch.equal(f(x), torch.nn.functional.silu(layer(x)))
+
+
+def test_gradients_are_refused_not_dropped(ts):
+    x = torch.randn(4, 256, device="cuda", requires_grad=True)
+    w = ts.fp4_quantize(torch.nn.Parameter(torch.randn(128, 256, device="cuda")))
+    y = ts.fp4_linear(x, w)
+    assert torch.equal(y.detach(), ts.fp4_linear(x.detach(), w))
+    with pytest.raises(RuntimeError, match="derivative for tensorshrink::fp4_linear is not implemented"):
+        y.sum().backward()
+    assert not w.global_scale.requires_grad

@@ -118,3 +118,39 @@ def test_the_cpu_is_refused_by_name():
             torch.zeros(1, dtype=torch.int32), None, None, 4, 0)):
         with pytest.raises(RuntimeError, match="CUDA tensors only"):
             call()
+
+
+def differentiable():
+    """Calls on tensors without memory whose results depend on something that wants a gradient."""
+    x = torch.randn(4, 256, device="meta", requires_grad=True)
+    bias = torch.randn(128, device="meta", requires_grad=True)
+    w, g = weight(128, 256, "nvfp4", "meta"), torch.ones(1, device="meta", requires_grad=True)
+    a = ts.Fp4Tensor(w.codes, w.scales, g, 128, 256, "nvfp4")
+    c = ts.PagedKVCache.allocate(2, 2, 64, 32, 16, device="meta", dtype=torch.float16)
+    qkv = torch.randn(2, 8 * 64, device="meta", dtype=torch.float16, requires_grad=True)
+    return {"x": lambda: ts.fp4_linear(x, w), "bias": lambda: ts.fp4_linear(x.detach(), w, bias=bias),
+            "input_scale": lambda: ts.fp4_linear(x.detach(), w, input_scale=g), "matmul": lambda: ts.fp4_matmul(a, w),
+            "dequantize": lambda: ts.fp4_dequantize(a), "attention": lambda: ts.paged_decode_attention(qkv, 4, c)}
+
+
+@pytest.mark.parametrize("name", ["x", "bias", "input_scale", "matmul", "dequantize", "attention"])
+def test_a_backward_pass_is_refused(name):
+    call = differentiable()[name]
+    with torch.no_grad():
+        assert not call().requires_grad
+    with pytest.raises(RuntimeError, match="derivative for tensorshrink::.* is not implemented"):
+        call().sum().backward()
+
+
+def test_nothing_else_gets_a_history():
+    x = torch.randn(4, 256, device="meta", requires_grad=True)
+    t = ts.fp4_quantize(x)
+    assert not t.global_scale.requires_grad and not ts.fp4_dequantize(t).requires_grad
+    assert not ts.fp4_linear(x.detach(), t).requires_grad
+    c = ts.PagedKVCache.allocate(2, 2, 64, 32, 16, device="meta", dtype=torch.float16)
+    kv = torch.randn(2, 3, 2, 64, device="meta", dtype=torch.float16, requires_grad=True)
+    ts.paged_append(kv, kv, c)
+    qkv = torch.randn(2, 8 * 64, device="meta", dtype=torch.float16, requires_grad=True)
+    out = torch.empty(2, 256, device="meta", dtype=torch.float16)
+    ts.paged_decode_attention(qkv, 4, c, out=out)
+    assert not (c.k_pages.requires_grad or c.v_pages.requires_grad or out.requires_grad)
