@@ -132,7 +132,8 @@ def fp4_linear(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = Non
 class Fp4Linear(nn.Module):
     """A linear layer with an Fp4Tensor weight. Buffers: `codes`, `scales`,
     `global_scale` (nvfp4) and `input_scale` (nvfp4: the activations' tensor
-    scale, 1 until `calibrate`), `bias`."""
+    scale, 1 until `calibrate`), `bias`. Casting the module (`.to(dtype)`,
+    `.half()`) casts the bias; the tensor scales stay fp32."""
 
     def __init__(self, weight: Fp4Tensor, bias: Optional[torch.Tensor] = None):
         super().__init__()
@@ -149,6 +150,15 @@ class Fp4Linear(nn.Module):
         """Quantise an nn.Linear whose weight is on the GPU."""
         b = layer.bias.detach() if layer.bias is not None else None
         return cls(fp4_quantize(layer.weight.detach(), format), b)
+
+    def _apply(self, fn, recurse=True):
+        scales = {name: getattr(self, name) for name in ("global_scale", "input_scale")}
+        super()._apply(fn, recurse)
+        for name, scale in scales.items():
+            cast = getattr(self, name)
+            if cast is not None and cast.dtype != torch.float32:
+                setattr(self, name, scale.to(cast.device))      # moved, but not rounded
+        return self
 
     def weight(self) -> Fp4Tensor:
         return Fp4Tensor(self.codes, self.scales, self.global_scale, self.out_features, self.in_features, self.format)

@@ -245,3 +245,12 @@ def test_gradients_are_refused_not_dropped(ts):
     with pytest.raises(RuntimeError, match="derivative for tensorshrink::fp4_linear is not implemented"):
         y.sum().backward()
     assert not w.global_scale.requires_grad
+
+
+def test_a_cast_module_multiplies_as_before(ts):
+    layer = ts.Fp4Linear(ts.fp4_quantize(torch.randn(128, 256, device="cuda")))
+    x = torch.randn(3, 256, device="cuda").to(torch.bfloat16)
+    layer.calibrate(x)
+    want = layer(x)
+    for dtype in (torch.bfloat16, torch.float16, torch.float64):
+        assert torch.equal(layer.to(dtype)(x), want)

@@ -154,3 +154,29 @@ def test_nothing_else_gets_a_history():
     out = torch.empty(2, 256, device="meta", dtype=torch.float16)
     ts.paged_decode_attention(qkv, 4, c, out=out)
     assert not (c.k_pages.requires_grad or c.v_pages.requires_grad or out.requires_grad)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(),
+                                  lambda m: torch.nn.Sequential(m).to(torch.float16)[0],
+                                  lambda m: m.bfloat16().float()])
+def test_a_cast_module_keeps_its_scales(cast):
+    """Values that bf16 and fp16 would round."""
+    w = weight(128, 256, "nvfp4", "meta")
+    with torch.device("meta"):
+        layer = ts.Fp4Linear(w, torch.randn(128))
+    layer.global_scale, layer.input_scale = torch.full((1,), 1.0001e-9), torch.full((1,), 0.0100001)
+    want = [layer.global_scale.clone(), layer.input_scale.clone()]
+    layer = cast(layer)
+    assert torch.equal(layer.global_scale, want[0]) and torch.equal(layer.input_scale, want[1])
+    assert layer.codes.dtype == torch.uint8 and layer.scales.dtype == torch.uint8
+    assert {"global_scale", "input_scale"} <= set(layer.state_dict())
+
+
+def test_a_cast_module_runs_and_moves(fake):
+    layer = ts.Fp4Linear(weight(128, 256, "nvfp4"), torch.empty(128, device=DEVICE)).to(torch.bfloat16)
+    x = torch.empty(3, 256, dtype=torch.bfloat16, device=DEVICE)
+    assert layer(x).shape == (3, 128) and layer.bias.dtype == torch.bfloat16
+    moved = layer.to("cpu", torch.float16)
+    assert moved.global_scale.device.type == "cpu" and moved.global_scale.dtype == torch.float32
+    mx = ts.Fp4Linear(weight(128, 256, "mxfp4")).half()
+    assert mx.global_scale is None and mx(x).shape == (3, 128)
