@@ -10,6 +10,7 @@ models through `CUDAGraphQuantModel`, modules.py:1589-1691, and leaves the
 cache to them). Weights are random, as in `QuantDecoder`.
 
     model = PagedDecoder(DecoderConfig(...), "cuda", max_batch=8, max_len=4096, budget=1024, recent=128)
+    model.calibrate(samples)                # nvfp4: the activations' tensor scales, once
     token = model.prefill(prompts)          # list of 1-D token tensors, one per sequence
     for _ in range(min(n, model.steps_left)):
         token = model.decode_step(token)    # may be captured in a CUDA graph
@@ -194,6 +195,23 @@ class PagedDecoder(nn.Module):
         self.positions.copy_(n_new)
         logits = self._logits(h[torch.arange(B, device=self.device), n_new.long() - 1])
         return logits if return_logits else logits.argmax(dim=-1)
+
+    @torch.no_grad()
+    def calibrate(self, prompts: Sequence[torch.Tensor]) -> None:
+        """Set the projections' input scales (nvfp4; mxfp4 has none) from a
+        prefill of sample prompts, each from what it is given behind the
+        projections already set. They are 1 before: a block whose largest value
+        is below 6 * 2^-6 then has a scale below E4M3's normal range, and its values
+        up to three bits less. The caches are left as after `prefill`."""
+        keep = torch.arange(max(map(len, prompts), default=0)) < torch.tensor([len(p) for p in prompts])[:, None]
+        keep = keep.to(self.device)                      # (not the padding)
+        hooks = [p.register_forward_pre_hook(lambda proj, args: proj.calibrate(args[0][keep]))
+                 for layer in self.layers for p in layer.projections()]
+        try:
+            self.prefill(prompts)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     @torch.no_grad()
     def decode_step(self, tokens: torch.Tensor, return_logits: bool = False) -> torch.Tensor:

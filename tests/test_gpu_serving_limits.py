@@ -188,3 +188,60 @@ def test_decoding_starts_from_the_prompts_weights():
                 s = torch.arange(n, device="cuda")
                 total = c.scores[c.page_table[b, s // 16].long(), :, s % 16].double().sum(0)
                 assert ((total - 2 * n).abs() <= 2.0 ** -16 * 2 * n).all()
+
+
+def projection_inputs(m, ps):
+    """What each projection is given by a prefill, without the padding, and the prefill's logits."""
+    seen, n = {}, [len(p) for p in ps]
+    keep = (torch.arange(max(n)) < torch.tensor(n)[:, None]).cuda()
+    names = {p: f"{i}.{name}" for i, layer in enumerate(m.layers) for name, p in zip(("qkv", "o", "gate_up", "down"),
+                                                                                     layer.projections())}
+    hooks = [p.register_forward_pre_hook(lambda p, args: seen.update({names[p]: (p, args[0][keep].clone())})) for p in names]
+    logits = m.prefill(ps, return_logits=True)
+    for h in hooks:
+        h.remove()
+    return seen, logits
+
+
+def test_calibrated_scales_are_those_of_the_samples():
+    """Each projection's scale is max|x| / 2688 of what a prefill of the samples
+    gives it, and with it 4 bits hold the small activations behind the attention
+    better than with 1, where block scales fall below E4M3's normal range."""
+    import tensorshrink_b200 as ts
+    m = build(max_len=64)
+    ps = prompts([30, 17])
+    before, _ = projection_inputs(m, ps)
+    m.calibrate(ps)
+    assert m.positions.tolist() == [30, 17] and m.caches[0].seq_lens.tolist() == [30, 17]
+    after, logits = projection_inputs(m, ps)
+    assert len(after) == 8
+    for name, (proj, x) in after.items():
+        assert proj.input_scale.item() == (x.float().abs().max() / 2688.0).item(), name
+
+    one, small = torch.ones(1, device="cuda"), 0
+    for name, (proj, x) in before.items():
+        own = (x.float().abs().max() / 2688.0).reshape(1)
+        blocks = x.float().reshape(x.shape[0], -1, 16)
+        low = (blocks.abs().amax(-1) < 6 * 2.0 ** -7) & (blocks.abs().amax(-1) > 0)
+        small += int(low.sum())
+
+        def off(g):
+            y = ts.fp4_dequantize(ts.fp4_quantize(x, "nvfp4", global_scale=g)).reshape(blocks.shape)
+            return (y - blocks)[low].norm()
+        assert low.sum() == 0 or off(own) < off(one), name
+    assert small > 0
+    again = m.prefill(ps, return_logits=True)
+    assert torch.equal(again, logits)
+
+
+def test_calibration_of_mxfp4_and_of_bad_samples():
+    m = build(max_len=64, format="mxfp4")
+    ps = prompts([30, 17])
+    want = m.prefill(ps, return_logits=True)
+    m.calibrate(ps)
+    assert torch.equal(m.prefill(ps, return_logits=True), want)
+    with pytest.raises(ValueError):
+        m.calibrate(ps[:1])
+    with pytest.raises(ValueError):
+        m.calibrate([])
+    assert not any(p._forward_pre_hooks for layer in m.layers for p in layer.projections())
