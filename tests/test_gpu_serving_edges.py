@@ -254,3 +254,30 @@ def test_a_cast_module_multiplies_as_before(ts):
     want = layer(x)
     for dtype in (torch.bfloat16, torch.float16, torch.float64):
         assert torch.equal(layer.to(dtype)(x), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,d", [([1500, 40], 64), ([700, 3], 128), ([300, 65], 256)])
+def test_attention_weights_have_both_their_terms(ts, dtype, lens, d):
+    """Against 64 bits with weights in two terms of the cache's type: the result's
+    rounding, half a unit (2^-8 of it in bf16, with 8 bits, 2^-11 in fp16, with 11);
+    2^-15 of sum p |v| for the weights' rounding (2^-16, 2^-22) and fp32 arithmetic on
+    scores of this size (2^-16); where fp16 weights underflow, 2^-25 of max |v| a
+    slot. One term alone would be off by up to 2^-8 (2^-11) of sum p |v|."""
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    g = torch.Generator(device="cuda").manual_seed(d)
+    c = ts.PagedKVCache.allocate(2, 2, d, max(lens) + 1, 16, dtype=dtype)
+    for t in (c.k_pages, c.v_pages):
+        t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+    c.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+    qkv = torch.randn(2, 10 * d, generator=g, device="cuda").to(dtype)
+    got = ts.paged_decode_attention(qkv, 6, c).double().view(2, 2, 3, d)
+    for b, n in enumerate(lens):
+        t = torch.arange(n + 1, device="cuda")
+        page = c.page_table[b, t // 16].long()
+        k, v = c.k_pages[page, :, t % 16].double(), c.v_pages[page, :, t % 16].double()
+        q = qkv[b].double().view(10, d)[:6].view(2, 3, d)
+        p = (torch.einsum("hgd,thd->hgt", q, k) * d ** -0.5).softmax(-1)
+        want, size = torch.einsum("hgt,thd->hgd", p, v), torch.einsum("hgt,thd->hgd", p, v.abs())
+        off = 2.0 ** -15 * size + (0 if dtype == torch.bfloat16 else (n + 1) * 2.0 ** -25 * v.abs().max())
+        assert ((got[b] - want).abs() <= half * (want.abs() + off) + off + 2.0 ** -25).all()

@@ -245,3 +245,49 @@ def test_calibration_of_mxfp4_and_of_bad_samples():
     with pytest.raises(ValueError):
         m.calibrate([])
     assert not any(p._forward_pre_hooks for layer in m.layers for p in layer.projections())
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_a_decode_step_is_its_parts(fmt):
+    """A step retraced from what its projections got and gave: every part but the
+    attention bit for bit, the attention against 64 bits over the cache that the
+    step leaves. Its bound: rounding to the 8 bits of bf16, 2^-8 of the result;
+    weights in two terms of bf16, 2^-8 of 2^-8 of each, and fp32 arithmetic on scores
+    of this size, 2^-16: 2^-15 of sum p |v|. (A result left out, or of another layer,
+    would be off by about 1 of the same; weights rounded once, by up to 2^-8.)"""
+    import torch.nn.functional as F
+    from tensorshrink_b200.decoder import _rms_norm
+    m = build(batch=3, max_len=300, format=fmt)
+    lens = [130, 1, 259]
+    m.prefill(prompts(lens))
+    names = {p: (i, name) for i, layer in enumerate(m.layers) for name, p in zip(("qkv", "o", "gate_up", "down"),
+                                                                                 layer.projections())}
+    seen = {}
+    for p in names:
+        p.register_forward_hook(lambda p, x, y: seen.update({names[p]: (x[0].clone(), y.clone())}))
+    tokens = torch.tensor([7, 77, 377], device="cuda")
+    logits = m.decode_step(tokens, return_logits=True)
+    h = m.embed[tokens].float()
+    for i, (layer, c) in enumerate(zip(m.layers, m.caches)):
+        assert torch.equal(seen[i, "qkv"][0], _rms_norm(h, layer.input_norm, m.cfg.rms_eps))
+        assert c.seq_lens.tolist() == [n + 1 for n in lens]
+        for b, n in enumerate(lens):
+            x = seen[i, "qkv"][1][b].view(8, 64)
+            cos, sin = m.rope_cos[n], m.rope_sin[n]
+            x1, x2 = x[:4].float().chunk(2, dim=-1)
+            q = torch.cat([x1 * cos - x2 * sin, x1 * sin + x2 * cos], dim=-1).to(x.dtype).double().view(2, 2, 64)
+            t = torch.arange(n + 1, device="cuda")
+            page = c.page_table[b, t // 16].long()
+            k, v = c.k_pages[page, :, t % 16].double(), c.v_pages[page, :, t % 16].double()
+            assert torch.equal(v[n], x[6:].double())
+            p = (torch.einsum("hgd,thd->hgt", q, k) * 64 ** -0.5).softmax(-1)
+            want = torch.einsum("hgt,thd->hgd", p, v).reshape(-1)
+            size = torch.einsum("hgt,thd->hgd", p, v.abs()).reshape(-1)
+            err = (seen[i, "o"][0][b].double() - want).abs()
+            assert (err <= 2.0 ** -8 * (want.abs() + 2.0 ** -15 * size) + 2.0 ** -15 * size).all()
+        h = h + seen[i, "o"][1]
+        assert torch.equal(seen[i, "gate_up"][0], _rms_norm(h, layer.post_norm, m.cfg.rms_eps))
+        gate, up = seen[i, "gate_up"][1].chunk(2, dim=-1)
+        assert torch.equal(seen[i, "down"][0], F.silu(gate) * up)
+        h = h + seen[i, "down"][1]
+    assert torch.equal(logits, F.linear(_rms_norm(h, m.final_norm, m.cfg.rms_eps), m.lm_head).float())
