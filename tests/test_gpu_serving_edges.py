@@ -281,3 +281,36 @@ def test_attention_weights_have_both_their_terms(ts, dtype, lens, d):
         want, size = torch.einsum("hgt,thd->hgd", p, v), torch.einsum("hgt,thd->hgd", p, v.abs())
         off = 2.0 ** -15 * size + (0 if dtype == torch.bfloat16 else (n + 1) * 2.0 ** -25 * v.abs().max())
         assert ((got[b] - want).abs() <= half * (want.abs() + off) + off + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,d", [(0, 64), (1, 64), (40, 128), (900, 64), (300, 256)])
+def test_infinite_values_come_out_as_the_formula_has_them(ts, dtype, n, d):
+    """sum p v with an infinity in v is that infinity, with two of unlike sign or a
+    NaN it is NaN, and the other columns are finite."""
+    c = ts.PagedKVCache.allocate(1, 1, d, n + 1, 16, dtype=dtype)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    for t in (c.k_pages, c.v_pages):
+        t.copy_(torch.randn(t.shape, generator=g, device="cuda") * 0.2)
+    c.seq_lens.fill_(n)
+    qkv = (torch.randn(1, 6 * d, generator=g, device="cuda") * 0.2).to(dtype)
+    clean = ts.paged_decode_attention(qkv, 4, c).view(4, d)
+    inf, nan = float("inf"), float("nan")
+    qkv[0, 5 * d] = inf                                      # the new token's v
+    want = {0: inf}
+    if n:
+        v = c.v_pages.view(-1, d)
+        for col, slots in ((1, {0: inf}), (2, {n - 1: -inf}), (3, {n // 2: nan}), (4, {0: inf, n - 1: inf}),
+                           (d - 1, {n // 3: -inf})):
+            for s, x in slots.items():
+                v[s, col] = x
+            want[col] = x
+        if n > 1:
+            v[0, 5], v[n - 1, 5] = inf, -inf
+            want[5] = nan
+    got = ts.paged_decode_attention(qkv, 4, c).view(4, d)
+    for col in range(d):
+        if col not in want:
+            assert torch.equal(got[:, col], clean[:, col]), col
+        else:
+            assert torch.equal(got[:, col].nan_to_num(nan=7.0), torch.full_like(got[:, col], want[col]).nan_to_num(nan=7.0)), col
