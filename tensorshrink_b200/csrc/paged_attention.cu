@@ -967,9 +967,10 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) paged_append_kernel(const A
 
 int make_cache(const ts_paged_cache* p, Cache* o) {
   TS_REQUIRE(p != nullptr, "NULL cache");
-  TS_REQUIRE(p->k_pages && p->v_pages && p->page_table && p->seq_lens, "NULL pointer in the cache");
+  // (of no sequences at all there may be no memory)
+  TS_REQUIRE(p->batch == 0 || (p->k_pages && p->v_pages && p->page_table && p->seq_lens), "NULL pointer in the cache");
   TS_UNSUPPORTED(p->dtype == TS_F16 || p->dtype == TS_BF16, "the cache holds fp16 or bf16");
-  TS_REQUIRE(p->batch >= 0 && p->n_kv > 0 && p->page_size > 0 && p->num_pages > 0 && p->max_pages > 0,
+  TS_REQUIRE(p->batch >= 0 && p->n_kv > 0 && p->page_size > 0 && (p->batch == 0 || (p->num_pages > 0 && p->max_pages > 0)),
              "bad cache sizes");
   TS_UNSUPPORTED(p->head_dim % 16 == 0 && p->head_dim >= 16 && p->head_dim <= 256,
                  "head_dim must be a multiple of 16, <= 256");
@@ -1070,14 +1071,14 @@ extern "C" int ts_paged_decode_attention(const void* qkv, int64_t qkv_row_stride
   AttnArgs a;
   const int rc = make_cache(cache, &a.c);
   if (rc != TS_OK) return rc;
-  TS_REQUIRE(qkv && out, "NULL pointer");
+  TS_REQUIRE(a.c.batch == 0 || (qkv && out), "NULL pointer");
   TS_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), "rope_cos and rope_sin come both or neither");
-  TS_REQUIRE(positions != nullptr || (rope_cos == nullptr && a.c.slot_pos == nullptr),
+  TS_REQUIRE(a.c.batch == 0 || positions != nullptr || (rope_cos == nullptr && a.c.slot_pos == nullptr),
              "positions are needed for the rotation and for slot_pos");
   TS_REQUIRE(n_q > 0 && n_q % a.c.n_kv == 0, "bad head counts");
   TS_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
   TS_REQUIRE(is_aligned(out, 4) && out_row_stride % 2 == 0, "rows of out must be 4-byte aligned");
-  TS_REQUIRE(!accumulate || a.c.scores != nullptr, "the cache has no scores to accumulate into");
+  TS_REQUIRE(a.c.batch == 0 || !accumulate || a.c.scores != nullptr, "the cache has no scores to accumulate into");
   if (a.c.batch == 0) return TS_OK;
   a.group = n_q / a.c.n_kv;
   a.head_tiles = (a.group + kHeads - 1) / kHeads;
@@ -1139,14 +1140,15 @@ extern "C" int ts_paged_append(const void* k, const int64_t* k_strides, const vo
   AppendArgs a;
   const int rc = make_cache(cache, &a.c);
   if (rc != TS_OK) return rc;
-  TS_REQUIRE(k && v && k_strides && v_strides && tokens >= 0, "bad tokens");
+  TS_REQUIRE(tokens >= 0, "bad tokens");
+  if (a.c.batch == 0 || tokens == 0) return TS_OK;     // (there may be no memory behind the pointers)
+  TS_REQUIRE(k && v && k_strides && v_strides, "NULL pointer");
   TS_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), "rope_cos and rope_sin come both or neither");
   TS_REQUIRE(scores == nullptr || (a.c.scores != nullptr && score_strides != nullptr),
              "scores were given for a cache that keeps none");
   for (int i = 0; i < 3; ++i)
     TS_REQUIRE(k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0, "k and v rows must be 16-byte aligned");
   TS_REQUIRE(is_aligned(k, 16) && is_aligned(v, 16), "k and v must be 16-byte aligned");
-  if (a.c.batch == 0 || tokens == 0) return TS_OK;
   a.k = reinterpret_cast<const uint16_t*>(k);
   a.v = reinterpret_cast<const uint16_t*>(v);
   a.kb = k_strides[0]; a.kt = k_strides[1]; a.kh = k_strides[2];

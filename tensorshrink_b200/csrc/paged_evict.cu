@@ -308,7 +308,7 @@ extern "C" int ts_paged_evict(const ts_paged_cache* cache, int budget, int recen
   EvictArgs a;
   const int rc = make_cache(cache, &a.c);
   if (rc != TS_OK) return rc;
-  TS_REQUIRE(a.c.scores != nullptr && a.c.slot_pos != nullptr, "eviction needs the cache's scores and slot_pos");
+  TS_REQUIRE(a.c.batch == 0 || (a.c.scores != nullptr && a.c.slot_pos != nullptr), "eviction needs the cache's scores and slot_pos");
   TS_REQUIRE(budget > 0, "budget must be positive");
   TS_REQUIRE(recent >= 0 && recent <= budget, "recent must be in [0, budget]");
   const int64_t cap = (int64_t)a.c.max_pages * a.c.page_size;

@@ -365,7 +365,7 @@ void paged_append(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tens
   int64_t ss[3] = {0, 0, 0};
   if (has(new_scores)) {
     on(*new_scores, dev, "scores");
-    TORCH_CHECK_VALUE(c.scores != nullptr, "scores were given for a cache that keeps none");
+    TORCH_CHECK_VALUE(has(scores), "scores were given for a cache that keeps none");
     TORCH_CHECK_VALUE(new_scores->scalar_type() == at::kFloat && new_scores->dim() == 3 && new_scores->size(0) == c.batch &&
                           new_scores->size(1) == c.n_kv && new_scores->size(2) == k.size(1),
                       "scores must be fp32 [batch, n_kv, tokens]");
@@ -392,9 +392,9 @@ at::Tensor attend(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, cons
   TORCH_CHECK_VALUE(qkv.scalar_type() == kp.scalar_type(), "qkv must have the cache's type");
   const int64_t rows = rope_rows(c, cos, sin, dev, "paged_decode_attention");
   per_sequence(positions, c, at::kLong, dev, "positions");
-  TORCH_CHECK_VALUE(has(positions) || (rows == 0 && c.slot_pos == nullptr),
+  TORCH_CHECK_VALUE(has(positions) || (rows == 0 && !has(slot_pos)),
                     "positions are needed for the rotation and for slot_pos");
-  TORCH_CHECK_VALUE(!accumulate || c.scores != nullptr, "the cache has no scores to accumulate into");
+  TORCH_CHECK_VALUE(!accumulate || has(scores), "the cache has no scores to accumulate into");
   at::Tensor out;
   if (has(out_)) {
     out = *out_;
@@ -432,7 +432,7 @@ at::Tensor& paged_decode_attention_out(const at::Tensor& qkv, int64_t n_q, const
 void paged_evict(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& table, const at::Tensor& lens,
                  const OptTensor& scores, const OptTensor& slot_pos, int64_t budget, int64_t recent) {
   const ts_paged_cache c = cache_view(kp, vp, table, lens, scores, slot_pos);
-  TORCH_CHECK_VALUE(c.scores != nullptr && c.slot_pos != nullptr, "eviction needs the cache's scores and slot_pos");
+  TORCH_CHECK_VALUE(has(scores) && has(slot_pos), "eviction needs the cache's scores and slot_pos");
   TORCH_CHECK_VALUE(budget > 0 && budget <= INT32_MAX && recent >= 0 && recent <= budget,
                     "budget must be positive and recent in [0, budget], got ", budget, " and ", recent);
   const at::Device dev = kp.device();

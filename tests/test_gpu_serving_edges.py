@@ -314,3 +314,27 @@ def test_infinite_values_come_out_as_the_formula_has_them(ts, dtype, n, d):
             assert torch.equal(got[:, col], clean[:, col]), col
         else:
             assert torch.equal(got[:, col].nan_to_num(nan=7.0), torch.full_like(got[:, col], want[col]).nan_to_num(nan=7.0)), col
+
+
+def test_nothing_to_do(ts):
+    c = filled_cache(ts, [30, 20])
+    before = [t.clone() for t in (c.k_pages, c.v_pages, c.scores, c.slot_pos, c.seq_lens)]
+    kv = torch.zeros(2, 0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    pos = torch.zeros(2, dtype=torch.int64, device="cuda")
+    ts.paged_append(kv, kv, c, pos, scores=torch.zeros(2, 2, 0, device="cuda"))
+    kv = torch.ones(2, 3, 2, 64, dtype=torch.bfloat16, device="cuda")
+    ts.paged_append(kv[:, 3:], kv[:, 3:], c)
+    ts.paged_append(kv, kv, c, n_new=torch.zeros(2, dtype=torch.int32, device="cuda"))
+    assert all(torch.equal(x, y) for x, y in zip(before, (c.k_pages, c.v_pages, c.scores, c.slot_pos, c.seq_lens)))
+    for none in (ts.PagedKVCache(c.k_pages, c.v_pages, c.page_table[:0], c.seq_lens[:0], c.scores, c.slot_pos),
+                 ts.PagedKVCache.allocate(0, 2, 64, 32, 16, track=True)):
+        qkv = torch.zeros(0, 8 * 64, dtype=torch.bfloat16, device="cuda")
+        out = ts.paged_decode_attention(qkv, 4, none, pos[:0], accumulate=True)
+        assert out.shape == (0, 256) and out.dtype == torch.bfloat16
+        ts.paged_append(kv[:0], kv[:0], none, pos[:0])
+        ts.paged_evict(none, 4, 1)
+    w = ts.fp4_quantize(torch.randn(8, 64, device="cuda"))
+    empty = ts.fp4_quantize(torch.zeros(0, 64, device="cuda"))
+    assert ts.fp4_matmul(empty, w).shape == (0, 8) and ts.fp4_matmul(w, empty).shape == (8, 0)
+    assert ts.fp4_linear(torch.zeros(2, 0, 64, device="cuda"), w).shape == (2, 0, 8)
+    assert ts.fp4_dequantize(empty).shape == (0, 64)
