@@ -327,7 +327,8 @@ int64_t rope_rows(const ts_paged_cache& c, const OptTensor& cos, const OptTensor
     TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(1) == c.head_dim / 2 && t->is_contiguous(),
                       what, ": the rotary tables must be contiguous fp32 [positions, head_dim / 2]");
   }
-  TORCH_CHECK_VALUE(cos->size(0) == sin->size(0), what, ": the rotary tables differ in length");
+  // (the library takes the NULL that an empty table's data is for no table)
+  TORCH_CHECK_VALUE(cos->size(0) == sin->size(0) && cos->size(0) > 0, what, ": the rotary tables are empty or differ in length");
   return cos->size(0);
 }
 

@@ -338,3 +338,17 @@ def test_nothing_to_do(ts):
     assert ts.fp4_matmul(empty, w).shape == (0, 8) and ts.fp4_matmul(w, empty).shape == (8, 0)
     assert ts.fp4_linear(torch.zeros(2, 0, 64, device="cuda"), w).shape == (2, 0, 8)
     assert ts.fp4_dequantize(empty).shape == (0, 64)
+
+
+def test_rotary_tables_without_rows_are_refused(ts):
+    """They used to count as no tables: keys were stored without their rotation."""
+    c = filled_cache(ts, [30, 20])
+    before = c.k_pages.clone()
+    none, pos = torch.zeros(0, 32, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    qkv = torch.ones(2, 8 * 64, dtype=torch.bfloat16, device="cuda")
+    kv = torch.ones(2, 3, 2, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="rotary tables are empty"):
+        ts.paged_decode_attention(qkv, 4, c, pos, none, none)
+    with pytest.raises(ValueError, match="rotary tables are empty"):
+        ts.paged_append(kv, kv, c, pos, none, none)
+    assert torch.equal(before, c.k_pages)
