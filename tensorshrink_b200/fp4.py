@@ -165,9 +165,11 @@ class Fp4Linear(nn.Module):
 
     @torch.no_grad()
     def calibrate(self, x: torch.Tensor) -> None:
-        """Set `input_scale` from sample activations: max|x| / 2688."""
+        """Set `input_scale` from sample activations: max|x| / 2688 over the
+        finite ones, as `fp4_quantize` finds a tensor's scale."""
         if self.input_scale is not None:
-            top = x.detach().float().abs().amax()
+            x = x.detach().float()
+            top = torch.where(x.isfinite(), x, torch.zeros_like(x)).abs().amax()
             self.input_scale.copy_((top / 2688.0).clamp(min=2.0 ** -100).reshape(1))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

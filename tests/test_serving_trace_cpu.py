@@ -180,3 +180,15 @@ def test_a_cast_module_runs_and_moves(fake):
     assert moved.global_scale.device.type == "cpu" and moved.global_scale.dtype == torch.float32
     mx = ts.Fp4Linear(weight(128, 256, "mxfp4")).half()
     assert mx.global_scale is None and mx(x).shape == (3, 128)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_calibration_takes_finite_samples(bad):
+    layer = ts.Fp4Linear(weight(128, 256, "nvfp4", "meta"))
+    layer.input_scale = torch.ones(1)
+    x = torch.linspace(-3, 2, 512).view(2, 256)
+    x[0, 5] = bad
+    layer.calibrate(x)
+    assert layer.input_scale.item() == (torch.tensor(3.0) / 2688.0).item()
+    layer.calibrate(torch.full((1, 256), bad))
+    assert layer.input_scale.item() == 2.0 ** -100
