@@ -330,7 +330,9 @@ TS_API int ts_paged_append(const void* k, const int64_t* k_strides, const void* 
  * and v stored in slot seq_lens[b], and every query head attends over slots
  * [0, seq_lens[b]] with scores scale * q.k. With accumulate != 0 each slot's
  * score grows by the weights that the kv head's query heads gave it (the new
- * slot's starts from 0; it is set to 0 too when nothing is accumulated). A
+ * slot's starts from 0; it is set to 0 too when nothing is accumulated);
+ * sequences must not share pages then, as one of two additions to the same score
+ * would be lost. A
  * sequence whose count is negative, that has no page left for the token, or
  * whose position has no rotary row answers with zeros and stores nothing.
  * seq_lens is not changed. qkv, out as in ts_decode_attention, in the

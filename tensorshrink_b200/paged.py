@@ -114,7 +114,8 @@ def paged_decode_attention(qkv: torch.Tensor, n_q: int, cache: PagedKVCache, pos
     given; k and v are stored in slot seq_lens[b]; every query head attends over
     slots [0, seq_lens[b]] with scores scale * q.k (default head_dim ** -0.5).
     `accumulate`: add to each slot's score the weights that its kv head's
-    query heads gave it. A sequence that has no slot for the token (negative
+    query heads gave it; sequences must not share pages then (each adds to its own
+    slots' scores, and one of two additions to the same would be lost). A sequence that has no slot for the token (negative
     seq_lens, no page left, a position without a rotary row) answers with
     zeros and stores nothing. Returns [batch, n_q head_dim] in qkv's type.
     seq_lens is not changed (see `PagedKVCache.advance`)."""
