@@ -644,9 +644,9 @@ __global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1) fp4_
 // complete on the leader's barrier; the leader's thread issues scale copies
 // and MMAs for both; commits release the stage in both. Tokens are the
 // accumulator's lanes, so that a thread stores runs of its token's outputs.
-// Measured: 8192 x 28672 x 8192 nvfp4, 720 to 760 us, 5.1 to 5.3 PFLOP/s at the
-// power limit (a lone CTA's tiles of 128 x 128: 1284 us); 2047 x 14336 x 4096,
-// 62 us, 3.9 PFLOP/s, in seven rounds of tiles where six hold all but four.
+// Measured: 8192 x 28672 x 8192 nvfp4, 720 to 815 us by card and by what ran
+// before, 4.7 to 5.3 PFLOP/s at the power limit (a lone CTA's tiles of 128 x 128:
+// 1284 us); 2047 x 14336 x 4096, 62 us, 3.9 PFLOP/s, in seven rounds of tiles where six hold all but four.
 // Bound by the loads into each SM (about 52 of 64 bytes a clock).
 
 constexpr int BN = 256, kHalf = BN / 2;

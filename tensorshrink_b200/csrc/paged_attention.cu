@@ -29,7 +29,7 @@
 //
 // Measured (bf16, 128 columns, 8 kv heads of 4 query heads): 64 sequences of up to
 // 8191 slots, 177 us, 6.1 TB/s, 94% of the copy bandwidth; 4 of 32768, 88 us, with
-// the logits kept 90 us (98 us with the cache read at the same L2 priority as
+// the logits kept 90 to 92 us (98 us with the cache read at the same L2 priority as
 // the logits are written); one of 512, 10.0 us, a chain of latencies (lengths,
 // pages, rows, the warps' and the CTAs' joins).
 #include <algorithm>
