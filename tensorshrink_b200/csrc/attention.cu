@@ -205,7 +205,14 @@ extern "C" int ts_decode_attention(const void* qkv, int64_t qkv_row_stride, int 
              "KV cache rows must be 16-byte aligned");
   if (batch == 0) return TS_OK;
   auto kern = attn::decode_attention_kernel;
-  if (smem > 48 * 1024) TS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static thread_local int configured_dev = -1;
+  int dev = 0;
+  TS_CUDA_TRY(cudaGetDevice(&dev));
+  if (configured_dev != dev) {
+    const int rc = open_smem(reinterpret_cast<const void*>(kern));
+    if (rc != TS_OK) return rc;
+    configured_dev = dev;
+  }
   kern<<<batch * n_kv, 32 * std::max(group, 4), smem, reinterpret_cast<cudaStream_t>(stream)>>>(
       reinterpret_cast<const __nv_bfloat16*>(qkv), qkv_row_stride, n_q, n_kv, head_dim, pos, rope_cos, rope_sin,
       reinterpret_cast<__nv_bfloat16*>(k_cache), reinterpret_cast<__nv_bfloat16*>(v_cache), cache_batch_stride,

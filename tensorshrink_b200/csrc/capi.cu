@@ -144,6 +144,14 @@ bool take_test_stall() {
 int sm_count() { return dev_info().sms; }
 int max_smem_optin() { return dev_info().smem_optin; }
 
+int open_smem(const void* kernel) {
+  cudaFuncAttributes attr;
+  TS_CUDA_TRY(cudaFuncGetAttributes(&attr, kernel));
+  TS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   max_smem_optin() - (int)attr.sharedSizeBytes));
+  return TS_OK;
+}
+
 static bool valid_act_dtype(int d) { return d == TS_F16 || d == TS_BF16; }
 static bool valid_dtype(int d) { return d == TS_F16 || d == TS_BF16 || d == TS_F32; }
 

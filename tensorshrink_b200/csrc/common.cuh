@@ -61,6 +61,11 @@ int sm_count();            // SMs of the current device (cached per device)
 uint64_t wait_limit_ns();
 bool take_test_stall();
 int max_smem_optin();      // opt-in shared memory per block of the current device
+// Lets a kernel's launches on the current device have all the dynamic shared
+// memory of a block next to its static. The limit is the function's, whoever
+// sets it, so that every thread sets the same: one that set what a call of its own
+// needs would lower it under a larger call of another.
+int open_smem(const void* kernel);
 
 inline bool is_aligned(const void* p, size_t a) {
   return (reinterpret_cast<uintptr_t>(p) % a) == 0;

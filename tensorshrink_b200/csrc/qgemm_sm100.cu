@@ -924,13 +924,12 @@ template <int BITS, bool CB, int XT, int BT>
 static int launch_qgemm(const CUtensorMap* maps, const qgemm::Args& a, int grid, size_t smem, cudaStream_t st) {
   auto k = qgemm::qgemm_kernel<BITS, CB, XT, BT>;
   static thread_local int configured_dev = -1;
-  static thread_local size_t configured_smem = 0;
   int dev = 0;
   TS_CUDA_TRY(cudaGetDevice(&dev));
-  if (configured_dev != dev || configured_smem < smem) {
-    TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (configured_dev != dev) {
+    const int rc = open_smem(reinterpret_cast<const void*>(k));
+    if (rc != TS_OK) return rc;
     configured_dev = dev;
-    configured_smem = smem;
   }
   k<<<grid, qgemm::kThreads, smem, st>>>(maps[0], maps[1], maps[2], maps[3], maps[4], a);
   TS_LAUNCH_CHECK();

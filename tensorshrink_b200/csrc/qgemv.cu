@@ -1270,13 +1270,12 @@ template <int BITS, bool CB, bool DQ, int SEG, int NL>
 int launch_one(const gemv::Chain<NL>& c, uint32_t grid, cudaStream_t stream, size_t smem) {
   auto kern = gemv::qgemv_kernel<BITS, CB, DQ, SEG, NL>;
   static thread_local int configured_dev = -1;
-  static thread_local size_t configured_smem = 0;
   int dev = 0;
   TS_CUDA_TRY(cudaGetDevice(&dev));
-  if (configured_dev != dev || configured_smem < smem) {
-    TS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (configured_dev != dev) {
+    const int rc = open_smem(reinterpret_cast<const void*>(kern));
+    if (rc != TS_OK) return rc;
     configured_dev = dev;
-    configured_smem = smem;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
