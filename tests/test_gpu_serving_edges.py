@@ -353,3 +353,25 @@ def test_rotary_tables_without_rows_are_refused(ts):
     with pytest.raises(ValueError, match="rotary tables are empty"):
         ts.paged_append(kv, kv, c, pos, none, none)
     assert torch.equal(before, c.k_pages)
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_a_compiled_step_over_the_cache_is_the_step(ts, backend):
+    """Append, attention and eviction traced as one graph: what they write is written."""
+    a, b = (filled_cache(ts, [20, 9], room=40) for _ in range(2))
+    pos = a.seq_lens.long()
+
+    def step(cache, qkv, kv, pos):
+        ts.paged_append(kv, kv, cache, pos)
+        cache.advance(5)
+        y = ts.paged_decode_attention(qkv, 4, cache, pos + 5, accumulate=True)
+        cache.advance()
+        ts.paged_evict(cache, 12, 2)
+        return y * 2
+    compiled = torch.compile(step, backend=backend, fullgraph=True)
+    for _ in range(3):
+        qkv, kv = torch.randn(2, 8 * 64, device="cuda").to(torch.bfloat16), torch.randn(2, 5, 2, 64, device="cuda").to(torch.bfloat16)
+        with torch.no_grad():
+            assert torch.equal(step(a, qkv, kv, pos), compiled(b, qkv, kv, pos))
+        for name in ("k_pages", "v_pages", "scores", "slot_pos", "seq_lens"):
+            assert torch.equal(getattr(a, name), getattr(b, name)), name
