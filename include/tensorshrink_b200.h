@@ -361,6 +361,148 @@ TS_API int ts_paged_evict(const ts_paged_cache* cache, int budget, int recent, v
                           size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * A paged key-value cache held in 8 bits. Pages hold codes [num_pages, n_kv,
+ * page_size, head_dim] (strides in elements = bytes), `block` neighbouring slots of
+ * a kv head share an fp32 scale: scales are contiguous [num_pages, n_kv, page_size /
+ * block], value = code * scale. page_size and block are multiples of 16, and
+ * block divides page_size. Everything else is as in ts_paged_cache.
+ */
+typedef enum ts_cache_code {
+  TS_CACHE_INT8 = 0,    /* signed integers, -127 .. 127 */
+  TS_CACHE_E4M3 = 1     /* 8-bit floating point, largest value 448 */
+} ts_cache_code;
+
+typedef struct ts_paged_cache8 {
+  void* k_pages;
+  void* v_pages;
+  int64_t page_stride, head_stride, token_stride;
+  float* k_scales;
+  float* v_scales;
+  const int32_t* page_table;  /* device [batch, max_pages] */
+  int64_t table_stride;
+  int32_t* seq_lens;          /* device [batch] */
+  int32_t code;               /* ts_cache_code */
+  int32_t batch, n_kv, head_dim, page_size, num_pages, max_pages, block;
+} ts_paged_cache8;
+
+/*
+ * Stores new tokens of each sequence in slots seq_lens[b] + t. k / v:
+ * [batch, tokens, n_kv, head_dim] of fp16 or bf16 with element strides (sequence,
+ * token, head) or, with offsets (device int32 [batch + 1]), packed: sequence b's
+ * tokens are rows offsets[b] to offsets[b + 1] of `tokens` in all, and the sequence
+ * stride is not used. n_new (device int32 [batch], or NULL): a smaller count per
+ * sequence. Rotation as ts_paged_append, k rounded to its type before it is
+ * quantised. For every block of slots that gets tokens, with a = max|new values|
+ * and q = 127 (TS_CACHE_INT8) or 448, in fp32:
+ *   need = max(a * fp32(1 / q), 2^-100)
+ *   scale = need                          the block holds no earlier tokens
+ *         = old                           need <= old
+ *         = max(need, 1.25 old)           otherwise; earlier codes become
+ *                                         round(code * (old / scale))
+ *   code = round(x * (1 / scale)), to nearest even, within +-q
+ * An infinity or a NaN among a block's values makes its scale NaN (and stays
+ * until the block begins anew); the new codes are 0 then. Tokens without a slot, a page or a
+ * rotary row are dropped. seq_lens is not changed; codes of slots behind the last token are left alone.
+ */
+TS_API int ts_paged8_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                            int kv_dtype, int64_t tokens, const int32_t* offsets, const int32_t* n_new,
+                            const ts_paged_cache8* cache, const int64_t* first, const float* rope_cos,
+                            const float* rope_sin, int64_t rope_rows, void* stream);
+
+/* The values of all pages, k and v contiguous [num_pages, n_kv, page_size,
+ * head_dim] of out_dtype, rounded once from the fp32 product code * scale. */
+TS_API int ts_paged8_dequantize(const ts_paged_cache8* cache, void* k, void* v, int out_dtype, void* stream);
+
+/*
+ * Attention of one query token per sequence over its cached tokens, slots [0,
+ * seq_lens[b]): q [batch, n_q * head_dim] fp16 or bf16, out alike. With tables q is
+ * rotated to positions[b]; a position without a rotary row, like a sequence
+ * without tokens, answers with zeros. Slots without a page do not count.
+ * Workspace as ts_paged_decode_attention.
+ */
+TS_API size_t ts_paged8_attention_workspace_size(const ts_paged_cache8* cache, int n_q);
+TS_API int ts_paged8_attention(const void* q, int q_dtype, int64_t q_row_stride, int n_q, const ts_paged_cache8* cache,
+                               const int64_t* positions, const float* rope_cos, const float* rope_sin,
+                               int64_t rope_rows, float scale, void* out, int64_t out_row_stride, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/*
+ * ts_paged_decode_attention for this cache: the new token's k and v (from qkv,
+ * [batch, (n_q + 2 n_kv) * head_dim]) are stored by ts_paged8_append, and
+ * every query head attends over slots [0, seq_lens[b]]. Workspace as above.
+ */
+TS_API int ts_paged8_decode_attention(const void* qkv, int qkv_dtype, int64_t qkv_row_stride, int n_q,
+                                      const ts_paged_cache8* cache, const int64_t* positions, const float* rope_cos,
+                                      const float* rope_sin, int64_t rope_rows, float scale, void* out,
+                                      int64_t out_row_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ts_int8_status for the 8-bit attention's flag. */
+TS_API int ts_paged8_status(int clear, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Norms of queries and keys for each head, and their rotation.
+ *
+ * x [tokens, (n_q + 2 n_kv) * head_dim] (fp16 or bf16, rows 16-byte aligned):
+ * query heads, key heads, value heads. Query and key heads become
+ *   y = x * rsqrt(mean(x^2) + eps) * w        (w: q_weight or k_weight, [head_dim]
+ *                                             of weight_dtype; NULL: y = x)
+ *   (y1 c - y2 s, y1 s + y2 c)                with tables, at positions[t]
+ * in fp32, rounded once; values are copied. out may be x. With a cache (16
+ * bits, x's type) key and value heads also go to slot slots[t] (device int64: page *
+ * page_size + offset) of its pages, whose score and position are set; a slot outside
+ * the pool is not written. A token whose position has no rotary row gets
+ * zeros and is not stored.
+ */
+TS_API int ts_qk_norm_rope(const void* x, int dtype, int64_t x_row_stride, int64_t tokens, int n_q, int n_kv, int head_dim,
+                           const void* q_weight, const void* k_weight, int weight_dtype, float eps,
+                           const int64_t* positions, const float* rope_cos, const float* rope_sin, int64_t rope_rows,
+                           void* out, int64_t out_row_stride, const ts_paged_cache* cache, const int64_t* slots,
+                           void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Page tables from request lengths. The pool is a stack of page numbers:
+ * free_pages[0 .. n_free[0]) of `capacity` are free, the last one is taken first.
+ */
+typedef struct ts_page_pool {
+  int32_t* free_pages;   /* device [capacity] */
+  int32_t* n_free;       /* device [1] */
+  int32_t capacity;
+  int32_t reserved0;
+} ts_page_pool;
+
+typedef struct ts_page_table {
+  int32_t* table;        /* device [batch, max_pages] */
+  int64_t table_stride;
+  int32_t* seq_lens;     /* device [batch] */
+  int32_t batch, max_pages, page_size, num_pages;
+} ts_page_table;
+
+/*
+ * Pages for n_new[b] (device; negative counts as 0) tokens behind each sequence's
+ * cached ones. An entry of the table that these tokens need and that names no page of
+ * [0, num_pages) gets one from the pool; sequences are served in order, all
+ * or nothing, until one needs more pages than are left: it and those behind
+ * it that need any get none. granted[b]: n_new[b], or 0 for a sequence that was
+ * not served, is out of use (negative seq_lens) or would pass the table's end. offsets
+ * [batch + 1]: where each sequence's tokens start in a packed batch of all n_new. For
+ * token t < capacity `tokens` of the packed batch: sequences[t] (-1 behind the
+ * last), slots[t] = page * page_size + offset (-1 without a page), positions[t] =
+ * (first[b], or without first the slot's number in the sequence) of a token with a slot, 0
+ * otherwise. seq_lens is not changed. Workspace as ts_paged_decode_attention.
+ */
+TS_API int ts_paged_reserve(const ts_page_pool* pool, const ts_page_table* table, const int32_t* n_new,
+                            const int64_t* first, int64_t tokens, int32_t* granted, int32_t* offsets, int64_t* slots,
+                            int64_t* positions, int32_t* sequences, void* stream);
+
+/*
+ * Cuts sequences back: where keep[b] (device) is not negative, seq_lens[b]
+ * becomes min(seq_lens[b], keep[b]) and the pages that it no longer needs go to the
+ * pool, in order of the sequences and of their pages; their entries become
+ * -1. Sequences must not share such pages.
+ */
+TS_API int ts_paged_release(const ts_page_pool* pool, const ts_page_table* table, const int32_t* keep, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Microscaled 4-bit floating point. Elements are E2M1, the even column in a
  * byte's low nibble, columns padded with zeros to a multiple of 64:
  *   TS_NVFP4  blocks of 16 columns with an E4M3 scale s and one fp32 scale g
@@ -424,6 +566,50 @@ TS_API size_t ts_fp4_linear_workspace_size(int64_t M, int64_t N, int64_t K, int 
 TS_API int ts_fp4_linear(const void* x, int x_dtype, int64_t M, int64_t x_row_stride, float* x_scale,
                          const ts_fp4_tensor* w, const void* bias, int bias_dtype, void* out, int out_dtype,
                          int64_t out_row_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit integers with a scale per row: value = code * scale[row]. Codes of a
+ * row lie on 16 bytes, `row_stride` bytes from the next row's; cols at most
+ * 131072 (a product's sums are 32-bit integers).
+ */
+typedef struct ts_int8_tensor {
+  int8_t* codes;         /* device, 16-byte aligned */
+  int64_t row_stride;    /* a multiple of 16, at least cols rounded up to 16 */
+  float* scales;         /* device [rows] */
+  int64_t rows, cols;
+} ts_int8_tensor;
+
+/*
+ * Quantises x [rows, cols] (fp16, bf16 or fp32) into t:
+ *   scale = max(max|row| * fp32(1 / 127), 2^-100),  code = rint(x * (1 / scale))
+ * with every operation rounded to fp32; columns up to the next multiple of 16
+ * get codes of 0. A row that holds an infinity or a NaN gets the scale NaN and
+ * codes of 0.
+ */
+TS_API int ts_int8_quantize(const void* x, int x_dtype, int64_t x_row_stride, const ts_int8_tensor* t, void* stream);
+
+/* The values of t in out_dtype, rounded once from the fp32 product code * scale. */
+TS_API int ts_int8_dequantize(const ts_int8_tensor* t, void* out, int out_dtype, int64_t out_row_stride, void* stream);
+
+/*
+ * out[M, N] = a . b^T (+ bias) for a [M, K] and b [N, K] on the integer tensor
+ * cores: exact 32-bit sums, then (sum * smaller scale) * larger scale + bias in fp32,
+ * rounded once to out_dtype. Workspace as ts_paged_decode_attention.
+ */
+TS_API size_t ts_int8_matmul_workspace_size(int64_t M, int64_t N, int64_t K);
+TS_API int ts_int8_matmul(const ts_int8_tensor* a, const ts_int8_tensor* b, const void* bias, int bias_dtype, void* out,
+                          int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[M, N] = x . w^T (+ bias): ts_int8_quantize of x [M, cols] by way of the
+ * workspace, then ts_int8_matmul, bit for bit. */
+TS_API size_t ts_int8_linear_workspace_size(int64_t M, int64_t N, int64_t K);
+TS_API int ts_int8_linear(const void* x, int x_dtype, int64_t M, int64_t x_row_stride, const ts_int8_tensor* w,
+                          const void* bias, int bias_dtype, void* out, int out_dtype, int64_t out_row_stride,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* ts_fp4_status for the int8 product's flag (the workspace's counters are the
+ * caller's to zero). */
+TS_API int ts_int8_status(int clear, void* stream);
 
 /* Bytes at a serving workspace's start that hold counters: zero before the
  * first call and between calls. */

@@ -92,7 +92,34 @@ class TsFp4Tensor(C.Structure):
                 ("format", _i32), ("reserved0", _i32)]
 
 
+class TsInt8Tensor(C.Structure):
+    """struct ts_int8_tensor."""
+    _fields_ = [("codes", _vp), ("row_stride", _i64), ("scales", _vp), ("rows", _i64), ("cols", _i64)]
+
+
+class TsPagedCache8(C.Structure):
+    """struct ts_paged_cache8."""
+    _fields_ = [
+        ("k_pages", _vp), ("v_pages", _vp), ("page_stride", _i64), ("head_stride", _i64), ("token_stride", _i64),
+        ("k_scales", _vp), ("v_scales", _vp), ("page_table", _vp), ("table_stride", _i64), ("seq_lens", _vp),
+        ("code", _i32), ("batch", _i32), ("n_kv", _i32), ("head_dim", _i32), ("page_size", _i32),
+        ("num_pages", _i32), ("max_pages", _i32), ("block", _i32),
+    ]
+
+
+class TsPagePool(C.Structure):
+    """struct ts_page_pool."""
+    _fields_ = [("free_pages", _vp), ("n_free", _vp), ("capacity", _i32), ("reserved0", _i32)]
+
+
+class TsPageTable(C.Structure):
+    """struct ts_page_table."""
+    _fields_ = [("table", _vp), ("table_stride", _i64), ("seq_lens", _vp), ("batch", _i32), ("max_pages", _i32),
+                ("page_size", _i32), ("num_pages", _i32)]
+
+
 TS_NVFP4, TS_MXFP4 = 0, 1
+TS_CACHE_INT8, TS_CACHE_E4M3 = 0, 1
 
 OP_GATED = 1
 OP_RMSNORM = 2
@@ -144,6 +171,29 @@ _SIGNATURES = [
                                 _i64, _vp, C.c_size_t, _vp]),
     ("ts_serving_counter_bytes", C.c_size_t, []),
     ("ts_fp4_status", C.c_int, [_vp, C.c_size_t, C.c_int, _vp]),
+    ("ts_int8_quantize", C.c_int, [_vp, C.c_int, _i64, C.POINTER(TsInt8Tensor), _vp]),
+    ("ts_int8_dequantize", C.c_int, [C.POINTER(TsInt8Tensor), _vp, C.c_int, _i64, _vp]),
+    ("ts_int8_matmul_workspace_size", C.c_size_t, [_i64, _i64, _i64]),
+    ("ts_int8_matmul", C.c_int, [C.POINTER(TsInt8Tensor), C.POINTER(TsInt8Tensor), _vp, C.c_int, _vp, C.c_int, _i64,
+                                 _vp, C.c_size_t, _vp]),
+    ("ts_int8_linear_workspace_size", C.c_size_t, [_i64, _i64, _i64]),
+    ("ts_int8_linear", C.c_int, [_vp, C.c_int, _i64, _i64, C.POINTER(TsInt8Tensor), _vp, C.c_int, _vp, C.c_int, _i64,
+                                 _vp, C.c_size_t, _vp]),
+    ("ts_int8_status", C.c_int, [C.c_int, _vp]),
+    ("ts_paged8_append", C.c_int, [_vp, C.POINTER(_i64), _vp, C.POINTER(_i64), C.c_int, _i64, _vp, _vp,
+                                   C.POINTER(TsPagedCache8), _vp, _vp, _vp, _i64, _vp]),
+    ("ts_paged8_dequantize", C.c_int, [C.POINTER(TsPagedCache8), _vp, _vp, C.c_int, _vp]),
+    ("ts_paged8_attention_workspace_size", C.c_size_t, [C.POINTER(TsPagedCache8), C.c_int]),
+    ("ts_paged8_attention", C.c_int, [_vp, C.c_int, _i64, C.c_int, C.POINTER(TsPagedCache8), _vp, _vp, _vp, _i64,
+                                      C.c_float, _vp, _i64, _vp, C.c_size_t, _vp]),
+    ("ts_paged8_decode_attention", C.c_int, [_vp, C.c_int, _i64, C.c_int, C.POINTER(TsPagedCache8), _vp, _vp, _vp, _i64,
+                                             C.c_float, _vp, _i64, _vp, C.c_size_t, _vp]),
+    ("ts_paged8_status", C.c_int, [C.c_int, _vp]),
+    ("ts_qk_norm_rope", C.c_int, [_vp, C.c_int, _i64, _i64, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, C.c_float,
+                                  _vp, _vp, _vp, _i64, _vp, _i64, C.POINTER(TsPagedCache), _vp, _vp]),
+    ("ts_paged_reserve", C.c_int, [C.POINTER(TsPagePool), C.POINTER(TsPageTable), _vp, _vp, _i64, _vp, _vp, _vp, _vp,
+                                   _vp, _vp]),
+    ("ts_paged_release", C.c_int, [C.POINTER(TsPagePool), C.POINTER(TsPageTable), _vp, _vp]),
     ("ts_dequantize_weight", C.c_int, [C.POINTER(TsQWeight), _vp, C.c_int, _i64, C.c_int, _vp]),
     ("ts_quantize_workspace_size", C.c_size_t, [C.POINTER(TsQuantParams)]),
     ("ts_quantize_pack", C.c_int, [_vp, C.c_int, C.POINTER(TsQuantParams), C.POINTER(TsQuantOutputs),

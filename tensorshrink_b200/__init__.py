@@ -43,11 +43,27 @@ from .fp4 import (
     fp4_matmul,
     fp4_linear,
 )
+from .int8 import (
+    Int8Tensor,
+    Int8Linear,
+    int8_quantize,
+    int8_dequantize,
+    int8_matmul,
+    int8_linear,
+)
 from .paged import (
     PagedKVCache,
+    PagedKVCache8,
+    PagePool,
+    PagedSlots,
     paged_append,
+    paged_attention,
     paged_decode_attention,
+    paged_dequantize,
     paged_evict,
+    paged_release,
+    paged_reserve,
+    qk_norm_rope,
 )
 
 __version__ = "0.1.0"
@@ -59,5 +75,8 @@ __all__ = [
     "quantize_tensor_gpu_adaptive", "quantize_module_gpu", "fused_quantized_linear",
     "apply_outlier_correction", "dequantize_weight", "ChainStep", "qlinear_chain",
     "Fp4Tensor", "Fp4Linear", "fp4_quantize", "fp4_dequantize", "fp4_matmul", "fp4_linear",
+    "Int8Tensor", "Int8Linear", "int8_quantize", "int8_dequantize", "int8_matmul", "int8_linear",
     "PagedKVCache", "paged_append", "paged_decode_attention", "paged_evict",
+    "PagedKVCache8", "paged_attention", "paged_dequantize", "PagePool", "PagedSlots", "paged_reserve", "paged_release",
+    "qk_norm_rope",
 ]

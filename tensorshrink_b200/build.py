@@ -29,7 +29,7 @@ LIBDIR = PKG / "_lib"
 OBJDIR = PKG / "_lib" / "obj"
 LIBNAME = "libtensorshrink_b200.so"
 TORCH_LIBNAME = "libtensorshrink_torch.so"
-TORCH_SRCS = [PKG / "csrc_torch" / "ops.cpp", PKG / "csrc_torch" / "serving.cpp"]
+TORCH_SRCS = [PKG / "csrc_torch" / name for name in ("ops.cpp", "serving.cpp", "serving8.cpp")]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
@@ -105,21 +105,32 @@ def build_torch_ops(lib: Path, verbose: bool = False) -> Path:
     thin C++ layer (host code only) over the C ABI library."""
     import torch.utils.cpp_extension as ce
     out = LIBDIR / TORCH_LIBNAME
-    deps = [*TORCH_SRCS, lib] + list(INCLUDE.glob("*.h"))
+    headers = [*INCLUDE.glob("*.h"), *TORCH_SRCS[0].parent.glob("*.h"), Path(__file__)]
+    deps = [*TORCH_SRCS, *headers, lib]
     if out.exists() and out.stat().st_mtime >= max(f.stat().st_mtime for f in deps):
         return out
     import torch
     cuda_inc = Path(nvcc()).resolve().parent.parent / "include"
-    cmd = ["g++", "-O2", "-shared", "-fPIC", "-std=c++17", *map(str, TORCH_SRCS), "-o", str(out),
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{p}" for p in ce.include_paths()], f"-I{cuda_inc}", f"-I{INCLUDE}",
-           *[f"-L{p}" for p in ce.library_paths()], "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-           "-ltorch_cuda", f"-L{LIBDIR}", "-ltensorshrink_b200", "-Wl,-rpath,$ORIGIN"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"torch ops build failed:\n{r.stdout}\n{r.stderr}")
+    flags = ["-O2", "-fPIC", "-std=c++17", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             *[f"-I{p}" for p in ce.include_paths()], f"-I{cuda_inc}", f"-I{INCLUDE}"]
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"torch ops build failed:\n{r.stdout}\n{r.stderr}")
+
+    def compile_one(src: Path) -> Path:
+        obj = OBJDIR / f"torch_{src.stem}.o"
+        if not obj.exists() or obj.stat().st_mtime < max(f.stat().st_mtime for f in [src, *headers]):
+            run(["g++", *flags, "-c", str(src), "-o", str(obj)])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(TORCH_SRCS)) as ex:
+        objs = list(ex.map(compile_one, TORCH_SRCS))
+    run(["g++", "-shared", *map(str, objs), "-o", str(out), *[f"-L{p}" for p in ce.library_paths()], "-lc10", "-lc10_cuda",
+         "-ltorch", "-ltorch_cpu", "-ltorch_cuda", f"-L{LIBDIR}", "-ltensorshrink_b200", "-Wl,-rpath,$ORIGIN"])
     return out
 
 

@@ -442,9 +442,9 @@ int ts_lloyd_fit(const float* values, int64_t n, int n_levels, int iters, float*
 
 namespace ts {
 
-int encode_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner,
-                   uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
-                   CUtensorMapSwizzle swizzle) {
+int encode_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int rank, const uint64_t* dims,
+                const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle,
+                CUtensorMapL2promotion promotion) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -455,13 +455,17 @@ int encode_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   });
   TS_REQUIRE(fn != nullptr, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dims[2] = {inner, outer};
-  const cuuint64_t strides[1] = {row_stride_bytes};
-  const cuuint32_t box[2] = {box_inner, box_outer};
-  const cuuint32_t estr[2] = {1, 1};
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    estr[i] = 1;
+    if (i + 1 < rank) s[i] = strides_bytes[i];
+  }
   auto encode = [&] {
-    return fn(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return fn(map, dtype, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = encode();
   if (r == CUDA_ERROR_INVALID_CONTEXT) {
@@ -472,10 +476,18 @@ int encode_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype
     TS_CUDA_TRY(cudaSetDevice(dev));
     r = encode();
   }
-  TS_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (%d): inner=%llu outer=%llu stride=%llu box=%ux%u",
-             (int)r, (unsigned long long)inner, (unsigned long long)outer,
-             (unsigned long long)row_stride_bytes, box_inner, box_outer);
+  TS_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (%d): rank=%d inner=%llu outer=%llu stride=%llu box=%ux%u",
+             (int)r, rank, (unsigned long long)dims[0], (unsigned long long)dims[1], (unsigned long long)strides_bytes[0],
+             box[0], box[1]);
   return TS_OK;
+}
+
+int encode_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner,
+                   uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
+                   CUtensorMapSwizzle swizzle) {
+  const uint64_t dims[2] = {inner, outer};
+  const uint32_t box[2] = {box_inner, box_outer};
+  return encode_tmap(map, base, dtype, 2, dims, &row_stride_bytes, box, swizzle);
 }
 
 }  // namespace ts

@@ -154,22 +154,6 @@ __device__ __forceinline__ uint32_t quantise16(const Lane<DT>& v, float g, float
   return sc;
 }
 
-// Clusters.
-__device__ __forceinline__ uint32_t cta_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// The address of the same shared-memory location in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_cta(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-}
-
 // Checks a tensor's description (`what` names it in messages).
 int check_tensor(const ts_fp4_tensor* t, const char* what);
 

@@ -39,6 +39,7 @@
 #include <algorithm>
 
 #include "fp4.cuh"
+#include "gemm.cuh"
 #include "paged.cuh"
 
 namespace ts {
@@ -120,16 +121,6 @@ __host__ __device__ constexpr uint32_t idesc_fp4(int M, int N, uint32_t sf) {
          ((uint32_t)(M >> 7) << 27) | (sf << 29);
 }
 
-// One lane of a converged warp. Unlike `lane == 0` it tells the compiler that
-// the code behind it runs once per warp, and the descriptors of tensor-core
-// instructions then go to uniform registers without a loop over lanes (the
-// same kernel, 8192 x 28672 x 8192: 2035 us with lane == 0, 1284 us with this).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
-  return p != 0;
-}
-
 template <bool NV>
 __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                         uint32_t accumulate) {
@@ -184,12 +175,6 @@ __device__ __forceinline__ void store_tokens(const GemmArgs& a, int64_t m, int64
     for (int j = 0; j < R; ++j, p += step)
       if (j < jn) *p = __float2half_rn(alpha(v[j], bias));
   }
-}
-
-__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
 }
 
 // Stores alpha * v + bias as output features n .. n + 3 of token m.
@@ -686,44 +671,6 @@ struct PairArgs {
   int stall, overlap;
 };
 
-// 128 consecutive fp32 columns of this warp's TMEM lane quadrant, four loads in flight.
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
-#pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    uint32_t* q = r + 32 * h;
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
-          "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]),
-          "=r"(q[15]), "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]),
-          "=r"(q[22]), "=r"(q[23]), "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]),
-          "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
-        : "r"(taddr + 32 * h));
-  }
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  // the registers hold the values from here on: no use moves before the wait
-#pragma unroll
-  for (int i = 0; i < 128; ++i) asm volatile("" : "+r"(r[i]));
-}
-
-// TMA tile load into this CTA's shared memory, completing on a barrier of either CTA of the pair.
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
 __device__ __forceinline__ void copy_scales_pair(uint32_t tmem, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
@@ -1104,31 +1051,6 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
     p.grid = 2 * (int)std::min<int64_t>(mb * nb, pairs);
   }
   return p;
-}
-
-// Launch; with `overlap` the kernel may start while the one before it (which
-// allows that, and whose results it waits for by itself) still runs.
-template <typename K, typename... Args>
-static cudaError_t launch_after(K k, int grid, int threads, size_t smem, cudaStream_t st, int overlap, int cluster,
-                                const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  cfg.attrs = attr;
-  if (overlap) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (cluster) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
-    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
-    ++cfg.numAttrs;
-  }
-  return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
 template <bool NV>

@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "fp4.cuh"
+#include "gemm.cuh"
 #include "paged.cuh"
 
 namespace ts {

@@ -309,4 +309,9 @@ int encode_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype
                    uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                    CUtensorMapSwizzle swizzle);
 
+// The same of `rank` <= 5 dimensions, the innermost first: strides of all but that one, in bytes.
+int encode_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int rank, const uint64_t* dims,
+                const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle,
+                CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+
 }  // namespace ts
