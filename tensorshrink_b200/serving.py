@@ -1,6 +1,8 @@
-"""A Llama-shaped decoder served from 4-bit floating-point projections and a
-paged key-value cache: `fp4_linear`, `paged_append`, `paged_decode_attention`
-and `paged_evict` as a serving program strings them together.
+"""A Llama-shaped decoder served from 4-bit floating-point or 8-bit integer
+projections and a paged key-value cache of 16 or 8 bits: `fp4_linear` or
+`int8_linear`, `qk_norm_rope`, `paged_append`, `paged_decode_attention` and
+`paged_evict`, `paged_reserve` and `paged_release`, as a serving program strings them
+together.
 
 `decoder.QuantDecoder` decodes a batch whose sequences all stand at one
 position of a dense cache. Here every sequence has its own length, and with a
@@ -14,6 +16,9 @@ cache to them). Weights are random, as in `QuantDecoder`.
     token = model.prefill(prompts)          # list of 1-D token tensors, one per sequence
     for _ in range(min(n, model.steps_left)):
         token = model.decode_step(token)    # may be captured in a CUDA graph
+
+    model = PagedDecoder(DecoderConfig(...), "cuda", format="int8", cache_dtype=torch.int8, qk_norm=True, pages=2000,
+                         max_batch=64, max_len=8192)    # 64 sequences of 8192 tokens would take 8192 pages of 64
 
 A step that a sequence has no rotary row or no slot for raises; the others go
 on once that one is taken out (`drop`). Replays of a captured step run without
@@ -32,7 +37,9 @@ from torch import nn
 
 from .decoder import DecoderConfig, _rms_norm, student_t_weight
 from .fp4 import Fp4Linear, fp4_quantize
-from .paged import PagedKVCache, paged_append, paged_decode_attention, paged_evict
+from .int8 import Int8Linear, int8_quantize
+from .paged import (PagedKVCache, PagedKVCache8, PagePool, paged_append, paged_decode_attention, paged_evict, paged_release,
+                    paged_reserve, qk_norm_rope)
 
 
 def _prompt_weights(q: torch.Tensor, k: torch.Tensor, lens: Sequence[int], most: int = 1 << 26) -> torch.Tensor:
@@ -64,18 +71,21 @@ def _prompt_weights(q: torch.Tensor, k: torch.Tensor, lens: Sequence[int], most:
 class PagedDecoderLayer(nn.Module):
     """One layer's projections (q/k/v and gate/up fused by rows) and norms."""
 
-    def __init__(self, cfg: DecoderConfig, layer_idx: int, format: str, device):
+    def __init__(self, cfg: DecoderConfig, layer_idx: int, format: str, device, qk_norm: bool = False):
         super().__init__()
         H, D = cfg.hidden, cfg.head_dim
         shapes = {"qkv": ((cfg.n_heads + 2 * cfg.n_kv_heads) * D, H), "o": (H, cfg.n_heads * D),
                   "gate_up": (2 * cfg.intermediate, H), "down": (H, cfg.intermediate)}
         for j, (name, shape) in enumerate(shapes.items()):
             w = student_t_weight(shape, seed=cfg.seed * 100003 + layer_idx * 16 + j, device=device)
-            setattr(self, name, Fp4Linear(fp4_quantize(w, format)))
+            setattr(self, name, Int8Linear(int8_quantize(w)) if format == "int8" else Fp4Linear(fp4_quantize(w, format)))
         self.input_norm = nn.Parameter(torch.ones(H, dtype=torch.float32, device=device), requires_grad=False)
         self.post_norm = nn.Parameter(torch.ones(H, dtype=torch.float32, device=device), requires_grad=False)
+        for name in ("q_norm", "k_norm"):
+            w = nn.Parameter(torch.ones(D, dtype=torch.float32, device=device), requires_grad=False) if qk_norm else None
+            self.register_parameter(name, w)
 
-    def projections(self) -> List[Fp4Linear]:
+    def projections(self) -> List[nn.Module]:
         return [self.qkv, self.o, self.gate_up, self.down]
 
 
@@ -86,31 +96,64 @@ class PagedDecoder(nn.Module):
     each slot's accumulated attention weight and position. max_position: the
     rotary tables' rows, tokens that a sequence can have in all; max_len by
     default, and LONG (33 MB of tables for heads of 128) with a budget, under
-    which sequences go on beyond max_len."""
+    which sequences go on beyond max_len.
+
+    format: "nvfp4", "mxfp4" or "int8". cache_dtype: the cache's type, bf16, or int8 or
+    float8_e4m3fn (not with a budget: such a cache evicts nothing). qk_norm: norms of
+    each query and key head in front of the rotation. pages: pages that the sequences
+    share, each taking them as it grows (None: every sequence has its own for max_len
+    tokens; not with a budget)."""
 
     LONG = 65536
 
     def __init__(self, cfg: DecoderConfig, device, format: str = "nvfp4", max_batch: int = 1, max_len: int = 2048,
-                 page_size: int = 64, max_position: Optional[int] = None, budget: Optional[int] = None, recent: int = 0):
+                 page_size: int = 64, max_position: Optional[int] = None, budget: Optional[int] = None, recent: int = 0,
+                 cache_dtype: torch.dtype = torch.bfloat16, qk_norm: bool = False, pages: Optional[int] = None):
         super().__init__()
         self.cfg, self.device = cfg, torch.device(device)
         self.budget, self.recent = budget, recent
         if budget is not None and not 0 <= recent <= budget < max_len:
             raise ValueError(f"recent <= budget < max_len is needed, got {recent}, {budget}, {max_len}")
+        self.packed = pages is not None or cache_dtype != torch.bfloat16
+        if self.packed and budget is not None:
+            raise ValueError("a budget needs a cache of bf16 and pages of each sequence's own")
         H, D = cfg.hidden, cfg.head_dim
         g = torch.Generator(device=self.device).manual_seed(cfg.seed + 7)
         self.embed = (torch.randn(cfg.vocab, H, generator=g, device=self.device) * 0.02).to(torch.bfloat16)
         self.lm_head = (torch.randn(cfg.vocab, H, generator=g, device=self.device) * 0.02).to(torch.bfloat16)
         self.final_norm = torch.ones(H, dtype=torch.float32, device=self.device)
-        self.layers = nn.ModuleList(PagedDecoderLayer(cfg, i, format, self.device) for i in range(cfg.n_layers))
+        self.layers = nn.ModuleList(PagedDecoderLayer(cfg, i, format, self.device, qk_norm) for i in range(cfg.n_layers))
         positions = max_position or (max_len if budget is None else max(max_len, self.LONG))
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, D, 2, device=self.device, dtype=torch.float32) / D))
         ang = torch.outer(torch.arange(positions, device=self.device, dtype=torch.float32), inv)
         self.rope_cos, self.rope_sin = ang.cos(), ang.sin()
-        self.caches = [PagedKVCache.allocate(max_batch, cfg.n_kv_heads, D, max_len, page_size, device=self.device,
-                                             track=budget is not None) for _ in range(cfg.n_layers)]
+        self.pages = pages
+        if self.packed:
+            self._share_pages(max_batch, max_len, page_size, cache_dtype)
+        else:
+            self.caches = [PagedKVCache.allocate(max_batch, cfg.n_kv_heads, D, max_len, page_size, device=self.device,
+                                                 track=budget is not None) for _ in range(cfg.n_layers)]
         self.positions = torch.zeros(max_batch, dtype=torch.int64, device=self.device)   # of the next token
         self._tokens: List[Optional[int]] = [0] * max_batch   # the same as the host counts them; None: dropped
+
+    def _share_pages(self, batch: int, max_len: int, page_size: int, dtype: torch.dtype) -> None:
+        """Caches of all layers with one page table and one count of tokens."""
+        cfg, per = self.cfg, -(-max_len // page_size)
+        table = torch.full((batch, per), -1, dtype=torch.int32, device=self.device)
+        self.pool = PagePool.allocate(self.pages or 0, self.device)
+        if self.pages is None:
+            table.copy_(torch.arange(batch * per, device=self.device).view(batch, per))
+        lens = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        shape = (batch * per if self.pages is None else self.pages, cfg.n_kv_heads, page_size, cfg.head_dim)
+        self.caches = []
+        for _ in range(cfg.n_layers):
+            k, v = (torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2))
+            if dtype == torch.bfloat16:
+                self.caches.append(PagedKVCache(k, v, table, lens))
+                continue
+            block = 16                                       # tokens that share a scale: 4 bytes to 16 * head_dim
+            ks, vs = (torch.ones(*shape[:2], page_size // block, dtype=torch.float32, device=self.device) for _ in range(2))
+            self.caches.append(PagedKVCache8(k, v, ks, vs, table, lens))
 
     def packed_nbytes(self) -> int:
         """Bytes of the projections' weights."""
@@ -124,23 +167,43 @@ class PagedDecoder(nn.Module):
 
     @property
     def steps_left(self) -> int:
-        """Decode steps until a sequence has no place for its token."""
-        return self.longest_sequence - max((n for n in self._tokens if n is not None), default=0)
+        """Decode steps until a sequence has no place for its token: no rotary row, no slot or no page."""
+        tokens = [n for n in self._tokens if n is not None]
+        steps = self.longest_sequence - max(tokens, default=0)
+        if self.pages is not None:
+            least, most = 0, steps                           # pages are enough for `least` steps
+            while least < most:
+                mid = (least + most + 1) // 2
+                if self._pages_for(n + mid for n in tokens) <= self.pages:
+                    least = mid
+                else:
+                    most = mid - 1
+            steps = least
+        return steps
+
+    def _pages_for(self, lens) -> int:
+        return sum(-(-n // self.caches[0].page_size) for n in lens)
 
     def count_steps(self, n: int = 1) -> None:
         """Count n decode steps (negative: steps that the program took back);
         raises if fewer are left. `decode_step` does it by itself, except while
         it is captured: a program that replays a captured step counts each replay."""
         if n > self.steps_left:
+            if self.pages is not None and n <= self.longest_sequence - max(t for t in self._tokens if t is not None):
+                raise RuntimeError(f"{n} decode steps, but {self.pages} pages hold {self.steps_left} (see pages and drop)")
             raise RuntimeError(f"{n} decode steps, but a sequence has {self.longest_sequence - self.steps_left} of "
                                f"{self.longest_sequence} tokens (see max_position, max_len and drop)")
         self._tokens = [None if t is None else t + n for t in self._tokens]
 
     def drop(self, sequence: int) -> None:
         """Take a sequence out of the steps that follow, until the next
-        prefill: it no longer counts, its cache is empty and its logits mean
-        nothing."""
+        prefill: it no longer counts, its cache is empty, its pages are the
+        others' and its logits mean nothing."""
         self._tokens[sequence] = None
+        if self.pages is not None:
+            keep = torch.full_like(self.caches[0].seq_lens, -1)
+            keep[sequence] = 0
+            paged_release(self.pool, self.caches[0], keep)
         for cache in self.caches:
             cache.seq_lens[sequence] = -1
 
@@ -165,6 +228,10 @@ class PagedDecoder(nn.Module):
         most = min(self.caches[0].capacity, self.rope_cos.shape[0])
         if B != self.positions.shape[0] or min(lens) < 1 or max(lens) > most:
             raise ValueError(f"{self.positions.shape[0]} prompts of 1 to {most} tokens are needed")
+        if self.pages is not None and self._pages_for(lens) > self.pages:
+            raise ValueError(f"the prompts take {self._pages_for(lens)} pages of {self.pages}")
+        if self.packed:
+            return self._prefill_packed(prompts, lens, return_logits)
         T = max(lens)
         self._tokens = list(lens)
         tokens = torch.zeros(B, T, dtype=torch.long, device=self.device)
@@ -181,11 +248,20 @@ class PagedDecoder(nn.Module):
 
         for layer, cache in zip(self.layers, self.caches):
             x = _rms_norm(h, layer.input_norm, cfg.rms_eps)
-            q, k, v = layer.qkv(x).view(B, T, -1, D).split([cfg.n_heads, cfg.n_kv_heads, cfg.n_kv_heads], dim=2)
-            rq, rk = rope(q), rope(k)
+            qkv, heads = layer.qkv(x), [cfg.n_heads, cfg.n_kv_heads, cfg.n_kv_heads]
             cache.seq_lens.zero_()
-            paged_append(k, v, cache, self.positions, self.rope_cos, self.rope_sin, n_new=n_new,
-                         scores=_prompt_weights(rq, rk, lens) if self.budget is not None else None)
+            if layer.q_norm is not None:
+                where = torch.arange(T, device=self.device).repeat(B)
+                qkv = qk_norm_rope(qkv.view(B * T, -1), *heads[:2], layer.q_norm, layer.k_norm, where, self.rope_cos,
+                                   self.rope_sin, cfg.rms_eps)
+                rq, rk, v = qkv.view(B, T, -1, D).split(heads, dim=2)
+                paged_append(rk, v, cache, self.positions, n_new=n_new,
+                             scores=_prompt_weights(rq, rk, lens) if self.budget is not None else None)
+            else:
+                q, k, v = qkv.view(B, T, -1, D).split(heads, dim=2)
+                rq, rk = rope(q), rope(k)
+                paged_append(k, v, cache, self.positions, self.rope_cos, self.rope_sin, n_new=n_new,
+                             scores=_prompt_weights(rq, rk, lens) if self.budget is not None else None)
             cache.seq_lens.copy_(n_new)
             self._evict(cache)
             # padding stands behind a prompt's tokens: causal attention never looks at it
@@ -196,17 +272,50 @@ class PagedDecoder(nn.Module):
         logits = self._logits(h[torch.arange(B, device=self.device), n_new.long() - 1])
         return logits if return_logits else logits.argmax(dim=-1)
 
+    def _prefill_packed(self, prompts: Sequence[torch.Tensor], lens: List[int], return_logits: bool) -> torch.Tensor:
+        """Prefill of prompts one behind the other, without padding, into caches
+        that share their pages."""
+        cfg, D, cache0 = self.cfg, self.cfg.head_dim, self.caches[0]
+        self._tokens = list(lens)
+        n_new = torch.tensor(lens, dtype=torch.int32, device=self.device)
+        if self.pages is not None:
+            paged_release(self.pool, cache0, torch.zeros_like(n_new))
+        cache0.seq_lens.zero_()
+        got = paged_reserve(self.pool, cache0, n_new, sum(lens))
+        ends = torch.tensor(lens).cumsum(0)
+        h = self.embed[torch.cat([p.to(self.device) for p in prompts])].float()
+        n_q, n_kv = cfg.n_heads, cfg.n_kv_heads
+        for layer, cache in zip(self.layers, self.caches):
+            qkv = layer.qkv(_rms_norm(h, layer.input_norm, cfg.rms_eps))
+            args = (qkv, n_q, n_kv, layer.q_norm, layer.k_norm, got.positions, self.rope_cos, self.rope_sin, cfg.rms_eps)
+            if isinstance(cache, PagedKVCache8):
+                qkv = qk_norm_rope(*args, out=qkv)
+            else:
+                qkv = qk_norm_rope(*args, out=qkv, cache=cache, slots=got.slots)
+            q, k, v = qkv.view(-1, n_q + 2 * n_kv, D).split([n_q, n_kv, n_kv], dim=1)
+            if isinstance(cache, PagedKVCache8):
+                paged_append(k, v, cache, n_new=got.granted, offsets=got.offsets)
+            a = torch.empty_like(q)
+            for end, n in zip(ends.tolist(), lens):
+                part = [x[end - n:end].transpose(0, 1)[None] for x in (q, k, v)]
+                a[end - n:end] = F.scaled_dot_product_attention(*part, is_causal=True, enable_gqa=True)[0].transpose(0, 1)
+            h = self._mlp(layer, h + layer.o(a.reshape(-1, n_q * D)))
+        cache0.advance(got.granted)                          # of all layers
+        self.positions.copy_(n_new)
+        logits = self._logits(h[ends.to(self.device) - 1])
+        return logits if return_logits else logits.argmax(dim=-1)
+
     @torch.no_grad()
     def calibrate(self, prompts: Sequence[torch.Tensor]) -> None:
         """Set the projections' input scales (nvfp4; mxfp4 has none) from a
         prefill of sample prompts, each from what it is given behind the
-        projections already set. They are 1 before: a block whose largest value
+        projections already set ("int8" finds its scales as it goes: nothing to set). They are 1 before: a block whose largest value
         is below 6 * 2^-6 then has a scale below E4M3's normal range, and its values
         up to three bits less. The caches are left as after `prefill`."""
         keep = torch.arange(max(map(len, prompts), default=0)) < torch.tensor([len(p) for p in prompts])[:, None]
         keep = keep.to(self.device)                      # (not the padding)
-        hooks = [p.register_forward_pre_hook(lambda proj, args: proj.calibrate(args[0][keep]))
-                 for layer in self.layers for p in layer.projections()]
+        hooks = [p.register_forward_pre_hook(lambda proj, args: proj.calibrate(args[0] if self.packed else args[0][keep]))
+                 for layer in self.layers for p in layer.projections() if isinstance(p, Fp4Linear)]
         try:
             self.prefill(prompts)
         finally:
@@ -223,14 +332,24 @@ class PagedDecoder(nn.Module):
             self.count_steps(-1)                         # nothing runs yet
         # which sequences' caches take the token: all but the dropped ones, and those of uncounted replays
         taken = ((self.positions < self.longest_sequence) & (self.caches[0].seq_lens >= 0)).to(torch.int32)
+        if self.packed:
+            # pages for the tokens; a sequence that gets none (in replays that nobody counts) stays as it is
+            taken = paged_reserve(self.pool, self.caches[0], taken, 0).granted
         h = self.embed[tokens].float()
         for layer, cache in zip(self.layers, self.caches):
             qkv = layer.qkv(_rms_norm(h, layer.input_norm, self.cfg.rms_eps))
-            a = paged_decode_attention(qkv, self.cfg.n_heads, cache, self.positions, self.rope_cos, self.rope_sin,
-                                       accumulate=self.budget is not None)
-            cache.advance(taken)
-            self._evict(cache)
+            rope = (self.rope_cos, self.rope_sin)
+            if layer.q_norm is not None:
+                qkv = qk_norm_rope(qkv, self.cfg.n_heads, self.cfg.n_kv_heads, layer.q_norm, layer.k_norm, self.positions, *rope,
+                                   self.cfg.rms_eps, out=qkv)
+                rope = (None, None)
+            a = paged_decode_attention(qkv, self.cfg.n_heads, cache, self.positions, *rope, accumulate=self.budget is not None)
+            if not self.packed:
+                cache.advance(taken)
+                self._evict(cache)
             h = self._mlp(layer, h + layer.o(a))
+        if self.packed:
+            self.caches[0].advance(taken)                    # of all layers
         self.positions.add_(1)
         logits = self._logits(h)
         return logits if return_logits else logits.argmax(dim=-1)
