@@ -3,9 +3,10 @@
 //   s_t = scale q . (a_t k_t),   p = softmax(s),   o = sum_t p_t (b_t v_t)
 //
 // over the cached slots t, a_t and b_t the scales of t's block. The scales stay
-// outside the products: codes become fp16 exactly (integers up to 127, e4m3), q is
-// exact in fp16 once its head's power of two is taken out, and a score is the product of
-// the fp32 sum with a_t. A weight enters the second product as p_t b_t over a power
+// outside the products. Scores of integers are sums of products of bytes, q being three
+// bytes of 24 bits (a head's power of two taken out), exact up to the last addition; those of
+// e4m3 (and of wide groups, for registers) take the codes as fp16, exactly, and q as
+// fp16 without its power of two. A score is the product of the sum with a_t. A weight enters the second product as p_t b_t over a power
 // of two that is at least every b_t so far (the output is scaled along when it
 // grows, as for the running maximum), in fp16: one term where the result is bf16,
 // whose own rounding is eight times larger, two where it is fp16.
@@ -22,11 +23,13 @@
 // maximum follows only when a score passes it by 2^4, found by one vote, so that
 // a tile usually needs no shuffles.
 //
-// The work is cut as in the 16-bit kernel (paged_split.cuh). Each warp streams tiles of
-// 16 slots through its own ring of stages, two TMA boxes (k, v) a tile, issued
-// by one lane and complete on the stage's barrier: no CTA barrier in the loop.
-// Lane i of a warp looks up page and scales of its tile 32 j + i, three batches deep. Every
-// wait is bounded; a warp whose wait runs out records it and stops.
+// The work is cut as in the 16-bit kernel (paged_split.cuh), in units of 128 slots, 32
+// of each to a warp, which streams them through its own ring of stages: a TMA
+// box each of k and v (two of 16 slots where pages are no multiple of 32), issued by
+// one lane and complete on the stage's barrier, no CTA barrier in the loop. (Copies of 16 slots
+// alone reach 5.1 TB/s where those of 32 reach 5.5.) Lane i of a warp looks up page and
+// scales of its tile 32 j + i, three batches deep. Every wait is bounded; a warp whose
+// wait runs out records it and stops.
 #include <algorithm>
 
 #include "gemm.cuh"
@@ -43,9 +46,7 @@ using paged::kCounterBytes;
 using paged::kCounters;
 using paged::kMaxPieces;
 using paged::kRowCost;
-using paged::kRows;
 using paged::kThreads;
-using paged::kUnit;
 using paged::kWarps;
 using paged::ldsm4;
 using paged::ldsm4t;
@@ -58,6 +59,9 @@ using paged::unpack2;
 
 __device__ int g_err;
 
+constexpr int kRows = 16;                  // slots of a tile, an MMA's rows
+constexpr int kPair = 2 * kRows;           // slots of a stage: two tiles
+constexpr int kUnit = kWarps * kPair;      // slots of a unit
 constexpr float kSlack = 4.f;              // log2 by which a weight may pass 1 before the maximum follows
 constexpr float kShift = 11.f;             // weights are 2^kShift times: at most 2^15, in fp16 down to 2^-35 times
 
@@ -77,6 +81,7 @@ struct AttnArgs {
   int* counters;
   float* partials;       // [grid][2][heads of a tile][D + 2]: the heads' rows, each with its max and sum
   int page_shift;        // log2(page_size), or -1
+  int whole_pairs;       // page_size % 32 == 0: both tiles of a stage share a page
   uint64_t wait_ns;
   int stall;             // test hook: nothing is loaded
 };
@@ -124,36 +129,55 @@ __device__ __forceinline__ void to_half(uint32_t w, uint32_t& x, uint32_t& y) {
   }
 }
 
-// Shared memory of a block: the warps' rings [kWarps][S][K, V][DP / kBox][16 rows][kBox],
-// their barriers, the query tile [heads][DP + 8] fp16, the heads' powers of two, and
-// the prefix sums of the sequences' units with their lengths.
-template <int DP>
-struct Ring {
-  static constexpr int kBox = DP < 128 ? DP : 128;              // columns of a TMA box
-  static constexpr int kHalf = kRows * DP;                      // bytes of a tile's K (or V)
-  static constexpr int kStage = 2 * kHalf;
-  static constexpr int S = DP == 64 ? 8 : DP == 128 ? 6 : 5;
-  static constexpr size_t kBytes = (size_t)kWarps * S * kStage;
-  static constexpr int kCtas = DP == 64 ? 3 : DP == 128 ? 2 : 1;
-};
+// Shared memory of a block: the warps' rings [kWarps][S][K, V][boxes][32 rows][kBox], their
+// barriers, the query tile ([heads][DP + 8] fp16, or three planes of bytes [heads][DP + 16]),
+// the heads' powers of two, and the prefix sums of the sequences' units with their lengths.
+//
+// DP: columns that are computed, head_dim rounded up (the copies fill the rest of a
+// box with zeros). Blocks per SM: as many as the registers allow, which hides more of a
+// tile's chain of latencies than longer rings do.
 template <int DP, int NT>
+struct Ring {
+  static constexpr int kCols = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;   // columns in shared memory
+  static constexpr int kBox = kCols < 128 ? kCols : 128;        // columns of a TMA box
+  static constexpr int kHalf = kPair * kCols;                   // bytes of a stage's K (or V)
+  static constexpr int kStage = 2 * kHalf;
+  static constexpr int S = kCols == 64 ? 6 : 3;
+  static constexpr size_t kBytes = (size_t)kWarps * S * kStage;
+  static constexpr int kCtas = kCols == 256 ? 1 : 2;
+};
+template <bool E4M3, int DP, int NT>
+constexpr bool int_scores() { return !E4M3 && DP * NT <= 128; }
+template <bool E4M3, int DP, int NT>
+constexpr size_t q_bytes() { return int_scores<E4M3, DP, NT>() ? 3 * 8 * NT * (DP + 16) : 8 * NT * (DP + 8) * 2; }
+template <bool E4M3, int DP, int NT>
 constexpr size_t attn_smem(int batch) {
-  return 1024 + Ring<DP>::kBytes + kWarps * Ring<DP>::S * 8 + 8 * NT * (DP + 8) * 2 + 8 * NT * 4 + (size_t)(2 * batch + 1) * 4;
+  return 1024 + Ring<DP, NT>::kBytes + kWarps * Ring<DP, NT>::S * 8 + q_bytes<E4M3, DP, NT>() + 8 * NT * 4 +
+         (size_t)(2 * batch + 1) * 4;
+}
+
+// 16 x 8 sums of 32 products of bytes.
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 template <bool BF, bool E4M3, int DP, int NT>
-__global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
+__global__ void __launch_bounds__(kThreads, Ring<DP, NT>::kCtas)
     paged8_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnArgs a) {
-  using P = Ring<DP>;
+  using P = Ring<DP, NT>;
+  constexpr bool kInt = int_scores<E4M3, DP, NT>();
   constexpr int S = P::S;
-  constexpr int kHeads = 8 * NT;                 // query heads of a tile
+  constexpr int kHeads = 8 * NT;                 // query heads of a tile: a multiple of kWarps
   constexpr int kBlocks = DP / 16;               // steps of 16 columns
   constexpr int kQPitch = DP + 8;
   extern __shared__ char smem_raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P::kBytes);                       // [kWarps][S]
   uint16_t* qs = reinterpret_cast<uint16_t*>(bars + kWarps * S);                        // [kHeads][kQPitch]
-  float* q_pow = reinterpret_cast<float*>(qs + kHeads * kQPitch);                       // [kHeads]
+  char* q8 = reinterpret_cast<char*>(qs);                                               // [3][kHeads][DP + 16]
+  float* q_pow = reinterpret_cast<float*>(q8 + q_bytes<E4M3, DP, NT>());                // [kHeads]
   int* prefix = reinterpret_cast<int*>(q_pow + kHeads);                                 // [batch + 1]
   __shared__ uint64_t warp_sums[kWarps];
   __shared__ int warp_most[kWarps];
@@ -162,7 +186,6 @@ __global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
   int* lens = prefix + c.batch + 1;                                                     // [batch]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int D = c.head_dim, rows_per_b = c.n_kv * a.head_tiles;
-  const int groups = (D + 31) / 32;              // pairs of 16-column steps
 
   if (tid == 0) {
     prefetch_tensormap(&kmap);
@@ -206,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
     // How the units are dealt out: a row of n units counts n + front, or, with
     // front < 0, -front whatever n is.
     const unsigned units = (unsigned)(uint32_t)all * rows_per_b, rows = (unsigned)(all >> 32) * rows_per_b;
-    deal = choose_deal(units, rows, longest, gridDim.x, min(a.group, kHeads), 1000);
+    deal = choose_deal(units, rows, longest, gridDim.x, min(a.group, kHeads));
     int v = 0;
     if (deal.front >= 0) v = (int)(uint32_t)at + deal.front * (int)(at >> 32);
     else v = -deal.front * (int)(at >> 32);
@@ -218,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
     if (b1 == c.batch && b0 < b1) prefix[c.batch] = v;
   }
   // query columns and heads that nothing fills: zeros, so that their scores are finite
-  for (int i = tid; i < kHeads * kQPitch / 2; i += kThreads) reinterpret_cast<uint32_t*>(qs)[i] = 0;
+  for (int i = tid; i < (int)q_bytes<E4M3, DP, NT>() / 4; i += kThreads) reinterpret_cast<uint32_t*>(qs)[i] = 0;
   if (tid < kHeads) q_pow[tid] = 0.f;
   __syncthreads();
   pdl_wait_primary();                                    // (the kernel that stores the new token)
@@ -266,18 +289,21 @@ __global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
     const int n = slots_of(a, lens[b]);
     const int32_t* table = c.table + b * c.table_stride;
 
-    // Tile j of this warp: slots t0 * 64 + warp * 16 + 64 j on. Lane i holds page and
-    // scales of tile i of the current batch of 32 (pg, ka, va) and of the next
-    // one (pg1, ...), and the pages of the one after that.
-    const int slot_base = t0 * kUnit + warp * kRows, tiles = min(t1 - t0, (n - slot_base + kUnit - 1) / kUnit);
+    // Stage k of this warp: slots t0 * 128 + warp * 32 + 128 k on, tiles 2 k and 2 k + 1. Lane i
+    // holds page and scales of tile i of the current batch of 32 (pg, ka, va) and of
+    // the next one (pg1, ...), and the pages of the one after that.
+    const int slot_base = t0 * kUnit + warp * kPair;
+    const int stages = min(t1 - t0, (n - slot_base + kUnit - 1) / kUnit);
+    auto slot_of_tile = [&](int j) { return slot_base + (j >> 1) * kUnit + (j & 1) * kRows; };
     auto page_of_tile = [&](int j) {
-      const int p = j < tiles ? table[page_index(a, slot_base + j * kUnit)] : -1;
+      const int slot = slot_of_tile(j);
+      const int p = j < 2 * stages && slot < n ? table[page_index(a, slot)] : -1;
       return (unsigned)p < (unsigned)c.num_pages ? p : -1;
     };
     auto scales_of_tile = [&](int j, int page, float& ka, float& va) {
       ka = va = 0.f;
       if (page >= 0) {
-        const int slot = slot_base + j * kUnit;
+        const int slot = slot_of_tile(j);
         const int64_t at = scale_at(c, page, h, (slot - page_index(a, slot) * c.page_size) / c.block);
         ka = c.k_scales[at];
         va = c.v_scales[at];
@@ -286,83 +312,145 @@ __global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
     int pg = page_of_tile(lane), pg1 = page_of_tile(32 + lane), pg2;
     float ka, va, ka1, va1;
 
-    // the tile's rotated query heads
+    // What the segment needs first is loaded before the copies, behind which it would wait: the
+    // position, the rotation, the query heads (each by a warp: elements j and j + D / 2).
     const bool turn = a.cos_t != nullptr;
     const int64_t pos_in = a.positions != nullptr ? a.positions[b] : lens[b];
+    constexpr int kPer = (DP / 2 + 31) / 32, kOwn = kHeads / kWarps;
+    uint32_t qx[kOwn][kPer];
+#pragma unroll
+    for (int w = 0; w < kOwn; ++w) {
+      const int g = warp + w * kWarps;
+      const uint16_t* qr = a.q + b * a.q_stride + (int64_t)(head0 + g) * D;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int j = lane + 32 * i;
+        qx[w][i] = g < heads && j < D / 2 ? (uint32_t)qr[j] | ((uint32_t)qr[j + D / 2] << 16) : 0;
+      }
+    }
     bool ok = !turn || (pos_in >= 0 && pos_in < a.rope_rows);
     if (a.extra) {
       // (a new token without a page answers with zeros)
       const int p = table[page_index(a, lens[b])];
       ok = ok && (unsigned)p < (unsigned)c.num_pages;
     }
-    const int64_t pos = ok ? pos_in : 0;
-
-    auto issue = [&](int j, int stage, int page) {
-      if (page < 0 || a.stall || broken) return;
-      if (elect_one()) {
-        const int slot = slot_base + j * kUnit, off = slot - page_index(a, slot) * c.page_size;
-        const uint32_t dst = ring_u + stage * P::kStage;
-        mbar_arrive_expect_tx(bar + stage, P::kStage);
+    float2 rot[kPer];
+    if (turn) {
+      const int64_t at = (ok ? pos_in : 0) * (D / 2);
 #pragma unroll
-        for (int x = 0; x < DP / P::kBox; ++x) {
-          tma_load_4d(dst + x * kRows * P::kBox, &kmap, x * P::kBox, off, h, page, bar + stage);
-          tma_load_4d(dst + P::kHalf + x * kRows * P::kBox, &vmap, x * P::kBox, off, h, page, bar + stage);
+      for (int i = 0; i < kPer; ++i) {
+        const int j = min(lane + 32 * i, D / 2 - 1);
+        rot[i] = make_float2(a.cos_t[at + j], a.sin_t[at + j]);
+      }
+    }
+    scales_of_tile(lane, pg, ka, va);
+
+    // Copies stage k to place `at` of the ring, tiles with a page; their bytes complete on its barrier.
+    auto issue = [&](int k, int at, int page0, int page1) {
+      if ((page0 < 0 && page1 < 0) || a.stall || broken) return;
+      if (elect_one()) {
+        const int slot = slot_of_tile(2 * k), i = page_index(a, slot), off = slot - i * c.page_size;
+        const uint32_t dst = ring_u + at * P::kStage;
+        if (a.whole_pairs) {                             // both tiles lie in one page
+          mbar_arrive_expect_tx(bar + at, P::kStage);
+#pragma unroll
+          for (int x = 0; x < P::kCols / P::kBox; ++x) {
+            tma_load_4d(dst + x * kPair * P::kBox, &kmap, x * P::kBox, off, h, page0, bar + at);
+            tma_load_4d(dst + P::kHalf + x * kPair * P::kBox, &vmap, x * P::kBox, off, h, page0, bar + at);
+          }
+        } else {
+          mbar_arrive_expect_tx(bar + at, (page0 >= 0 && page1 >= 0 ? 1 : 0) * (P::kStage / 2) + P::kStage / 2);
+          const int off1 = off + kRows < c.page_size ? off + kRows : 0;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int page = e == 0 ? page0 : page1, o = e == 0 ? off : off1;
+            if (page < 0) continue;
+#pragma unroll
+            for (int x = 0; x < P::kCols / P::kBox; ++x) {
+              const uint32_t d = dst + (x * kPair + e * kRows) * P::kBox;
+              tma_load_4d(d, &kmap, x * P::kBox, o, h, page, bar + at);
+              tma_load_4d(d + P::kHalf, &vmap, x * P::kBox, o, h, page, bar + at);
+            }
+          }
         }
       }
       __syncwarp();
     };
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) issue(s, s, __shfl_sync(0xffffffffu, pg, s));
-    scales_of_tile(lane, pg, ka, va);
+    for (int k = 0; k < S; ++k)
+      issue(k, k, __shfl_sync(0xffffffffu, pg, 2 * k), __shfl_sync(0xffffffffu, pg, 2 * k + 1));
     scales_of_tile(32 + lane, pg1, ka1, va1);
     pg2 = page_of_tile(64 + lane);
 
-    // Each head by a warp: rotated, rounded to its type as a cached query would be,
-    // the power of two of its largest magnitude taken out, in fp16.
-    for (int g = warp; g < heads; g += kWarps) {
-      const uint16_t* qr = a.q + b * a.q_stride + (int64_t)(head0 + g) * D;
-      constexpr int kPer = (DP / 2 + 31) / 32;
-      uint32_t x[kPer];                                // elements j and j + D / 2
+    // Each head by a warp: rotated and rounded to its type, then either in fp16 with the
+    // power of two of its largest magnitude taken out, or as an integer of 2^21
+    // times that, in three signed bytes (24 bits under the largest magnitude).
+#pragma unroll
+    for (int w = 0; w < kOwn; ++w) {
+      const int g = warp + w * kWarps;
+      if (g >= heads) break;
+      uint32_t* x = qx[w];
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int j = lane + 32 * i;
-        x[i] = 0;
-        if (j < D / 2) {
-          x[i] = (uint32_t)qr[j] | ((uint32_t)qr[j + D / 2] << 16);
-          if (turn) {
-            const float2 f = unpack2<BF>(x[i]);
-            const float2 y = rotate(f.x, f.y, a.cos_t[pos * (D / 2) + j], a.sin_t[pos * (D / 2) + j]);
-            x[i] = pack2<BF>(y.x, y.y);
-          }
+        if (turn) {
+          const float2 f = unpack2<BF>(x[i]);
+          const float2 y = rotate(f.x, f.y, rot[i].x, rot[i].y);
+          x[i] = lane + 32 * i < D / 2 ? pack2<BF>(y.x, y.y) : 0;
         }
         top = __vmaxu2(top, x[i] & 0x7FFF7FFFu);
       }
       top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
-      // 2^e of the largest magnitude (infinities and NaN make their own way); 2^-e is its inverse
-      const uint32_t e = min(max(__float_as_uint(unpack2<BF>(top).x) >> 23, 20u), 234u);
+      const uint32_t e = min(max(__float_as_uint(unpack2<BF>(top).x) >> 23, 20u), 253u);
       const float down = __uint_as_float((254u - e) << 23);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int j = lane + 32 * i;
         if (j < D / 2) {
           const float2 f = unpack2<BF>(x[i]);
-          const uint32_t w = pack2<false>(f.x * down, f.y * down);
-          qs[g * kQPitch + j] = (uint16_t)w;
-          qs[g * kQPitch + j + D / 2] = (uint16_t)(w >> 16);
+          if constexpr (kInt) {
+            auto put = [&](float y, int at) {
+              const int v = max(-8355711, min(8355711, __float2int_rn(y * down * 2097152.f)));   // (the largest three bytes)
+              const int b0 = (int8_t)v, v1 = (v - b0) >> 8, b1 = (int8_t)v1;
+              char* p = q8 + g * (DP + 16) + at;
+              p[0] = (char)b0;
+              p[kHeads * (DP + 16)] = (char)b1;
+              p[2 * kHeads * (DP + 16)] = (char)((v1 - b1) >> 8);
+            };
+            put(f.x, j);
+            put(f.y, j + D / 2);
+          } else {
+            const uint32_t w = pack2<false>(f.x * down, f.y * down);
+            qs[g * kQPitch + j] = (uint16_t)w;
+            qs[g * kQPitch + j + D / 2] = (uint16_t)(w >> 16);
+          }
         }
       }
-      if (lane == 0) q_pow[g] = __uint_as_float(e << 23);
+      // (a head with an infinity or a NaN has no scores)
+      const float unit = kInt ? 4.76837158203125e-7f : 1.f;     // 2^-21
+      if (lane == 0) q_pow[g] = top < (BF ? 0x7F80u : 0x7C00u) ? __uint_as_float(e << 23) * unit : __uint_as_float(0x7FC00000u);
     }
     __syncthreads();
-    // operand registers of q: columns 4 i .. 4 i + 3 of every 16 of head lane / 4
-    uint2 qf[kBlocks][NT];
+    // operand registers of q, of head lane / 4: columns 4 i .. 4 i + 3 of every 16 (fp16); or 4 i .. and
+    // 16 + 4 i .. of every 32, for each plane of bytes
+    uint2 qf[kInt ? 3 * kBlocks / 2 : kBlocks][NT];
     float f[NT][2];                                    // scale and power of two of this thread's heads
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      if constexpr (kInt) {
 #pragma unroll
-      for (int s = 0; s < kBlocks; ++s)
-        qf[s][t] = *reinterpret_cast<const uint2*>(qs + (8 * t + (lane >> 2)) * kQPitch + 16 * s + 4 * (lane & 3));
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+          for (int s = 0; s < kBlocks / 2; ++s) {
+            const char* src = q8 + (p * kHeads + 8 * t + (lane >> 2)) * (DP + 16) + 32 * s + 4 * (lane & 3);
+            qf[p * (kBlocks / 2) + s][t] =
+                make_uint2(*reinterpret_cast<const uint32_t*>(src), *reinterpret_cast<const uint32_t*>(src + 16));
+          }
+      } else {
+#pragma unroll
+        for (int s = 0; s < kBlocks; ++s)
+          qf[s][t] = *reinterpret_cast<const uint2*>(qs + (8 * t + (lane >> 2)) * kQPitch + 16 * s + 4 * (lane & 3));
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) f[t][e] = q_pow[8 * t + 2 * (lane & 3) + e] * a.scale2;
     }
@@ -384,77 +472,77 @@ __global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
     float v_pow = 0.f, v_inv = 0.f;                    // the power of two over the values' scales, and its inverse
 
     const int g8 = lane >> 2;
-    int stage = 0;
-    for (int j = 0; j < tiles && !broken; ++j) {
-      const int i = j & 31;
-      if (i == 0 && j > 0) {
-        pg = pg1; ka = ka1; va = va1;
-        pg1 = pg2;
-        scales_of_tile(j + 32 + lane, pg1, ka1, va1);
-        pg2 = page_of_tile(j + 64 + lane);
-      }
-      {
-        const int ahead = i + S - 1;
-        const int p = __shfl_sync(0xffffffffu, ahead < 32 ? pg : pg1, ahead & 31);
-        issue(j + S - 1, stage == 0 ? S - 1 : stage - 1, p);
-      }
-      const int page = __shfl_sync(0xffffffffu, pg, i);
-      const float ks = __shfl_sync(0xffffffffu, ka, i), vs = __shfl_sync(0xffffffffu, va, i);
-      const int at = stage;
-      stage = stage + 1 == S ? 0 : stage + 1;
-      if (page < 0) continue;                          // nothing was loaded
-      if (!__all_sync(0xffffffffu, mbar_wait_hint(bar + at, (phases >> at) & 1, &g_err, 61, a.wait_ns))) {
-        broken = true;
-        // (the copies that are on their way land before the block ends)
-        if (!a.stall)
-          for (int k = 0; k < S; ++k) {
-            const int jj = j + k, ss = (at + k) % S;
-            const int pp = jj < tiles ? __shfl_sync(0xffffffffu, i + k < 32 ? pg : pg1, (i + k) & 31) : -1;
-            if (pp >= 0) mbar_wait_hint(bar + ss, (phases >> ss) & 1, nullptr, 0, a.wait_ns);
-          }
-        break;
-      }
+    // Byte (row r, column d) of a box: 16-byte chunk d / 16 is kept at another place of its row,
+    // its number xor r % 8 (of rows of 64 bytes: r / 2 % 4), so that eight rows of a chunk
+    // touch every bank once. This lane's row and chunk of an ldmatrix, whose matrices are (slots 0-7,
+    // chunk 2 s), (8-15, 2 s), (0-7, 2 s + 1), (8-15, 2 s + 1):
+    const uint32_t l_at = (lane & 15) * P::kBox + (((lane >> 4) ^ (P::kBox == 128 ? lane & 7 : (lane >> 1) & 3)) << 4);
+    auto chunks_at = [&](uint32_t base, int s) {       // (tiles start on multiples of their size)
+      return ((base + l_at) ^ ((s << 5) % P::kBox)) + (s << 5) / P::kBox * (kPair * P::kBox);
+    };
+
+    // Waits for the stage at `at`; false if that took too long.
+    auto arrived = [&](int at) {
+      if (!__all_sync(0xffffffffu, mbar_wait_hint(bar + at, (phases >> at) & 1, &g_err, 61, a.wait_ns))) return false;
       phases ^= 1u << at;
-      const uint32_t kb = ring_u + at * P::kStage, vb = kb + P::kHalf;
-      const int live = n - (slot_base + j * kUnit);    // slots of the tile that count
+      return true;
+    };
+
+    // Takes the tile at byte `at` of the ring, whose block has the scales ks, vs and whose first
+    // `live` slots count.
+    auto consume = [&](int at, float ks, float vs, int live) {
+      const uint32_t kb = ring_u + at, vb = kb + P::kHalf;
       if (live < kRows) {
         // values behind the last token may be anything, an e4m3 NaN too, which no weight of 0 hides
-        for (int x = lane; x < (kRows - live) * (DP / 16); x += 32) {
-          const int r = live + x / (DP / 16), ch = x % (DP / 16);
-          *reinterpret_cast<uint4*>(ring + (vb - ring_u) + (ch * 16 / P::kBox) * kRows * P::kBox + r * P::kBox +
-                                    (ch * 16 % P::kBox)) = make_uint4(0, 0, 0, 0);
+        char* v = ring + at + P::kHalf;
+        for (int x = lane; x < (kRows - live) * (P::kCols / 16); x += 32) {
+          const int r = live + x / (P::kCols / 16), ch = x % (P::kCols / 16);
+          *reinterpret_cast<uint4*>(v + (ch * 16 / P::kBox) * kPair * P::kBox + r * P::kBox + (ch * 16 % P::kBox)) =
+              make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __syncwarp();
       }
-      // byte (row r, column d) of a box: 16-byte chunk d / 16 is kept at another place
-      // of its row, so that eight rows of a chunk touch every bank once
-      auto chunk_at = [&](uint32_t base, int r, int ch) {
-        const uint32_t box = base + (ch * 16 / P::kBox) * (kRows * P::kBox) + r * P::kBox;
-        const int cb = ch % (P::kBox / 16);
-        return box + ((P::kBox == 128 ? cb ^ (r & 7) : cb ^ ((r >> 1) & 3)) << 4);
-      };
-
-      // scores of 16 slots x the tile's heads
-      float sc[NT][4];
+      float sc[NT][4];                                 // scores of 16 slots x the tile's heads
+      if constexpr (kInt) {
+        int si[NT][3][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[t][e] = 0.f;
-      // matrices of an ldmatrix: (slots 0-7, chunk 2 s), (8-15, 2 s), (0-7, 2 s + 1), (8-15, 2 s + 1)
-      const int lrow = (lane & 7) + (lane & 8), lch = lane >> 4;
+          for (int p = 0; p < 3; ++p)
 #pragma unroll
-      for (int s = 0; s < kBlocks / 2; ++s) {
-        if (s >= groups) break;
-        uint32_t w[4];
-        ldsm4(chunk_at(kb, lrow, 2 * s + lch), w);
+            for (int e = 0; e < 4; ++e) si[t][p][e] = 0;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t k4[4];
-          to_half<E4M3, false>(w[2 * e], k4[0], k4[2]);
-          to_half<E4M3, false>(w[2 * e + 1], k4[1], k4[3]);
+        for (int s = 0; s < kBlocks / 2; ++s) {
+          uint32_t w[4];
+          ldsm4(chunks_at(kb, s), w);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma<false>(sc[t], k4, qf[2 * s + e][t].x, qf[2 * s + e][t].y);
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int p = 0; p < 3; ++p) mma_s8(si[t][p], w, qf[p * (kBlocks / 2) + s][t].x, qf[p * (kBlocks / 2) + s][t].y);
+        }
+        // (the lower two planes together stay below 2^31)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[t][e] = fmaf((float)si[t][2][e], 65536.f, (float)(si[t][1][e] * 256 + si[t][0][e]));
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[t][e] = 0.f;
+#pragma unroll
+        for (int s = 0; s < kBlocks / 2; ++s) {
+          uint32_t w[4];
+          ldsm4(chunks_at(kb, s), w);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t k4[4];
+            to_half<E4M3, false>(w[2 * e], k4[0], k4[2]);
+            to_half<E4M3, false>(w[2 * e + 1], k4[1], k4[3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma<false>(sc[t], k4, qf[2 * s + e][t].x, qf[2 * s + e][t].y);
+          }
         }
       }
       // in log2 units
@@ -522,12 +610,10 @@ __global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
           }
         }
       }
-      // matrices of a transposing ldmatrix: (slots 0-7, chunk 2 s), (8-15, 2 s), (0-7, 2 s + 1), (8-15, 2 s + 1)
 #pragma unroll
       for (int s = 0; s < kBlocks / 2; ++s) {
-        if (s >= groups) break;
         uint32_t w[4];
-        ldsm4t(chunk_at(vb, lrow, 2 * s + lch), w);
+        ldsm4t(chunks_at(vb, s), w);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint32_t v4[4];
@@ -540,7 +626,45 @@ __global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
           }
         }
       }
-      __syncwarp();   // the stage is refilled at the top of the next round
+    };
+
+    int place = 0;
+    for (int k = 0; k < stages && !broken; ++k) {
+      const int i = 2 * k & 31;                        // of the batch
+      if (i == 0 && k > 0) {
+        pg = pg1; ka = ka1; va = va1;
+        pg1 = pg2;
+        scales_of_tile(2 * k + 32 + lane, pg1, ka1, va1);
+        pg2 = page_of_tile(2 * k + 64 + lane);
+      }
+      const int page[2] = {__shfl_sync(0xffffffffu, pg, i), __shfl_sync(0xffffffffu, pg, i + 1)};   // (-1: nothing was loaded)
+      const float ks[2] = {__shfl_sync(0xffffffffu, ka, i), __shfl_sync(0xffffffffu, ka, i + 1)};
+      const float vs[2] = {__shfl_sync(0xffffffffu, va, i), __shfl_sync(0xffffffffu, va, i + 1)};
+      if (page[0] >= 0 || page[1] >= 0) {
+        if (!arrived(place)) {
+          broken = true;
+          // the copies that are on their way land before the block ends
+          if (!a.stall)
+            for (int e = 0; e < S; ++e) {
+              const int x = i + 2 * e, st = (place + e) % S;
+              const int p0 = __shfl_sync(0xffffffffu, x < 32 ? pg : pg1, x & 31), p1 = __shfl_sync(0xffffffffu, x < 32 ? pg : pg1, (x + 1) & 31);
+              if (k + e < stages && (p0 >= 0 || p1 >= 0)) mbar_wait_hint(bar + st, (phases >> st) & 1, nullptr, 0, a.wait_ns);
+            }
+          break;
+        }
+#pragma unroll 1
+        for (int e = 0; e < 2; ++e)
+          if ((e == 0 ? page[0] : page[1]) >= 0)
+            consume(place * P::kStage + e * kRows * P::kBox, e == 0 ? ks[0] : ks[1], e == 0 ? vs[0] : vs[1],
+                    n - slot_of_tile(2 * k + e));
+        __syncwarp();
+      }
+      {
+        const int x = i + 2 * S;
+        issue(k + S, place, __shfl_sync(0xffffffffu, x < 32 ? pg : pg1, x & 31),
+              __shfl_sync(0xffffffffu, x < 32 ? pg : pg1, (x + 1) & 31));
+      }
+      place = place + 1 == S ? 0 : place + 1;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -719,7 +843,9 @@ __global__ void __launch_bounds__(kThreads, Ring<DP>::kCtas)
   }
 }
 
-static size_t grid_of(int head_dim) { return (size_t)sm_count() * (head_dim > 128 ? 1 : head_dim > 64 ? 2 : 3); }
+static size_t grid_of(int head_dim) {
+  return (size_t)sm_count() * (head_dim > 128 ? Ring<256, 1>::kCtas : Ring<128, 1>::kCtas);
+}
 
 static size_t workspace_bytes_of(int head_dim) {
   return kCounterBytes + grid_of(head_dim) * 2 * 16 * (head_dim + 2) * 4;
@@ -730,7 +856,7 @@ static int encode_map(CUtensorMap* map, const Cache& c, const void* base, int bo
   // (of a dimension of one the stride does not matter, but it has to be a valid one)
   auto stride = [&](int64_t s, int n) { return (uint64_t)(n > 1 ? s : std::max<int64_t>(s, 16)); };
   const uint64_t strides[3] = {stride(c.token_stride, c.page_size), stride(c.head_stride, c.n_kv), stride(c.page_stride, c.num_pages)};
-  const uint32_t boxes[4] = {(uint32_t)box, (uint32_t)kRows, 1, 1};
+  const uint32_t boxes[4] = {(uint32_t)box, (uint32_t)(c.page_size % kPair == 0 ? kPair : kRows), 1, 1};
   return encode_tmap(map, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, dims, strides, boxes,
                      box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
@@ -738,7 +864,7 @@ static int encode_map(CUtensorMap* map, const Cache& c, const void* base, int bo
 template <bool BF, bool E4M3, int DP, int NT>
 static int launch(const AttnArgs& a, int overlap, cudaStream_t st) {
   auto k = paged8_attention_kernel<BF, E4M3, DP, NT>;
-  const size_t smem = attn_smem<DP, NT>(a.c.batch);
+  const size_t smem = attn_smem<E4M3, DP, NT>(a.c.batch);
   // (the same value for all host threads, as for the 16-bit kernel)
   static thread_local int configured_dev = -1;
   static thread_local size_t most = 0;
@@ -753,8 +879,8 @@ static int launch(const AttnArgs& a, int overlap, cudaStream_t st) {
   }
   TS_UNSUPPORTED(smem <= most, "batch too large for the kernel's tables");
   CUtensorMap km, vm;
-  int rc = encode_map(&km, a.c, a.c.k, Ring<DP>::kBox);
-  if (rc == TS_OK) rc = encode_map(&vm, a.c, a.c.v, Ring<DP>::kBox);
+  int rc = encode_map(&km, a.c, a.c.k, Ring<DP, NT>::kBox);
+  if (rc == TS_OK) rc = encode_map(&vm, a.c, a.c.v, Ring<DP, NT>::kBox);
   if (rc != TS_OK) return rc;
   TS_CUDA_TRY(launch_after(k, (int)grid_of(a.c.head_dim), kThreads, smem, st, overlap, 0, km, vm, a));
   TS_LAUNCH_CHECK();
@@ -765,6 +891,7 @@ template <bool BF, bool E4M3>
 static int launch(const AttnArgs& a, int overlap, cudaStream_t st) {
   // one column tile of eight query heads, or two where a group has more
   const bool wide = a.group > 8;
+  if (a.c.head_dim > 64 && a.c.head_dim <= 96) return wide ? launch<BF, E4M3, 96, 2>(a, overlap, st) : launch<BF, E4M3, 96, 1>(a, overlap, st);
   if (a.c.head_dim <= 64) return wide ? launch<BF, E4M3, 64, 2>(a, overlap, st) : launch<BF, E4M3, 64, 1>(a, overlap, st);
   if (a.c.head_dim <= 128) return wide ? launch<BF, E4M3, 128, 2>(a, overlap, st) : launch<BF, E4M3, 128, 1>(a, overlap, st);
   return wide ? launch<BF, E4M3, 256, 2>(a, overlap, st) : launch<BF, E4M3, 256, 1>(a, overlap, st);
@@ -807,6 +934,7 @@ static int make_args(AttnArgs* a, int q_dtype, int n_q, const ts_paged_cache8* c
   a->counters = reinterpret_cast<int*>(workspace);
   a->partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + kCounterBytes);
   a->page_shift = log2_of(a->c.page_size);
+  a->whole_pairs = a->c.page_size % kPair == 0 ? 1 : 0;
   a->wait_ns = wait_limit_ns();
   a->stall = take_test_stall() ? 1 : 0;
   return TS_OK;
