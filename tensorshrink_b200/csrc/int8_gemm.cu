@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
   }
 }
 
-// ---- prefill: tiles of 256 tokens x 256 weight rows on CTA pairs ------------------
+// ---- prefill: tiles of 256 tokens x BN <= 256 weight rows on CTA pairs ------------
 //
 // Two CTAs of a cluster share one MMA (cta_group::2, M = 256): each holds its
 // 128 token rows of A, half of B's rows and the accumulator of its own tokens, so
@@ -470,18 +470,22 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
 // cores. Loads of both CTAs complete on the leader's barrier; the leader's
 // thread issues the MMAs for both; commits release the stage in both. Tokens are
 // the accumulator's lanes, so that a thread stores runs of its token's outputs.
-// Two accumulators: a tile's epilogue runs under the next one's products.
+// Two accumulators: a tile's epilogue runs under the next one's products. BN is chosen so
+// that the tiles come out as few rounds of all pairs as their size allows.
 
-constexpr int BN = 256, kHalf = BN / 2;
 constexpr int kPairEpi = 8, kPairThreads = (2 + kPairEpi) * 32;
 constexpr int kOutWords = 32 * 17;         // an epilogue warp's staging: 32 rows of 16 words, one word apart
 
+template <int BN>
 struct Pair {
+  static constexpr int kHalf = BN / 2;                         // columns of an epilogue warp, B's rows of a CTA
   static constexpr int kBBytes = BN / 2 * kBK;
   static constexpr int kStage = kABytes + kBBytes;
   static constexpr int kAcc = 2;
+  static constexpr int kAccCols = 256;                          // tensor memory comes in powers of two
   static constexpr int kEpi = 192 + kPairEpi * (2 * kHalf + kOutWords) * 4;   // barriers, then the epilogue warps' words
-  static constexpr int S = (227 * 1024 - 1024 - kEpi) / kStage;
+  static constexpr int kFit = (227 * 1024 - 1024 - kEpi) / kStage;
+  static constexpr int S = kFit < 8 ? kFit : 8;
   static_assert((2 * S + 2 * kAcc + 1) * 8 + 4 <= 192, "barriers");
   static constexpr size_t kSmem = 1024 + (size_t)S * kStage + kEpi;
 };
@@ -502,10 +506,30 @@ struct PairArgs {
   int stall;
 };
 
-__global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
+// N consecutive 32-bit columns of this warp's TMEM lane quadrant, all loads in flight.
+template <int N>
+__device__ __forceinline__ void tmem_ld_all(uint32_t taddr, uint32_t (&r)[N]) {
+  static_assert(N % 16 == 0, "columns");
+#pragma unroll
+  for (int h = 0; h < N / 16; ++h) {
+    uint32_t* q = r + 16 * h;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
+          "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15])
+        : "r"(taddr + 16 * h));
+  }
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  // the registers hold the values from here on: no use moves before the wait
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const PairArgs a) {
-  using P = Pair;
-  constexpr int S = P::S;
+  using P = Pair<BN>;
+  constexpr int S = P::S, kHalf = P::kHalf;
   extern __shared__ char smem_raw[];
   // both CTAs have one layout: the dynamic area starts at the same address in each
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -539,7 +563,7 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(P::kAcc * BN)
+                 "r"(P::kAcc * P::kAccCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -550,21 +574,31 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    const bool leads = elect_one();
-    if (leads) pdl_wait_primary();                     // (the kernel that writes the tokens' codes)
-    if (leads && !a.stall) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int tile = pair; ok && tile < ntiles; tile += pairs) {
+    if (elect_one()) {
+      // Both CTAs' copies count on the leader's barrier. The first stages' weights are loaded
+      // while the kernel that writes the tokens' codes may still run; everything
+      // else follows its end.
+      const int ahead = a.stall ? 0 : min(S, a.kblocks);     // (a pair has at least one tile)
+      const int brow0 = pair / a.mblocks * BN + (int)rank * (BN / 2);
+      for (int kb = 0; kb < ahead; ++kb) {
+        if (rank == 0) mbar_arrive_expect_tx(full + kb, 2 * P::kStage);
+        tma_load_pair(smem_u32(s_b + kb * P::kBBytes), &bmap, kb * kBK, brow0, map_cta(smem_u32(full + kb), 0));
+      }
+      pdl_wait_primary();
+      for (int kb = 0; kb < ahead; ++kb)
+        tma_load_pair(smem_u32(s_a + kb * kABytes), &amap, kb * kBK, pair % a.mblocks * 256 + (int)rank * 128,
+                      map_cta(smem_u32(full + kb), 0));
+      int s = ahead == S ? 0 : ahead, kb = ahead;
+      uint32_t ph = ahead == S ? 1 : 0;
+      bool ok = !a.stall;
+      for (int tile = pair; ok && tile < ntiles; tile += pairs, kb = 0) {
         const int mb = tile % a.mblocks, nb = tile / a.mblocks;
         const int arow = mb * 256 + (int)rank * 128, brow = nb * BN + (int)rank * (BN / 2);
-        for (int kb = 0; kb < a.kblocks; ++kb) {
+        for (; kb < a.kblocks; ++kb) {
           if (!mbar_wait_hint(empty + s, ph ^ 1, &g_err, 51, a.wait_ns)) {
             ok = false;
             break;
           }
-          // both CTAs' copies count on the leader's barrier
           const uint32_t bar = map_cta(smem_u32(full + s), 0);
           if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * P::kStage);
           tma_load_pair(smem_u32(s_a + s * kABytes), &amap, kb * kBK, arow, bar);
@@ -577,7 +611,7 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
       }
       // every stage has been released to this CTA before it ends; after a
       // timeout, the copies in flight have landed
-      for (int i = 0; i < S; ++i) {
+      for (int i = 0; i < S && !a.stall; ++i) {
         if (ok) {
           if (!mbar_wait_hint(empty + s, ph ^ 1, &g_err, 55, a.wait_ns)) break;
         } else if (rank == 0) {
@@ -601,7 +635,7 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
       for (int tile = pair; ok && tile < ntiles; tile += pairs) {
         if (!mbar_wait_hint(tempty + buf, bph ^ 1, &g_err, 52, a.wait_ns)) break;
         tc_fence_after();
-        const uint32_t d = tmem + buf * BN;
+        const uint32_t d = tmem + buf * P::kAccCols;
         for (int kb = 0; kb < a.kblocks; ++kb) {
           if (!mbar_wait_hint(full + s, ph, &g_err, 53, a.wait_ns)) {
             ok = false;
@@ -646,8 +680,9 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
       const int rows = (int)max((int64_t)0, min((int64_t)32, a.M - m0));
       __syncwarp();                                    // (the last tile's scales have been used)
 #pragma unroll
-      for (int i = 0; i < kHalf / 32; ++i) {
+      for (int i = 0; i < (kHalf + 31) / 32; ++i) {
         const int col = i * 32 + lane;
+        if (col >= kHalf) break;
         s_ws[col] = col < cols ? a.wscales[n0 + col] : 0.f;
         s_bias[col] = a.bias != nullptr && col < cols ? load_f(a.bias, a.bias_dtype, n0 + col) : 0.f;
       }
@@ -659,7 +694,7 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
       // the sums wait in registers, so that the accumulator is free again
       // before the first of them is stored
       uint32_t v[kHalf];
-      tmem_ld128(acc0 + buf * BN, v);
+      tmem_ld_all(acc0 + buf * P::kAccCols, v);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(map_cta(smem_u32(tempty + buf), 0));
@@ -720,7 +755,8 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
       for (int c = 0; c < kHalf / 2; c += 16) {
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s_out[lane * 17 + j] = v[c + j];
+        for (int j = 0; j < 16; ++j)
+          if (c + j < kHalf / 2) s_out[lane * 17 + j] = v[c + j];
         __syncwarp();
         if (words) {
           const int col = 2 * (c + (lane & 15));
@@ -746,14 +782,14 @@ __global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
   cluster_sync();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::kAcc * BN) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::kAcc * P::kAccCols) : "memory");
   }
 }
 
 // ---- host -------------------------------------------------------------------
 
 struct Plan {
-  bool pair;        // CTA pairs on tiles of 256 tokens x 256 weight rows
+  int pair;         // CTA pairs on tiles of 256 tokens x this many weight rows, or 0
   int BT, tblocks, wblocks, kblocks, ntiles, grid;
   int cluster;      // CTAs that share a tile as a cluster, or 0
 };
@@ -793,8 +829,8 @@ static int max_clusters(int size) {
   return known[size];
 }
 
-// Cycles that a call takes at least: a stage of a pair's tile 560 and the change from
-// tile to tile 500; a stage of a lone CTA's tile 400, or what its bytes take at
+// Cycles that a call takes at least: a stage of a pair's tile what its bytes take into an
+// SM (60 a cycle) and the change from tile to tile 500; a stage of a lone CTA's tile 400, or what its bytes take at
 // DRAM's rate; a join of up to four pieces 3000 and 2500 per 32 tokens, of a
 // cluster 1500 and 600. Only their order matters.
 static Plan plan(int64_t M, int64_t N, int64_t K) {
@@ -828,15 +864,20 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
   }
   p.ntiles = (int)std::min<int64_t>(ntiles, INT32_MAX);
   if (M <= 128) return p;
-  const int64_t mb = (M + 255) / 256, nb = (N + BN - 1) / BN;
-  const double pair = (double)((mb * nb + pairs - 1) / pairs) * (560.0 * p.kblocks + 500) + 1500;
-  if (pair <= best || ntiles > (int64_t)paged::kCounters) {
-    p.pair = true;
+  const int64_t mb = (M + 255) / 256;
+  bool take = ntiles > (int64_t)paged::kCounters;
+  for (int bn : {256, 224, 192, 160, 128}) {
+    const int64_t nb = (N + bn - 1) / bn, tiles = mb * nb;
+    const double c = (double)((tiles + pairs - 1) / pairs) * ((kABytes + bn * 64) / 60.0 * p.kblocks + 500) + 1500;
+    if (take ? p.pair != 0 && c >= best : c >= best) continue;
+    best = c;
+    take = true;
+    p.pair = bn;
     p.cluster = 0;
     p.tblocks = (int)mb;
-    p.wblocks = (int)nb;
-    p.ntiles = (int)std::min<int64_t>(mb * nb, INT32_MAX);
-    p.grid = 2 * (int)std::min<int64_t>(mb * nb, pairs);
+    p.wblocks = (int)std::min<int64_t>(nb, INT32_MAX);
+    p.ntiles = (int)std::min<int64_t>(tiles, INT32_MAX);
+    p.grid = 2 * (int)std::min<int64_t>(tiles, pairs);
   }
   return p;
 }
@@ -858,17 +899,19 @@ static int launch(const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& 
   return TS_OK;
 }
 
+template <int BN>
 static int launch_pair(const CUtensorMap& am, const CUtensorMap& bm, const PairArgs& a, int grid, int overlap, cudaStream_t st) {
-  constexpr size_t smem = Pair::kSmem;
+  constexpr size_t smem = Pair<BN>::kSmem;
   static_assert(smem <= 227 * 1024, "shared memory");
+  auto k = int8_pair_kernel<BN>;
   static thread_local int configured_dev = -1;
   int dev = 0;
   TS_CUDA_TRY(cudaGetDevice(&dev));
   if (configured_dev != dev) {
-    TS_CUDA_TRY(cudaFuncSetAttribute(int8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_dev = dev;
   }
-  TS_CUDA_TRY(launch_after(int8_pair_kernel, grid, kPairThreads, smem, st, overlap, 0, am, bm, a));
+  TS_CUDA_TRY(launch_after(k, grid, kPairThreads, smem, st, overlap, 0, am, bm, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
@@ -901,7 +944,7 @@ static int matmul(const Plan& p, const ts_int8_tensor* x, const ts_int8_tensor* 
                           (uint64_t)t->row_stride, kBK, rows, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   CUtensorMap wm, xm;
-  int rc = map(&wm, w, 128);
+  int rc = map(&wm, w, p.pair ? p.pair / 2 : kBW);
   if (rc == TS_OK) rc = map(&xm, x, p.pair ? 128 : p.BT);
   if (rc != TS_OK) return rc;
   if (p.pair) {
@@ -923,7 +966,13 @@ static int matmul(const Plan& p, const ts_int8_tensor* x, const ts_int8_tensor* 
     a.vec = w->rows % per == 0 && out_row_stride % per == 0 && is_aligned(out, 16);
     a.wait_ns = wait_limit_ns();
     a.stall = stall;
-    return launch_pair(xm, wm, a, p.grid, overlap, st);
+    switch (p.pair) {
+      case 128: return launch_pair<128>(xm, wm, a, p.grid, overlap, st);
+      case 160: return launch_pair<160>(xm, wm, a, p.grid, overlap, st);
+      case 192: return launch_pair<192>(xm, wm, a, p.grid, overlap, st);
+      case 224: return launch_pair<224>(xm, wm, a, p.grid, overlap, st);
+      default: return launch_pair<256>(xm, wm, a, p.grid, overlap, st);
+    }
   }
   GemmArgs a;
   a.wscales = w->scales;
