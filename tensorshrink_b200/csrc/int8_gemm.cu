@@ -483,10 +483,10 @@ struct Pair {
   static constexpr int kStage = kABytes + kBBytes;
   static constexpr int kAcc = 2;
   static constexpr int kAccCols = 256;                          // tensor memory comes in powers of two
-  static constexpr int kEpi = 192 + kPairEpi * (2 * kHalf + kOutWords) * 4;   // barriers, then the epilogue warps' words
+  static constexpr int kEpi = 256 + kPairEpi * (2 * kHalf + kOutWords) * 4;   // barriers, then the epilogue warps' words
   static constexpr int kFit = (227 * 1024 - 1024 - kEpi) / kStage;
-  static constexpr int S = kFit < 8 ? kFit : 8;
-  static_assert((2 * S + 2 * kAcc + 1) * 8 + 4 <= 192, "barriers");
+  static constexpr int S = kFit < 10 ? kFit : 10;
+  static_assert((2 * S + 2 * kAcc + 1) * 8 + 4 <= 256, "barriers");
   static constexpr size_t kSmem = 1024 + (size_t)S * kStage + kEpi;
 };
 
@@ -506,25 +506,6 @@ struct PairArgs {
   int stall;
 };
 
-// N consecutive 32-bit columns of this warp's TMEM lane quadrant, all loads in flight.
-template <int N>
-__device__ __forceinline__ void tmem_ld_all(uint32_t taddr, uint32_t (&r)[N]) {
-  static_assert(N % 16 == 0, "columns");
-#pragma unroll
-  for (int h = 0; h < N / 16; ++h) {
-    uint32_t* q = r + 16 * h;
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
-          "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15])
-        : "r"(taddr + 16 * h));
-  }
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  // the registers hold the values from here on: no use moves before the wait
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
-}
-
 template <int BN>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const PairArgs a) {
@@ -541,7 +522,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   uint64_t* tempty = tfull + P::kAcc;
   uint64_t* drain = tempty + P::kAcc;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  char* s_epi = reinterpret_cast<char*>(full) + 192;
+  char* s_epi = reinterpret_cast<char*>(full) + 256;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
@@ -691,86 +672,91 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       const bool got = mbar_wait_hint(tfull + buf, bph, &g_err, 54, a.wait_ns);
       if (!__all_sync(0xffffffffu, got)) break;
       tc_fence_after();
-      // the sums wait in registers, so that the accumulator is free again
-      // before the first of them is stored
-      uint32_t v[kHalf];
-      tmem_ld_all(acc0 + buf * P::kAccCols, v);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_cluster(map_cta(smem_u32(tempty + buf), 0));
-      if (++buf == P::kAcc) {
-        buf = 0;
-        bph ^= 1;
-      }
-      if (rows == 0) continue;
+      // A few columns at a time, by one short loop: a tile's whole epilogue unrolled is 16 KB of
+      // instructions, which cost a small call 4 us to fetch.
+      constexpr int CW = kHalf % 32 == 0 ? 32 : 16;
+      const uint32_t acc = acc0 + buf * P::kAccCols;
+      const bool words = (reinterpret_cast<uintptr_t>(a.out) & 3) == 0 && (a.out_stride & 1) == 0;
+#pragma unroll 1
+      for (int c = 0; c < kHalf; c += CW) {
+        float f[CW];
+        if constexpr (CW == 32) tmem_ld32(acc + c, f);
+        else tmem_ld16(acc + c, f);
+        if (c + CW >= kHalf) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_cluster(map_cta(smem_u32(tempty + buf), 0));
+        }
+        if (rows == 0 || c >= cols) continue;
 #pragma unroll
-      for (int i = 0; i < kHalf; i += 4) {
-        const float4 ws = *reinterpret_cast<const float4*>(s_ws + i), bs = *reinterpret_cast<const float4*>(s_bias + i);
-        v[i] = __float_as_uint(scaled((int)v[i], xs, ws.x, bs.x));
-        v[i + 1] = __float_as_uint(scaled((int)v[i + 1], xs, ws.y, bs.y));
-        v[i + 2] = __float_as_uint(scaled((int)v[i + 2], xs, ws.z, bs.z));
-        v[i + 3] = __float_as_uint(scaled((int)v[i + 3], xs, ws.w, bs.w));
-      }
-      if (a.out_dtype == TS_F32) {
-        float* out = reinterpret_cast<float*>(a.out) + m0 * a.out_stride + n0;
-        if (a.vec) {                                   // N is a multiple of 4
-          float* row = out + lane * a.out_stride;
+        for (int i = 0; i < CW; i += 4) {
+          const float4 ws = *reinterpret_cast<const float4*>(s_ws + c + i), bs = *reinterpret_cast<const float4*>(s_bias + c + i);
+          f[i] = scaled(__float_as_int(f[i]), xs, ws.x, bs.x);
+          f[i + 1] = scaled(__float_as_int(f[i + 1]), xs, ws.y, bs.y);
+          f[i + 2] = scaled(__float_as_int(f[i + 2]), xs, ws.z, bs.z);
+          f[i + 3] = scaled(__float_as_int(f[i + 3]), xs, ws.w, bs.w);
+        }
+        if (a.out_dtype == TS_F32) {
+          float* out = reinterpret_cast<float*>(a.out) + m0 * a.out_stride + n0 + c;
+          if (a.vec) {                                 // N is a multiple of 4
+            float* row = out + lane * a.out_stride;
 #pragma unroll
-          for (int i = 0; i < kHalf; i += 4)
-            if (lane < rows && i < cols) *reinterpret_cast<uint4*>(row + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            for (int i = 0; i < CW; i += 4)
+              if (lane < rows && c + i < cols) *reinterpret_cast<float4*>(row + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+            continue;
+          }
+          // 16 columns of the warp's rows at a time through shared memory, two
+          // rows of them per store
+#pragma unroll
+          for (int h = 0; h < CW; h += 16) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s_out[lane * 17 + j] = __float_as_uint(f[h + j]);
+            __syncwarp();
+            const int col = h + (lane & 15);
+            for (int r = lane >> 4; r < rows; r += 2)
+              if (c + col < cols) out[r * a.out_stride + col] = __uint_as_float(s_out[r * 17 + (lane & 15)]);
+          }
           continue;
         }
-        // 16 columns of the warp's rows at a time through shared memory, two
-        // rows of them per store
+        uint32_t v[CW / 2];
 #pragma unroll
-        for (int c = 0; c < kHalf; c += 16) {
-          __syncwarp();
+        for (int i = 0; i < CW / 2; ++i)
+          v[i] = a.out_dtype == TS_BF16 ? paged::pack2<true>(f[2 * i], f[2 * i + 1]) : paged::pack2<false>(f[2 * i], f[2 * i + 1]);
+        uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + m0 * a.out_stride + n0 + c;
+        if (a.vec) {                                   // N is a multiple of 8
+          uint16_t* row = out + lane * a.out_stride;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) s_out[lane * 17 + j] = v[c + j];
-          __syncwarp();
-          const int col = c + (lane & 15);
-          for (int r = lane >> 4; r < rows; r += 2)
-            if (col < cols) out[r * a.out_stride + col] = __uint_as_float(s_out[r * 17 + (lane & 15)]);
+          for (int i = 0; i < CW / 8; ++i)
+            if (lane < rows && c + i * 8 < cols)
+              *reinterpret_cast<uint4*>(row + i * 8) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          continue;
         }
-        continue;
-      }
-#pragma unroll
-      for (int i = 0; i < kHalf / 2; ++i) {
-        const float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
-        v[i] = a.out_dtype == TS_BF16 ? paged::pack2<true>(x, y) : paged::pack2<false>(x, y);
-      }
-      uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + m0 * a.out_stride + n0;
-      if (a.vec) {                                     // N is a multiple of 8
-        uint16_t* row = out + lane * a.out_stride;
-#pragma unroll
-        for (int i = 0; i < kHalf / 8; ++i)
-          if (lane < rows && i * 8 < cols)
-            *reinterpret_cast<uint4*>(row + i * 8) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        continue;
-      }
-      // 32 columns of the warp's rows at a time through shared memory: two rows
-      // per store where rows start on words, one row of elements otherwise
-      const bool words = (reinterpret_cast<uintptr_t>(a.out) & 3) == 0 && (a.out_stride & 1) == 0;
-#pragma unroll
-      for (int c = 0; c < kHalf / 2; c += 16) {
+        // through shared memory: rows by words where they start on words, else by elements
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c + j < kHalf / 2) s_out[lane * 17 + j] = v[c + j];
+        for (int j = 0; j < CW / 2; ++j) s_out[lane * 17 + j] = v[j];
         __syncwarp();
         if (words) {
-          const int col = 2 * (c + (lane & 15));
-          for (int r = lane >> 4; r < rows; r += 2) {
-            const uint32_t x = s_out[r * 17 + (lane & 15)];
+          constexpr int kPer = 64 / CW;                // rows of a store
+          const int w = lane % (CW / 2), col = 2 * w;
+          for (int r = lane / (CW / 2); r < rows; r += kPer) {
+            const uint32_t x = s_out[r * 17 + w];
             uint16_t* dst = out + r * a.out_stride + col;
-            if (col + 1 < cols) *reinterpret_cast<uint32_t*>(dst) = x;
-            else if (col < cols) *dst = (uint16_t)x;
+            if (c + col + 1 < cols) *reinterpret_cast<uint32_t*>(dst) = x;
+            else if (c + col < cols) *dst = (uint16_t)x;
           }
         } else {
           const uint16_t* h = reinterpret_cast<const uint16_t*>(s_out);
-          for (int r = 0; r < rows; ++r)
-            if (2 * c + lane < cols) out[r * a.out_stride + 2 * c + lane] = h[r * 34 + lane];
+          constexpr int kPer = 32 / CW;                // rows of a store
+          const int col = lane % CW;
+          for (int r = lane / CW; r < rows; r += kPer)
+            if (c + col < cols) out[r * a.out_stride + col] = h[r * 34 + col];
         }
+      }
+      if (++buf == P::kAcc) {
+        buf = 0;
+        bph ^= 1;
       }
     }
   }
@@ -866,7 +852,7 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
   if (M <= 128) return p;
   const int64_t mb = (M + 255) / 256;
   bool take = ntiles > (int64_t)paged::kCounters;
-  for (int bn : {256, 224, 192, 160, 128}) {
+  for (int bn : {256, 224, 192, 160, 128, 96, 64}) {
     const int64_t nb = (N + bn - 1) / bn, tiles = mb * nb;
     const double c = (double)((tiles + pairs - 1) / pairs) * ((kABytes + bn * 64) / 60.0 * p.kblocks + 500) + 1500;
     if (take ? p.pair != 0 && c >= best : c >= best) continue;
@@ -967,6 +953,8 @@ static int matmul(const Plan& p, const ts_int8_tensor* x, const ts_int8_tensor* 
     a.wait_ns = wait_limit_ns();
     a.stall = stall;
     switch (p.pair) {
+      case 64: return launch_pair<64>(xm, wm, a, p.grid, overlap, st);
+      case 96: return launch_pair<96>(xm, wm, a, p.grid, overlap, st);
       case 128: return launch_pair<128>(xm, wm, a, p.grid, overlap, st);
       case 160: return launch_pair<160>(xm, wm, a, p.grid, overlap, st);
       case 192: return launch_pair<192>(xm, wm, a, p.grid, overlap, st);
