@@ -815,10 +815,13 @@ static int max_clusters(int size) {
   return known[size];
 }
 
-// Cycles that a call takes at least: a stage of a pair's tile what its bytes take into an
-// SM (60 a cycle) and the change from tile to tile 500; a stage of a lone CTA's tile 400, or what its bytes take at
-// DRAM's rate; a join of up to four pieces 3000 and 2500 per 32 tokens, of a
-// cluster 1500 and 600. Only their order matters.
+// Cycles that a call takes, as measured (0.5 to 2 us of launch and first loads aside): a stage
+// of a pair's tile what its bytes take into an SM at 60 a cycle, the change from tile to
+// tile 500; a stage of a lone CTA's tile its bytes at 40 a cycle, or the weight's at DRAM's
+// rate, 1400 for the results of each 32 tokens, 500 and 1200 per 32 tokens for the join of up to four
+// pieces, 1500 and 600 for a cluster's. Both kinds of plan tried on 28 shapes: the one taken is
+// within 5% of the best. Up to 32 tokens a pair's tile of 256 is all but empty (1 x 14336
+// x 4096: 23 us, a lone CTA's 13.6).
 static Plan plan(int64_t M, int64_t N, int64_t K) {
   Plan p{};
   const int sms = std::max(2, sm_count()), pairs = sms / 2;
@@ -830,9 +833,9 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
   const int rounds = (int)(std::min<int64_t>(M, p.BT) + 31) / 32;
   const double stream = (double)units * kABytes / 3300;   // the weight's bytes, at DRAM's bytes per cycle
   auto cost = [&](int64_t grid, int pieces) {
-    const double own = (double)((units + grid - 1) / grid) * 400;
-    return std::max(own, stream) + (pieces > 1 ? 3000 + 2500.0 * rounds * ((pieces + 3) / 4) : 0) +
-           (double)((ntiles + grid - 1) / grid) * rounds * 400;
+    const double own = (double)((units + grid - 1) / grid) * (kABytes + p.BT * kBK) / 40;
+    return std::max(own, stream) + (pieces > 1 ? 500 + 1200.0 * rounds * ((pieces + 3) / 4) : 0) +
+           (double)((ntiles + grid - 1) / grid) * rounds * 1400;
   };
   // whole tiles, or whole parts of them, where the SMs hold them all at once;
   // else, or if that is better, equal shares of all stages
@@ -849,7 +852,7 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
     }
   }
   p.ntiles = (int)std::min<int64_t>(ntiles, INT32_MAX);
-  if (M <= 128) return p;
+  if (M <= 32) return p;
   const int64_t mb = (M + 255) / 256;
   bool take = ntiles > (int64_t)paged::kCounters;
   for (int bn : {256, 224, 192, 160, 128, 96, 64}) {
