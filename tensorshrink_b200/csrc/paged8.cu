@@ -82,7 +82,6 @@ __global__ void __launch_bounds__(256) paged8_append_kernel(const AppendArgs a) 
     const int hv = i % (c.n_kv * 2), h = hv % c.n_kv, is_v = hv / c.n_kv;
     const int slot0 = (blk0 + i / (c.n_kv * 2)) * bs;           // of the block
     const int page = c.table[b * c.table_stride + slot0 / c.page_size];
-    if ((unsigned)page >= (unsigned)c.num_pages) continue;
     const int off0 = slot0 % c.page_size;
     const int r0 = max(0, len - slot0), r1 = min(bs, len + tokens - slot0);   // the rows that get tokens
     const uint16_t* src = is_v ? a.v + h * a.vh : a.k + h * a.kh;
@@ -109,6 +108,8 @@ __global__ void __launch_bounds__(256) paged8_append_kernel(const AppendArgs a) 
         any = true;
       }
     }
+    // (the tokens are on their way while the page is looked up)
+    if ((unsigned)page >= (unsigned)c.num_pages) continue;
     uint8_t* out = (is_v ? c.v : c.k) + row_at(c, page, h, off0) + cc * 8;
     float* sp = (is_v ? c.v_scales : c.k_scales) + scale_at(c, page, h, off0 / bs);
     const float old = r0 > 0 ? *sp : 0.f;
