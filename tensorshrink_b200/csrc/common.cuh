@@ -120,6 +120,40 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// Two fp32 values in one register pair, and the operations that take two at once.
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float a, float b) {
+  Two d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 both(Two v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Products that stay rounded where a sum follows: the assembler makes one operation
+// of mul2 and add2.
+__device__ __forceinline__ Two mul2_rn(Two a, Two b) {
+  const float2 x = both(a), y = both(b);
+  return two(__fmul_rn(x.x, y.x), __fmul_rn(x.y, y.y));
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
 // Programmatic dependent launch: let the next kernel in the stream start its
 // prologue, and wait for the previous kernel's results before reading them.
 __device__ __forceinline__ void pdl_launch_dependents() {

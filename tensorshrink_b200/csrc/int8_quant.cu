@@ -90,20 +90,23 @@ __device__ __forceinline__ uint32_t top8(const uint32_t (&w)[N]) {
   }
 }
 
+// Eight codes x r to nearest even: what adding 1.5 * 2^23 leaves in the sums' low bits.
 template <int DT, int N>
 __device__ __forceinline__ uint2 codes8(const uint32_t (&w)[N], float r) {
-  int q[8];
+  const Two rr = two(r, r), magic = two(12582912.f, 12582912.f);
+  float2 q[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float f;
-    if constexpr (DT == TS_F32) f = __uint_as_float(w[i % N]);
-    else f = Elem<DT>::f((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu));
-    q[i] = __float2int_rn(__fmul_rn(f, r));
+  for (int i = 0; i < 4; ++i) {
+    Two f;
+    if constexpr (DT == TS_F32) f = two(__uint_as_float(w[(2 * i) % N]), __uint_as_float(w[(2 * i + 1) % N]));
+    else f = two(Elem<DT>::f((uint16_t)(w[i] & 0xFFFFu)), Elem<DT>::f((uint16_t)(w[i] >> 16)));
+    q[i] = both(add2(mul2_rn(f, rr), magic));
   }
-  auto pack = [](int a, int b, int c, int d) {
-    return prmt(prmt((uint32_t)a, (uint32_t)b, 0x0040), prmt((uint32_t)c, (uint32_t)d, 0x0040), 0x5410);
+  auto pack = [](float2 a, float2 b) {
+    return prmt(prmt(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), prmt(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040),
+                0x5410);
   };
-  return make_uint2(pack(q[0], q[1], q[2], q[3]), pack(q[4], q[5], q[6], q[7]));
+  return make_uint2(pack(q[0], q[1]), pack(q[2], q[3]));
 }
 
 // G: threads of a row (a warp to 1024); rows of more than kHold * G chunks are read twice.

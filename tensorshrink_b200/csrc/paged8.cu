@@ -52,9 +52,12 @@ __device__ __forceinline__ uint32_t top_bits(const uint4& w) {
 
 template <bool BF, bool E4M3>
 __device__ __forceinline__ uint2 codes_of(const uint4& w, float r) {
-  const float2 a = unpack2<BF>(w.x), b = unpack2<BF>(w.y), c = unpack2<BF>(w.z), d = unpack2<BF>(w.w);
-  return make_uint2(encode4<E4M3>(__fmul_rn(a.x, r), __fmul_rn(a.y, r), __fmul_rn(b.x, r), __fmul_rn(b.y, r)),
-                    encode4<E4M3>(__fmul_rn(c.x, r), __fmul_rn(c.y, r), __fmul_rn(d.x, r), __fmul_rn(d.y, r)));
+  const Two rr = two(r, r);
+  auto pair = [&](uint32_t x) {
+    const float2 f = unpack2<BF>(x);
+    return mul2_rn(two(f.x, f.y), rr);
+  };
+  return make_uint2(encode4<E4M3>(pair(w.x), pair(w.y)), encode4<E4M3>(pair(w.z), pair(w.w)));
 }
 
 template <bool BF, bool E4M3, bool ROPE>
@@ -90,12 +93,18 @@ __global__ void __launch_bounds__(256) paged8_append_kernel(const AppendArgs a) 
     const bool turn = ROPE && !is_v;
     const int64_t pos0 = first + (slot0 - len);
     // (a key whose position has no rotary row is dropped, and its value with it)
-    auto has = [&](int r) { return on && r < r1 && (!ROPE || (pos0 + r >= 0 && pos0 + r < a.rope_rows)); };
-    auto load = [&](int r) {
-      const int64_t p = pos0 + r;
-      return load_row<BF, ROPE>(tok0 + r * step, cc, chunks, turn ? a.cos_t + p * (c.head_dim / 2) : nullptr,
-                                turn ? a.sin_t + p * (c.head_dim / 2) : nullptr);
+    int lo = r0, hi = on ? r1 : 0;                              // the rows that this lane may take
+    if (ROPE) {
+      lo = (int)max((int64_t)lo, min(-pos0, (int64_t)bs));
+      hi = (int)min((int64_t)hi, max(a.rope_rows - pos0, (int64_t)0));
+    }
+    auto has = [&](int r) { return r < hi && (!ROPE || r >= lo); };
+    auto load = [&](const uint16_t* row, int r) {
+      const int64_t p = (pos0 + r) * (c.head_dim / 2);
+      return load_row<BF, ROPE>(row, cc, chunks, turn ? a.cos_t + p : nullptr, turn ? a.sin_t + p : nullptr);
     };
+    const uint16_t* row0 = tok0 + (r0 + rl) * step;             // of this lane's first row
+    const int64_t row_step = per * step;
     uint4 w[kHold];
     uint32_t top = 0;
     bool any = false;
@@ -104,7 +113,7 @@ __global__ void __launch_bounds__(256) paged8_append_kernel(const AppendArgs a) 
       const int r = r0 + s * per + rl;
       w[s] = make_uint4(0, 0, 0, 0);
       if (has(r)) {
-        w[s] = load(r);
+        w[s] = load(row0 + s * row_step, r);
         any = true;
       }
     }
@@ -117,7 +126,7 @@ __global__ void __launch_bounds__(256) paged8_append_kernel(const AppendArgs a) 
     for (int s = 0; s < kHold; ++s) top = max(top, top_bits(w[s]));
     for (int r = r0 + kHold * per + rl; r < r1; r += per)
       if (has(r)) {
-        top = max(top, top_bits(load(r)));
+        top = max(top, top_bits(load(tok0 + r * step, r)));
         any = true;
       }
     if (!__any_sync(0xffffffffu, any)) continue;
@@ -136,15 +145,12 @@ __global__ void __launch_bounds__(256) paged8_append_kernel(const AppendArgs a) 
             if (on) {
               uint2* p = reinterpret_cast<uint2*>(out + r * c.token_stride);
               const uint2 q = *p;
+              const Two rr = two(ratio, ratio);
               float x[4], y[4];
               decode4<E4M3>(q.x, x);
               decode4<E4M3>(q.y, y);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                x[e] = __fmul_rn(x[e], ratio);
-                y[e] = __fmul_rn(y[e], ratio);
-              }
-              *p = make_uint2(encode4<E4M3>(x[0], x[1], x[2], x[3]), encode4<E4M3>(y[0], y[1], y[2], y[3]));
+              *p = make_uint2(encode4<E4M3>(mul2_rn(two(x[0], x[1]), rr), mul2_rn(two(x[2], x[3]), rr)),
+                              encode4<E4M3>(mul2_rn(two(y[0], y[1]), rr), mul2_rn(two(y[2], y[3]), rr)));
             }
         } else {
           scale = old;                                 // (a NaN stays)
@@ -154,56 +160,79 @@ __global__ void __launch_bounds__(256) paged8_append_kernel(const AppendArgs a) 
     if (lane == 0) *sp = scale;
     const bool number = scale == scale;
     const float r = number ? __frcp_rn(scale) : 0.f;
-    auto put = [&](int row, const uint4& x) {
-      *reinterpret_cast<uint2*>(out + row * c.token_stride) = number ? codes_of<BF, E4M3>(x, r) : make_uint2(0, 0);
+    auto put = [&](uint8_t* row, const uint4& x) {
+      *reinterpret_cast<uint2*>(row) = number ? codes_of<BF, E4M3>(x, r) : make_uint2(0, 0);
     };
+    uint8_t* out0 = out + (r0 + rl) * c.token_stride;
+    const int64_t out_step = per * c.token_stride;
 #pragma unroll
     for (int s = 0; s < kHold; ++s) {
       const int row = r0 + s * per + rl;
-      if (has(row)) put(row, w[s]);
+      if (has(row)) put(out0 + s * out_step, w[s]);
     }
     for (int row = r0 + kHold * per + rl; row < r1; row += per)
-      if (has(row)) put(row, load(row));
+      if (has(row)) put(out + row * c.token_stride, load(tok0 + row * step, row));
   }
 }
 
-// The values of all pages: a thread takes 16 columns of a slot.
-template <bool E4M3>
-__global__ void __launch_bounds__(256) paged8_dequantize_kernel(const Cache c, void* k_out, void* v_out, int dtype) {
-  const int chunks = c.head_dim / 16;
-  const int64_t n = (int64_t)c.num_pages * c.n_kv * c.page_size * chunks;
+// The values of all pages: a block takes a head's part of a page at a time, a thread 16
+// columns of a slot, four of them on their way at once.
+template <bool E4M3, int DT>
+__global__ void __launch_bounds__(256) paged8_dequantize_kernel(const Cache c, void* k_out, void* v_out) {
+  const int chunks = c.head_dim / 16, n = c.page_size * chunks;
   const bool is_v = blockIdx.y != 0;
   const uint8_t* src = is_v ? c.v : c.k;
   const float* scales = is_v ? c.v_scales : c.k_scales;
-  void* out = is_v ? v_out : k_out;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t slot = i / chunks;                   // (page, head, offset)
-    const int ch = (int)(i - slot * chunks);
-    const int64_t ph = slot / c.page_size;
-    const int off = (int)(slot - ph * c.page_size), page = (int)(ph / c.n_kv), h = (int)(ph - (int64_t)page * c.n_kv);
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + row_at(c, page, h, off) + ch * 16));
-    const float s = __ldg(scales + ph * c.blocks + off / c.block);
-    float f[16];
-    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+  char* out = reinterpret_cast<char*>(is_v ? v_out : k_out);
+  constexpr int kAhead = 4, kBytes = DT == TS_F32 ? 64 : 32;       // of a thread's 16 values
+  const int off0 = threadIdx.x / chunks, ch0 = threadIdx.x - off0 * chunks;
+  const int off_step = blockDim.x / chunks, ch_step = blockDim.x - off_step * chunks;
+  for (int64_t ph = blockIdx.x; ph < (int64_t)c.num_pages * c.n_kv; ph += gridDim.x) {
+    const int page = (int)(ph / c.n_kv), h = (int)(ph - (int64_t)page * c.n_kv);
+    const uint8_t* rows = src + row_at(c, page, h, 0);
+    const float* sc = scales + ph * c.blocks;
+    int off = off0, ch = ch0;
+    for (int i = threadIdx.x; i < n; i += kAhead * blockDim.x) {
+      uint4 w[kAhead];
+      float s[kAhead];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x[4];
-      decode4<E4M3>(q[e], x);
+      for (int k = 0; k < kAhead; ++k) {
+        if (i + k * (int)blockDim.x < n) {
+          w[k] = __ldg(reinterpret_cast<const uint4*>(rows + off * c.token_stride + ch * 16));
+          s[k] = __ldg(sc + off / c.block);
+        }
+        off += off_step;
+        ch += ch_step;
+        if (ch >= chunks) {
+          ch -= chunks;
+          ++off;
+        }
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[4 * e + j] = __fmul_rn(x[j], s);
-    }
-    if (dtype == TS_F32) {
-      float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + i * 16);
+      for (int k = 0; k < kAhead; ++k) {
+        const int at = i + k * (int)blockDim.x;
+        if (at >= n) break;
+        const Two ss = two(s[k], s[k]);
+        const uint32_t q[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+        uint4* p = reinterpret_cast<uint4*>(out + (ph * n + at) * kBytes);
+        uint32_t d[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-    } else {
-      uint32_t d[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        d[e] = dtype == TS_BF16 ? pack2<true>(f[2 * e], f[2 * e + 1]) : pack2<false>(f[2 * e], f[2 * e + 1]);
-      uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + i * 16);
-      p[0] = make_uint4(d[0], d[1], d[2], d[3]);
-      p[1] = make_uint4(d[4], d[5], d[6], d[7]);
+        for (int e = 0; e < 4; ++e) {
+          float x[4];
+          decode4<E4M3>(q[e], x);
+          const float2 f = both(mul2(two(x[0], x[1]), ss)), g = both(mul2(two(x[2], x[3]), ss));
+          if constexpr (DT == TS_F32) {
+            p[e] = make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(g.x), __float_as_uint(g.y));
+          } else {
+            d[2 * e] = pack2<DT == TS_BF16>(f.x, f.y);
+            d[2 * e + 1] = pack2<DT == TS_BF16>(g.x, g.y);
+          }
+        }
+        if constexpr (DT != TS_F32) {
+          p[0] = make_uint4(d[0], d[1], d[2], d[3]);
+          p[1] = make_uint4(d[4], d[5], d[6], d[7]);
+        }
+      }
     }
   }
 }
@@ -303,14 +332,21 @@ extern "C" int ts_paged8_dequantize(const ts_paged_cache8* cache, void* k, void*
   const int rc = make_cache(cache, &c);
   if (rc != TS_OK) return rc;
   TS_UNSUPPORTED(out_dtype == TS_F16 || out_dtype == TS_BF16 || out_dtype == TS_F32, "unknown output type %d", out_dtype);
-  const int64_t n = (int64_t)c.num_pages * c.n_kv * c.page_size * (c.head_dim / 16);
-  if (n == 0) return TS_OK;
+  if ((int64_t)c.num_pages * c.n_kv * c.page_size == 0) return TS_OK;
   TS_REQUIRE(c.k && c.v && c.k_scales && c.v_scales && k && v && is_aligned(k, 16) && is_aligned(v, 16),
              "NULL or unaligned pointer");
-  const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, (int64_t)sm_count() * 32), 2);
+  const dim3 grid((unsigned)std::min<int64_t>((int64_t)c.num_pages * c.n_kv, (int64_t)sm_count() * 16), 2);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (cache->code == TS_CACHE_E4M3) paged8_dequantize_kernel<true><<<grid, 256, 0, st>>>(c, k, v, out_dtype);
-  else paged8_dequantize_kernel<false><<<grid, 256, 0, st>>>(c, k, v, out_dtype);
+  auto run = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(c, k, v); };
+  if (cache->code == TS_CACHE_E4M3) {
+    if (out_dtype == TS_BF16) run(paged8_dequantize_kernel<true, TS_BF16>);
+    else if (out_dtype == TS_F16) run(paged8_dequantize_kernel<true, TS_F16>);
+    else run(paged8_dequantize_kernel<true, TS_F32>);
+  } else {
+    if (out_dtype == TS_BF16) run(paged8_dequantize_kernel<false, TS_BF16>);
+    else if (out_dtype == TS_F16) run(paged8_dequantize_kernel<false, TS_F16>);
+    else run(paged8_dequantize_kernel<false, TS_F32>);
+  }
   TS_LAUNCH_CHECK();
   return TS_OK;
 }

@@ -38,18 +38,22 @@ __device__ __forceinline__ float scale_of(float top) {
   return fmaxf(__fmul_rn(top, E4M3 ? (float)(1.0 / 448.0) : (float)(1.0 / 127.0)), 7.888609052210118e-31f);   // 2^-100
 }
 
-// Four codes of values that were divided by their scale.
+// Four codes of values that were divided by their scale, at most the largest code's size
+// (give or take fp32's rounding, which stays below half a step): to nearest even. An
+// integer is what adding 1.5 * 2^23 leaves in the sum's low bits.
 template <bool E4M3>
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+__device__ __forceinline__ uint32_t encode4(Two a, Two b) {
   if constexpr (E4M3) {
-    // (to nearest even, saturating)
+    const float2 x = both(a), y = both(b);
     uint32_t w;
     asm("{\n .reg .b16 lo, hi;\n cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n"
-        " mov.b32 %0, {lo, hi};\n}" : "=r"(w) : "f"(a), "f"(b), "f"(c), "f"(d));
+        " mov.b32 %0, {lo, hi};\n}" : "=r"(w) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
     return w;
   } else {
-    auto code = [](float x) { return (uint32_t)max(-127, min(127, __float2int_rn(x))); };
-    return prmt(prmt(code(a), code(b), 0x0040), prmt(code(c), code(d), 0x0040), 0x5410);
+    const Two magic = two(12582912.f, 12582912.f);
+    const float2 x = both(add2(a, magic)), y = both(add2(b, magic));
+    return prmt(prmt(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040), prmt(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040),
+                0x5410);
   }
 }
 

@@ -40,34 +40,6 @@ struct NormArgs {
   int page_shift;
 };
 
-// Two fp32 values in one register pair, and the operations that take two at once.
-typedef unsigned long long Two;
-__device__ __forceinline__ Two two(float a, float b) {
-  Two d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float2 both(Two v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ Two mul2(Two a, Two b) {
-  Two d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ Two add2(Two a, Two b) {
-  Two d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-  Two d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
 // Eight values from column j on.
 __device__ __forceinline__ void load8(const void* w, int dtype, int j, Two (&f)[4]) {
   if (dtype == TS_F32) {
@@ -184,8 +156,8 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_kernel(const NormArgs a) 
           // (products and sums rounded one by one, as `rotate` does)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const Two y = add2(mul2(x[e], cs[e]), mul2(x[4 + e], ns[e]));
-            x[4 + e] = add2(mul2(x[e], sn[e]), mul2(x[4 + e], cs[e]));
+            const Two y = add2(mul2_rn(x[e], cs[e]), mul2_rn(x[4 + e], ns[e]));
+            x[4 + e] = add2(mul2_rn(x[e], sn[e]), mul2_rn(x[4 + e], cs[e]));
             x[e] = y;
           }
         }
