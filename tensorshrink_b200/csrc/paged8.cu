@@ -61,7 +61,7 @@ __device__ __forceinline__ uint2 codes_of(const uint4& w, float r) {
 }
 
 template <bool BF, bool E4M3, bool ROPE>
-__global__ void __launch_bounds__(256) paged8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, ROPE ? 2 : 4) paged8_append_kernel(const AppendArgs a) {
   const Cache& c = a.c;
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, b = blockIdx.y, len = c.seq_lens[b];
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256) paged8_append_kernel(const AppendArgs a) 
 }
 
 // The values of all pages: a block takes a head's part of a page at a time, a thread 16
-// columns of a slot, four of them on their way at once.
+// columns of a slot, two of them on their way at once.
 template <bool E4M3, int DT>
 __global__ void __launch_bounds__(256) paged8_dequantize_kernel(const Cache c, void* k_out, void* v_out) {
   const int chunks = c.head_dim / 16, n = c.page_size * chunks;
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) paged8_dequantize_kernel(const Cache c, v
   const uint8_t* src = is_v ? c.v : c.k;
   const float* scales = is_v ? c.v_scales : c.k_scales;
   char* out = reinterpret_cast<char*>(is_v ? v_out : k_out);
-  constexpr int kAhead = 4, kBytes = DT == TS_F32 ? 64 : 32;       // of a thread's 16 values
+  constexpr int kAhead = 2, kBytes = DT == TS_F32 ? 64 : 32;       // of a thread's 16 values
   const int off0 = threadIdx.x / chunks, ch0 = threadIdx.x - off0 * chunks;
   const int off_step = blockDim.x / chunks, ch_step = blockDim.x - off_step * chunks;
   for (int64_t ph = blockIdx.x; ph < (int64_t)c.num_pages * c.n_kv; ph += gridDim.x) {
@@ -335,7 +335,7 @@ extern "C" int ts_paged8_dequantize(const ts_paged_cache8* cache, void* k, void*
   if ((int64_t)c.num_pages * c.n_kv * c.page_size == 0) return TS_OK;
   TS_REQUIRE(c.k && c.v && c.k_scales && c.v_scales && k && v && is_aligned(k, 16) && is_aligned(v, 16),
              "NULL or unaligned pointer");
-  const dim3 grid((unsigned)std::min<int64_t>((int64_t)c.num_pages * c.n_kv, (int64_t)sm_count() * 16), 2);
+  const dim3 grid((unsigned)std::min<int64_t>((int64_t)c.num_pages * c.n_kv, (int64_t)1 << 24), 2);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(c, k, v); };
   if (cache->code == TS_CACHE_E4M3) {

@@ -19,7 +19,7 @@ namespace paged {
 constexpr int kTableThreads = 1024;
 constexpr int kTableWarps = kTableThreads / 32;
 constexpr int kTableCtas = 8;              // of the cluster
-constexpr int kMaxSequences = 16384;
+constexpr int kMaxSequences = 8192;      // (three words of each in shared memory)
 
 struct TableArgs {
   int32_t* free_pages;
@@ -89,22 +89,27 @@ __device__ __forceinline__ void exclusive_sums(int64_t* v, int n, int64_t* total
   if (lane == 0) *total = before;
 }
 
-// What the CTAs in front of this one have in `total`, and what all have.
-__device__ __forceinline__ void cluster_sums(const int64_t* total, int64_t* front, int64_t* all) {
-  const int n = cluster_ctas(), rank = (int)cta_rank();
-  int64_t f = 0, s = 0;
-  for (int i = 0; i < n; ++i) {
-    const int64_t x = ld_cluster64(map_cta(smem_u32(total), i));
-    if (i < rank) f += x;
-    s += x;
+// What the CTAs in front of this one have in `total`, and what all have, in out[0], out[1]. By one warp, a
+// lane a CTA.
+__device__ __forceinline__ void cluster_sums(const int64_t* total, int64_t* out) {
+  const int lane = threadIdx.x & 31, rank = (int)cta_rank();
+  const int64_t x = lane < cluster_ctas() ? ld_cluster64(map_cta(smem_u32(total), lane)) : 0;
+  int64_t front = lane < rank ? x : 0, all = x;
+  static_assert(kTableCtas <= 8, "lanes");
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    front += __shfl_xor_sync(0xffffffffu, front, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
   }
-  *front = f;
-  *all = s;
+  if (lane == 0) {
+    out[0] = front;
+    out[1] = all;
+  }
 }
 
 __global__ void __launch_bounds__(kTableThreads, 1) paged_reserve_kernel(const TableArgs a) {
   extern __shared__ int64_t sums[];                 // [per] pages of the run's sequences, [per] tokens; [batch + 1] offsets
-  __shared__ int64_t total[2], popped;
+  __shared__ int64_t total[2], popped, across[2][2];
   int64_t* tokens = sums + a.per;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cta_rank();
   const int b0 = rank * a.per, mine = max(0, min(a.per, a.batch - b0));
@@ -127,9 +132,9 @@ __global__ void __launch_bounds__(kTableThreads, 1) paged_reserve_kernel(const T
   __syncthreads();
   if (warp < 2) exclusive_sums(warp == 0 ? sums : tokens, mine, total + warp);
   cluster_sync();
-  int64_t front, front_tokens, all;
-  cluster_sums(total, &front, &all);
-  cluster_sums(total + 1, &front_tokens, &all);
+  if (warp < 2) cluster_sums(total + warp, across[warp]);
+  __syncthreads();
+  const int64_t front = across[0][0], front_tokens = across[1][0];
   // the entries
   for (int i = warp; i < mine; i += kTableWarps) {
     const int b = b0 + i, len = a.seq_lens[b], n = max(0, a.n_new[b]);
@@ -139,12 +144,20 @@ __global__ void __launch_bounds__(kTableThreads, 1) paged_reserve_kernel(const T
       int32_t* row = a.table + b * a.table_stride;
       const int p0 = len / a.page_size, p1 = (int)pages_for(a, len + (int64_t)n);
       int k = (int)at;                                 // (end is at most n_free)
-      for (int q = p0; q < p1; q += 32) {
-        const int p = q + lane;
-        const bool empty = p < p1 && !is_page(a, row[p]);
-        const unsigned mask = __ballot_sync(0xffffffffu, empty);
-        if (empty) row[p] = a.free_pages[n_free - 1 - (k + __popc(mask & ((1u << lane) - 1)))];
-        k += __popc(mask);
+      for (int q = p0 + lane; q - lane < p1; q += 128) {
+        int to[4];                                     // place in the pool of each empty entry
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = q + 32 * i < p1 ? row[q + 32 * i] : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool empty = q + 32 * i < p1 && !is_page(a, to[i]);
+          const unsigned mask = __ballot_sync(0xffffffffu, empty);
+          to[i] = empty ? n_free - 1 - (k + __popc(mask & ((1u << lane) - 1))) : -1;
+          k += __popc(mask);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (to[i] >= 0) row[q + 32 * i] = a.free_pages[to[i]];
       }
     }
     if (lane == 0) {
@@ -157,7 +170,11 @@ __global__ void __launch_bounds__(kTableThreads, 1) paged_reserve_kernel(const T
   }
   cluster_sync();                                    // the entries, counts and offsets are everybody's
   int* off = reinterpret_cast<int*>(sums + 2 * a.per);   // [batch + 1]
-  for (int i = threadIdx.x; i <= a.batch; i += kTableThreads) off[i] = __ldcg(a.offsets + i);
+  int* len_of = off + a.batch + 1;                       // [batch] cached tokens, -1 of a sequence that got nothing
+  for (int i = threadIdx.x; i <= a.batch; i += kTableThreads) {
+    off[i] = __ldcg(a.offsets + i);
+    if (i < a.batch) len_of[i] = __ldcg(a.granted + i) > 0 ? a.seq_lens[i] : -1;
+  }
   if (rank == 0 && warp == 0) {
     // (served sequences need the pool's first pages: as many as the last of them ends at)
     int64_t top = 0;
@@ -165,37 +182,44 @@ __global__ void __launch_bounds__(kTableThreads, 1) paged_reserve_kernel(const T
     if (lane == 0) *a.n_free = n_free - (int)top;
   }
   __syncthreads();
+  // kAhead tokens of a thread at a time, so that their look-ups in the table overlap
+  constexpr int kAhead = 4;
   const int64_t step = (int64_t)cluster_ctas() * kTableThreads;
-  for (int64_t t = (int64_t)rank * kTableThreads + threadIdx.x; t < a.tokens; t += step) {
-    int64_t slot = -1, pos = 0;
-    int b = -1;
-    if (t < off[a.batch]) {
+  for (int64_t t0 = (int64_t)rank * kTableThreads + threadIdx.x; t0 < a.tokens; t0 += kAhead * step) {
+    int b[kAhead], s[kAhead], page[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t t = t0 + k * step;
+      b[k] = s[k] = page[k] = -1;
+      if (t >= a.tokens || t >= off[a.batch]) continue;
       // the last sequence that starts at t or in front of it (those without tokens start where the next one does)
-      b = 0;
-      for (int hi = a.batch - 1; b < hi;) {
-        const int mid = (b + hi + 1) >> 1;
-        if (off[mid] <= t) b = mid; else hi = mid - 1;
+      int lo = 0;
+      for (int hi = a.batch - 1; lo < hi;) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (off[mid] <= t) lo = mid; else hi = mid - 1;
       }
-      if (__ldcg(a.granted + b) > 0) {
-        const int i = (int)(t - off[b]), s = a.seq_lens[b] + i;
-        const int p = a.page_shift >= 0 ? s >> a.page_shift : s / a.page_size;
-        const int page = __ldcg(a.table + b * a.table_stride + p);
-        if (is_page(a, page)) {
-          slot = (int64_t)page * a.page_size + (s - p * a.page_size);
-          pos = a.first != nullptr ? a.first[b] + i : s;
-        }
-      }
+      b[k] = lo;
+      if (len_of[lo] < 0) continue;
+      s[k] = len_of[lo] + (int)(t - off[lo]);
+      page[k] = __ldcg(a.table + lo * a.table_stride + (a.page_shift >= 0 ? s[k] >> a.page_shift : s[k] / a.page_size));
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
-    a.sequences[t] = b;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t t = t0 + k * step;
+      if (t >= a.tokens) break;
+      const bool has = is_page(a, page[k]);
+      const int in_page = a.page_shift >= 0 ? s[k] & (a.page_size - 1) : s[k] % a.page_size;
+      a.slots[t] = has ? (int64_t)page[k] * a.page_size + in_page : -1;
+      a.positions[t] = !has ? 0 : a.first != nullptr ? a.first[b[k]] + (t - off[b[k]]) : s[k];
+      a.sequences[t] = b[k];
+    }
   }
   cluster_sync();                                    // nobody leaves while its sums may be read
 }
 
 __global__ void __launch_bounds__(kTableThreads, 1) paged_release_kernel(const TableArgs a) {
   extern __shared__ int64_t sums[];                 // [per] pages of the run's sequences
-  __shared__ int64_t total;
+  __shared__ int64_t total, across[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b0 = (int)cta_rank() * a.per, mine = max(0, min(a.per, a.batch - b0));
   const int n_free = max(0, min(*a.n_free, a.capacity));
@@ -209,8 +233,9 @@ __global__ void __launch_bounds__(kTableThreads, 1) paged_release_kernel(const T
   __syncthreads();
   if (warp == 0) exclusive_sums(sums, mine, &total);
   cluster_sync();
-  int64_t front, all;
-  cluster_sums(&total, &front, &all);
+  if (warp == 0) cluster_sums(&total, across);
+  __syncthreads();
+  const int64_t front = across[0], all = across[1];
   for (int i = warp; i < mine; i += kTableWarps) {
     const int b = b0 + i, keep = a.n_new[b];
     if (keep < 0) continue;
@@ -218,16 +243,21 @@ __global__ void __launch_bounds__(kTableThreads, 1) paged_release_kernel(const T
     const int len = a.seq_lens[b];
     int64_t at = n_free + front + sums[i];
     const int64_t end = n_free + front + (i + 1 < mine ? sums[i + 1] : total);
-    for (int q = first_page(len, keep); at < end && q < a.max_pages; q += 32) {
-      const int p = q + lane, e = p < a.max_pages ? row[p] : -1;
-      const bool full = p < a.max_pages && is_page(a, e);
-      const unsigned mask = __ballot_sync(0xffffffffu, full);
-      if (full) {
-        const int64_t to = at + __popc(mask & ((1u << lane) - 1));
-        if (to < a.capacity) a.free_pages[to] = e;   // (more pages than the pool has: some were shared)
-        row[p] = -1;
+    for (int q = first_page(len, keep) + lane; at < end && q - lane < a.max_pages; q += 128) {
+      int e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = q + 32 * i < a.max_pages ? row[q + 32 * i] : -1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool full = is_page(a, e[i]);
+        const unsigned mask = __ballot_sync(0xffffffffu, full);
+        if (full) {
+          const int64_t to = at + __popc(mask & ((1u << lane) - 1));
+          if (to < a.capacity) a.free_pages[to] = e[i];   // (more pages than the pool has: some were shared)
+          row[q + 32 * i] = -1;
+        }
+        at += __popc(mask);
       }
-      at += __popc(mask);
     }
     __syncwarp();
     if (lane == 0 && len > keep) a.seq_lens[b] = keep;
@@ -297,7 +327,7 @@ extern "C" int ts_paged_reserve(const ts_page_pool* pool, const ts_page_table* t
   a.slots = slots;
   a.positions = positions;
   a.sequences = sequences;
-  return launch_tables(paged_reserve_kernel, a, tokens, (size_t)(a.batch + 1) * 4, reinterpret_cast<cudaStream_t>(stream));
+  return launch_tables(paged_reserve_kernel, a, tokens, (size_t)(2 * a.batch + 1) * 4, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ts_paged_release(const ts_page_pool* pool, const ts_page_table* table, const int32_t* keep, void* stream) {

@@ -145,7 +145,7 @@ def test_table_calls_are_checked():
         return lib.ts_paged_reserve(p, t, n_new, None, tokens, P, P, slots, P, P, None)
     assert reserve(n_new=None) == INVALID and reserve(tokens=-1) == INVALID and reserve(slots=None) == INVALID
     assert reserve(page_size=0) == INVALID and reserve(max_pages=1 << 28) == INVALID and reserve(seq_lens=None) == INVALID
-    assert reserve(batch=0) == INVALID and reserve(batch=16385) == UNSUPPORTED and reserve(free_pages=None) == INVALID
+    assert reserve(batch=0) == INVALID and reserve(batch=8193) == UNSUPPORTED and reserve(free_pages=None) == INVALID
     p, t = views(batch=0)
     assert lib.ts_paged_release(p, t, None, None) == 0
     p, t = views()
