@@ -495,6 +495,7 @@ struct PairArgs {
   const float* xscales;
   int64_t M, N;
   int mblocks, nblocks, kblocks;
+  int group;                       // token blocks that are taken through all weight rows together
   int steps;
   const void* bias;
   int bias_dtype;
@@ -505,6 +506,16 @@ struct PairArgs {
   uint64_t wait_ns;
   int stall;
 };
+
+// Tile -> blocks of tokens and of weight rows: `group` token blocks at a time, the
+// tokens running fastest, so that what the pairs read together, and the group's tokens over all
+// rounds, stay in each half of L2 (8191 x 28672 x 8192 in one group of all 32: 1.9 GB from DRAM).
+__device__ __forceinline__ void tile_at(const PairArgs& a, int tile, int* mb, int* nb) {
+  const int g = tile / (a.group * a.nblocks), r = tile - g * a.group * a.nblocks;
+  const int wide = min(a.group, a.mblocks - g * a.group);
+  *nb = r / wide;
+  *mb = g * a.group + r - *nb * wide;
+}
 
 template <int BN>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
@@ -560,20 +571,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       // while the kernel that writes the tokens' codes may still run; everything
       // else follows its end.
       const int ahead = a.stall ? 0 : min(S, a.kblocks);     // (a pair has at least one tile)
-      const int brow0 = pair / a.mblocks * BN + (int)rank * (BN / 2);
+      int mb, nb;
+      tile_at(a, pair, &mb, &nb);
+      const int brow0 = nb * BN + (int)rank * (BN / 2), arow0 = mb * 256 + (int)rank * 128;
       for (int kb = 0; kb < ahead; ++kb) {
         if (rank == 0) mbar_arrive_expect_tx(full + kb, 2 * P::kStage);
         tma_load_pair(smem_u32(s_b + kb * P::kBBytes), &bmap, kb * kBK, brow0, map_cta(smem_u32(full + kb), 0));
       }
       pdl_wait_primary();
       for (int kb = 0; kb < ahead; ++kb)
-        tma_load_pair(smem_u32(s_a + kb * kABytes), &amap, kb * kBK, pair % a.mblocks * 256 + (int)rank * 128,
+        tma_load_pair(smem_u32(s_a + kb * kABytes), &amap, kb * kBK, arow0,
                       map_cta(smem_u32(full + kb), 0));
       int s = ahead == S ? 0 : ahead, kb = ahead;
       uint32_t ph = ahead == S ? 1 : 0;
       bool ok = !a.stall;
       for (int tile = pair; ok && tile < ntiles; tile += pairs, kb = 0) {
-        const int mb = tile % a.mblocks, nb = tile / a.mblocks;
+        tile_at(a, tile, &mb, &nb);
         const int arow = mb * 256 + (int)rank * 128, brow = nb * BN + (int)rank * (BN / 2);
         for (; kb < a.kblocks; ++kb) {
           if (!mbar_wait_hint(empty + s, ph ^ 1, &g_err, 51, a.wait_ns)) {
@@ -655,8 +668,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     uint32_t* s_out = reinterpret_cast<uint32_t*>(s_bias + kHalf);                           // [32 rows][17 words]
     pdl_wait_primary();                                // (the token scales)
     for (int tile = pair; tile < ntiles; tile += pairs) {
-      const int64_t m0 = (int64_t)(tile % a.mblocks) * 256 + rank * 128 + quad * 32;
-      const int64_t n0 = (int64_t)(tile / a.mblocks) * BN + half * kHalf;
+      int mb, nb;
+      tile_at(a, tile, &mb, &nb);
+      const int64_t m0 = (int64_t)mb * 256 + rank * 128 + quad * 32;
+      const int64_t n0 = (int64_t)nb * BN + half * kHalf;
       const int cols = (int)max((int64_t)0, min((int64_t)kHalf, a.N - n0));
       const int rows = (int)max((int64_t)0, min((int64_t)32, a.M - m0));
       __syncwarp();                                    // (the last tile's scales have been used)
@@ -945,6 +960,7 @@ static int matmul(const Plan& p, const ts_int8_tensor* x, const ts_int8_tensor* 
     a.mblocks = p.tblocks;
     a.nblocks = p.wblocks;
     a.kblocks = p.kblocks;
+    a.group = (int)std::max<int64_t>(1, std::min<int64_t>(a.mblocks, (32 << 20) / (256 * w->cols)));
     a.steps = steps;
     a.bias = bias;
     a.bias_dtype = bias_dtype;

@@ -167,6 +167,7 @@ at::Tensor norm_rope(const at::Tensor& x_in, int64_t n_q, int64_t n_kv, const Op
     TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && out.stride(1) == 1 &&
                           out.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
                       "out must have x's shape and type, and contiguous rows that start on 16 bytes");
+    TORCH_CHECK(!at::GradMode::is_enabled() || !out.requires_grad(), "qk_norm_rope: out wants a gradient, and there is none");
   } else {
     out = fresh(x.sizes(), x.scalar_type(), dev);
   }

@@ -104,8 +104,8 @@ class PagedKVCache8(_Paged):
     v_scales: fp32, contiguous [num_pages, n_kv, page_size / block]: `block`
     neighbouring slots (a multiple of 16) of a kv head share a scale, and a
     code stands for code * scale. page_table and seq_lens as in
-    `PagedKVCache`. There is no eviction from such a cache: slots that
-    move to another block would be rounded anew."""
+    `PagedKVCache`. int8 codes are -127 to 127. There is no eviction from such a
+    cache: slots that move to another block would be rounded anew."""
 
     __slots__ = ("k_pages", "v_pages", "k_scales", "v_scales", "page_table", "seq_lens")
 
@@ -161,7 +161,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache: AnyCache, positions: O
     that holds earlier tokens keeps its scale if that is large enough;
     otherwise the scale grows, by a quarter at least, and the earlier tokens' codes
     are rounded anew. An infinity or a NaN makes its block's scale NaN, which
-    stays until a token comes to the block's first slot again."""
+    stays until a token comes to the block's first slot again. Sequences must
+    not share a page that gets tokens."""
     if isinstance(cache, PagedKVCache8):
         if scores is not None:
             raise ValueError("scores were given for a cache that keeps none")
@@ -319,7 +320,7 @@ def qk_norm_rope(qkv: torch.Tensor, n_q: int, n_kv: int, q_weight: Optional[torc
     With a cache of 16 bits and slots (int64 [tokens], as `paged_reserve` gives
     them) key and value heads also go to their slots in the pages, whose scores
     become 0 and positions the tokens', if the cache keeps them. A slot outside the pool
-    is not written. (For a cache of 8 bits, whose tokens share scales:
+    is not written; no slot may be given twice. (For a cache of 8 bits, whose tokens share scales:
     `paged_append`.)"""
     args = (qkv, n_q, n_kv, q_weight, k_weight, positions, rope_cos, rope_sin, eps)
     name = "qk_norm_rope"

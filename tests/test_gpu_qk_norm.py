@@ -214,3 +214,8 @@ def test_refusals(ts):
     y = f(x.clone().requires_grad_(), 2, 1, qw, kw)
     with pytest.raises(RuntimeError):
         y.float().sum().backward()
+    z = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError):
+        f(z, 2, 1, qw, kw, out=z)
+    with torch.no_grad():
+        f(z, 2, 1, qw, kw, out=z)
