@@ -175,16 +175,17 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) paged8_append_kernel(const 
   }
 }
 
-// The values of all pages: a block takes a head's part of a page at a time, a thread 16
-// columns of a slot, two of them on their way at once.
+// The values of all pages: a block takes a head's part of a page at a time, a thread eight
+// columns of a slot (so that a warp's stores of 16 bits are whole lines: with sixteen, two
+// stores of half a sector pair each, L1 was the limit), four of them on their way at once.
 template <bool E4M3, int DT>
 __global__ void __launch_bounds__(256) paged8_dequantize_kernel(const Cache c, void* k_out, void* v_out) {
-  const int chunks = c.head_dim / 16, n = c.page_size * chunks;
+  const int chunks = c.head_dim / 8, n = c.page_size * chunks;
   const bool is_v = blockIdx.y != 0;
   const uint8_t* src = is_v ? c.v : c.k;
   const float* scales = is_v ? c.v_scales : c.k_scales;
   char* out = reinterpret_cast<char*>(is_v ? v_out : k_out);
-  constexpr int kAhead = 2, kBytes = DT == TS_F32 ? 64 : 32;       // of a thread's 16 values
+  constexpr int kAhead = 4, kBytes = DT == TS_F32 ? 32 : 16;       // of a thread's eight values
   const int off0 = threadIdx.x / chunks, ch0 = threadIdx.x - off0 * chunks;
   const int off_step = blockDim.x / chunks, ch_step = blockDim.x - off_step * chunks;
   for (int64_t ph = blockIdx.x; ph < (int64_t)c.num_pages * c.n_kv; ph += gridDim.x) {
@@ -193,12 +194,12 @@ __global__ void __launch_bounds__(256) paged8_dequantize_kernel(const Cache c, v
     const float* sc = scales + ph * c.blocks;
     int off = off0, ch = ch0;
     for (int i = threadIdx.x; i < n; i += kAhead * blockDim.x) {
-      uint4 w[kAhead];
+      uint2 w[kAhead];
       float s[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         if (i + k * (int)blockDim.x < n) {
-          w[k] = __ldg(reinterpret_cast<const uint4*>(rows + off * c.token_stride + ch * 16));
+          w[k] = __ldg(reinterpret_cast<const uint2*>(rows + off * c.token_stride + ch * 8));
           s[k] = __ldg(sc + off / c.block);
         }
         off += off_step;
@@ -213,24 +214,21 @@ __global__ void __launch_bounds__(256) paged8_dequantize_kernel(const Cache c, v
         const int at = i + k * (int)blockDim.x;
         if (at >= n) break;
         const Two ss = two(s[k], s[k]);
-        const uint32_t q[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+        float x[4], y[4];
+        decode4<E4M3>(w[k].x, x);
+        decode4<E4M3>(w[k].y, y);
+        const float2 f[4] = {both(mul2(two(x[0], x[1]), ss)), both(mul2(two(x[2], x[3]), ss)), both(mul2(two(y[0], y[1]), ss)),
+                             both(mul2(two(y[2], y[3]), ss))};
         uint4* p = reinterpret_cast<uint4*>(out + (ph * n + at) * kBytes);
-        uint32_t d[8];
+        if constexpr (DT == TS_F32) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x[4];
-          decode4<E4M3>(q[e], x);
-          const float2 f = both(mul2(two(x[0], x[1]), ss)), g = both(mul2(two(x[2], x[3]), ss));
-          if constexpr (DT == TS_F32) {
-            p[e] = make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(g.x), __float_as_uint(g.y));
-          } else {
-            d[2 * e] = pack2<DT == TS_BF16>(f.x, f.y);
-            d[2 * e + 1] = pack2<DT == TS_BF16>(g.x, g.y);
-          }
-        }
-        if constexpr (DT != TS_F32) {
-          p[0] = make_uint4(d[0], d[1], d[2], d[3]);
-          p[1] = make_uint4(d[4], d[5], d[6], d[7]);
+          for (int e = 0; e < 2; ++e)
+            p[e] = make_uint4(__float_as_uint(f[2 * e].x), __float_as_uint(f[2 * e].y), __float_as_uint(f[2 * e + 1].x),
+                              __float_as_uint(f[2 * e + 1].y));
+        } else {
+          constexpr bool kBF = DT == TS_BF16;
+          *p = make_uint4(pack2<kBF>(f[0].x, f[0].y), pack2<kBF>(f[1].x, f[1].y), pack2<kBF>(f[2].x, f[2].y),
+                          pack2<kBF>(f[3].x, f[3].y));
         }
       }
     }
