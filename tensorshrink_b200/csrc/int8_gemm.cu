@@ -20,7 +20,9 @@
 // into whole parts, whose CTAs are a cluster and add their sums through
 // distributed shared memory, or, where clusters do not fit the tiles, into
 // equal shares of all stages laid end to end, whose sums the last CTA of a
-// tile to arrive adds from the workspace.
+// tile to arrive adds from the workspace. Measured, other weights each call: 14336 x
+// 4096, 1 token 11.6 us, 4096 x 14336, 33 tokens 14.3 (59 MB, 9.0 us at the copy
+// bandwidth; the rest is start, first loads and epilogue).
 //
 // Every wait is bounded in wall-clock time: a role whose wait runs out records
 // a code and unwinds; the TMEM is freed at the end in any case.
@@ -471,7 +473,9 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
 // thread issues the MMAs for both; commits release the stage in both. Tokens are
 // the accumulator's lanes, so that a thread stores runs of its token's outputs.
 // Two accumulators: a tile's epilogue runs under the next one's products. BN is chosen so
-// that the tiles come out as few rounds of all pairs as their size allows.
+// that the tiles come out as few rounds of all pairs as their size allows. Measured: 8191 x 28672 x
+// 8192 1.17 to 1.25 ms, 3.1 to 3.3 POP/s at the power limit (1.4 GHz, 92% of the tensor pipe's cycles);
+// 2047 x 14336 x 4096 81 us, 3.0 POP/s; 256 x 4096 x 4096 9.9 us.
 
 constexpr int kPairEpi = 8, kPairThreads = (2 + kPairEpi) * 32;
 constexpr int kOutWords = 32 * 17;         // an epilogue warp's staging: 32 rows of 16 words, one word apart

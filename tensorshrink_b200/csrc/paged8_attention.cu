@@ -6,10 +6,11 @@
 // outside the products. Scores of integers are sums of products of bytes, q being three
 // bytes of 24 bits (a head's power of two taken out), exact up to the last addition; those of
 // e4m3 (and of wide groups, for registers) take the codes as fp16, exactly, and q as
-// fp16 without its power of two. A score is the product of the sum with a_t. A weight enters the second product as p_t b_t over a power
-// of two that is at least every b_t so far (the output is scaled along when it
-// grows, as for the running maximum), in fp16: one term where the result is bf16,
-// whose own rounding is eight times larger, two where it is fp16.
+// fp16 without its power of two. A score is the product of the sum with a_t. A weight
+// enters the second product as p_t b_t over a power of two that is at least every
+// b_t so far (the output is scaled along when it grows, as for the running
+// maximum), in fp16: one term where the result is bf16, whose own rounding is
+// eight times larger, two where it is fp16.
 //
 // What bounds it: 2 len D bytes per kv head are read once, DRAM bandwidth does, but at
 // half the bytes of a 16-bit cache the instructions per slot come close. So the
@@ -18,8 +19,8 @@
 // to eight half the products, exponentials and registers of the other
 // orientation. Codes come from shared memory as bytes, four of a register making two
 // operand registers, with the order of columns inside a 16-column step permuted
-// alike in q (scores) or in the output (where a thread then holds four
-// neighbouring columns); P turns from sums to operand by movmatrix. The running
+// alike in q (scores) or in the output (whose accumulator rows g and g + 8 are the
+// neighbouring columns 2 g and 2 g + 1); P turns from sums to operand by movmatrix. The running
 // maximum follows only when a score passes it by 2^4, found by one vote, so that
 // a tile usually needs no shuffles.
 //
@@ -30,6 +31,11 @@
 // alone reach 5.1 TB/s where those of 32 reach 5.5.) Lane i of a warp looks up page and
 // scales of its tile 32 j + i, three batches deep. Every wait is bounded; a warp whose
 // wait runs out records it and stops.
+//
+// Measured (128 columns, 8 kv heads): 64 sequences of up to 8191 slots, 8 query heads to a kv
+// head, int8, token-major pages, 106 to 111 us, 5.0 TB/s (the copies alone 104 us: rows of
+// 128 bytes a KB apart); 4 of 32768, e4m3, fp16 results, 52 us, 5.2 TB/s; one of 512, 10 us, a
+// chain of latencies and of first instruction fetches.
 #include <algorithm>
 
 #include "gemm.cuh"
