@@ -2,6 +2,8 @@
 // product, norms of queries and keys, the paged cache of 8 bits and the page
 // tables (C ABI: ts_int8_*, ts_qk_norm_rope, ts_paged8_*, ts_paged_reserve,
 // ts_paged_release). Conventions as in serving.cpp.
+#include <ATen/MemoryOverlap.h>
+
 #include "serving_common.h"
 
 namespace {
@@ -168,6 +170,7 @@ at::Tensor norm_rope(const at::Tensor& x_in, int64_t n_q, int64_t n_kv, const Op
                           out.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
                       "out must have x's shape and type, and contiguous rows that start on 16 bytes");
     TORCH_CHECK(!at::GradMode::is_enabled() || !out.requires_grad(), "qk_norm_rope: out wants a gradient, and there is none");
+    at::assert_no_partial_overlap(out, x);
   } else {
     out = fresh(x.sizes(), x.scalar_type(), dev);
   }
@@ -345,6 +348,7 @@ at::Tensor attend_out(const OptTensor& out_, const ts_paged_cache8& c, int64_t w
   TORCH_CHECK_VALUE(out_->dim() == 2 && out_->size(0) == c.batch && out_->size(1) == width &&
                         out_->scalar_type() == q.scalar_type() && out_->stride(1) == 1,
                     "out must be [batch, n_q head_dim] of the queries' type with contiguous rows");
+  at::assert_no_partial_overlap(*out_, q);
   return *out_;
 }
 

@@ -188,10 +188,12 @@ class PagedDecoder(nn.Module):
         """Count n decode steps (negative: steps that the program took back);
         raises if fewer are left. `decode_step` does it by itself, except while
         it is captured: a program that replays a captured step counts each replay."""
-        if n > self.steps_left:
-            if self.pages is not None and n <= self.longest_sequence - max(t for t in self._tokens if t is not None):
-                raise RuntimeError(f"{n} decode steps, but {self.pages} pages hold {self.steps_left} (see pages and drop)")
-            raise RuntimeError(f"{n} decode steps, but a sequence has {self.longest_sequence - self.steps_left} of "
+        tokens = [t for t in self._tokens if t is not None]
+        slots = self.longest_sequence - max(tokens, default=0)
+        if n <= slots and self.pages is not None and n > 0 and self._pages_for(t + n for t in tokens) > self.pages:
+            raise RuntimeError(f"{n} decode steps, but {self.pages} pages hold {self.steps_left} (see pages and drop)")
+        if n > slots:
+            raise RuntimeError(f"{n} decode steps, but a sequence has {self.longest_sequence - slots} of "
                                f"{self.longest_sequence} tokens (see max_position, max_len and drop)")
         self._tokens = [None if t is None else t + n for t in self._tokens]
 

@@ -219,3 +219,6 @@ def test_refusals(ts):
         f(z, 2, 1, qw, kw, out=z)
     with torch.no_grad():
         f(z, 2, 1, qw, kw, out=z)
+    buf = torch.zeros(5, 256, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError):
+        f(buf[:4], 2, 1, qw, kw, out=buf[1:])                    # rows of the one are rows of the other

@@ -216,3 +216,93 @@ def test_refusals():
         build(torch.float16)
     with pytest.raises(ValueError):
         build(pages=3).prefill(prompts())
+
+
+def test_all_dropped():
+    m = build(pages=20)
+    m.prefill(prompts())
+    for i in range(4):
+        m.drop(i)
+    assert int(m.pool.n_free) == 20 and m.steps_left == m.longest_sequence
+    with pytest.raises(RuntimeError, match="decode steps"):
+        m.count_steps(10 ** 6)
+    m.decode_step(torch.zeros(4, dtype=torch.long, device="cuda"))
+    assert m.caches[0].seq_lens.tolist() == [-1] * 4 and int(m.pool.n_free) == 20
+
+
+def test_threads_share_a_stream():
+    """Host threads call all operators on one stream, with tensors of their own."""
+    import threading
+    import tensorshrink_b200 as ts
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+
+    def round_of(i):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        w = ts.int8_quantize(torch.randn(16 * 64, 300, generator=g, device="cuda"))
+        cache, pool = ts.PagedKVCache8.allocate(3, 4, 64, 96, page_size=32, dtype=(torch.int8, E4M3)[i % 2]), ts.PagePool.allocate(9)
+        cache.page_table.fill_(-1)
+        qw = torch.rand(64, generator=g, device="cuda")
+        x = torch.randn(3, 300, generator=g, device="cuda").bfloat16()
+        one = torch.ones(3, dtype=torch.int32, device="cuda")
+        outs = []
+        for _ in range(40):
+            got = ts.paged_reserve(pool, cache, one, 3)
+            qkv = ts.qk_norm_rope(ts.int8_linear(x, w), 8, 4, qw, qw)
+            outs.append(ts.paged_decode_attention(qkv, 8, cache))
+            cache.advance(got.granted)
+            x = torch.roll(x, 1, 1)
+        ts.paged_release(pool, cache, torch.zeros_like(one))
+        return torch.stack(outs), pool.free.clone(), cache.seq_lens.clone()
+
+    want = [round_of(i) for i in range(4)]
+    found = [None] * 4
+    torch.cuda.synchronize()
+
+    def work(i):
+        found[i] = round_of(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for a, b in zip(want, found):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_schemas_hold():
+    """What the operators write is what their schemas say, and their shapes under tracing are the real ones."""
+    import tensorshrink_b200 as ts
+    from tensorshrink_b200 import _C
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    ops, utils = _C.serving_ops(), ("test_schema", "test_faketensor")
+
+    def check(op, *args, **kw):
+        torch.library.opcheck(op, args, kw, test_utils=utils)
+    x = torch.randn(5, 200, device="cuda").bfloat16()
+    w = ts.int8_quantize(torch.randn(64, 200, device="cuda"))
+    check(ops.int8_quantize.default, x)
+    check(ops.int8_dequantize.default, w.codes, w.scales, 200, torch.float16)
+    check(ops.int8_matmul.default, w.codes, w.scales, w.codes, w.scales, 200, None, torch.float32)
+    check(ops.int8_linear.default, x, w.codes, w.scales, 200, None)
+    qkv = torch.randn(4, 8 * 64, device="cuda").bfloat16()
+    qw = torch.rand(64, device="cuda")
+    check(ops.qk_norm_rope.default, qkv, 4, 2, qw, qw, None, None, None, 1e-6)
+    check(ops.qk_norm_rope.out, qkv, 4, 2, qw, qw, None, None, None, 1e-6, out=torch.empty_like(qkv))
+    c16 = ts.PagedKVCache.allocate(4, 2, 64, 64, page_size=16)
+    check(ops.qk_norm_rope_store.default, qkv, 4, 2, qw, qw, None, None, None, 1e-6, *c16._args(),
+          torch.arange(4, device="cuda"))
+    c = ts.PagedKVCache8.allocate(4, 2, 64, 64, page_size=16)
+    c.seq_lens.fill_(3)
+    kv = qkv.view(4, 1, 8, 64)
+    check(ops.paged8_append.default, kv[:, :, 4:6], kv[:, :, 6:], *c._args(), None, None, None, None, None)
+    check(ops.paged8_dequantize.default, *c._args(), torch.bfloat16)
+    check(ops.paged8_attention.default, qkv[:, :256], *c._args(), None, None, None, None)
+    check(ops.paged8_decode_attention.default, qkv, 4, *c._args(), None, None, None, None)
+    pool, one = ts.PagePool.allocate(8), torch.ones(4, dtype=torch.int32, device="cuda")
+    c.page_table[:, 1:] = -1
+    check(ops.paged_reserve.default, pool.free, pool.n_free, c.page_table, c.seq_lens, 16, 16, one * 20, None, 80)
+    check(ops.paged_release.default, pool.free, pool.n_free, c.page_table, c.seq_lens, 16, 16, one)
