@@ -600,8 +600,9 @@ TS_API size_t ts_int8_matmul_workspace_size(int64_t M, int64_t N, int64_t K);
 TS_API int ts_int8_matmul(const ts_int8_tensor* a, const ts_int8_tensor* b, const void* bias, int bias_dtype, void* out,
                           int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes, void* stream);
 
-/* out[M, N] = x . w^T (+ bias): ts_int8_quantize of x [M, cols] by way of the
- * workspace, then ts_int8_matmul, bit for bit. */
+/* out[M, N] = x . w^T (+ bias): ts_int8_quantize of x [M, cols], then ts_int8_matmul,
+ * bit for bit; by way of the workspace, or for one or two short tokens in one
+ * kernel. out does not overlap x. */
 TS_API size_t ts_int8_linear_workspace_size(int64_t M, int64_t N, int64_t K);
 TS_API int ts_int8_linear(const void* x, int x_dtype, int64_t M, int64_t x_row_stride, const ts_int8_tensor* w,
                           const void* bias, int bias_dtype, void* out, int out_dtype, int64_t out_row_stride,

@@ -16,12 +16,14 @@
 //               128-byte swizzle
 //   warp 1      one thread issues the MMAs
 //   warps 2-5   epilogue: tcgen05.ld, scales, bias, stores
+//   warps 6-13  (kernels of few tokens that come unquantised) find the tokens' scales and
+//               quantise the stages' columns into shared memory, a stage per warp in turn
 // Bound by the weight's bytes. The tiles are few, so they are split along K:
 // into whole parts, whose CTAs are a cluster and add their sums through
 // distributed shared memory, or, where clusters do not fit the tiles, into
 // equal shares of all stages laid end to end, whose sums the last CTA of a
 // tile to arrive adds from the workspace. Measured, other weights each call: 14336 x
-// 4096, 1 token 11.6 us, 4096 x 14336, 33 tokens 14.3 (59 MB, 9.0 us at the copy
+// 4096, 1 token 11.6 us (13.6 with its quantisation), 4096 x 14336, 33 tokens 14.3 (59 MB, 9.0 us at the copy
 // bandwidth; the rest is start, first loads and epilogue).
 //
 // Every wait is bounded in wall-clock time: a role whose wait runs out records
@@ -42,6 +44,15 @@ constexpr int kEpiWarps = 4;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr int kABytes = kBW * kBK;
 constexpr int kMaxCluster = 8;           // CTAs of a cluster that share a tile
+constexpr int kQuantWarps = 8;
+
+// Up to this many tokens, of this many elements together, the kernel quantises them itself:
+// every CTA finds their scales (each reads all of them, from L2) while its first weights
+// are on their way. More come from a quantiser in front, which the kernel's start
+// overlaps. 14336 x 4096: one token 13.6 us by itself, 14.7 behind a quantiser, two
+// 14.3 and 14.6, four 16.1 and 14.8; 8192 x 28672, one token 47.3 and 44.5.
+constexpr int kOwnTokens = 2;
+constexpr int64_t kOwnElements = 16384;
 
 __device__ int g_err;
 
@@ -62,6 +73,9 @@ struct GemmArgs {
   int stall;                       // test hook: the producer issues nothing
   int cluster;                     // CTAs that share a tile as a cluster, or 0
   int out_vec;                     // rows of out take stores of four values
+  const void* x;                   // tokens to be quantised by the kernel itself
+  int x_dtype, x_aligned;          // x_aligned: rows start on 16 bytes
+  int64_t x_stride, K;
 };
 
 template <int BT>
@@ -184,11 +198,69 @@ struct Items {
   }
 };
 
-template <int BT>
-__global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap wmap,
-                                                                const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
+// By the quantising warps: the scales of all tokens to xs[] (and to r[] their inverses, 0
+// of a token that is not finite).
+template <int DT>
+__device__ __forceinline__ void token_scales(const GemmArgs& a, float* xs, float* r, uint32_t (*tops)[kOwnTokens]) {
+  using T = typename Elem<DT>::T;
+  const int t = threadIdx.x - kThreads, warp = t >> 5, chunks = (int)((a.K + 7) / 8), M = (int)a.M;
+  for (int m = 0; m < M; ++m) {
+    const T* row = reinterpret_cast<const T*>(a.x) + m * a.x_stride;
+    uint32_t top = 0;
+    constexpr int kAhead = 4, N = DT == TS_F32 ? 8 : 4;
+    for (int c = t; c < chunks; c += kAhead * kQuantWarps * 32) {
+      uint32_t w[kAhead][N];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int ci = c + i * kQuantWarps * 32;
+        const int64_t cols = ci < chunks ? a.K : 0;      // (nothing is loaded behind the last column)
+        if (a.x_aligned) load8<DT, true>(row, ci, cols, w[i]);
+        else load8<DT, false>(row, ci, cols, w[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) top = max(top, top8<DT>(w[i]));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((t & 31) == 0) tops[warp][m] = top;
+  }
+  named_bar_sync(4, kQuantWarps * 32);
+  if (t < M) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < kQuantWarps; ++w) top = max(top, tops[w][t]);
+    const bool finite = top < 0x7F800000u;
+    const float s = finite ? scale_of(__uint_as_float(top)) : __uint_as_float(0x7FC00000u);
+    xs[t] = s;
+    r[t] = finite ? __frcp_rn(s) : 0.f;
+  }
+  named_bar_sync(4, kQuantWarps * 32);
+}
+
+// Columns [128 kb, 128 kb + 128) of all tokens into a stage, as TMA would swizzle them: 16 lanes a
+// row, eight columns each.
+template <int DT>
+__device__ __forceinline__ void quantise_stage(const GemmArgs& a, int kb, char* sx, const float* r) {
+  using T = typename Elem<DT>::T;
+  const int lane = threadIdx.x & 31, j = lane & 15;
+  for (int m = lane >> 4; m < a.M; m += 2) {
+    const T* row = reinterpret_cast<const T*>(a.x) + m * a.x_stride;
+    uint32_t w[DT == TS_F32 ? 8 : 4];
+    if (a.x_aligned) load8<DT, true>(row, kb * 16 + j, a.K, w);
+    else load8<DT, false>(row, kb * 16 + j, a.K, w);
+    const float f = r[m];
+    *reinterpret_cast<uint2*>(sx + m * 128 + (((j >> 1) ^ (m & 7)) << 4) + (j & 1) * 8) =
+        f != 0.f ? codes8<DT>(w, f) : make_uint2(0, 0);
+  }
+}
+
+template <int BT, bool Q>
+__global__ void __launch_bounds__(kThreads + (Q ? kQuantWarps * 32 : 0), 1)
+int8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const GemmArgs a) {
   using P = Shape<BT>;
   constexpr int S = P::S;
+  static_assert(!Q || BT >= kOwnTokens, "tokens of a stage");
+  __shared__ uint32_t q_tops[kQuantWarps][kOwnTokens];
+  __shared__ float q_inv[kOwnTokens];
   extern __shared__ char smem_raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   char* s_w = smem;                                  // [S][128][128]
@@ -206,9 +278,9 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
   const int ntiles = a.wblocks * a.tblocks;
   if (warp == 0 && lane == 0) {
     prefetch_tensormap(&wmap);
-    prefetch_tensormap(&xmap);
+    if (!Q) prefetch_tensormap(&xmap);
     for (int i = 0; i < S; ++i) {
-      mbar_init(full + i, 1);
+      mbar_init(full + i, Q ? 2 : 1);
       mbar_init(empty + i, 1);
     }
     for (int i = 0; i < P::kAcc; ++i) {
@@ -230,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
   if (warp == 0) {
     if (elect_one()) {
       auto load_w = [&](const Item& x, int kb, int s) {
-        mbar_arrive_expect_tx(full + s, P::kStage);
+        mbar_arrive_expect_tx(full + s, Q ? kABytes : P::kStage);
         tma_load_2d(s_w + s * kABytes, &wmap, kb * kBK, x.tile / a.tblocks * kBW, full + s);
       };
       // The weight's first S stages are loaded while the kernel that writes
@@ -255,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
             }
             load_w(x, kb, s);
           }
-          tma_load_2d(s_x + s * P::kXBytes, &xmap, kb * kBK, x.tile % a.tblocks * BT, full + s);
+          if (!Q) tma_load_2d(s_x + s * P::kXBytes, &xmap, kb * kBK, x.tile % a.tblocks * BT, full + s);
           ++issued;
           if (++s == S) {
             s = 0;
@@ -309,6 +381,29 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
       umma_commit(drain);
       mbar_wait_hint(drain, 0, nullptr, 0, a.wait_ns);
     }
+  } else if (Q && warp >= 2 + kEpiWarps) {
+    if (a.x_dtype == TS_BF16) token_scales<TS_BF16>(a, s_xs, q_inv, q_tops);
+    else if (a.x_dtype == TS_F16) token_scales<TS_F16>(a, s_xs, q_inv, q_tops);
+    else token_scales<TS_F32>(a, s_xs, q_inv, q_tops);
+    int n = 0;                                       // of the CTA's stages
+    bool ok = true;
+    Items it(a, ntiles);
+    Item x;
+    while (ok && it.next(a, x)) {
+      for (int kb = x.k0; kb < x.k1; ++kb, ++n) {
+        if (n % kQuantWarps != warp - (2 + kEpiWarps)) continue;
+        const int s = n % S;
+        ok = __all_sync(0xffffffffu, mbar_wait_hint(empty + s, (uint32_t)(n / S & 1) ^ 1, &g_err, 45, a.wait_ns));
+        if (!ok) break;
+        char* sx = s_x + s * P::kXBytes;
+        if (a.x_dtype == TS_BF16) quantise_stage<TS_BF16>(a, kb, sx, q_inv);
+        else if (a.x_dtype == TS_F16) quantise_stage<TS_F16>(a, kb, sx, q_inv);
+        else quantise_stage<TS_F32>(a, kb, sx, q_inv);
+        fence_proxy_async_smem();                    // the tensor cores read what was written
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + s);
+      }
+    }
   } else {
     const int quad = warp & 3;
     const int r = quad * 32 + lane;                  // this thread's row of the tile
@@ -324,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
       const int jn_all = (int)min((int64_t)BT, a.M - m0);
       const bool valid = n < a.N;
       named_bar_sync(3, kEpiWarps * 32);             // (the last tile's scales have been used)
-      if (r < jn_all) s_xs[r] = a.xscales[m0 + r];
+      if (!Q && r < jn_all) s_xs[r] = a.xscales[m0 + r];   // (else its quantisers have put them there)
       const float ws = valid ? a.wscales[n] : 0.f;
       const float bias = a.bias && valid ? load_f(a.bias, a.bias_dtype, n) : 0.f;
       if (!named_bar_and(3, kEpiWarps * 32, mbar_wait_hint(tfull + buf, bph, &g_err, 44, a.wait_ns))) break;
@@ -443,7 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
     const int rank = (int)cta_rank(), tile = blockIdx.x / a.cluster;
     const int64_t m0 = (int64_t)(tile % a.tblocks) * BT, n = (int64_t)(tile / a.tblocks) * kBW + 4 * lane;
     const int jn = (int)min((int64_t)BT, a.M - m0);
-    for (int j = rank + a.cluster * warp; j < jn; j += a.cluster * (kThreads / 32)) {
+    constexpr int kWarpsAll = kThreads / 32 + (Q ? kQuantWarps : 0);
+    for (int j = rank + a.cluster * warp; j < jn; j += a.cluster * kWarpsAll) {
       const uint32_t at = smem_u32(s_w) + (uint32_t)(j * kBW + 4 * lane) * 4;
       float4 v[kMaxCluster];
 #pragma unroll
@@ -458,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
           sum[2] += __float_as_int(v[p].z);
           sum[3] += __float_as_int(v[p].w);
         }
-      if (n < a.N) store_four(a, m0 + j, n, sum, a.xscales[m0 + j]);
+      if (n < a.N) store_four(a, m0 + j, n, sum, Q ? s_xs[j] : a.xscales[m0 + j]);
     }
     cluster_sync();                                    // nobody leaves while its sums may be read
   }
@@ -812,7 +908,7 @@ static int max_clusters(int size) {
     known_dev = dev;
   }
   if (known[size] < 0) {
-    auto k = int8_gemm_kernel<128>;
+    auto k = int8_gemm_kernel<128, false>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(sm_count() / size * size));
     cfg.blockDim = dim3((unsigned)kThreads);
@@ -890,9 +986,9 @@ static Plan plan(int64_t M, int64_t N, int64_t K) {
   return p;
 }
 
-template <int BT>
+template <int BT, bool Q>
 static int launch(const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& a, int grid, int overlap, cudaStream_t st) {
-  auto k = int8_gemm_kernel<BT>;
+  auto k = int8_gemm_kernel<BT, Q>;
   constexpr size_t smem = Shape<BT>::kSmem;
   static_assert(smem <= 227 * 1024, "shared memory");
   static thread_local int configured_dev = -1;
@@ -902,7 +998,7 @@ static int launch(const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& 
     TS_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_dev = dev;
   }
-  TS_CUDA_TRY(launch_after(k, grid, kThreads, smem, st, overlap, a.cluster, wm, xm, a));
+  TS_CUDA_TRY(launch_after(k, grid, kThreads + (Q ? kQuantWarps * 32 : 0), smem, st, overlap, a.cluster, wm, xm, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
@@ -929,8 +1025,16 @@ static size_t plan_bytes(const Plan& p) {
   return paged::kCounterBytes + (!p.pair && !p.cluster ? (size_t)p.grid * 2 * kBW * p.BT * 4 : 0);
 }
 
+// Tokens that the product quantises itself.
+struct Tokens {
+  const void* x;
+  int dtype;
+  int64_t stride;
+};
+
 static int matmul(const Plan& p, const ts_int8_tensor* x, const ts_int8_tensor* w, const void* bias, int bias_dtype, void* out,
-                  int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes, int overlap, void* stream) {
+                  int out_dtype, int64_t out_row_stride, void* workspace, size_t workspace_bytes, int overlap, const Tokens* own,
+                  void* stream) {
   TS_UNSUPPORTED(out_dtype == TS_F16 || out_dtype == TS_BF16 || out_dtype == TS_F32, "unknown output type %d", out_dtype);
   TS_UNSUPPORTED(!bias || bias_dtype == TS_F16 || bias_dtype == TS_BF16 || bias_dtype == TS_F32, "unknown bias type %d",
                  bias_dtype);
@@ -953,7 +1057,8 @@ static int matmul(const Plan& p, const ts_int8_tensor* x, const ts_int8_tensor* 
   };
   CUtensorMap wm, xm;
   int rc = map(&wm, w, p.pair ? p.pair / 2 : kBW);
-  if (rc == TS_OK) rc = map(&xm, x, p.pair ? 128 : p.BT);
+  if (own) xm = wm;                                    // (not used)
+  else if (rc == TS_OK) rc = map(&xm, x, p.pair ? 128 : p.BT);
   if (rc != TS_OK) return rc;
   if (p.pair) {
     PairArgs a;
@@ -1006,11 +1111,18 @@ static int matmul(const Plan& p, const ts_int8_tensor* x, const ts_int8_tensor* 
   a.cluster = p.cluster;
   const int wide = out_dtype == TS_F32 ? 16 : 8;       // bytes of four values
   a.out_vec = is_aligned(out, wide) && out_row_stride % 4 == 0;
+  a.x = own ? own->x : nullptr;
+  a.x_dtype = own ? own->dtype : 0;
+  a.x_stride = own ? own->stride : 0;
+  a.x_aligned = own && is_aligned(own->x, 16) && own->stride * (own->dtype == TS_F32 ? 4 : 2) % 16 == 0;
+  a.K = w->cols;
+  static_assert(kOwnTokens <= 16, "tokens of the kernel that quantises them");
+  if (own) return launch<16, true>(wm, xm, a, p.grid, 0, st);
   switch (p.BT) {
-    case 16: return launch<16>(wm, xm, a, p.grid, overlap, st);
-    case 32: return launch<32>(wm, xm, a, p.grid, overlap, st);
-    case 64: return launch<64>(wm, xm, a, p.grid, overlap, st);
-    default: return launch<128>(wm, xm, a, p.grid, overlap, st);
+    case 16: return launch<16, false>(wm, xm, a, p.grid, overlap, st);
+    case 32: return launch<32, false>(wm, xm, a, p.grid, overlap, st);
+    case 64: return launch<64, false>(wm, xm, a, p.grid, overlap, st);
+    default: return launch<128, false>(wm, xm, a, p.grid, overlap, st);
   }
 }
 
@@ -1034,7 +1146,7 @@ extern "C" int ts_int8_matmul(const ts_int8_tensor* a, const ts_int8_tensor* b, 
   TS_REQUIRE(a->cols == b->cols, "a has %lld columns, b %lld", (long long)a->cols, (long long)b->cols);
   if (a->rows == 0 || b->rows == 0) return TS_OK;
   return matmul(plan(a->rows, b->rows, b->cols), a, b, bias, bias_dtype, out, out_dtype, out_row_stride, workspace,
-                workspace_bytes, 0, stream);
+                workspace_bytes, 0, nullptr, stream);
 }
 
 extern "C" int ts_int8_status(int clear, void* stream) {
@@ -1085,7 +1197,13 @@ extern "C" int ts_int8_linear(const void* x, int x_dtype, int64_t M, int64_t x_r
   t.scales = reinterpret_cast<float*>(t.codes + align_up((size_t)M * (size_t)t.row_stride, 256));
   t.rows = M;
   t.cols = w->cols;
+  if (M <= kOwnTokens && M * w->cols <= kOwnElements) {
+    TS_UNSUPPORTED(x_dtype == TS_F16 || x_dtype == TS_BF16 || x_dtype == TS_F32, "unknown element type %d", x_dtype);
+    TS_REQUIRE(x && is_aligned(x, x_dtype == TS_F32 ? 4 : 2), "x must be aligned to its elements");
+    const Tokens own = {x, x_dtype, x_row_stride};
+    return matmul(p, &t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, 0, &own, stream);
+  }
   rc = ts_int8_quantize(x, x_dtype, x_row_stride, &t, stream);
   if (rc != TS_OK) return rc;
-  return matmul(p, &t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, 1, stream);
+  return matmul(p, &t, w, bias, bias_dtype, out, out_dtype, out_row_stride, workspace, at, 1, nullptr, stream);
 }

@@ -116,7 +116,8 @@ def test_matmul(ts, m, n, k):
                                product(a.codes[:, :k], a.scales, b.codes[:, :k], b.scales, z, dtype)), (dtype, z is None)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (8, 300, 1000), (40, 1024, 4096), (300, 520, 777)])
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (1, 130, 1), (1, 1000, 16384), (1, 200, 16385), (2, 4000, 8192), (2, 77, 333),
+                                   (3, 512, 4096), (8, 300, 1000), (40, 1024, 4096), (300, 520, 777)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_is_quantize_then_matmul(ts, m, n, k, dtype):
     x, w = matrix(m, k, dtype, 3), ts.int8_quantize(matrix(n, k, torch.float32, 4))
@@ -183,6 +184,20 @@ def test_shapes_and_module(ts):
     assert ts.int8_linear(x, ts.int8_quantize(x[:0])).shape == (6, 0)
     big = matrix(6, 401, torch.float16, 8)
     assert torch.equal(m.half()(big[:, 1:201]), m(big[:, 1:201].contiguous()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_and_two_tokens_as_they_come(ts, dtype):
+    # rows that start anywhere, of any size and content, through the kernel that quantises them itself
+    w = ts.int8_quantize(matrix(300, 515, torch.float32, 4))
+    base = matrix(6, 1200, dtype, 5)
+    base[4] = 0
+    base[5, 530] = float("nan")
+    for rows in (slice(0, 1), slice(1, 3), slice(4, 5), slice(4, 6)):
+        for at in (0, 1, 3, 8):
+            x = base[rows, at:at + 515]
+            q, s = rows_of(x)
+            same(ts.int8_linear(x, w), product(q, s, w.codes[:, :515], w.scales, None, dtype))
 
 
 def test_refusals(ts):
