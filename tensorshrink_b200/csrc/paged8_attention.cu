@@ -33,9 +33,8 @@
 // wait runs out records it and stops.
 //
 // Measured (128 columns, 8 kv heads): 64 sequences of up to 8191 slots, 8 query heads to a kv
-// head, int8, token-major pages, 106 to 111 us, 5.0 TB/s (the copies alone 104 us: rows of
-// 128 bytes a KB apart); 4 of 32768, e4m3, fp16 results, 52 us, 5.2 TB/s; one of 512, 10 us, a
-// chain of latencies and of first instruction fetches.
+// head, int8, token-major pages, 96 us, 5.6 TB/s; 4 of 32768, e4m3, fp16 results, 52 us,
+// 5.2 TB/s; one of 512, 10 us, a chain of latencies and of first instruction fetches.
 #include <algorithm>
 
 #include "gemm.cuh"
@@ -76,6 +75,7 @@ struct AttnArgs {
   const uint16_t* q;
   int64_t q_stride;
   int n_q, group, head_tiles;
+  int abreast;           // rows of a sequence that CTAs of neighbouring numbers take side by side
   int extra;             // 1: slot seq_lens[b] holds the new token and counts
   const int64_t* positions;
   const float* cos_t;
@@ -192,6 +192,9 @@ __global__ void __launch_bounds__(kThreads, Ring<DP, NT>::kCtas)
   int* lens = prefix + c.batch + 1;                                                     // [batch]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int D = c.head_dim, rows_per_b = c.n_kv * a.head_tiles;
+  const int laid = rows_per_b / a.abreast;               // rows of a sequence that lie end to end
+  // CTAs abreast work as one on the rows laid end to end, each on a row of its own of every `abreast`
+  const unsigned cta = blockIdx.x / a.abreast, side = blockIdx.x - cta * a.abreast;
 
   if (tid == 0) {
     prefetch_tensormap(&kmap);
@@ -234,8 +237,8 @@ __global__ void __launch_bounds__(kThreads, Ring<DP, NT>::kCtas)
     }
     // How the units are dealt out: a row of n units counts n + front, or, with
     // front < 0, -front whatever n is.
-    const unsigned units = (unsigned)(uint32_t)all * rows_per_b, rows = (unsigned)(all >> 32) * rows_per_b;
-    deal = choose_deal(units, rows, longest, gridDim.x, min(a.group, kHeads));
+    const unsigned units = (unsigned)(uint32_t)all * laid, rows = (unsigned)(all >> 32) * laid;
+    deal = choose_deal(units, rows, longest, gridDim.x / a.abreast, min(a.group, kHeads));
     int v = 0;
     if (deal.front >= 0) v = (int)(uint32_t)at + deal.front * (int)(at >> 32);
     else v = -deal.front * (int)(at >> 32);
@@ -256,12 +259,12 @@ __global__ void __launch_bounds__(kThreads, Ring<DP, NT>::kCtas)
     if (prefix[b] == prefix[b + 1])
       for (int i = tid; i < a.n_q * D; i += kThreads) a.out[b * a.out_stride + i] = 0;
 
-  const unsigned total = (unsigned)prefix[c.batch] * rows_per_b;   // (the host keeps it below 2^31)
+  const unsigned total = (unsigned)prefix[c.batch] * laid;         // (the host keeps it below 2^31)
   if (total == 0) return;
   const unsigned n_cta = min(deal.n_cta, total);
-  if (blockIdx.x >= n_cta) return;
+  if (cta >= n_cta) return;
   const Shares shares(total, n_cta);
-  const unsigned u1 = shares.begin(blockIdx.x + 1);
+  const unsigned u1 = shares.begin(cta + 1);
 
   char* ring = smem + (size_t)warp * S * P::kStage;
   const uint32_t ring_u = smem_u32(ring);
@@ -269,26 +272,27 @@ __global__ void __launch_bounds__(kThreads, Ring<DP, NT>::kCtas)
   uint32_t phases = 0;                                   // a bit per stage: the parity of its next completion
   bool broken = false;
 
-  // the first row: sequence b is the last with prefix[b] * rows_per_b <= u
-  unsigned u = shares.begin(blockIdx.x);
+  // the first row: sequence b is the last with prefix[b] * laid <= u
+  unsigned u = shares.begin(cta);
   int b = 0;
   for (int hi = c.batch - 1; b < hi;) {
     const int mid = (b + hi + 1) >> 1;
-    if ((unsigned)prefix[mid] * rows_per_b <= u) b = mid; else hi = mid - 1;
+    if ((unsigned)prefix[mid] * laid <= u) b = mid; else hi = mid - 1;
   }
-  int row = (int)((u - (unsigned)prefix[b] * rows_per_b) / (unsigned)(prefix[b + 1] - prefix[b]));
-  for (; u < u1; ++row) {
+  int nth = (int)((u - (unsigned)prefix[b] * laid) / (unsigned)(prefix[b + 1] - prefix[b]));
+  for (; u < u1; ++nth) {
     // the segment: units [t0, t1) of (sequence b, kv head h, head tile ht)
-    if (row == rows_per_b) {
-      row = 0;
+    if (nth == laid) {
+      nth = 0;
       do ++b; while (prefix[b + 1] == prefix[b]);
     }
     const int cost = prefix[b + 1] - prefix[b], nt = units_of(a, lens[b]), front = cost - nt;
-    const unsigned row_u = (unsigned)prefix[b] * rows_per_b + (unsigned)(row * cost);
+    const unsigned row_u = (unsigned)prefix[b] * laid + (unsigned)(nth * cost);
     const int v0 = (int)(u - row_u), v1 = (int)min((unsigned)cost, v0 + (u1 - u));
     u += v1 - v0;
     if (v1 <= front) continue;                         // only the row's front
     const int t0 = max(v0 - front, 0), t1 = v1 - front;
+    const int row = nth * a.abreast + (int)side;
     const int h = row / a.head_tiles, ht = row - h * a.head_tiles;
     const int heads = min(kHeads, a.group - ht * kHeads);
     const int head0 = h * a.group + ht * kHeads;       // first query head of the tile
@@ -764,9 +768,9 @@ __global__ void __launch_bounds__(kThreads, Ring<DP, NT>::kCtas)
       if (is_last) {
         const int pieces = cta1 - cta0 + 1;          // at most kMaxPieces + 1
         // a row's pieces lie first in their CTAs' slots, but for its beginning
-        const float* begun = a.partials + ((int64_t)cta0 * 2 + 1) * prow;
-        const float* others = a.partials + (int64_t)cta0 * 2 * prow;
-        auto piece = [&](int i) { return i == 0 ? begun : others + (int64_t)i * 2 * prow; };
+        const float* others = a.partials + ((int64_t)cta0 * a.abreast + side) * 2 * prow;
+        const int64_t next = (int64_t)a.abreast * 2 * prow;
+        auto piece = [&](int i) { return i == 0 ? others + prow : others + i * next; };
         // Two heads per warp, which needs no other: the pieces' factors
         // 2^(m_piece - m), lane i those of pieces i, i + 32, ..., and their sums, four
         // values a lane, eight pieces in flight ahead of their use.
@@ -920,6 +924,13 @@ static int make_args(AttnArgs* a, int q_dtype, int n_q, const ts_paged_cache8* c
   a->group = n_q / a->c.n_kv;
   const int heads = a->group > 8 ? 16 : 8;
   a->head_tiles = (a->group + heads - 1) / heads;
+  // Where a token's heads lie next to each other, up to four CTAs of neighbouring numbers
+  // take as many heads of the same slots at about the same time, so that DRAM serves longer
+  // runs: 64 sequences of up to 8191 slots 96 us for 103 to 108 (two heads 96, eight 97). Pages of
+  // whole heads gain nothing (53 us for 53) and keep all CTAs.
+  a->abreast = 1;
+  for (int n = 2; n <= 4; ++n)
+    if (a->c.head_stride < a->c.token_stride && a->c.n_kv * a->head_tiles % n == 0) a->abreast = n;
   TS_UNSUPPORTED((int64_t)a->c.batch * a->c.n_kv * a->head_tiles < (int64_t)kCounters, "too many heads in one call");
   TS_UNSUPPORTED(((int64_t)a->c.max_pages * a->c.page_size / kUnit + 1 + kRowCost) * a->c.batch * a->c.n_kv * a->head_tiles <
                      (int64_t)1 << 31,

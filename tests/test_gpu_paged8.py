@@ -302,6 +302,19 @@ def test_attention(ts, case, dtype, held):
 
 
 @pytest.mark.parametrize("held", [INT8, E4M3])
+@pytest.mark.parametrize("n_q,n_kv,d,page,lens", [
+    (6, 3, 128, 64, [1, 900, 0, 129, 6000]), (12, 6, 64, 16, [700, 33]), (5, 5, 128, 64, [2000, 128]), (40, 2, 128, 64, [300, 5000, 0]),
+    (34, 2, 80, 32, [1500]), (14, 7, 96, 64, [40] * 90), (24, 3, 256, 64, [70, 3000, 1]), (12, 12, 128, 64, [5000, 1, 700] * 6)])
+def test_heads_taken_side_by_side(ts, n_q, n_kv, d, page, lens, held):
+    # token-major pages, numbers of heads that two, three, four or no CTAs share
+    c = make(ts, lens, n_kv, d, page, 16, held, 3, layout="tokens")
+    q = torch.randn(len(lens), n_q * d, device="cuda").to(torch.bfloat16)
+    out = ts.paged_attention(q, c)
+    close(out, *reference(c, q, lens))
+    assert torch.equal(ts.paged_attention(q, c), out)
+
+
+@pytest.mark.parametrize("held", [INT8, E4M3])
 def test_attention_without_pages_lengths_and_rows(ts, held):
     c = make(ts, [200, 64, 40, 100, 10], 2, 64, 16, 16, held, 4, room=1)
     c.page_table[0, 3] = -1                                       # holes
