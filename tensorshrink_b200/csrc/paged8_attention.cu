@@ -140,25 +140,35 @@ __device__ __forceinline__ void to_half(uint32_t w, uint32_t& x, uint32_t& y) {
 // the heads' powers of two, and the prefix sums of the sequences' units with their lengths.
 //
 // DP: columns that are computed, head_dim rounded up (the copies fill the rest of a
-// box with zeros). Blocks per SM: as many as the registers allow, which hides more of a
-// tile's chain of latencies than longer rings do.
-template <int DP, int NT>
+// box with zeros). C: blocks per SM, as many as the registers allow, which hides more of a
+// tile's chain of latencies, and of a row's start, than longer rings do. 64 columns, 64 sequences
+// of up to 16000 slots: four blocks 99 us, three 104, two with rings of six stages 130;
+// 16 query heads to a kv head, 32 of up to 8000: 49, 48, 53. 96 columns, 64 of up to
+// 16000: three blocks 139, two 146; 128 columns: see kManyRows.
+template <int DP, int NT, int C>
 struct Ring {
   static constexpr int kCols = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;   // columns in shared memory
   static constexpr int kBox = kCols < 128 ? kCols : 128;        // columns of a TMA box
   static constexpr int kHalf = kPair * kCols;                   // bytes of a stage's K (or V)
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int S = kCols == 64 ? 6 : 3;
+  static constexpr int S = kCols == 128 && C == 3 ? 2 : 3;
   static constexpr size_t kBytes = (size_t)kWarps * S * kStage;
-  static constexpr int kCtas = kCols == 256 ? 1 : 2;
 };
+
+// 128 columns: three blocks per SM with rings of two stages where the rows are many and short (150
+// sequences of 8 kv heads, of up to 300 slots 26 us for 29 with two blocks of three stages, of
+// up to 3000 85 for 96), else two (128 of 8000 slots 316 us for 339, 64 of up to 16000 167 for
+// 171, 4 of 4000 14.7 for 15.8). The host knows the tables' capacity, not the lengths.
+constexpr int kManyRows = 2;               // kv heads of all sequences per SM, from which three are taken
+constexpr int64_t kShortTable = 4096;      // slots
+
 template <bool E4M3, int DP, int NT>
 constexpr bool int_scores() { return !E4M3 && DP * NT <= 128; }
 template <bool E4M3, int DP, int NT>
 constexpr size_t q_bytes() { return int_scores<E4M3, DP, NT>() ? 3 * 8 * NT * (DP + 16) : 8 * NT * (DP + 8) * 2; }
-template <bool E4M3, int DP, int NT>
+template <bool E4M3, int DP, int NT, int C>
 constexpr size_t attn_smem(int batch) {
-  return 1024 + Ring<DP, NT>::kBytes + kWarps * Ring<DP, NT>::S * 8 + q_bytes<E4M3, DP, NT>() + 8 * NT * 4 +
+  return 1024 + Ring<DP, NT, C>::kBytes + kWarps * Ring<DP, NT, C>::S * 8 + q_bytes<E4M3, DP, NT>() + 8 * NT * 4 +
          (size_t)(2 * batch + 1) * 4;
 }
 
@@ -169,10 +179,10 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <bool BF, bool E4M3, int DP, int NT>
-__global__ void __launch_bounds__(kThreads, Ring<DP, NT>::kCtas)
+template <bool BF, bool E4M3, int DP, int NT, int C>
+__global__ void __launch_bounds__(kThreads, C)
     paged8_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnArgs a) {
-  using P = Ring<DP, NT>;
+  using P = Ring<DP, NT, C>;
   constexpr bool kInt = int_scores<E4M3, DP, NT>();
   constexpr int S = P::S;
   constexpr int kHeads = 8 * NT;                 // query heads of a tile: a multiple of kWarps
@@ -853,12 +863,9 @@ __global__ void __launch_bounds__(kThreads, Ring<DP, NT>::kCtas)
   }
 }
 
-static size_t grid_of(int head_dim) {
-  return (size_t)sm_count() * (head_dim > 128 ? Ring<256, 1>::kCtas : Ring<128, 1>::kCtas);
-}
-
 static size_t workspace_bytes_of(int head_dim) {
-  return kCounterBytes + grid_of(head_dim) * 2 * 16 * (head_dim + 2) * 4;
+  const int ctas = head_dim > 128 ? 1 : head_dim > 64 ? 3 : 4;   // blocks per SM at most
+  return kCounterBytes + (size_t)sm_count() * ctas * 2 * 16 * (head_dim + 2) * 4;
 }
 
 static int encode_map(CUtensorMap* map, const Cache& c, const void* base, int box) {
@@ -871,10 +878,10 @@ static int encode_map(CUtensorMap* map, const Cache& c, const void* base, int bo
                      box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
-template <bool BF, bool E4M3, int DP, int NT>
+template <bool BF, bool E4M3, int DP, int NT, int C>
 static int launch(const AttnArgs& a, int overlap, cudaStream_t st) {
-  auto k = paged8_attention_kernel<BF, E4M3, DP, NT>;
-  const size_t smem = attn_smem<E4M3, DP, NT>(a.c.batch);
+  auto k = paged8_attention_kernel<BF, E4M3, DP, NT, C>;
+  const size_t smem = attn_smem<E4M3, DP, NT, C>(a.c.batch);
   // (the same value for all host threads, as for the 16-bit kernel)
   static thread_local int configured_dev = -1;
   static thread_local size_t most = 0;
@@ -889,10 +896,10 @@ static int launch(const AttnArgs& a, int overlap, cudaStream_t st) {
   }
   TS_UNSUPPORTED(smem <= most, "batch too large for the kernel's tables");
   CUtensorMap km, vm;
-  int rc = encode_map(&km, a.c, a.c.k, Ring<DP, NT>::kBox);
-  if (rc == TS_OK) rc = encode_map(&vm, a.c, a.c.v, Ring<DP, NT>::kBox);
+  int rc = encode_map(&km, a.c, a.c.k, Ring<DP, NT, C>::kBox);
+  if (rc == TS_OK) rc = encode_map(&vm, a.c, a.c.v, Ring<DP, NT, C>::kBox);
   if (rc != TS_OK) return rc;
-  TS_CUDA_TRY(launch_after(k, (int)grid_of(a.c.head_dim), kThreads, smem, st, overlap, 0, km, vm, a));
+  TS_CUDA_TRY(launch_after(k, sm_count() * C, kThreads, smem, st, overlap, 0, km, vm, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
@@ -901,10 +908,15 @@ template <bool BF, bool E4M3>
 static int launch(const AttnArgs& a, int overlap, cudaStream_t st) {
   // one column tile of eight query heads, or two where a group has more
   const bool wide = a.group > 8;
-  if (a.c.head_dim > 64 && a.c.head_dim <= 96) return wide ? launch<BF, E4M3, 96, 2>(a, overlap, st) : launch<BF, E4M3, 96, 1>(a, overlap, st);
-  if (a.c.head_dim <= 64) return wide ? launch<BF, E4M3, 64, 2>(a, overlap, st) : launch<BF, E4M3, 64, 1>(a, overlap, st);
-  if (a.c.head_dim <= 128) return wide ? launch<BF, E4M3, 128, 2>(a, overlap, st) : launch<BF, E4M3, 128, 1>(a, overlap, st);
-  return wide ? launch<BF, E4M3, 256, 2>(a, overlap, st) : launch<BF, E4M3, 256, 1>(a, overlap, st);
+  if (a.c.head_dim <= 64) return wide ? launch<BF, E4M3, 64, 2, 3>(a, overlap, st) : launch<BF, E4M3, 64, 1, 4>(a, overlap, st);
+  if (a.c.head_dim <= 96) return wide ? launch<BF, E4M3, 96, 2, 2>(a, overlap, st) : launch<BF, E4M3, 96, 1, 3>(a, overlap, st);
+  if (a.c.head_dim <= 128) {
+    if (wide) return launch<BF, E4M3, 128, 2, 2>(a, overlap, st);
+    const bool many = (int64_t)a.c.batch * a.c.n_kv >= (int64_t)kManyRows * sm_count() &&
+                      (int64_t)a.c.max_pages * a.c.page_size <= kShortTable;
+    return many ? launch<BF, E4M3, 128, 1, 3>(a, overlap, st) : launch<BF, E4M3, 128, 1, 2>(a, overlap, st);
+  }
+  return wide ? launch<BF, E4M3, 256, 2, 1>(a, overlap, st) : launch<BF, E4M3, 256, 1, 1>(a, overlap, st);
 }
 
 // Fills `a` from the arguments that both entry points share, and checks them.

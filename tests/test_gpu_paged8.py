@@ -315,6 +315,18 @@ def test_heads_taken_side_by_side(ts, n_q, n_kv, d, page, lens, held):
 
 
 @pytest.mark.parametrize("held", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,layout", [(128, "heads"), (112, "tokens"), (96, "heads"), (64, "tokens"), (48, "heads")])
+def test_many_rows(ts, d, layout, dtype, held):
+    lens = [1, 900, 64, 0, 2500] * 16
+    c = make(ts, lens, 4, d, 64, 32, held, 4, layout=layout)
+    q = torch.randn(len(lens), 12 * d, device="cuda").to(dtype)
+    out = ts.paged_attention(q, c)
+    close(out, *reference(c, q, lens))
+    assert torch.equal(ts.paged_attention(q, c), out)
+
+
+@pytest.mark.parametrize("held", [INT8, E4M3])
 def test_attention_without_pages_lengths_and_rows(ts, held):
     c = make(ts, [200, 64, 40, 100, 10], 2, 64, 16, 16, held, 4, room=1)
     c.page_table[0, 3] = -1                                       # holes
