@@ -33,8 +33,9 @@
 // wait runs out records it and stops.
 //
 // Measured (128 columns, 8 kv heads): 64 sequences of up to 8191 slots, 8 query heads to a kv
-// head, int8, token-major pages, 96 us, 5.6 TB/s; 4 of 32768, e4m3, fp16 results, 52 us,
-// 5.2 TB/s; one of 512, 10 us, a chain of latencies and of first instruction fetches.
+// head, int8, token-major pages, 96 us repeated on one input, 5.6 TB/s, 106 on others each
+// time; 4 of 32768, e4m3, fp16 results, 52 us, 5.2 TB/s; one of 512, 10 us, a chain of
+// latencies and of first instruction fetches.
 #include <algorithm>
 
 #include "gemm.cuh"
@@ -938,7 +939,8 @@ static int make_args(AttnArgs* a, int q_dtype, int n_q, const ts_paged_cache8* c
   a->head_tiles = (a->group + heads - 1) / heads;
   // Where a token's heads lie next to each other, up to four CTAs of neighbouring numbers
   // take as many heads of the same slots at about the same time, so that DRAM serves longer
-  // runs: 64 sequences of up to 8191 slots 96 us for 103 to 108 (two heads 96, eight 97). Pages of
+  // runs: 64 sequences of up to 8191 slots 96 us for 103 to 108 (two heads 96, eight 97), on other
+  // inputs each time 108 for 110. Pages of
   // whole heads gain nothing (53 us for 53) and keep all CTAs.
   a->abreast = 1;
   for (int n = 2; n <= 4; ++n)
