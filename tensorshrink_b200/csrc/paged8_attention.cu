@@ -9,8 +9,8 @@
 // fp16 without its power of two. A score is the product of the sum with a_t. A weight
 // enters the second product as p_t b_t over a power of two that is at least every
 // b_t so far (the output is scaled along when it grows, as for the running
-// maximum), in fp16: one term where the result is bf16, whose own rounding is
-// eight times larger, two where it is fp16.
+// maximum), as two terms of fp16, 22 bits (one term turned the last bits of bf16
+// results).
 //
 // What bounds it: 2 len D bytes per kv head are read once, DRAM bandwidth does, but at
 // half the bytes of a 16-bit cache the instructions per slot come close. So the
@@ -624,11 +624,9 @@ __global__ void __launch_bounds__(kThreads, C)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t w = pack2<false>(p[2 * e], p[2 * e + 1]);
+          const float2 x = unpack2<false>(w);
           pf[t][e] = transpose8(w);
-          if (!BF) {
-            const float2 x = unpack2<false>(w);
-            pr[t][e] = transpose8(pack2<false>(p[2 * e] - x.x, p[2 * e + 1] - x.y));
-          }
+          pr[t][e] = transpose8(pack2<false>(p[2 * e] - x.x, p[2 * e + 1] - x.y));
         }
       }
 #pragma unroll
@@ -643,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, C)
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             mma<false>(o[2 * s + e][t], v4, pf[t][0], pf[t][1]);
-            if (!BF) mma<false>(o[2 * s + e][t], v4, pr[t][0], pr[t][1]);
+            mma<false>(o[2 * s + e][t], v4, pr[t][0], pr[t][1]);
           }
         }
       }
