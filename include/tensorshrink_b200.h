@@ -417,7 +417,8 @@ TS_API int ts_paged8_dequantize(const ts_paged_cache8* cache, void* k, void* v, 
  * Attention of one query token per sequence over its cached tokens, slots [0,
  * seq_lens[b]): q [batch, n_q * head_dim] fp16 or bf16, out alike. With tables q is
  * rotated to positions[b]; a position without a rotary row, like a sequence
- * without tokens, answers with zeros. Slots without a page do not count.
+ * without tokens, answers with zeros. Slots without a page do not count. out may be q
+ * (of a projection's output: its query columns), and overlaps it in no other way.
  * Workspace as ts_paged_decode_attention.
  */
 TS_API size_t ts_paged8_attention_workspace_size(const ts_paged_cache8* cache, int n_q);
@@ -447,7 +448,7 @@ TS_API int ts_paged8_status(int clear, void* stream);
  *   y = x * rsqrt(mean(x^2) + eps) * w        (w: q_weight or k_weight, [head_dim]
  *                                             of weight_dtype; NULL: y = x)
  *   (y1 c - y2 s, y1 s + y2 c)                with tables, at positions[t]
- * in fp32, rounded once; values are copied. out may be x. With a cache (16
+ * in fp32, rounded once; values are copied. out may be x, and overlaps it in no other way. With a cache (16
  * bits, x's type) key and value heads also go to slot slots[t] (device int64: page *
  * page_size + offset) of its pages, whose score and position are set; a slot outside
  * the pool is not written. A token whose position has no rotary row gets

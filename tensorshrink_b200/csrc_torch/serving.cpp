@@ -208,6 +208,7 @@ at::Tensor attend(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, cons
     TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == c.batch && out.size(1) == owidth &&
                           out.scalar_type() == qkv.scalar_type() && out.stride(1) == 1,
                       "out must be [batch, n_q head_dim] of qkv's type with contiguous rows");
+    apart(out, qkv, "paged_decode_attention");
   } else {
     out = fresh({c.batch, owidth}, qkv.scalar_type(), dev);
   }

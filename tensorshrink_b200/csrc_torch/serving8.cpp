@@ -2,8 +2,6 @@
 // product, norms of queries and keys, the paged cache of 8 bits and the page
 // tables (C ABI: ts_int8_*, ts_qk_norm_rope, ts_paged8_*, ts_paged_reserve,
 // ts_paged_release). Conventions as in serving.cpp.
-#include <ATen/MemoryOverlap.h>
-
 #include "serving_common.h"
 
 namespace {
@@ -170,11 +168,11 @@ at::Tensor norm_rope(const at::Tensor& x_in, int64_t n_q, int64_t n_kv, const Op
                           out.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
                       "out must have x's shape and type, and contiguous rows that start on 16 bytes");
     TORCH_CHECK(!at::GradMode::is_enabled() || !out.requires_grad(), "qk_norm_rope: out wants a gradient, and there is none");
-    at::assert_no_partial_overlap(out, x);
   } else {
     out = fresh(x.sizes(), x.scalar_type(), dev);
   }
   x = fit_rows(x);
+  if (has(out_)) apart(out, x, "qk_norm_rope");
   const int wdt = has(qw) ? code_of(qw->scalar_type(), "qk_norm_rope") : has(kw) ? code_of(kw->scalar_type(), "qk_norm_rope") : 0;
   done(ts_qk_norm_rope(x.data_ptr(), code_of(x.scalar_type(), "qk_norm_rope"), x.stride(0), tokens, (int)n_q, (int)n_kv, (int)d,
                        ptr(qw), ptr(kw), wdt, (float)eps, ptr<int64_t>(positions), ptr<float>(ct), ptr<float>(st), rows,
@@ -342,13 +340,14 @@ std::tuple<at::Tensor, at::Tensor> paged8_dequantize(const at::Tensor& kp, const
 }
 
 // The output of an attention call: the caller's, or a new one.
-at::Tensor attend_out(const OptTensor& out_, const ts_paged_cache8& c, int64_t width, const at::Tensor& q) {
+// (q: the queries, or their projection, as they are read)
+at::Tensor attend_out(const OptTensor& out_, const ts_paged_cache8& c, int64_t width, const at::Tensor& q, const char* what) {
   if (!has(out_)) return fresh({c.batch, width}, q.scalar_type(), q.device());
   on(*out_, q.device(), "out");
   TORCH_CHECK_VALUE(out_->dim() == 2 && out_->size(0) == c.batch && out_->size(1) == width &&
                         out_->scalar_type() == q.scalar_type() && out_->stride(1) == 1,
                     "out must be [batch, n_q head_dim] of the queries' type with contiguous rows");
-  at::assert_no_partial_overlap(*out_, q);
+  apart(*out_, q, what);
   return *out_;
 }
 
@@ -370,7 +369,7 @@ at::Tensor attend8(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& 
   per_sequence(positions, sz, at::kLong, dev, "positions");
   TORCH_CHECK_VALUE(has(positions) || rows == 0, "positions are needed for the rotation");
   const int64_t n_q = q.size(1) / c.head_dim;
-  at::Tensor out = attend_out(out_, c, q.size(1), q);
+  at::Tensor out = attend_out(out_, c, q.size(1), q, "paged_attention");
   cudaStream_t s = stream_of(dev);
   const Scratch ws = workspace(dev, s, ts_paged8_attention_workspace_size(&c, (int)n_q));
   done(ts_paged8_attention(q.data_ptr(), code_of(q.scalar_type(), "paged_attention"), q.stride(0), (int)n_q, &c,
@@ -407,8 +406,8 @@ at::Tensor decode8(const at::Tensor& qkv_in, int64_t n_q, const at::Tensor& kp, 
   const int64_t rows = rope_rows(sz, cos, sin, dev, "paged_decode_attention");
   per_sequence(positions, sz, at::kLong, dev, "positions");
   TORCH_CHECK_VALUE(has(positions) || rows == 0, "positions are needed for the rotation");
-  at::Tensor out = attend_out(out_, c, n_q * c.head_dim, qkv_in);
   const at::Tensor qkv = fit_rows(qkv_in);
+  at::Tensor out = attend_out(out_, c, n_q * c.head_dim, qkv, "paged_decode_attention");
   cudaStream_t s = stream_of(dev);
   const Scratch ws = workspace(dev, s, ts_paged8_attention_workspace_size(&c, (int)n_q));
   done(ts_paged8_decode_attention(qkv.data_ptr(), code_of(qkv.scalar_type(), "paged_decode_attention"), qkv.stride(0), (int)n_q,

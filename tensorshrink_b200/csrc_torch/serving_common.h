@@ -114,6 +114,25 @@ inline at::Tensor forward_only(at::Tensor y, const char* name, std::initializer_
   return y;
 }
 
+// Refuses an `out` whose rows share memory with one another, or with rows of x that kernels read
+// where they lie: but for the same columns of the same rows, some warps may have yet to read
+// what others write. Both are matrices with as many rows, of contiguous elements of one size. (ATen's own check passes
+// over tensors with gaps between their rows.)
+inline void apart(const at::Tensor& out, const at::Tensor& x, const char* what) {
+  const int64_t rows = out.size(0), item = out.element_size(), width = out.size(1) * item, x_width = x.size(1) * item;
+  if (rows == 0 || width == 0 || x_width == 0) return;
+  const int64_t step = out.stride(0) * item, x_step = x.stride(0) * item;
+  TORCH_CHECK_VALUE(rows == 1 || step >= width, what, ": the rows of out overlap");
+  const auto at = reinterpret_cast<intptr_t>(out.data_ptr()), x_at = reinterpret_cast<intptr_t>(x.data_ptr());
+  if (at + (rows - 1) * step + width <= x_at || x_at + (rows - 1) * x_step + x_width <= at) return;
+  if (rows == 1 || step == x_step) {
+    if (at == x_at && width <= x_width) return;
+    const int64_t gap = rows == 1 ? 0 : ((at - x_at) % step + step) % step;   // from a row of x to the next of out
+    if (rows > 1 && gap >= x_width && gap + width <= step) return;
+  }
+  TORCH_CHECK(false, what, ": out overlaps the input");
+}
+
 // Raises the exception that the library's status stands for.
 inline void done(int rc, const char* what) {
   if (rc == TS_OK) return;

@@ -187,7 +187,8 @@ def paged_decode_attention(qkv: torch.Tensor, n_q: int, cache: AnyCache, positio
     query heads gave it; sequences must not share pages then (each adds to its own
     slots' scores, and one of two additions to the same would be lost). A sequence that has no slot for the token (negative
     seq_lens, no page left, a position without a rotary row) answers with
-    zeros and stores nothing. Returns [batch, n_q head_dim] in qkv's type.
+    zeros and stores nothing. Returns [batch, n_q head_dim] in qkv's type, or
+    `out`, which may be qkv's own query columns and shares no other memory with it.
     seq_lens is not changed (see `PagedKVCache.advance`).
 
     Over a cache of 8 bits (which accumulates nothing) the token is stored as
@@ -213,7 +214,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache8, positions: Optional[t
     (fp16 or bf16) is rotated to positions[b] when rotary tables are given;
     scores are scale * q.k (default head_dim ** -0.5). Slots without a page do
     not count; a sequence without tokens, or with a position that has no
-    rotary row, answers with zeros. Returns [batch, n_q head_dim] in q's type."""
+    rotary row, answers with zeros. Returns [batch, n_q head_dim] in q's type, or
+    `out`, which may be q itself and overlaps it in no other way."""
     if not isinstance(cache, PagedKVCache8):
         raise NotImplementedError("paged_attention reads a cache of 8 bits (paged_decode_attention reads both)")
     args = (q, *cache._args(), positions, rope_cos, rope_sin, scale)
@@ -315,7 +317,7 @@ def qk_norm_rope(qkv: torch.Tensor, n_q: int, n_kv: int, q_weight: Optional[torc
     rotated to positions[t] (int64 [tokens]) when rotary tables are given, all in
     fp32 and rounded once; values are copied. A token whose position has no
     rotary row comes out as zeros. Returns a tensor like qkv, or `out`, which
-    may be qkv itself.
+    may be qkv itself and overlaps it in no other way.
 
     With a cache of 16 bits and slots (int64 [tokens], as `paged_reserve` gives
     them) key and value heads also go to their slots in the pages, whose scores
