@@ -208,6 +208,7 @@ at::Tensor attend(const at::Tensor& qkv, int64_t n_q, const at::Tensor& kp, cons
     TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == c.batch && out.size(1) == owidth &&
                           out.scalar_type() == qkv.scalar_type() && out.stride(1) == 1,
                       "out must be [batch, n_q head_dim] of qkv's type with contiguous rows");
+    no_history(out, "paged_decode_attention");
     apart(out, qkv, "paged_decode_attention");
   } else {
     out = fresh({c.batch, owidth}, qkv.scalar_type(), dev);
@@ -376,6 +377,7 @@ at::Tensor& paged_decode_attention_out_meta(const at::Tensor& qkv, int64_t n_q, 
                                             const OptTensor& sin, c10::optional<double> scale, bool accumulate,
                                             at::Tensor& out) {
   paged_decode_attention_meta(qkv, n_q, kp, vp, table, lens, scores, slot_pos, positions, cos, sin, scale, accumulate);
+  no_history(out, "paged_decode_attention");
   return out;
 }
 

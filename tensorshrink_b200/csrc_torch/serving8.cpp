@@ -167,7 +167,7 @@ at::Tensor norm_rope(const at::Tensor& x_in, int64_t n_q, int64_t n_kv, const Op
     TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && out.stride(1) == 1 &&
                           out.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
                       "out must have x's shape and type, and contiguous rows that start on 16 bytes");
-    TORCH_CHECK(!at::GradMode::is_enabled() || !out.requires_grad(), "qk_norm_rope: out wants a gradient, and there is none");
+    no_history(out, "qk_norm_rope");
   } else {
     out = fresh(x.sizes(), x.scalar_type(), dev);
   }
@@ -347,6 +347,7 @@ at::Tensor attend_out(const OptTensor& out_, const ts_paged_cache8& c, int64_t w
   TORCH_CHECK_VALUE(out_->dim() == 2 && out_->size(0) == c.batch && out_->size(1) == width &&
                         out_->scalar_type() == q.scalar_type() && out_->stride(1) == 1,
                     "out must be [batch, n_q head_dim] of the queries' type with contiguous rows");
+  no_history(*out_, what);
   apart(*out_, q, what);
   return *out_;
 }
@@ -561,6 +562,7 @@ at::Tensor& qk_norm_rope_out_meta(const at::Tensor& x, int64_t n_q, int64_t n_kv
                                   const OptTensor& positions, const OptTensor& cos, const OptTensor& sin, double eps,
                                   at::Tensor& out) {
   qk_norm_rope_meta(x, n_q, n_kv, qw, kw, positions, cos, sin, eps);
+  no_history(out, "qk_norm_rope");
   return out;
 }
 at::Tensor qk_norm_rope_store_meta(const at::Tensor& x, int64_t n_q, int64_t n_kv, const OptTensor& qw, const OptTensor& kw,
@@ -576,6 +578,7 @@ at::Tensor& qk_norm_rope_store_out_meta(const at::Tensor& x, int64_t n_q, int64_
                                         const OptTensor&, const OptTensor&, const at::Tensor&, at::Tensor& out) {
   TORCH_CHECK_VALUE(x.scalar_type() == kp.scalar_type(), "qk_norm_rope: the cache's heads or type differ from x's");
   qk_norm_rope_meta(x, n_q, n_kv, qw, kw, positions, cos, sin, eps);
+  no_history(out, "qk_norm_rope");
   return out;
 }
 
@@ -616,6 +619,7 @@ at::Tensor& paged8_attention_out_meta(const at::Tensor& q, const at::Tensor& kp,
                                       const OptTensor& positions, const OptTensor& cos, const OptTensor& sin,
                                       c10::optional<double> scale, at::Tensor& out) {
   paged8_attention_meta(q, kp, vp, ks, vs, table, lens, positions, cos, sin, scale);
+  no_history(out, "paged_attention");
   return out;
 }
 
@@ -632,6 +636,7 @@ at::Tensor& paged8_decode_attention_out_meta(const at::Tensor& qkv, int64_t n_q,
                                              const at::Tensor& lens, const OptTensor& positions, const OptTensor& cos,
                                              const OptTensor& sin, c10::optional<double> scale, at::Tensor& out) {
   paged8_decode_attention_meta(qkv, n_q, kp, vp, ks, vs, table, lens, positions, cos, sin, scale);
+  no_history(out, "paged_decode_attention");
   return out;
 }
 

@@ -133,6 +133,11 @@ inline void apart(const at::Tensor& out, const at::Tensor& x, const char* what) 
   TORCH_CHECK(false, what, ": out overlaps the input");
 }
 
+// What is written into a given result has no history: one that wants a gradient is refused.
+inline void no_history(const at::Tensor& out, const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled() || !out.requires_grad(), what, ": out wants a gradient, and there is none");
+}
+
 // Raises the exception that the library's status stands for.
 inline void done(int rc, const char* what) {
   if (rc == TS_OK) return;

@@ -116,3 +116,19 @@ def test_attention_outputs(ts, kind):
     with pytest.raises(RuntimeError, match="overlap"):
         call(one[:width].view(1, -1), one[8:8 + w].view(1, -1))
     call(one[:width].view(1, -1), one[width:width + w].view(1, -1))
+
+
+@pytest.mark.parametrize("kind", ["attention", "decode 8", "decode 16"])
+def test_a_result_that_wants_a_gradient_is_refused(ts, kind):
+    cache = caches(ts, 2)[kind == "decode 16"]
+    x = rows(2, 8 * 64 if kind == "attention" else 12 * 64)
+
+    def call(out):
+        return ts.paged_attention(x, cache, out=out) if kind == "attention" else ts.paged_decode_attention(x, 8, cache, out=out)
+    leaf = torch.full((2, 8 * 64), 3.0, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(RuntimeError, match="wants a gradient"):
+        call(leaf)
+    assert (leaf == 3).all()
+    with torch.no_grad():
+        call(leaf)
+        assert not (leaf == 3).any() and torch.equal(leaf, call(None))
