@@ -226,6 +226,7 @@ at::Tensor paged_decode_attention(const at::Tensor& qkv, int64_t n_q, const at::
                                   const at::Tensor& table, const at::Tensor& lens, const OptTensor& scores,
                                   const OptTensor& slot_pos, const OptTensor& positions, const OptTensor& cos,
                                   const OptTensor& sin, c10::optional<double> scale, bool accumulate) {
+  no_tangents("paged_decode_attention", {&qkv});
   return forward_only(attend(qkv, n_q, kp, vp, table, lens, scores, slot_pos, positions, cos, sin, scale, accumulate,
                              c10::nullopt), "paged_decode_attention", {&qkv});
 }

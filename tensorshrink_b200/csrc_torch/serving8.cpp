@@ -208,6 +208,7 @@ at::Tensor qk_norm_rope_store(const at::Tensor& x, int64_t n_q, int64_t n_kv, co
                               const OptTensor& positions, const OptTensor& cos, const OptTensor& sin, double eps,
                               const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& table, const at::Tensor& lens,
                               const OptTensor& scores, const OptTensor& slot_pos, const at::Tensor& slots) {
+  no_tangents("qk_norm_rope_store", {&x, in(qw), in(kw)});
   return forward_only(store(x, n_q, n_kv, qw, kw, positions, cos, sin, eps, kp, vp, table, lens, scores, slot_pos, slots,
                             c10::nullopt), "qk_norm_rope_store", {&x, in(qw), in(kw)});
 }
@@ -421,6 +422,7 @@ at::Tensor paged8_decode_attention(const at::Tensor& qkv, int64_t n_q, const at:
                                    const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& table, const at::Tensor& lens,
                                    const OptTensor& positions, const OptTensor& cos, const OptTensor& sin,
                                    c10::optional<double> scale) {
+  no_tangents("paged_decode_attention", {&qkv});
   return forward_only(decode8(qkv, n_q, kp, vp, ks, vs, table, lens, positions, cos, sin, scale, c10::nullopt),
                       "paged_decode_attention", {&qkv});
 }

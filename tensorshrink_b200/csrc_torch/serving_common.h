@@ -5,6 +5,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -99,10 +100,21 @@ inline void on(const OptTensor& t, const at::Device& dev, const char* name) {
 
 // The operators compute no gradients. A floating-point result of inputs that want
 // them says so when a backward pass reaches it, instead of ending it silently;
-// the forward pass is the same. (Codes are integers, and what is written into a
-// cache or into a given result is held without its history.)
+// the forward pass is the same. Inputs with tangents (derivatives in forward mode) are
+// refused at once, as the result would come without one. (Codes are integers, and what is
+// quantised or written into a cache or a given result is held without its history.)
 inline const at::Tensor* in(const OptTensor& t) { return has(t) ? &*t : nullptr; }
+inline bool has_tangent(const at::Tensor& t) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined();
+}
+// (By itself in front of what writes into a cache.)
+inline void no_tangents(const char* name, std::initializer_list<const at::Tensor*> of) {
+  for (const at::Tensor* t : of)
+    TORCH_CHECK_NOT_IMPLEMENTED(t == nullptr || !has_tangent(*t), "tensorshrink::", name,
+                                " has no derivative in forward mode, and an input has a tangent");
+}
 inline at::Tensor forward_only(at::Tensor y, const char* name, std::initializer_list<const at::Tensor*> of) {
+  no_tangents(name, of);
   if (!at::GradMode::is_enabled()) return y;
   std::vector<at::Tensor> in;
   for (const at::Tensor* t : of)
@@ -133,9 +145,10 @@ inline void apart(const at::Tensor& out, const at::Tensor& x, const char* what) 
   TORCH_CHECK(false, what, ": out overlaps the input");
 }
 
-// What is written into a given result has no history: one that wants a gradient is refused.
+// What is written into a given result has no history: one that wants a gradient, or has a tangent, is refused.
 inline void no_history(const at::Tensor& out, const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled() || !out.requires_grad(), what, ": out wants a gradient, and there is none");
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(out), what, ": out has a tangent, and there is no derivative in forward mode");
 }
 
 // Raises the exception that the library's status stands for.

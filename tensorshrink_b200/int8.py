@@ -11,7 +11,7 @@ weights, dequantised on the way to 16-bit tensor cores, activations kept
 The functions are thin layers over `torch.ops.tensorshrink.int8_*`, with the
 conventions of `fp4`: the current stream of the tensors' device, no
 synchronisation, CUDA tensors only, no gradients (a backward pass that reaches a
-result raises).
+result raises, and inputs with tangents are refused; a quantised tensor has no history).
 """
 
 from __future__ import annotations

@@ -132,3 +132,18 @@ def test_a_result_that_wants_a_gradient_is_refused(ts, kind):
     with torch.no_grad():
         call(leaf)
         assert not (leaf == 3).any() and torch.equal(leaf, call(None))
+
+
+@pytest.mark.parametrize("kind", ["attention", "decode 8", "decode 16", "norm and store", "product"])
+def test_derivatives_in_forward_mode_are_refused(ts, kind):
+    import torch.autograd.forward_ad as fwd
+    cache = caches(ts, 2)[kind in ("decode 16", "norm and store")]
+    before = [t.clone() for t in cache._args() if t is not None]
+    x = rows(2, 8 * 64 if kind == "attention" else 12 * 64)
+    w = ts.int8_quantize(rows(16, 12 * 64, 1))
+    calls = {"attention": lambda y: ts.paged_attention(y, cache), "product": lambda y: ts.int8_linear(y, w),
+             "norm and store": lambda y: ts.qk_norm_rope(y, 8, 2, cache=cache, slots=torch.arange(2, device="cuda"))}
+    call = calls.get(kind, lambda y: ts.paged_decode_attention(y, 8, cache))
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+        call(fwd.make_dual(x, torch.ones_like(x)))
+    assert all(torch.equal(a, b) for a, b in zip(before, [t for t in cache._args() if t is not None]))
