@@ -645,11 +645,11 @@ at::Tensor& paged8_decode_attention_out_meta(const at::Tensor& qkv, int64_t n_q,
 void pool_check_meta(const at::Tensor& free, const at::Tensor& n_free) { pool_fits(free, n_free); }
 
 Slots paged_reserve_meta(const at::Tensor& free, const at::Tensor&, const at::Tensor&, const at::Tensor& lens, int64_t, int64_t,
-                         const at::Tensor&, const OptTensor&, int64_t tokens) {
-  TORCH_CHECK_VALUE(tokens >= 0, "paged_reserve: bad number of tokens ", tokens);
+                         const at::Tensor&, const OptTensor&, SymInt tokens) {
+  TORCH_CHECK_VALUE(!tokens.maybe_as_int() || *tokens.maybe_as_int() >= 0, "paged_reserve: bad number of tokens ", tokens);
   const auto i32 = free.options().dtype(at::kInt), i64 = free.options().dtype(at::kLong);
-  return {at::empty_symint({lens.sym_size(0)}, i32), at::empty_symint({lens.sym_size(0) + 1}, i32), at::empty({tokens}, i64),
-          at::empty({tokens}, i64), at::empty({tokens}, i32)};
+  return {at::empty_symint({lens.sym_size(0)}, i32), at::empty_symint({lens.sym_size(0) + 1}, i32), at::empty_symint({tokens}, i64),
+          at::empty_symint({tokens}, i64), at::empty_symint({tokens}, i32)};
 }
 
 void paged_release_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, int64_t,
@@ -687,7 +687,7 @@ TORCH_LIBRARY_FRAGMENT(tensorshrink, m) {
         "Tensor(f!) out) -> Tensor(f!)");
   m.def("pool_check(Tensor free, Tensor n_free) -> ()");
   m.def("paged_reserve(Tensor free, Tensor(a!) n_free, Tensor(b!) page_table, Tensor seq_lens, int page_size, int num_pages, "
-        "Tensor n_new, Tensor? positions, int tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+        "Tensor n_new, Tensor? positions, SymInt tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("paged_release(Tensor(a!) free, Tensor(b!) n_free, Tensor(c!) page_table, Tensor(d!) seq_lens, int page_size, "
         "int num_pages, Tensor keep) -> ()");
 }
