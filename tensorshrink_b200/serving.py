@@ -337,15 +337,21 @@ class PagedDecoder(nn.Module):
         if self.packed:
             # pages for the tokens; a sequence that gets none (in replays that nobody counts) stays as it is
             taken = paged_reserve(self.pool, self.caches[0], taken, 0).granted
+        views = self.caches
+        if self.budget is not None and self.layers[0].q_norm is not None:
+            # The rotation in front of the attention turns a sequence past its limit away; the attention, which has
+            # no tables then, would still give its slots weights: there it takes no part.
+            lens = self.caches[0].seq_lens.masked_fill(taken == 0, -1)
+            views = [PagedKVCache(c.k_pages, c.v_pages, c.page_table, lens, c.scores, c.slot_pos) for c in self.caches]
         h = self.embed[tokens].float()
-        for layer, cache in zip(self.layers, self.caches):
+        for layer, cache, view in zip(self.layers, self.caches, views):
             qkv = layer.qkv(_rms_norm(h, layer.input_norm, self.cfg.rms_eps))
             rope = (self.rope_cos, self.rope_sin)
             if layer.q_norm is not None:
                 qkv = qk_norm_rope(qkv, self.cfg.n_heads, self.cfg.n_kv_heads, layer.q_norm, layer.k_norm, self.positions, *rope,
                                    self.cfg.rms_eps, out=qkv)
                 rope = (None, None)
-            a = paged_decode_attention(qkv, self.cfg.n_heads, cache, self.positions, *rope, accumulate=self.budget is not None)
+            a = paged_decode_attention(qkv, self.cfg.n_heads, view, self.positions, *rope, accumulate=self.budget is not None)
             if not self.packed:
                 cache.advance(taken)
                 self._evict(cache)
