@@ -6,9 +6,11 @@
 // the tokens came into; rows behind the first eight loads of a lane (blocks of more
 // than 16 rows of 128 columns) are read a second time, from L1 or L2. A block that
 // holds earlier tokens keeps its scale where that is large enough. Where it is not, the
-// scale grows by a quarter at least and the earlier codes are rounded anew: a code is
+// scale grows by a quarter at least and the earlier codes are rounded anew. An int8 code is
 // then off by 1/2 (1 + 0.8 + 0.64 + ...) < 2.5 steps at most however often its block's scale
-// grows, where growth to what is needed would let the half steps of 15 tokens add up.
+// grows, where growth to what is needed would let the half steps of 15 tokens add up. An e4m3
+// code's step shrinks with the code: m growths leave a value within (1 + 2^-4)^(m + 1) - 1 of itself (of
+// 15 growths in a row, chosen to make it worst, 105%), which is at most 15% of the block's largest.
 // Bound by DRAM traffic: the tokens are read once, codes of half the size written. 30000 packed
 // tokens of 16 sequences, 8 heads of 128 columns, bf16 to e4m3: 38.5 us, 4.9 TB/s; the
 // values of the pages that they fill 32 us, 5.9 TB/s; one token of 64 sequences 3.8 us.

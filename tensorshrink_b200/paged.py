@@ -160,7 +160,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache: AnyCache, positions: O
     or bf16; k after its rotation) are quantised block by block. A block
     that holds earlier tokens keeps its scale if that is large enough;
     otherwise the scale grows, by a quarter at least, and the earlier tokens' codes
-    are rounded anew. An infinity or a NaN makes its block's scale NaN, which
+    are rounded anew: int8 codes are off by 2.5 steps at most then, e4m3 values by
+    (1 + 2^-4)^(growths + 1) - 1 of themselves, 15% of the block's largest. An infinity or a NaN makes its block's scale NaN, which
     stays until a token comes to the block's first slot again. Sequences must
     not share a page that gets tokens."""
     if isinstance(cache, PagedKVCache8):
