@@ -489,7 +489,7 @@ typedef struct ts_page_table {
  * token t < capacity `tokens` of the packed batch: sequences[t] (-1 behind the
  * last), slots[t] = page * page_size + offset (-1 without a page), positions[t] =
  * (first[b], or without first the slot's number in the sequence) of a token with a slot, 0
- * otherwise. seq_lens is not changed. Workspace as ts_paged_decode_attention.
+ * otherwise. seq_lens is not changed. There is no workspace.
  */
 TS_API int ts_paged_reserve(const ts_page_pool* pool, const ts_page_table* table, const int32_t* n_new,
                             const int64_t* first, int64_t tokens, int32_t* granted, int32_t* offsets, int64_t* slots,

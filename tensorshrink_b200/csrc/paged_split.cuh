@@ -1,6 +1,7 @@
-// How the attention kernels over the paged cache cut their work: units of 64
-// slots of one kv head, dealt out to CTAs, 16 slots of each unit to a warp; and the
-// matrix instructions that both use.
+// How the attention kernels over the paged cache cut their work: units of a kv head's
+// slots, dealt out to CTAs, a quarter of each unit to a warp (64 slots and 16 in the 16-bit
+// kernel, whose constants stand here, 128 and 32 in the 8-bit one); and the matrix
+// instructions that both use.
 #pragma once
 
 #include "paged.cuh"
@@ -12,6 +13,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;                  // slots of a warp's share of a unit
 constexpr int kUnit = kWarps * kRows;      // slots of a unit
+constexpr unsigned kUnitCost = 1800;       // cycles of a unit, see choose_deal
 constexpr int kRowCost = 6;                // units that starting and joining a row costs
 constexpr int kFullUnits = 8;              // units per CTA from which that cost is counted
 constexpr int kMaxPieces = 96;             // CTAs that share a kv head's units at most
@@ -59,11 +61,11 @@ struct Deal {
   unsigned n_cta;
 };
 
-// Cycles, as measured where CTAs have little to do: a unit `unit`; a row's start
+// Cycles, as measured in the 16-bit kernel where CTAs have little to do: a unit 1800; a row's start
 // and its warps' join 6000; the join of pieces 3000, and for each eight query
-// heads 2500 and 1200 for each eight pieces. (A whole warp calls it.)
-__device__ __forceinline__ Deal choose_deal(unsigned units, unsigned rows, int longest, unsigned grid, int heads,
-                                            unsigned unit = 1800) {
+// heads 2500 and 1200 for each eight pieces. The 8-bit kernel takes the same numbers for its own units,
+// which have as many bytes. (A whole warp calls it.)
+__device__ __forceinline__ Deal choose_deal(unsigned units, unsigned rows, int longest, unsigned grid, int heads) {
   if (rows == 0) return {0, 0};
   const unsigned turns = (heads + 2 * kWarps - 1) / (2 * kWarps);
   auto join = [&](unsigned pieces) { return pieces > 1 ? 3000 + turns * (2500 + (pieces + 7) / 8 * 1200) : 0; };
@@ -80,14 +82,14 @@ __device__ __forceinline__ Deal choose_deal(unsigned units, unsigned rows, int l
   // Where a launch has few units: each row in equal parts of CTAs of its own,
   // if that lets the last of them finish sooner.
   const unsigned share = (units + d.n_cta - 1) / d.n_cta;
-  const unsigned shares_cost = share * unit + (rows > 1 ? 6000 : 0) + join((longest + share - 1) / share + 1);
+  const unsigned shares_cost = share * kUnitCost + (rows > 1 ? 6000 : 0) + join((longest + share - 1) / share + 1);
   // lane i looks at i + 1 and at 34 + 2 i parts
   unsigned best = 0xFFFFFFFFu;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const unsigned p = k == 0 ? (threadIdx.x & 31) + 1 : 34 + 2 * (threadIdx.x & 31);
     const unsigned q = (longest + p - 1) / p;
-    if (p <= (unsigned)min(longest, kMaxPieces) && rows * p <= grid) best = min(best, (q * unit + join(p)) << 7 | p);
+    if (p <= (unsigned)min(longest, kMaxPieces) && rows * p <= grid) best = min(best, (q * kUnitCost + join(p)) << 7 | p);
   }
   best = __reduce_min_sync(0xffffffffu, best);
   if (best >> 7 < shares_cost) {
