@@ -396,8 +396,8 @@ typedef struct ts_paged_cache8 {
  * and q = 127 (TS_CACHE_INT8) or 448, in fp32:
  *   need = max(a * fp32(1 / q), 2^-100)
  *   scale = need                          the block holds no earlier tokens
- *         = old                           need <= old
- *         = max(need, 1.25 old)           otherwise; earlier codes become
+ *         = old                           need <= |old|
+ *         = max(need, 1.25 |old|)         otherwise; earlier codes become
  *                                         round(code * (old / scale))
  *   code = round(x * (1 / scale)), to nearest even, within +-q
  * An infinity or a NaN among a block's values makes its scale NaN (and stays

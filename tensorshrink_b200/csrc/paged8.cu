@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) paged8_append_kernel(const 
     if (finite) {
       scale = scale_of<E4M3>(unpack2<BF>(top).x);
       if (r0 > 0) {
-        if (scale > old) {
-          scale = fmaxf(scale, __fmul_rn(1.25f, old));
+        if (scale > fabsf(old)) {
+          scale = fmaxf(scale, __fmul_rn(1.25f, fabsf(old)));
           // the earlier tokens' codes, rounded anew
           const float ratio = __fdiv_rn(old, scale);
           for (int r = rl; r < r0; r += per)

@@ -8,7 +8,7 @@
 // e4m3 (and of wide groups, for registers) take the codes as fp16, exactly, and q as
 // fp16 without its power of two. A score is the product of the sum with a_t. A weight
 // enters the second product as p_t b_t over a power of two that is at least every
-// b_t so far (the output is scaled along when it grows, as for the running
+// |b_t| so far (the output is scaled along when it grows, as for the running
 // maximum), as two terms of fp16, 22 bits (one term turned the last bits of bf16
 // results).
 //
@@ -581,10 +581,10 @@ __global__ void __launch_bounds__(kThreads, C)
         }
         past = past || fmaxf(sc[t][0], sc[t][2]) > m[t][0] + kSlack || fmaxf(sc[t][1], sc[t][3]) > m[t][1] + kSlack;
       }
-      if (__any_sync(0xffffffffu, past || vs > v_pow)) {
+      if (__any_sync(0xffffffffu, past || fabsf(vs) > v_pow)) {
         float grow = 1.f;
-        if (vs > v_pow) {
-          const uint32_t e = min((__float_as_uint(vs) + 0x7FFFFFu) >> 23, 253u);     // 2^e >= vs
+        if (fabsf(vs) > v_pow) {
+          const uint32_t e = min((__float_as_uint(fabsf(vs)) + 0x7FFFFFu) >> 23, 253u);     // 2^e >= |vs|
           const float inv = __uint_as_float((254u - e) << 23);
           grow = v_pow * inv;
           v_pow = __uint_as_float(e << 23);
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, C)
             }
           }
       }
-      const float vf = vs * v_inv;                     // at most 1
+      const float vf = vs * v_inv;                     // 1 in size at most
       uint32_t pf[NT][2], pr[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
