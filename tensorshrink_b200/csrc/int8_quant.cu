@@ -11,7 +11,7 @@
 // read once: up to 32 columns a thread, groups of a warp to a CTA of 1024 threads;
 // rows of more than 32768 columns are read a second time, from L2. Rows that do
 // not start on 16 bytes are read in words, shifted where they start in the
-// middle of one. Bound by DRAM traffic: 8191 x 8192 bf16 35 us, 5.8 TB/s; one row of
+// middle of one. Bound by DRAM traffic: 8191 x 8192 bf16 33 to 35 us, 5.8 to 6.0 TB/s; one row of
 // 4096, 2.0 us.
 #include <algorithm>
 
@@ -80,7 +80,8 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) int8_quantize_kernel(const 
   }
 }
 
-// The values q s of the first `cols` columns, a thread eight of them.
+// The values q s of the first `cols` columns, a thread eight of them. 14336 x 4096 to bf16 50 us, 3.5 TB/s (27 us at the
+// copy's bandwidth), to fp32 79, 3.7 TB/s (45): every eight values take a 64-bit division and the choice of the type.
 __global__ void __launch_bounds__(256) int8_dequantize_kernel(const int8_t* codes, int64_t ld, const float* scales, int64_t rows,
                                                               int64_t cols, void* out, int dtype, int64_t out_stride, int vec) {
   const int64_t chunks = (cols + 7) / 8;

@@ -32,10 +32,12 @@
 // scales of its tile 32 j + i, three batches deep. Every wait is bounded; a warp whose
 // wait runs out records it and stops.
 //
-// Measured (128 columns, 8 kv heads): 64 sequences of up to 8191 slots, 8 query heads to a kv
-// head, int8, token-major pages, 96 us repeated on one input, 5.6 TB/s, 106 on others each
-// time; 4 of 32768, e4m3, fp16 results, 52 us, 5.2 TB/s; one of 512, 10 us, a chain of
-// latencies and of first instruction fetches.
+// Measured (128 columns, 8 kv heads, other inputs each time, in a graph): 64 sequences of up to 8191 slots,
+// 8 query heads to a kv head, int8, token-major pages, 102 us, 5.3 TB/s (a call 111, with one term for
+// a weight 106); 4 of 32768, e4m3, fp16 results, 53 us, 5.1 TB/s; one of 512, 10.5 us, a chain of
+// latencies and of first instruction fetches. Groups of more than eight heads, whose second column tile
+// doubles the instructions of a slot, are bound by those: 16 heads, 32 sequences of up to 8000 slots
+// 77 us (e4m3 71), 3.4 TB/s; 32 heads over one, each 16 of them reading the slots again, 32 of up to 20000 51 us for 81 MB.
 #include <algorithm>
 
 #include "gemm.cuh"
@@ -143,9 +145,9 @@ __device__ __forceinline__ void to_half(uint32_t w, uint32_t& x, uint32_t& y) {
 // DP: columns that are computed, head_dim rounded up (the copies fill the rest of a
 // box with zeros). C: blocks per SM, as many as the registers allow, which hides more of a
 // tile's chain of latencies, and of a row's start, than longer rings do. 64 columns, 64 sequences
-// of up to 16000 slots: four blocks 99 us, three 104, two with rings of six stages 130;
-// 16 query heads to a kv head, 32 of up to 8000: 49, 48, 53. 96 columns, 64 of up to
-// 16000: three blocks 139, two 146; 128 columns: see kManyRows.
+// of up to 16000 slots: four blocks 108 us, three 112, two with rings of six stages 139;
+// 16 query heads to a kv head, 32 of up to 8000: 54, 53, 57. 96 columns, 64 of up to
+// 16000: three blocks 141, two 156; 128 columns: see kManyRows.
 template <int DP, int NT, int C>
 struct Ring {
   static constexpr int kCols = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;   // columns in shared memory
@@ -157,9 +159,10 @@ struct Ring {
 };
 
 // 128 columns: three blocks per SM with rings of two stages where the rows are many and short (150
-// sequences of 8 kv heads, of up to 300 slots 26 us for 29 with two blocks of three stages, of
-// up to 3000 85 for 96), else two (128 of 8000 slots 316 us for 339, 64 of up to 16000 167 for
-// 171, 4 of 4000 14.7 for 15.8). The host knows the tables' capacity, not the lengths.
+// sequences of 8 kv heads, of up to 300 slots 30 us for 33 with two blocks of three stages, of
+// up to 3000 91 for 103), else two (128 of 8000 slots 328 us for 337, 64 of up to 16000 175 for
+// 176, 4 of 4000 17.9 for 18.9). The host knows the tables' capacity, not the lengths: 256 of up to 1000 slots
+// in tables with room for more than 4096 take 81 us, 68 with three blocks.
 constexpr int kManyRows = 2;               // kv heads of all sequences per SM, from which three are taken
 constexpr int64_t kShortTable = 4096;      // slots
 
@@ -404,8 +407,9 @@ __global__ void __launch_bounds__(kThreads, C)
     pg2 = page_of_tile(64 + lane);
 
     // Each head by a warp: rotated and rounded to its type, then either in fp16 with the
-    // power of two of its largest magnitude taken out, or as an integer of 2^21
-    // times that, in three signed bytes (24 bits under the largest magnitude).
+    // power of two of its largest magnitude taken out (off by 2^-25 of that power at most, where an
+    // element lies under fp16's normal range, else not at all), or as an integer of 2^21
+    // times that, in three signed bytes (24 bits under the largest magnitude, off by 2^-22 of the power at most).
 #pragma unroll
     for (int w = 0; w < kOwn; ++w) {
       const int g = warp + w * kWarps;
@@ -937,9 +941,8 @@ static int make_args(AttnArgs* a, int q_dtype, int n_q, const ts_paged_cache8* c
   a->head_tiles = (a->group + heads - 1) / heads;
   // Where a token's heads lie next to each other, up to four CTAs of neighbouring numbers
   // take as many heads of the same slots at about the same time, so that DRAM serves longer
-  // runs: 64 sequences of up to 8191 slots 96 us for 103 to 108 (two heads 96, eight 97), on other
-  // inputs each time 108 for 110. Pages of
-  // whole heads gain nothing (53 us for 53) and keep all CTAs.
+  // runs: 64 sequences of up to 8191 slots 102 us for 112 (two heads 103, eight 102). Pages of
+  // whole heads gain nothing (57 us for 57) and keep all CTAs.
   a->abreast = 1;
   for (int n = 2; n <= 4; ++n)
     if (a->c.head_stride < a->c.token_stride && a->c.n_kv * a->head_tiles % n == 0) a->abreast = n;
