@@ -881,8 +881,9 @@ static int encode_map(CUtensorMap* map, const Cache& c, const void* base, int bo
                      box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
+// `token`: what is appended first, once nothing can be refused any more; or NULL.
 template <bool BF, bool E4M3, int DP, int NT, int C>
-static int launch(const AttnArgs& a, int overlap, cudaStream_t st) {
+static int launch(const AttnArgs& a, const AppendArgs* token, cudaStream_t st) {
   auto k = paged8_attention_kernel<BF, E4M3, DP, NT, C>;
   const size_t smem = attn_smem<E4M3, DP, NT, C>(a.c.batch);
   // (the same value for all host threads, as for the 16-bit kernel)
@@ -901,25 +902,26 @@ static int launch(const AttnArgs& a, int overlap, cudaStream_t st) {
   CUtensorMap km, vm;
   int rc = encode_map(&km, a.c, a.c.k, Ring<DP, NT, C>::kBox);
   if (rc == TS_OK) rc = encode_map(&vm, a.c, a.c.v, Ring<DP, NT, C>::kBox);
+  if (rc == TS_OK && token != nullptr) rc = launch_append(*token, BF ? TS_BF16 : TS_F16, E4M3 ? TS_CACHE_E4M3 : TS_CACHE_INT8, 1, st);
   if (rc != TS_OK) return rc;
-  TS_CUDA_TRY(launch_after(k, sm_count() * C, kThreads, smem, st, overlap, 0, km, vm, a));
+  TS_CUDA_TRY(launch_after(k, sm_count() * C, kThreads, smem, st, token != nullptr, 0, km, vm, a));
   TS_LAUNCH_CHECK();
   return TS_OK;
 }
 
 template <bool BF, bool E4M3>
-static int launch(const AttnArgs& a, int overlap, cudaStream_t st) {
+static int launch(const AttnArgs& a, const AppendArgs* token, cudaStream_t st) {
   // one column tile of eight query heads, or two where a group has more
   const bool wide = a.group > 8;
-  if (a.c.head_dim <= 64) return wide ? launch<BF, E4M3, 64, 2, 3>(a, overlap, st) : launch<BF, E4M3, 64, 1, 4>(a, overlap, st);
-  if (a.c.head_dim <= 96) return wide ? launch<BF, E4M3, 96, 2, 2>(a, overlap, st) : launch<BF, E4M3, 96, 1, 3>(a, overlap, st);
+  if (a.c.head_dim <= 64) return wide ? launch<BF, E4M3, 64, 2, 3>(a, token, st) : launch<BF, E4M3, 64, 1, 4>(a, token, st);
+  if (a.c.head_dim <= 96) return wide ? launch<BF, E4M3, 96, 2, 2>(a, token, st) : launch<BF, E4M3, 96, 1, 3>(a, token, st);
   if (a.c.head_dim <= 128) {
-    if (wide) return launch<BF, E4M3, 128, 2, 2>(a, overlap, st);
+    if (wide) return launch<BF, E4M3, 128, 2, 2>(a, token, st);
     const bool many = (int64_t)a.c.batch * a.c.n_kv >= (int64_t)kManyRows * sm_count() &&
                       (int64_t)a.c.max_pages * a.c.page_size <= kShortTable;
-    return many ? launch<BF, E4M3, 128, 1, 3>(a, overlap, st) : launch<BF, E4M3, 128, 1, 2>(a, overlap, st);
+    return many ? launch<BF, E4M3, 128, 1, 3>(a, token, st) : launch<BF, E4M3, 128, 1, 2>(a, token, st);
   }
-  return wide ? launch<BF, E4M3, 256, 2, 1>(a, overlap, st) : launch<BF, E4M3, 256, 1, 1>(a, overlap, st);
+  return wide ? launch<BF, E4M3, 256, 2, 1>(a, token, st) : launch<BF, E4M3, 256, 1, 1>(a, token, st);
 }
 
 // Fills `a` from the arguments that both entry points share, and checks them.
@@ -972,9 +974,9 @@ static int make_args(AttnArgs* a, int q_dtype, int n_q, const ts_paged_cache8* c
   return TS_OK;
 }
 
-static int attend(const AttnArgs& a, int dtype, int code, int overlap, cudaStream_t st) {
-  if (dtype == TS_BF16) return code == TS_CACHE_E4M3 ? launch<true, true>(a, overlap, st) : launch<true, false>(a, overlap, st);
-  return code == TS_CACHE_E4M3 ? launch<false, true>(a, overlap, st) : launch<false, false>(a, overlap, st);
+static int attend(const AttnArgs& a, const AppendArgs* token, int dtype, int code, cudaStream_t st) {
+  if (dtype == TS_BF16) return code == TS_CACHE_E4M3 ? launch<true, true>(a, token, st) : launch<true, false>(a, token, st);
+  return code == TS_CACHE_E4M3 ? launch<false, true>(a, token, st) : launch<false, false>(a, token, st);
 }
 
 }  // namespace paged8
@@ -999,7 +1001,7 @@ extern "C" int ts_paged8_attention(const void* q, int q_dtype, int64_t q_row_str
   a.q = reinterpret_cast<const uint16_t*>(q);
   a.q_stride = q_row_stride;
   a.extra = 0;
-  return paged8::attend(a, q_dtype, cache->code, 0, reinterpret_cast<cudaStream_t>(stream));
+  return paged8::attend(a, nullptr, q_dtype, cache->code, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ts_paged8_decode_attention(const void* qkv, int qkv_dtype, int64_t qkv_row_stride, int n_q,
@@ -1007,7 +1009,7 @@ extern "C" int ts_paged8_decode_attention(const void* qkv, int qkv_dtype, int64_
                                           const float* rope_sin, int64_t rope_rows, float scale, void* out,
                                           int64_t out_row_stride, void* workspace, size_t workspace_bytes, void* stream) {
   paged8::AttnArgs a;
-  int rc = paged8::make_args(&a, qkv_dtype, n_q, cache, positions, rope_cos, rope_sin, rope_rows, scale, out, out_row_stride,
+  const int rc = paged8::make_args(&a, qkv_dtype, n_q, cache, positions, rope_cos, rope_sin, rope_rows, scale, out, out_row_stride,
                              workspace, workspace_bytes);
   if (rc != TS_OK || a.c.batch == 0) return rc;
   TS_REQUIRE(qkv && is_aligned(qkv, 16) && qkv_row_stride % 8 == 0, "qkv rows must be 16-byte aligned");
@@ -1028,10 +1030,7 @@ extern "C" int ts_paged8_decode_attention(const void* qkv, int qkv_dtype, int64_
   p.cos_t = rope_cos;
   p.sin_t = rope_sin;
   p.rope_rows = rope_rows;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  rc = paged8::launch_append(p, qkv_dtype, cache->code, 1, st);
-  if (rc != TS_OK) return rc;
-  return paged8::attend(a, qkv_dtype, cache->code, 1, st);
+  return paged8::attend(a, &p, qkv_dtype, cache->code, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ts_paged8_status(int clear, void* stream) {
