@@ -934,8 +934,10 @@ static int max_clusters(int size) {
 // of a pair's tile what its bytes take into an SM at 60 a cycle, the change from tile to
 // tile 500; a stage of a lone CTA's tile its bytes at 40 a cycle, or the weight's at DRAM's
 // rate, 1400 for the results of each 32 tokens, 500 and 1200 per 32 tokens for the join of up to four
-// pieces, 1500 and 600 for a cluster's. Both kinds of plan tried on 28 shapes: the one taken is
-// within 5% of the best. Up to 32 tokens a pair's tile of 256 is all but empty (1 x 14336
+// pieces, 1500 and 600 for a cluster's. Both kinds of plan tried on 4 weights x 12 numbers of tokens from 1 to
+// 4096: the one taken is within 5% of the best, but for 33 to 64 tokens, where the costs of a lone CTA's results are not
+// told well (6144 x 4096 14.4 us, pairs of 96 rows 11.4; 14336 x 4096 18.1 us, lone CTAs 16.7; 4096 x 4096, 64 tokens 11.2,
+// pairs of 64 rows 10.1). Up to 32 tokens a pair's tile of 256 is all but empty (1 x 14336
 // x 4096: 23 us, a lone CTA's 13.6).
 static Plan plan(int64_t M, int64_t N, int64_t K) {
   Plan p{};
